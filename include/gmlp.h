@@ -317,6 +317,55 @@ int gmlp_hidden_bwd(const void* dh, const void* x, const void* w_gate, const voi
                     int64_t K, int64_t N, int dtype, int act, float dropout_p, uint64_t seed, uint64_t offset,
                     void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * 4-bit weights and expert layers, for serving a few token rows (M <= 64).  fp16 and bf16 activations, inference only.
+ * The reference has neither; the math is its gated MLP (EagerGatedMLP, src/triton_gated_mlp/gated_mlp.py:73-98), per
+ * expert, on weights scale·n.
+ *
+ * Storage of a 4-bit matrix [rows, cols] (multiples of 8) with one scale per row and `group` columns, group = 32, 64
+ * or 128: padded to whole tiles of 16 rows and blocks of 128 columns.
+ *   codes   uint8 [tiles][blocks][4 q][16 r][4 s][4 bytes]: the 4 bytes of (q, r, s) are columns 32 s + 8 q + 0..7 of row r as
+ *           n + 8, -8 <= n <= 7: columns 0, 2, 4, 6 in nibbles 0..3, columns 1, 3, 5, 7 in nibbles 4..7 (a byte's low
+ *           nibble first).  A tile's block is 1 KiB, in the order in which a wavefront's lanes load it.
+ *   scales  dtype [tiles][blocks][4][128 / group][4]: quarter of the tile's rows, group, row of the quarter.
+ * What lies in the padding is not used, but its scales have to be finite.  Several matrices of one size (experts)
+ * follow each other.
+ *
+ * gmlp_q4_quantize: scale = (largest magnitude of the group) / 7 rounded to dtype, n = w / scale rounded to nearest (even); padding
+ *   is n = 0, and scale 0 where a whole group is padding.  gmlp_q4_dequantize: w = scale·n rounded to dtype.
+ * gmlp_q4_linear_fwd: y[M,C] = x[M,R]·Wᵀ + bias, W [C,R] 4-bit; bias may be NULL.  The products are of scale·n itself, not
+ *   of its rounding.
+ * gmlp_q4_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) in dtype [M,N] (scratch), y = h·W_downᵀ + b_down.
+ */
+int gmlp_q4_quantize(const void* w, void* codes, void* scales, int64_t count, int64_t rows, int64_t cols, int group, int dtype,
+                     void* stream);
+int gmlp_q4_dequantize(const void* codes, const void* scales, void* w, int64_t count, int64_t rows, int64_t cols, int group,
+                       int dtype, void* stream);
+int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, const void* bias, void* y, int64_t M, int64_t R,
+                       int64_t C, int group, int dtype, void* stream);
+int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_gate, const void* codes_up, const void* scales_up,
+                    const void* codes_down, const void* scales_down, const void* b_gate, const void* b_up, const void* b_down,
+                    void* h, void* y, int64_t M, int64_t K, int64_t N, int group, int dtype, int act, void* stream);
+
+/*
+ * gmlp_moe_route: p = softmax(logits[m, 0..E)) in fp32; experts [M, top_k] are the numbers of the top_k largest logits in
+ *   descending order (the lowest number first among equals, NaN above everything), weights [M, top_k] their p, divided
+ *   by their sum if `normalize`.  dtype: of the logits (any GMLP_* one); weights are float, experts int64_t.  A logit of -inf
+ *   is an expert that the token cannot have: weight 0; a row of nothing else has weights 0.  A row with NaN or +inf has
+ *   weights NaN, as softmax does.  logits, weights and experts need the alignment of their elements only.  1 <= top_k <= 16, top_k <= E <= 512, any M.
+ * gmlp_moe_fwd: y[m] = sum over m's experts e of weight·MLP_e(x[m]), MLP_e the gated MLP with w_gate[e], w_up[e] [N,K] and
+ *   w_down[e] [K,N] (group = 0: dtype, s_* NULL; otherwise 4-bit codes with scales s_*); the hidden states are rounded to
+ *   dtype, the sum over experts is fp32.  Experts that no token chose are not read; one with weight 0 through -inf is not
+ *   run.  M <= 64.  workspace: gmlp_moe_workspace_bytes.
+ */
+int gmlp_moe_route(const void* logits, float* weights, int64_t* experts, int64_t M, int64_t E, int64_t top_k, int normalize, int dtype,
+                   void* stream);
+size_t gmlp_moe_workspace_bytes(int64_t M, int64_t N, int64_t E, int64_t top_k, int dtype);
+int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const void* w_up, const void* w_down, const void* s_gate,
+                 const void* s_up, const void* s_down, void* y, int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k,
+                 int normalize, int group, int dtype, int logits_dtype, int act, void* workspace, size_t workspace_bytes,
+                 void* stream);
+
 /* Writes the dropout keep mask (1 = keep) for an [M,N] tensor; the test oracle of the generator. */
 int gmlp_dropout_mask(uint8_t* mask, int64_t M, int64_t N, float dropout_p, uint64_t seed,
                       uint64_t offset, void* stream);

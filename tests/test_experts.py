@@ -1,0 +1,626 @@
+"""4-bit weights, expert routing and expert layers against plain implementations in 64 bits.
+
+Tolerances.  u is half a unit in the last place of the output type (2^-11 fp16, 2^-8 bf16), s the smallest subnormal's half.
+A sum of n products accumulated in fp32 (rounded or truncated at each addition) is off by at most (n + 16) 2^-23 of the sum
+of their magnitudes.  So a linear layer is held, element by element, to u |y| + (n + 16) 2^-23 (|x| |W|ᵀ + |b|) + s.  A gated
+MLP adds what its hidden states are off by, carried through |W_down|: their own rounding, and act(g) u with g and u off by
+their sums' bounds (every activation's slope is at most 1.13, the device's activations are within 2e-6 of theirs).  Those
+bounds grow with n while errors grow with its root, so the 2-norm is held too: a rounding is at most u / sqrt(3) in the mean
+square, two of them 0.82 u, so the norm of the error is at most u times the result's (one rounding: 0.6 u).
+"""
+
+import math
+
+import pytest
+import torch
+
+from triton_gated_mlp import _cabi
+from triton_gated_mlp.ops import moe, quant
+
+U = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8}
+SUB = {torch.float16: 2.0**-25, torch.bfloat16: 2.0**-134}
+HALF = [torch.float16, torch.bfloat16]
+
+
+# ------------------------------------------------------------------ plain implementations
+def numbers_of(q):
+    """(n, scale of each) of a single Q4Weight as float64 [rows, cols], looked up one place at a time."""
+    codes, scales = q.codes.cpu().reshape(-1), q.scales.cpu().double().reshape(-1)
+    KB, g = q.codes.shape[-5], q.group_size
+    r = torch.arange(q.rows).unsqueeze(1)
+    c = torch.arange(q.cols).unsqueeze(0)
+    block = (r // 16) * KB + c // 128
+    nibble = torch.where(c % 2 == 0, (c % 8) // 2, 4 + (c % 8) // 2)
+    byte = block * 1024 + ((c % 32) // 8) * 256 + (r % 16) * 16 + ((c % 128) // 32) * 4 + nibble // 2
+    n = ((codes[byte].int() >> (4 * (nibble % 2))) & 15) - 8
+    at = block * (16 * 128 // g) + ((r % 16) // 4) * (4 * 128 // g) + ((c % 128) // g) * 4 + r % 4
+    return n.double(), scales[at]
+
+
+def weights_of(q):
+    n, s = numbers_of(q)
+    return n * s
+
+
+def sliced(q, e):
+    return quant.Q4Weight(q.codes[e], q.scales[e], q.rows, q.cols, q.group_size)
+
+
+ACT = {
+    "silu": lambda g: g * torch.sigmoid(g),
+    "gelu": torch.nn.functional.gelu,
+    "relu": torch.relu,
+    "leaky_relu": torch.nn.functional.leaky_relu,
+    "sigmoid": torch.sigmoid,
+    "tanh": torch.tanh,
+    "no_act": lambda g: g,
+}
+
+
+def linear64(x, w, b, dtype):
+    """(y, bound) in float64."""
+    y, mass = x @ w.T, x.abs() @ w.abs().T
+    if b is not None:
+        y, mass = y + b, mass + b.abs()
+    return y, U[dtype] * y.abs() + (x.shape[1] + 16) * 2.0**-23 * mass + SUB[dtype]
+
+
+def mlp64(x, wg, bg, wu, bu, wd, bd, act, dtype):
+    """(y, bound) before the rounding of y, in float64."""
+    u = U[dtype]
+    g, dg = linear64(x, wg, bg, dtype)
+    v, dv = linear64(x, wu, bu, dtype)
+    dg, dv = dg - u * g.abs(), dv - u * v.abs()  # these two stay in fp32
+    a = ACT[act](g)
+    h = a * v
+    da = 1.13 * dg + 2e-6 * (1 + a.abs())
+    dh = da * (v.abs() + dv) + a.abs() * dv + u * h.abs() + SUB[dtype]
+    y, mass = h @ wd.T, h.abs() @ wd.abs().T
+    if bd is not None:
+        y, mass = y + bd, mass + bd.abs()
+    return y, dh @ wd.abs().T + (h.shape[1] + 16) * 2.0**-23 * mass
+
+
+def route64(logits, k, normalize):
+    """(weights, experts): the largest that is left, one after the other."""
+    rows = []
+    for row in logits.double().tolist():
+        left = list(range(len(row)))
+        picks = []
+        for _ in range(k):
+            best = left[0]
+            for e in left[1:]:
+                if row[e] > row[best]:
+                    best = e
+            picks.append(best)
+            left.remove(best)
+        top = max(row)
+        if top == -math.inf:
+            rows.append(([0.0] * k, picks))
+            continue
+        p = [math.exp(v - top) for v in row]
+        total = sum(p[e] for e in picks) if normalize else sum(p)
+        rows.append(([p[e] / total for e in picks], picks))
+    return torch.tensor([w for w, _ in rows], dtype=torch.float64), torch.tensor([e for _, e in rows])
+
+
+def moe64(x, logits, k, normalize, act, dtype, weights):
+    """weights(e) -> (W_gate, W_up, W_down) in float64; (y, bound)."""
+    w, experts = route64(logits, k, normalize)
+    y, bound = torch.zeros_like(x), torch.zeros_like(x)
+    mass = torch.zeros_like(x)
+    for e in sorted(set(experts.reshape(-1).tolist())):
+        t, j = torch.nonzero((experts == e) & (w > 0), as_tuple=True)
+        if len(t) == 0:
+            continue
+        wg, wu, wd = weights(e)
+        out, off = mlp64(x[t], wg, None, wu, None, wd, None, act, dtype)
+        y[t] += w[t, j, None] * out
+        bound[t] += w[t, j, None] * (off + 1e-6 * out.abs())  # (a weight is within 1e-6 of its own)
+        mass[t] += (w[t, j, None] * out).abs()
+    return y, bound + U[dtype] * y.abs() + (k + 16) * 2.0**-23 * mass + SUB[dtype]
+
+
+def hold(got, y, bound, dtype, roundings):
+    got = got.detach().double().cpu().reshape(y.shape)
+    assert torch.isfinite(got).all()
+    off = (got - y).abs()
+    assert (off <= bound).all(), f"off by {(off / bound).max().item():.3f} of the bound"
+    if y.numel() >= 64 and y.norm() > 0:
+        rel = ((got - y).norm() / y.norm()).item()
+        assert rel <= U[dtype] * (0.6 if roundings == 1 else 1.0), f"2-norm off by {rel / U[dtype]:.3f} u"
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def normal(shape, std, dtype, g):
+    return (std * torch.randn(shape, generator=g)).to(dtype)
+
+
+# ------------------------------------------------------------------ without a GPU
+def test_refusals_of_the_c_interface():
+    import ctypes
+
+    lib = _cabi.lib()
+    raw = ctypes.create_string_buffer(4096 + 64)
+    a = (ctypes.addressof(raw) + 63) & ~63
+    err = lambda: lib.gmlp_last_error().decode()
+    # NULL, group size, dtype, widths, rows, alignment
+    assert lib.gmlp_q4_linear_fwd(None, a, a, None, a, 1, 64, 64, 128, 0, None) == -1 and "NULL" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 48, 0, None) == -1 and "group" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 128, 2, None) == -2
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 128, 9, None) == -1
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 60, 64, 128, 0, None) == -2 and "multiple of 8" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 60, 128, 0, None) == -2
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 65, 64, 64, 128, 0, None) == -2 and "64" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 0, 64, 64, 128, 0, None) == -2
+    assert lib.gmlp_q4_linear_fwd(a + 8, a, a, None, a, 1, 64, 64, 128, 0, None) == -3
+    assert lib.gmlp_q4_linear_fwd(a, a, a, a + 2, a, 1, 64, 64, 128, 0, None) == -3
+    mlp = lambda x, M, K, N, group, dtype, act: lib.gmlp_q4_mlp_fwd(x, a, a, a, a, a, a, None, None, None, a, a, M, K, N, group, dtype, act, None)
+    assert mlp(None, 1, 64, 64, 32, 0, 0) == -1 and mlp(a, 1, 64, 64, 32, 0, 7) == -1 and "act" in err()
+    assert mlp(a, 1, 64, 68, 32, 0, 0) == -2 and mlp(a, 65, 64, 64, 32, 0, 0) == -2 and mlp(a, 1, 64, 64, 16, 0, 0) == -1
+    for quantize in (lib.gmlp_q4_quantize, lib.gmlp_q4_dequantize):
+        assert quantize(a, None, a, 1, 16, 128, 32, 0, None) == -1
+        assert quantize(a, a, a, 1, 16, 128, 100, 0, None) == -1
+        assert quantize(a, a, a, 0, 16, 128, 32, 0, None) == -2
+        assert quantize(a, a, a, 1, 12, 128, 32, 0, None) == -2
+        assert quantize(a, a, a, 1, 16, 128, 32, 2, None) == -2
+        assert quantize(a, a, a, 1 << 40, 16, 128, 32, 0, None) == -2
+    assert lib.gmlp_moe_route(a, a, None, 1, 8, 2, 1, 2, None) == -1
+    assert lib.gmlp_moe_route(a, a, a, 1, 8, 9, 1, 2, None) == -2 and "top_k" in err()
+    assert lib.gmlp_moe_route(a, a, a, 1, 8, 0, 1, 2, None) == -2
+    assert lib.gmlp_moe_route(a, a, a, 1, 513, 2, 1, 2, None) == -2
+    assert lib.gmlp_moe_route(a, a, a, 1, 64, 17, 1, 2, None) == -2
+    assert lib.gmlp_moe_route(a, a, a, 0, 8, 2, 1, 2, None) == -2
+    assert lib.gmlp_moe_route(a, a, a, 1, 8, 2, 1, 5, None) == -1
+    need = lib.gmlp_moe_workspace_bytes(4, 64, 8, 2, 0)
+    assert need >= 4 * 2 * 64 * 2
+    assert lib.gmlp_moe_workspace_bytes(65, 64, 8, 2, 0) == 0
+
+    def layer(x=a, logits=a, s=None, y=a, M=4, K=64, N=64, E=8, k=2, group=0, dtype=0, ld=2, act=0, ws=a, n=need):
+        return lib.gmlp_moe_fwd(x, logits, a, a, a, s, s, s, y, M, K, N, E, k, 1, group, dtype, ld, act, ws, n, None)
+
+    assert layer(x=None) == -1 and layer(logits=None) == -1 and layer(ws=None) == -1
+    assert layer(n=need - 1) == -1 and "workspace" in err()
+    assert layer(M=65) == -2 and layer(M=0) == -2 and layer(K=60) == -2 and layer(N=4) == -2 and layer(k=9) == -2 and layer(E=600) == -2
+    assert layer(group=128) == -1 and layer(group=5, s=a) == -1 and layer(dtype=2) == -2 and layer(ld=3) == -1 and layer(act=9) == -1
+    assert layer(x=a + 4) == -3 and layer(ws=a + 8) == -3
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.zeros(2, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        moe.moe_route(torch.zeros(2, 8), 2)
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        quant.quantize_q4(x)
+    w = torch.zeros(8, 64, 64, dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        moe.moe_mlp_fwd(x, torch.zeros(2, 8), w, w, w, 2)
+
+
+# ------------------------------------------------------------------ 4-bit weights
+gpu = pytest.mark.gpu
+
+
+def device():
+    assert torch.cuda.is_available(), "GPU tests need a visible AMD GPU"
+    return torch.device("cuda", 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("shape", [(8, 8), (16, 128), (40, 200), (3, 24, 328)])
+def test_quantize_and_dequantize(shape, group, dtype):
+    w = normal(shape, 0.02, dtype, gen(1))
+    w[..., 0, :] = 0  # a row of zeros
+    q = quant.quantize_q4(w.to(device()), group)
+    back = quant.dequantize_q4(q)
+    assert back.shape == w.shape and back.dtype == dtype
+    experts = [(w, q, back)] if w.dim() == 2 else [(w[e], sliced(q, e), back[e]) for e in range(shape[0])]
+    for dense, one, again in experts:
+        n, s = numbers_of(one)
+        cols = dense.shape[1]
+        for first in range(0, cols, group):
+            part = dense[:, first : first + group].float()
+            scale = (part.abs().amax(1) / 7).to(dtype)
+            assert torch.equal(s[:, first].to(dtype), scale)
+            step = torch.where(scale > 0, scale.float(), 1.0).unsqueeze(1)
+            assert torch.equal(n[:, first : first + group], (part / step).round().clamp(-8, 7).double())
+        assert torch.equal(again.cpu(), (n * s).to(dtype))  # (a product of 11 by 4 bits is exact in fp32)
+    # the padding holds n = 0
+    full = quant.Q4Weight(q.codes, q.scales, q.codes.shape[-6] * 16, q.codes.shape[-5] * 128, group)
+    one = full if w.dim() == 2 else sliced(full, 0)
+    n, _ = numbers_of(one)
+    assert (n[w.shape[-2] :] == 0).all() and (n[:, w.shape[-1] :] == 0).all()
+
+
+def q4(shape, group, dtype, g):
+    return quant.quantize_q4(normal(shape, 0.02, dtype, g).to(device()), group)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize(
+    "M,R,C,group,bias",
+    [
+        (1, 8, 8, 128, False), (1, 128, 16, 32, True), (1, 2048, 256, 128, False), (2, 1160, 3096, 32, True), (7, 264, 72, 64, True),
+        (16, 4096, 40, 128, False), (17, 1000, 136, 64, False), (32, 136, 1000, 32, False), (33, 520, 264, 32, True),
+        (64, 1032, 520, 128, True), (64, 2048, 48, 64, False), (65, 264, 392, 64, True), (300, 1160, 264, 32, False),
+    ],
+)
+def test_q4_linear(M, R, C, group, bias, dtype):
+    g = gen(M + R)
+    x, q = normal((M, R), 1.0, dtype, g), q4((C, R), group, dtype, g)
+    b = normal((C,), 0.5, dtype, g) if bias else None
+    y = quant.q4_linear_fwd(x.to(device()), q, None if b is None else b.to(device()))
+    w = weights_of(q)
+    if M > 64:  # on the weights rounded to 16 bits
+        w = w.to(dtype).double()
+    ref, bound = linear64(x.double(), w, None if b is None else b.double(), dtype)
+    hold(y, ref, bound, dtype, 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+def test_q4_linear_takes_every_code_scale_and_padding(dtype):
+    """All sixteen numbers in all places, a scale for every row and group, and padding that holds something else."""
+    dev, g = device(), gen(5)
+    rows, cols, group = 24, 200, 32
+    codes = torch.randint(0, 256, (2, 2, 4, 16, 4, 4), generator=g, dtype=torch.uint8)
+    scales = (0.01 + torch.rand((2, 2, 4, 4, 4), generator=g)).to(dtype)
+    q = quant.Q4Weight(codes.to(dev), scales.to(dev), rows, cols, group)
+    x = normal((3, cols), 1.0, dtype, g)
+    ref, bound = linear64(x.double(), weights_of(q), None, dtype)
+    hold(quant.q4_linear_fwd(x.to(dev), q), ref, bound, dtype, 1)
+    # one column at a time: the result is scale * n, rounded once
+    eye = torch.eye(cols, dtype=dtype)[:64]
+    assert torch.equal(quant.q4_linear_fwd(eye.to(dev), q).cpu(), weights_of(q)[:, :64].T.to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize(
+    "M,K,N,group,bias,act",
+    [
+        (1, 8, 8, 32, False, "silu"), (1, 2048, 264, 128, False, "silu"), (3, 264, 1032, 32, True, "gelu"), (16, 520, 640, 64, True, "tanh"),
+        (17, 136, 392, 128, False, "relu"), (48, 264, 520, 64, True, "gelu"), (64, 1032, 264, 32, False, "leaky_relu"),
+        (5, 128, 128, 128, True, "sigmoid"), (9, 256, 384, 32, False, "no_act"), (130, 264, 520, 64, True, "silu"),
+    ],
+)
+def test_q4_mlp(M, K, N, group, bias, act, dtype):
+    dev, g = device(), gen(M + K)
+    x = normal((M, K), 1.0, dtype, g)
+    qs = [q4((N, K), group, dtype, g), q4((N, K), group, dtype, g), q4((K, N), group, dtype, g)]
+    bs = [normal((n,), 0.1, dtype, g) if bias else None for n in (N, N, K)]
+    on = [None if b is None else b.to(dev) for b in bs]
+    y = quant.q4_mlp_fwd(x.to(dev), qs[0], on[0], qs[1], on[1], qs[2], on[2], act_fn=act)
+    ws = [weights_of(q) for q in qs]
+    if M > 64:
+        ws = [w.to(dtype).double() for w in ws]
+    b64 = [None if b is None else b.double() for b in bs]
+    ref, bound = mlp64(x.double(), ws[0], b64[0], ws[1], b64[1], ws[2], b64[2], act, dtype)
+    hold(y, ref, bound + U[dtype] * ref.abs() + SUB[dtype], dtype, 2)
+
+
+@gpu
+def test_q4_operators_take_leading_dimensions_strides_and_no_rows():
+    dev, g, dtype = device(), gen(3), torch.bfloat16
+    q = q4((72, 136), 64, dtype, g)
+    x = normal((136, 6), 1.0, dtype, g).to(dev)
+    y = quant.q4_linear_fwd(x.T.contiguous(), q)
+    assert torch.equal(quant.q4_linear_fwd(x.T, q), y)
+    assert torch.equal(quant.q4_linear_fwd(x.T.reshape(2, 3, 136), q), y.reshape(2, 3, 72))
+    assert torch.equal(quant.q4_linear_fwd(x.T[1], q), y[1])
+    wide = torch.zeros(6, 272, dtype=dtype, device=dev)
+    wide[:, ::2] = x.T
+    assert torch.equal(quant.q4_linear_fwd(wide[:, ::2], q), y)
+    assert quant.q4_linear_fwd(x.T[:0], q).shape == (0, 72)
+    up, down = q4((72, 136), 64, dtype, g), q4((136, 72), 64, dtype, g)
+    out = quant.q4_mlp_fwd(x.T, q, None, up, None, down, None)
+    assert torch.equal(quant.q4_mlp_fwd(x.T.reshape(3, 2, 136), q, None, up, None, down, None), out.reshape(3, 2, 136))
+    assert quant.q4_mlp_fwd(x.T[:0], q, None, up, None, down, None).shape == (0, 136)
+    # a row's result does not depend on the rows beside it in a tile
+    for m in (0, 5):
+        assert torch.equal(quant.q4_linear_fwd(x.T[m : m + 1], q)[0], y[m])
+
+
+@gpu
+def test_q4_refusals():
+    dev, g, dtype = device(), gen(3), torch.float16
+    q = q4((72, 136), 64, dtype, g)
+    x = normal((4, 136), 1.0, dtype, g).to(dev)
+    with pytest.raises(ValueError, match="expected"):
+        quant.q4_linear_fwd(x[:, :128].contiguous(), q)
+    with pytest.raises(TypeError):
+        quant.q4_linear_fwd(x.bfloat16(), q)
+    with pytest.raises(TypeError):
+        quant.q4_linear_fwd(x.float(), q)
+    with pytest.raises(ValueError, match="bias"):
+        quant.q4_linear_fwd(x, q, torch.zeros(71, dtype=dtype, device=dev))
+    with pytest.raises(ValueError, match="group size"):
+        quant.q4_linear_fwd(x, q._replace(group_size=16))
+    with pytest.raises(ValueError, match="codes"):
+        quant.q4_linear_fwd(x, q._replace(codes=q.codes[:4]))
+    with pytest.raises(ValueError, match="scales"):
+        quant.q4_linear_fwd(x, q._replace(scales=q.scales.reshape(-1)))
+    with pytest.raises(TypeError, match="uint8"):
+        quant.q4_linear_fwd(x, q._replace(codes=q.codes.to(torch.int8)))
+    with pytest.raises(RuntimeError, match="device"):
+        quant.q4_linear_fwd(x, q._replace(codes=q.codes.cpu()))
+    with pytest.raises(RuntimeError, match="no backward"):
+        quant.q4_linear_fwd(x.clone().requires_grad_(True), q)
+    with torch.no_grad():
+        quant.q4_linear_fwd(x.clone().requires_grad_(True), q)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda t: quant.q4_linear_fwd(t, q), (x,))
+    with pytest.raises(ValueError):
+        quant.quantize_q4(x[0])
+    with pytest.raises(ValueError, match="group size"):
+        quant.quantize_q4(x, 48)
+    with pytest.raises(NotImplementedError):
+        quant.quantize_q4(torch.zeros(12, 128, dtype=dtype, device=dev))
+    with pytest.raises(TypeError):
+        quant.quantize_q4(x.float())
+    with pytest.raises(ValueError, match="group sizes"):
+        quant.q4_mlp_fwd(x, q, None, q, None, q4((136, 72), 32, dtype, g), None)
+    with pytest.raises(NotImplementedError):
+        quant.q4_mlp_fwd(x, q, None, q, None, q4((136, 72), 64, dtype, g), None, act_fn="softsign")
+
+
+# ------------------------------------------------------------------ routing
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("M,E,k", [(1, 1, 1), (1, 8, 2), (5, 60, 6), (64, 64, 8), (3, 65, 4), (9, 128, 8), (130, 160, 6), (4, 257, 1), (7, 512, 16), (2, 16, 16)])
+def test_route(M, E, k, normalize, dtype):
+    logits = normal((M, E), 1.5, dtype, gen(M + E))
+    w, e = moe.moe_route(logits.to(device()), k, normalize)
+    assert w.dtype == torch.float32 and e.dtype == torch.int64 and w.shape == e.shape == (M, k)
+    ref, experts = route64(logits, k, normalize)
+    assert torch.equal(e.cpu(), experts)
+    # an exponential and a quotient in fp32, over a sum of at most 512 terms
+    assert torch.allclose(w.cpu().double(), ref, rtol=5e-6, atol=1e-30)
+
+
+@gpu
+@pytest.mark.parametrize("E", [8, 70, 300])
+def test_route_ties_masks_and_what_is_not_finite(E):
+    inf, nan, low = math.inf, math.nan, torch.finfo(torch.float32).min
+    logits = torch.full((8, E), -inf)
+    logits[1] = 0.25                      # all equal
+    logits[2, 3] = 1.0                    # one is available
+    logits[3, 1::2] = torch.arange(len(logits[3, 1::2])).float() % 3  # ties among every other one
+    logits[4] = low                       # the type's lowest value is a number
+    logits[5], logits[5, 2] = 0.0, -0.0   # the two zeros are equal
+    logits[6], logits[6, 4] = 0.0, nan
+    logits[7], logits[7, 5] = 0.0, inf
+    for normalize in (True, False):
+        w, e = moe.moe_route(logits.to(device()), 4, normalize)
+        w, e = w.cpu(), e.cpu()
+        ref, experts = route64(logits[:6], 4, normalize)
+        assert torch.equal(e[:6], experts)
+        assert torch.allclose(w[:6].double(), ref, rtol=5e-6, atol=1e-30)
+        assert (w[0] == 0).all() and (w[2, 1:] == 0).all()
+        assert torch.isnan(w[6]).all() and torch.isnan(w[7]).any()
+        assert e[6, 0] == 4 and e[7, 0] == 5
+
+
+@gpu
+def test_route_strides_leading_dimensions_and_refusals():
+    dev = device()
+    logits = normal((6, 24), 1.5, torch.bfloat16, gen(1)).to(dev)
+    w, e = moe.moe_route(logits, 3)
+    for view in (logits.T.contiguous().T, logits.reshape(2, 3, 24)):
+        w2, e2 = moe.moe_route(view, 3)
+        assert w2.shape == (*view.shape[:-1], 3)
+        assert torch.equal(w2.reshape(6, 3), w) and torch.equal(e2.reshape(6, 3), e)
+    # rows that begin at odd addresses
+    odd = torch.empty(1 + 6 * 24, dtype=torch.bfloat16, device=dev)[1:].reshape(6, 24).copy_(logits)
+    assert torch.equal(moe.moe_route(odd, 3).weights, w)
+    assert moe.moe_route(logits[:0], 3).experts.shape == (0, 3)
+    for k in (0, 25):
+        with pytest.raises(ValueError, match="top_k"):
+            moe.moe_route(logits, k)
+    with pytest.raises(NotImplementedError):
+        moe.moe_route(torch.zeros(2, 600, device=dev), 2)
+    with pytest.raises(NotImplementedError):
+        moe.moe_route(torch.zeros(2, 64, device=dev), 17)
+    with pytest.raises(TypeError):
+        moe.moe_route(logits.double(), 2)
+    with pytest.raises(RuntimeError, match="no backward"):
+        moe.moe_route(torch.zeros(2, 8, device=dev, requires_grad=True), 2)
+
+
+# ------------------------------------------------------------------ expert layers
+def experts_of(E, K, N, bits, group, dtype, g):
+    """(gate, up, down) for the operator, and a function that gives one expert's in float64."""
+    ws = [normal(shape, 0.05, dtype, g).to(device()) for shape in ((E, N, K), (E, N, K), (E, K, N))]
+    if bits == 4:
+        qs = [quant.quantize_q4(w, group) for w in ws]
+        return qs, lambda e: tuple(weights_of(sliced(q, e)) for q in qs)
+    return ws, lambda e: tuple(w[e].cpu().double() for w in ws)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize(
+    "M,K,N,E,k,bits,group,act,normalize",
+    [
+        (1, 8, 8, 1, 1, 16, 0, "silu", True), (1, 256, 136, 8, 2, 16, 0, "silu", True), (1, 264, 392, 8, 2, 4, 32, "gelu", True),
+        (2, 136, 72, 4, 4, 16, 0, "relu", False), (7, 200, 328, 16, 4, 4, 64, "silu", False), (16, 264, 136, 60, 6, 16, 0, "silu", True),
+        (16, 392, 264, 8, 2, 4, 128, "silu", True), (17, 72, 200, 4, 2, 16, 0, "tanh", True), (33, 136, 264, 128, 8, 16, 0, "silu", False),
+        (40, 264, 136, 8, 3, 4, 32, "silu", True), (64, 128, 64, 512, 16, 16, 0, "silu", True), (64, 136, 72, 2, 1, 4, 64, "gelu", True),
+        (100, 72, 136, 8, 2, 16, 0, "silu", True), (130, 72, 136, 8, 2, 4, 128, "silu", True),
+    ],
+)
+def test_moe_mlp(M, K, N, E, k, bits, group, act, normalize, dtype):
+    g = gen(M + K + N)
+    x, logits = normal((M, K), 1.0, dtype, g), normal((M, E), 1.5, torch.float32, g)
+    ws, one = experts_of(E, K, N, bits, group, dtype, g)
+    y = moe.moe_mlp_fwd(x.to(device()), logits.to(device()), *ws, k, normalize=normalize, act_fn=act)
+    ref, bound = moe64(x.double(), logits, k, normalize, act, dtype, one)
+    hold(y, ref, bound, dtype, 2)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("M", [1, 16, 50])
+def test_moe_mlp_with_masked_experts(M, bits):
+    """Rows that leave fewer experts than top_k, rows that leave none, and everything on one expert."""
+    dev, dtype, E, K, N = device(), torch.bfloat16, 8, 136, 72
+    g = gen(M)
+    x, logits = normal((M, K), 1.0, dtype, g), normal((M, E), 1.5, torch.float32, g)
+    ws, one = experts_of(E, K, N, bits, 32, dtype, g)
+    logits[:, 1:] = logits[:, 1:].masked_fill(torch.rand((M, E - 1), generator=g) < 0.7, -math.inf)
+    if M > 2:
+        logits[2] = -math.inf
+    y = moe.moe_mlp_fwd(x.to(dev), logits.to(dev), *ws, 3)
+    ref, bound = moe64(x.double(), logits, 3, True, "silu", dtype, one)
+    hold(y, ref, bound, dtype, 2)
+    if M > 2:
+        assert (y[2] == 0).all()
+    logits[:, 1:] = -math.inf
+    y = moe.moe_mlp_fwd(x.to(dev), logits.to(dev), *ws, 3)
+    ref, bound = moe64(x.double(), logits, 1, True, "silu", dtype, one)
+    hold(y, ref, bound, dtype, 2)
+    assert (moe.moe_mlp_fwd(x.to(dev), torch.full((M, E), -math.inf, device=dev), *ws, 3) == 0).all()
+
+
+@gpu
+def test_what_is_not_finite_stays_with_its_token_and_its_expert():
+    dev, dtype, E, K, N, M = device(), torch.float16, 4, 136, 72, 16
+    g = gen(0)
+    x, logits = normal((M, K), 1.0, dtype, g).to(dev), normal((M, E), 1.5, torch.float32, g).to(dev)
+    (gate, up, down), _ = experts_of(E, K, N, 16, 0, dtype, g)
+    y = moe.moe_mlp_fwd(x, logits, gate, up, down, 2)
+    experts = moe.moe_route(logits, 2).experts
+    for ruined in range(3):
+        ws = [t.clone() for t in (gate, up, down)]
+        ws[ruined][3] = math.nan
+        out = moe.moe_mlp_fwd(x, logits, *ws, 2)
+        chose = (experts == 3).any(1)
+        assert chose.any() and (~chose).any()
+        assert torch.equal(out[~chose], y[~chose]) and torch.isnan(out[chose]).all()
+    bad = x.clone()
+    bad[5] = math.nan
+    out = moe.moe_mlp_fwd(bad, logits, gate, up, down, 2)
+    keep = torch.arange(M, device=dev) != 5
+    assert torch.equal(out[keep], y[keep]) and torch.isnan(out[5]).all()
+    # a token whose logits are not finite, in the way softmax has it
+    wrong = logits.clone()
+    wrong[7, 1] = math.nan
+    out = moe.moe_mlp_fwd(x, wrong, gate, up, down, 2)
+    keep = torch.arange(M, device=dev) != 7
+    assert torch.equal(out[keep], y[keep]) and torch.isnan(out[7]).all()
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_moe_mlp_rows_stand_alone_and_repeat(bits):
+    """Other tokens of the batch change nothing but rounding (the sums' order may differ), leading dimensions and strides
+    nothing at all, and neither does another call."""
+    dev, dtype, E, K, N, M = device(), torch.bfloat16, 8, 264, 136, 12
+    g = gen(9)
+    x, logits = normal((M, K), 1.0, dtype, g).to(dev), normal((M, E), 1.5, torch.float32, g).to(dev)
+    ws, one = experts_of(E, K, N, bits, 64, dtype, g)
+    y = moe.moe_mlp_fwd(x, logits, *ws, 2)
+    assert torch.equal(moe.moe_mlp_fwd(x.T.contiguous().T, logits.T.contiguous().T, *ws, 2), y)
+    assert torch.equal(moe.moe_mlp_fwd(x.reshape(3, 4, K), logits.reshape(3, 4, E), *ws, 2), y.reshape(3, 4, K))
+    assert torch.equal(moe.moe_mlp_fwd(x, logits, *ws, 2), y)
+    assert moe.moe_mlp_fwd(x[:0], logits[:0], *ws, 2).shape == (0, K)
+    for m in (0, 7):
+        alone = moe.moe_mlp_fwd(x[m], logits[m], *ws, 2)
+        ref, bound = moe64(x[m : m + 1].cpu().double(), logits[m : m + 1].cpu(), 2, True, "silu", dtype, one)
+        hold(alone, ref, bound, dtype, 2)
+    if bits == 16:  # weights in another order of their elements
+        turned = [w.transpose(1, 2).contiguous().transpose(1, 2) for w in ws]
+        assert torch.equal(moe.moe_mlp_fwd(x, logits, *turned, 2), y)
+    for dt in HALF:  # logits of the activations' type
+        low = logits.to(dt)
+        assert torch.equal(moe.moe_mlp_fwd(x, low, *ws, 2), moe.moe_mlp_fwd(x, low.float(), *ws, 2))
+
+
+@gpu
+def test_moe_refusals():
+    dev, dtype, g = device(), torch.float16, gen(2)
+    ws, _ = experts_of(4, 72, 136, 16, 0, dtype, g)
+    qs, _ = experts_of(4, 72, 136, 4, 32, dtype, g)
+    x, logits = normal((3, 72), 1.0, dtype, g).to(dev), torch.zeros(3, 4, device=dev)
+    call = moe.moe_mlp_fwd
+    with pytest.raises(TypeError, match="either all"):
+        call(x, logits, ws[0], qs[1], ws[2], 2)
+    with pytest.raises(TypeError):
+        call(x.float(), logits, *ws, 2)
+    with pytest.raises(TypeError):
+        call(x.bfloat16(), logits, *qs, 2)
+    with pytest.raises(ValueError, match="token rows"):
+        call(x, logits[:2], *ws, 2)
+    with pytest.raises(ValueError, match="W_gate"):
+        call(x, torch.zeros(3, 5, device=dev), *ws, 2)
+    with pytest.raises(ValueError, match="W_up"):
+        call(x, logits, ws[0], ws[1][:, :128], ws[2], 2)
+    with pytest.raises(ValueError, match="W_down"):
+        call(x, logits, ws[0], ws[1], ws[0], 2)
+    with pytest.raises(ValueError, match="codes"):
+        call(x, torch.zeros(3, 5, device=dev), *qs, 2)
+    for k in (0, 5):
+        with pytest.raises(ValueError, match="top_k"):
+            call(x, logits, *ws, k)
+    with pytest.raises(NotImplementedError):
+        call(x, logits, *ws, 2, act_fn="softsign")
+    with pytest.raises(RuntimeError, match="no backward"):
+        call(x, logits, ws[0].clone().requires_grad_(True), ws[1], ws[2], 2)
+    with pytest.raises(RuntimeError, match="traced"):
+        torch.jit.trace(lambda t: call(t, logits, *ws, 2), (x,))
+
+
+# ------------------------------------------------------------------ streams and graphs
+def _calls(bits):
+    dev, dtype, g = device(), torch.bfloat16, gen(4)
+    E, K, N, M = 16, 264, 392, 5
+    ws, _ = experts_of(E, K, N, bits, 64, dtype, g)
+    x, logits = normal((M, K), 1.0, dtype, g).to(dev), normal((M, E), 1.5, torch.float32, g).to(dev)
+    if bits == 16:
+        return x, logits, lambda: [moe.moe_mlp_fwd(x, logits, *ws, 3), *moe.moe_route(logits, 3)]
+    one = [sliced(q, 2) for q in ws]
+    return x, logits, lambda: [moe.moe_mlp_fwd(x, logits, *ws, 3), quant.q4_mlp_fwd(x, one[0], None, one[1], None, one[2], None),
+                               quant.q4_linear_fwd(x, one[0])]
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_operators_run_on_the_current_stream(bits):
+    x, logits, call = _calls(bits)
+    ref = call()
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        held = x.clone()
+        x.fill_(math.nan)
+        x.copy_(held)  # on the side stream: a call on another stream would read NaN, or race
+        out = call()
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(ref, out))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_operators_replay_in_a_graph(bits):
+    x, logits, call = _calls(bits)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    g = gen(8)
+    for _ in range(4):  # other inputs and another routing each time
+        x.copy_(normal(x.shape, 1.0, x.dtype, g))
+        logits.copy_(normal(logits.shape, 1.5, logits.dtype, g))
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = call()
+        assert all(torch.equal(a, b) for a, b in zip(ref, out))
+        torch.cuda.synchronize()

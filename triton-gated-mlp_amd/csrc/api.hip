@@ -11,6 +11,7 @@
 #include <mutex>
 #include <vector>
 
+#include "experts.hpp"
 #include "launch.hpp"
 
 namespace {
@@ -1425,6 +1426,219 @@ int gmlp_hidden_bwd(const void* dh, const void* x, const void* w_gate, const voi
   if (db_up) { cs_in[nb] = du; cs_out[nb] = db_up; ++nb; }
   return run_gradients(__func__, dg, du, w_gate, w_up, dx, n, lhs, rhs, dws, M, K, N, R, C, nb, cs_in, cs_out, R, dtype,
                        workspace, ws_bytes, stream);
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ 4-bit weights, expert layers
+namespace {
+
+int check_q4(const char* fn, int group, int dtype) {
+  if (group != 32 && group != 64 && group != 128)
+    return fail(GMLP_EINVAL, "%s: group = %d is not 32, 64 or 128", fn, group);
+  if (dtype != GMLP_F16 && dtype != GMLP_BF16)
+    return fail(dtype == GMLP_F32 ? GMLP_ESHAPE : GMLP_EINVAL, "%s: dtype %d is not GMLP_F16/GMLP_BF16", fn, dtype);
+  return 0;
+}
+int check_rows(const char* fn, int64_t M) {
+  if (M > gmlp::EXPERTS_MAX_M)
+    return fail(GMLP_ESHAPE, "%s: M = %lld exceeds the %d token rows of a call", fn, (long long)M, gmlp::EXPERTS_MAX_M);
+  return 0;
+}
+// The kernels address a tile of weights, the token rows and the hidden states with 32-bit byte offsets, and a grid
+// has a workgroup per tile.
+int check_expert_sizes(const char* fn, int64_t M, int64_t K, int64_t N, int64_t experts, int64_t pairs) {
+  const int64_t limit = (int64_t)1 << 31, most = K > N ? K : N;
+  if (most * 32 >= limit || M * K * 2 >= limit || pairs * N * 2 >= limit || experts * cdiv(most, 16) >= limit)
+    return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
+  return 0;
+}
+int check_storage(const char* fn, int64_t count, int64_t rows, int64_t cols) {
+  if (count < 1 || rows < 1 || cols < 1 || rows > kMaxDim || cols > kMaxDim ||
+      count > ((int64_t)1 << 32) / cdiv(rows, 16) / cdiv(cols, 128))
+    return fail(GMLP_ESHAPE, "%s: count, rows, cols must be >= 1 and not too large (got %lld, %lld, %lld)", fn, (long long)count,
+                (long long)rows, (long long)cols);
+  if (int rc = check_mult8(fn, "rows", rows)) return rc;
+  return check_mult8(fn, "cols", cols);
+}
+int check_routing(const char* fn, int64_t E, int64_t top_k) {
+  if (E < 1 || E > gmlp::EXPERTS_MAX_E || top_k < 1 || top_k > gmlp::EXPERTS_MAX_K || top_k > E)
+    return fail(GMLP_ESHAPE, "%s: needs 1 <= top_k <= %d and top_k <= E <= %d (got top_k %lld, E %lld)", fn, gmlp::EXPERTS_MAX_K,
+                gmlp::EXPERTS_MAX_E, (long long)top_k, (long long)E);
+  return 0;
+}
+template <typename F>
+hipError_t by_half(int dtype, F&& f) {
+  return dtype == GMLP_F16 ? f(gmlp::f16{}) : f(gmlp::bf16{});
+}
+// Where the parts of gmlp_moe_fwd's workspace begin.
+struct MoeWorkspace {
+  size_t active, slot, tokens, count, weight, bytes;
+  MoeWorkspace(int64_t M, int64_t N, int64_t E, int64_t top_k) {
+    const size_t pairs = (size_t)(M * top_k), experts = (size_t)E < pairs ? (size_t)E : pairs;
+    size_t at = pairs * (size_t)N * 2;
+    auto part = [&](size_t n) {
+      const size_t begin = (at + 255) / 256 * 256;
+      at = begin + n;
+      return begin;
+    };
+    active = part((1 + experts) * sizeof(int));
+    slot = part(experts * gmlp::EXPERTS_MAX_M);
+    tokens = part(experts * gmlp::EXPERTS_MAX_M);
+    count = part(experts);
+    weight = part(pairs * sizeof(float));
+    bytes = at;
+  }
+};
+
+}  // namespace
+
+extern "C" {
+
+int gmlp_q4_quantize(const void* w, void* codes, void* scales, int64_t count, int64_t rows, int64_t cols, int group, int dtype,
+                     void* stream) {
+  GMLP_REQUIRE_PTR(w); GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales);
+  if (int rc = check_q4(__func__, group, dtype)) return rc;
+  if (int rc = check_storage(__func__, count, rows, cols)) return rc;
+  GMLP_REQUIRE_ALIGNED(w); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales);
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    return gmlp::launch_q4_quantize<T>((const T*)w, (uint8_t*)codes, (T*)scales, count, rows, cols, group, (hipStream_t)stream);
+  }));
+}
+
+int gmlp_q4_dequantize(const void* codes, const void* scales, void* w, int64_t count, int64_t rows, int64_t cols, int group,
+                       int dtype, void* stream) {
+  GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales); GMLP_REQUIRE_PTR(w);
+  if (int rc = check_q4(__func__, group, dtype)) return rc;
+  if (int rc = check_storage(__func__, count, rows, cols)) return rc;
+  GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(w);
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    return gmlp::launch_q4_dequantize<T>((const uint8_t*)codes, (const T*)scales, (T*)w, count, rows, cols, group, (hipStream_t)stream);
+  }));
+}
+
+int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, const void* bias, void* y, int64_t M, int64_t R,
+                       int64_t C, int group, int dtype, void* stream) {
+  GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales); GMLP_REQUIRE_PTR(y);
+  if (int rc = check_q4(__func__, group, dtype)) return rc;
+  if (int rc = check_dims(__func__, M, R, C)) return rc;
+  if (int rc = check_rows(__func__, M)) return rc;
+  if (int rc = check_mult8(__func__, "R", R)) return rc;
+  if (int rc = check_mult8(__func__, "C", C)) return rc;
+  if (int rc = check_expert_sizes(__func__, M, C, R, 1, M)) return rc;
+  GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(bias);
+  GMLP_REQUIRE_ALIGNED(y);
+  gmlp::ExpertArgs a = {};
+  a.h = const_cast<void*>(x);  // read only
+  a.y = y;
+  a.bias[2] = bias;
+  a.down = {codes, scales};
+  a.M = (int)M; a.K = (int)C; a.N = (int)R; a.E = a.top_k = a.dense = 1;
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    return gmlp::launch_experts_down<decltype(tag)>(a, group, (hipStream_t)stream);
+  }));
+}
+
+int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_gate, const void* codes_up, const void* scales_up,
+                    const void* codes_down, const void* scales_down, const void* b_gate, const void* b_up, const void* b_down,
+                    void* h, void* y, int64_t M, int64_t K, int64_t N, int group, int dtype, int act, void* stream) {
+  GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(codes_gate); GMLP_REQUIRE_PTR(scales_gate); GMLP_REQUIRE_PTR(codes_up);
+  GMLP_REQUIRE_PTR(scales_up); GMLP_REQUIRE_PTR(codes_down); GMLP_REQUIRE_PTR(scales_down); GMLP_REQUIRE_PTR(h);
+  GMLP_REQUIRE_PTR(y);
+  if (int rc = check_q4(__func__, group, dtype)) return rc;
+  GMLP_REQUIRE_ACT(act);
+  if (int rc = check_dims(__func__, M, K, N)) return rc;
+  if (int rc = check_rows(__func__, M)) return rc;
+  if (int rc = check_mult8(__func__, "K", K)) return rc;
+  if (int rc = check_mult8(__func__, "N", N)) return rc;
+  if (int rc = check_expert_sizes(__func__, M, K, N, 1, M)) return rc;
+  GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(scales_gate); GMLP_REQUIRE_ALIGNED(codes_up);
+  GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(codes_down); GMLP_REQUIRE_ALIGNED(scales_down);
+  GMLP_REQUIRE_ALIGNED(b_gate); GMLP_REQUIRE_ALIGNED(b_up); GMLP_REQUIRE_ALIGNED(b_down); GMLP_REQUIRE_ALIGNED(h);
+  GMLP_REQUIRE_ALIGNED(y);
+  gmlp::ExpertArgs a = {};
+  a.x = x;
+  a.h = h;
+  a.y = y;
+  a.bias[0] = b_gate; a.bias[1] = b_up; a.bias[2] = b_down;
+  a.gate = {codes_gate, scales_gate};
+  a.up = {codes_up, scales_up};
+  a.down = {codes_down, scales_down};
+  a.M = (int)M; a.K = (int)K; a.N = (int)N; a.act = act; a.E = a.top_k = a.dense = 1;
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    if (hipError_t e = gmlp::launch_experts_gateup<T>(a, group, (hipStream_t)stream)) return e;
+    return gmlp::launch_experts_down<T>(a, group, (hipStream_t)stream);
+  }));
+}
+
+int gmlp_moe_route(const void* logits, float* weights, int64_t* experts, int64_t M, int64_t E, int64_t top_k, int normalize, int dtype,
+                   void* stream) {
+  GMLP_REQUIRE_PTR(logits); GMLP_REQUIRE_PTR(weights); GMLP_REQUIRE_PTR(experts);
+  GMLP_REQUIRE_DTYPE(dtype);
+  if (int rc = check_routing(__func__, E, top_k)) return rc;
+  if (M < 1 || M > kMaxDim) return fail(GMLP_ESHAPE, "%s: M = %lld must be in [1, 2^30]", __func__, (long long)M);
+  return hip_result(__func__, by_dtype(dtype, [&](auto tag) {
+    typedef decltype(tag) L;
+    return gmlp::launch_route<L>((const L*)logits, weights, experts, M, (int)E, (int)top_k, normalize, (hipStream_t)stream);
+  }));
+}
+
+size_t gmlp_moe_workspace_bytes(int64_t M, int64_t N, int64_t E, int64_t top_k, int dtype) {
+  if (M < 1 || M > gmlp::EXPERTS_MAX_M || N < 1 || N > kMaxDim || E < 1 || E > gmlp::EXPERTS_MAX_E || top_k < 1 ||
+      top_k > gmlp::EXPERTS_MAX_K || (dtype != GMLP_F16 && dtype != GMLP_BF16))
+    return 0;
+  return MoeWorkspace(M, N, E, top_k).bytes;
+}
+
+int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const void* w_up, const void* w_down, const void* s_gate,
+                 const void* s_up, const void* s_down, void* y, int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k,
+                 int normalize, int group, int dtype, int logits_dtype, int act, void* workspace, size_t workspace_bytes,
+                 void* stream) {
+  GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(logits); GMLP_REQUIRE_PTR(w_gate); GMLP_REQUIRE_PTR(w_up); GMLP_REQUIRE_PTR(w_down);
+  GMLP_REQUIRE_PTR(y); GMLP_REQUIRE_PTR(workspace);
+  if (group != 0) {
+    GMLP_REQUIRE_PTR(s_gate); GMLP_REQUIRE_PTR(s_up); GMLP_REQUIRE_PTR(s_down);
+  }
+  if (int rc = check_q4(__func__, group == 0 ? 32 : group, dtype)) return rc;
+  GMLP_REQUIRE_DTYPE(logits_dtype);
+  GMLP_REQUIRE_ACT(act);
+  if (int rc = check_routing(__func__, E, top_k)) return rc;
+  if (int rc = check_dims(__func__, M, K, N)) return rc;
+  if (int rc = check_rows(__func__, M)) return rc;
+  if (int rc = check_mult8(__func__, "K", K)) return rc;
+  if (int rc = check_mult8(__func__, "N", N)) return rc;
+  if (int rc = check_expert_sizes(__func__, M, K, N, E, M * top_k)) return rc;
+  GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(w_gate); GMLP_REQUIRE_ALIGNED(w_up);
+  GMLP_REQUIRE_ALIGNED(w_down); GMLP_REQUIRE_ALIGNED(s_gate); GMLP_REQUIRE_ALIGNED(s_up); GMLP_REQUIRE_ALIGNED(s_down);
+  GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
+  const MoeWorkspace ws(M, N, E, top_k);
+  if (workspace_bytes < ws.bytes)
+    return fail(GMLP_EINVAL, "%s: workspace of %zu bytes, needs %zu", __func__, workspace_bytes, ws.bytes);
+  char* const base = (char*)workspace;
+  gmlp::ExpertArgs a = {};
+  a.x = x;
+  a.h = base;
+  a.y = y;
+  a.gate = {w_gate, s_gate};
+  a.up = {w_up, s_up};
+  a.down = {w_down, s_down};
+  a.M = (int)M; a.K = (int)K; a.N = (int)N; a.E = (int)E; a.top_k = (int)top_k; a.act = act;
+  a.plan = {(int*)(base + ws.active), (uint8_t*)(base + ws.count), (uint8_t*)(base + ws.tokens), (int8_t*)(base + ws.slot),
+            (float*)(base + ws.weight)};
+  const hipStream_t s = (hipStream_t)stream;
+  const hipError_t planned = by_dtype(logits_dtype, [&](auto tag) {
+    typedef decltype(tag) L;
+    return gmlp::launch_experts_plan<L>((const L*)logits, a.plan, a.M, a.E, a.top_k, normalize, s);
+  });
+  if (planned != hipSuccess) return hip_result(__func__, planned);
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    if (hipError_t e = gmlp::launch_experts_gateup<T>(a, group, s)) return e;
+    return gmlp::launch_experts_down<T>(a, group, s);
+  }));
 }
 
 }  // extern "C"

@@ -1,0 +1,56 @@
+// 4-bit weights and expert layers: what the kernels of experts.hip and the C entry points share.
+#pragma once
+#include "common.hpp"
+
+namespace gmlp {
+
+constexpr int Q4_TILE = 16;          // weight rows of a tile
+constexpr int Q4_BLOCK = 128;        // weight columns of a block
+constexpr int EXPERTS_MAX_M = 64;    // token rows of a call
+constexpr int EXPERTS_MAX_E = 512;   // experts
+constexpr int EXPERTS_MAX_K = 16;    // experts of a token
+
+// One matrix of weights per expert: 16-bit [experts, rows, cols], or codes and scales of the 4-bit storage (gmlp.h).
+struct ExpertWeights {
+  const void* w;
+  const void* scales;  // 4-bit weights only
+};
+
+// The routing of a call, which plan_kernel makes of the logits: device pointers into the caller's workspace.
+struct ExpertPlan {
+  int* active;      // [1 + experts]: how many experts any token chose, then their numbers in ascending order
+  uint8_t* count;   // [active experts]: tokens of the expert
+  uint8_t* tokens;  // [active experts][EXPERTS_MAX_M]: which, ascending
+  int8_t* slot;     // [active experts][EXPERTS_MAX_M]: the token's how-manieth choice the expert is, -1: not chosen
+  float* weight;    // [M * top_k]
+};
+
+struct ExpertArgs {
+  const void* x;      // [M, K]
+  const void* bias[3];
+  ExpertWeights gate, up, down;
+  void* h;            // [M * top_k, N]
+  void* y;            // [M, K]
+  int M, K, N, E, top_k, act;
+  int dense;          // one expert, every token's, with weight 1: plan is not read
+  ExpertPlan plan;
+};
+
+// Gate/up, then down, on 16-bit (group = 0) or 4-bit weights (group = 32, 64 or 128).
+template <typename T>
+hipError_t launch_experts_gateup(const ExpertArgs& a, int group, hipStream_t s);
+// y[M, a.K] = sum over experts of weight * h[., a.N]·W_downᵀ (+ bias[2])
+template <typename T>
+hipError_t launch_experts_down(const ExpertArgs& a, int group, hipStream_t s);
+template <typename L>
+hipError_t launch_experts_plan(const L* logits, const ExpertPlan& plan, int M, int E, int top_k, int normalize, hipStream_t s);
+template <typename L>
+hipError_t launch_route(const L* logits, float* weights, int64_t* experts, int64_t M, int E, int top_k, int normalize, hipStream_t s);
+
+template <typename T>
+hipError_t launch_q4_quantize(const T* w, uint8_t* codes, T* scales, int64_t count, int64_t rows, int64_t cols, int group, hipStream_t s);
+template <typename T>
+hipError_t launch_q4_dequantize(const uint8_t* codes, const T* scales, T* w, int64_t count, int64_t rows, int64_t cols, int group,
+                                hipStream_t s);
+
+}  // namespace gmlp

@@ -42,7 +42,8 @@ typedef std::optional<Tensor> OptTensor;
 #define GMLP_ENTRY_POINTS(X)                                                                     \
   X(gmlp_last_error) X(gmlp_workspace_bytes) X(gmlp_mlp_workspace_bytes) X(gmlp_mlp_fwd)         \
   X(gmlp_mlp_bwd) X(gmlp_gateup_fwd) X(gmlp_decode_fwd) X(gmlp_decode_stream_fwd) X(gmlp_hidden_bwd) \
-  X(gmlp_grads_workspace_bytes)
+  X(gmlp_grads_workspace_bytes) X(gmlp_linear_fwd) X(gmlp_q4_quantize) X(gmlp_q4_dequantize) X(gmlp_q4_linear_fwd) \
+  X(gmlp_q4_mlp_fwd) X(gmlp_moe_route) X(gmlp_moe_workspace_bytes) X(gmlp_moe_fwd)
 struct Library {
 #define GMLP_MEMBER(name) decltype(&::name) name = nullptr;
   GMLP_ENTRY_POINTS(GMLP_MEMBER)
@@ -477,6 +478,218 @@ Tensor hidden(const Tensor& x_in, const Tensor& Wu_in, const OptTensor& bu_in, c
   return h;
 }
 
+// ------------------------------------------------------------------ 4-bit weights, expert layers
+// Inference operators: nothing is recorded for autograd, so a call that autograd would have to record is refused, and
+// so is a trace, which would see the output's allocation only.
+void inference_only(const char* name, std::initializer_list<std::reference_wrapper<const Tensor>> tensors) {
+  refuse_transforms(name, tensors);
+  bool graph = false;
+  for (const Tensor& t : tensors) graph = graph || (t.defined() && t.requires_grad());
+  TORCH_CHECK(!(graph && at::GradMode::is_enabled()), name, " has no backward pass: call it under torch.no_grad()");
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be traced");
+}
+constexpr int64_t FEW_ROWS = 64;  // token rows of the weight-streaming kernels
+
+// triton_gated_mlp.ops.quant.Q4Weight: codes, scales, rows, cols, group size
+typedef std::tuple<Tensor, Tensor, int64_t, int64_t, int64_t> Q4;
+struct Q4Matrix {
+  Tensor codes, scales;
+  int64_t rows, cols, count = 1;
+  int group;
+  // `experts`: 0 for a single matrix
+  Q4Matrix(const char* name, const Q4& q, const Tensor& x, int64_t experts, int64_t rows_, int64_t cols_)
+      : codes(std::get<0>(q)), scales(std::get<1>(q)), rows(std::get<2>(q)), cols(std::get<3>(q)), group((int)std::get<4>(q)) {
+    TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, name, ": group size ", group, " is not 32, 64 or 128");
+    TORCH_CHECK_VALUE(rows == rows_ && cols == cols_, name, " is [", rows, ", ", cols, "], expected [", rows_, ", ", cols_, "]");
+    const int64_t tiles = (rows + 15) / 16, blocks = (cols + 127) / 128;
+    std::vector<int64_t> c, s;
+    if (experts > 0) c.push_back(experts), s.push_back(experts), count = experts;
+    c.insert(c.end(), {tiles, blocks, 4, 16, 4, 4});
+    s.insert(s.end(), {tiles, blocks, 4, 128 / group, 4});
+    TORCH_CHECK_VALUE(codes.sizes() == at::IntArrayRef(c), name, ": codes of size ", codes.sizes(), ", expected ", c);
+    TORCH_CHECK_VALUE(scales.sizes() == at::IntArrayRef(s), name, ": scales of size ", scales.sizes(), ", expected ", s);
+    TORCH_CHECK_TYPE(codes.scalar_type() == at::kByte, name, ": codes are ", codes.scalar_type(), ", expected uint8");
+    TORCH_CHECK_TYPE(scales.scalar_type() == x.scalar_type(), name, ": scales are ", scales.scalar_type(), ", the input ",
+                     x.scalar_type());
+    TORCH_CHECK(codes.device() == x.device() && scales.device() == x.device(), name, " is on another device than the input");
+    codes = codes.contiguous();
+    scales = scales.contiguous();
+  }
+  // the weights in 16 bits
+  Tensor dense(int code) const {
+    const Tensor w = at::empty({rows, cols}, scales.options());
+    check(lib.gmlp_q4_dequantize(ptr(codes), ptr(scales), out_ptr(w), 1, rows, cols, group, code, stream_of(w)));
+    return w;
+  }
+};
+int require_half(const char* name, std::initializer_list<std::reference_wrapper<const Tensor>> tensors) {
+  const int code = require_gpu(tensors);
+  TORCH_CHECK_TYPE(code != GMLP_F32, name, " takes float16 or bfloat16 activations");
+  return code;
+}
+void check_bias(const char* name, const Tensor& b, int64_t n) {
+  TORCH_CHECK_VALUE(!b.defined() || (b.dim() == 1 && b.size(0) == n), "dimension mismatch in ", name);
+}
+
+Tensor q4_linear(const Tensor& x_in, const Q4& q, const OptTensor& bias_in) {
+  const Tensor& b_in = or_undefined(bias_in);
+  inference_only("q4_linear_fwd", {x_in, std::get<1>(q), b_in});
+  const int code = require_half("q4_linear_fwd", {x_in, b_in});
+  TORCH_CHECK_VALUE(x_in.dim() >= 1, "x needs at least one dimension");
+  const int64_t R = x_in.size(-1), C = std::get<2>(q), M = R > 0 ? x_in.numel() / R : 0;
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x_in.device());
+  const Q4Matrix w("weight", q, x_in, 0, C, R);
+  check_bias("bias", b_in, C);
+  const Tensor x = x_in.contiguous(), b = contiguous(b_in);
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = C;
+  const Tensor y = at::empty(sizes, x.options());
+  if (M == 0) return y;
+  if (M <= FEW_ROWS) {
+    check(lib.gmlp_q4_linear_fwd(ptr(x), ptr(w.codes), ptr(w.scales), ptr(b), out_ptr(y), M, R, C, w.group, code, stream_of(x)));
+    return y;
+  }
+  const Tensor dense = w.dense(code);
+  const size_t bytes = lib.gmlp_workspace_bytes(GMLP_OP_LINEAR_FWD, M, R, C, code);
+  const Tensor ws = scratch(bytes, x);
+  check(lib.gmlp_linear_fwd(ptr(x), ptr(dense), ptr(b), out_ptr(y), M, R, C, code, out_ptr(ws), bytes, stream_of(x)));
+  return y;
+}
+
+Tensor q4_mlp(const Tensor& x_in, const Q4& gate, const OptTensor& bg_in, const Q4& up, const OptTensor& bu_in, const Q4& down,
+              const OptTensor& bd_in, int64_t act) {
+  const Tensor &bg_o = or_undefined(bg_in), &bu_o = or_undefined(bu_in), &bd_o = or_undefined(bd_in);
+  inference_only("q4_mlp_fwd", {x_in, std::get<1>(gate), std::get<1>(up), std::get<1>(down), bg_o, bu_o, bd_o});
+  const int code = require_half("q4_mlp_fwd", {x_in, bg_o, bu_o, bd_o});
+  TORCH_CHECK_VALUE(x_in.dim() >= 1, "x needs at least one dimension");
+  const int64_t K = x_in.size(-1), N = std::get<2>(gate), M = K > 0 ? x_in.numel() / K : 0;
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x_in.device());
+  const Q4Matrix wg("W_gate", gate, x_in, 0, N, K), wu("W_up", up, x_in, 0, N, K), wd("W_down", down, x_in, 0, K, N);
+  TORCH_CHECK_VALUE(wg.group == wu.group && wg.group == wd.group, "the matrices have different group sizes");
+  check_bias("b_gate", bg_o, N);
+  check_bias("b_up", bu_o, N);
+  check_bias("b_down", bd_o, K);
+  const Tensor x = x_in.contiguous(), bg = contiguous(bg_o), bu = contiguous(bu_o), bd = contiguous(bd_o);
+  const Tensor y = at::empty(x.sizes(), x.options());
+  if (M == 0) return y;
+  if (M <= FEW_ROWS) {
+    const Tensor h = at::empty({M, N}, x.options());
+    check(lib.gmlp_q4_mlp_fwd(ptr(x), ptr(wg.codes), ptr(wg.scales), ptr(wu.codes), ptr(wu.scales), ptr(wd.codes), ptr(wd.scales),
+                              ptr(bg), ptr(bu), ptr(bd), out_ptr(h), out_ptr(y), M, K, N, wg.group, code, (int)act, stream_of(x)));
+    return y;
+  }
+  return mlp_infer(x, wg.dense(code), bg.defined() ? OptTensor(bg) : OptTensor(), wu.dense(code),
+                   bu.defined() ? OptTensor(bu) : OptTensor(), wd.dense(code), bd.defined() ? OptTensor(bd) : OptTensor(), act);
+}
+
+std::tuple<Tensor, Tensor> q4_quantize(const Tensor& w_in, int64_t group) {
+  inference_only("quantize_q4", {w_in});
+  const int code = require_half("quantize_q4", {w_in});
+  TORCH_CHECK_VALUE(w_in.dim() == 2 || w_in.dim() == 3, "quantize_q4 takes [rows, cols] or [experts, rows, cols], got ", w_in.sizes());
+  TORCH_CHECK_VALUE(group == 32 || group == 64 || group == 128, "group size ", group, " is not 32, 64 or 128");
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(w_in.device());
+  const Tensor w = w_in.contiguous();
+  const int64_t rows = w.size(-2), cols = w.size(-1), count = w.dim() == 3 ? w.size(0) : 1;
+  std::vector<int64_t> c, s;
+  if (w.dim() == 3) c.push_back(count), s.push_back(count);
+  c.insert(c.end(), {(rows + 15) / 16, (cols + 127) / 128, 4, 16, 4, 4});
+  s.insert(s.end(), {(rows + 15) / 16, (cols + 127) / 128, 4, 128 / group, 4});
+  const Tensor codes = at::empty(c, w.options().dtype(at::kByte)), scales = at::empty(s, w.options());
+  check(lib.gmlp_q4_quantize(ptr(w), out_ptr(codes), out_ptr(scales), count, rows, cols, (int)group, code, stream_of(w)));
+  return {codes, scales};
+}
+Tensor q4_dequantize(const Q4& q) {
+  const Tensor& s = std::get<1>(q);
+  inference_only("dequantize_q4", {s});
+  const int code = require_half("dequantize_q4", {s});
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(s.device());
+  const int64_t experts = s.dim() == 6 ? s.size(0) : 0;
+  const Q4Matrix w("weight", q, s, experts, std::get<2>(q), std::get<3>(q));
+  std::vector<int64_t> sizes;
+  if (experts > 0) sizes.push_back(experts);
+  sizes.insert(sizes.end(), {w.rows, w.cols});
+  const Tensor out = at::empty(sizes, s.options());
+  check(lib.gmlp_q4_dequantize(ptr(w.codes), ptr(w.scales), out_ptr(out), w.count, w.rows, w.cols, w.group, code, stream_of(out)));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> moe_route(const Tensor& logits_in, int64_t top_k, bool normalize) {
+  inference_only("moe_route", {logits_in});
+  const int code = require_gpu({logits_in});
+  TORCH_CHECK_VALUE(logits_in.dim() >= 1, "logits need at least one dimension");
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(logits_in.device());
+  const Tensor logits = logits_in.contiguous();
+  const int64_t E = logits.size(-1), M = E > 0 ? logits.numel() / E : 0;
+  std::vector<int64_t> sizes = logits.sizes().vec();
+  sizes.back() = top_k;
+  TORCH_CHECK_VALUE(top_k >= 1 && top_k <= E, "top_k = ", top_k, " of ", E, " experts");
+  const Tensor weights = at::empty(sizes, logits.options().dtype(at::kFloat)), experts = at::empty(sizes, logits.options().dtype(at::kLong));
+  if (M > 0)
+    check(lib.gmlp_moe_route(ptr(logits), (float*)out_ptr(weights), (int64_t*)out_ptr(experts), M, E, top_k, normalize, code,
+                             stream_of(logits)));
+  return {weights, experts};
+}
+
+// gate, up, down: pointers to the experts' weights, and to their scales
+Tensor moe_rows(const Tensor& x_in, const Tensor& logits_in, int code, int logits_code, const void* const (&w)[3],
+                const void* const (&sc)[3], int64_t N, int64_t E, int64_t top_k, bool normalize, int group, int64_t act) {
+  const Tensor x = x_in.contiguous(), logits = logits_in.contiguous();
+  const int64_t K = x.size(-1), M = K > 0 ? x.numel() / K : 0;
+  const Tensor y = at::empty(x.sizes(), x.options());
+  if (M == 0) return y;
+  const size_t bytes = lib.gmlp_moe_workspace_bytes(std::min(M, FEW_ROWS), N, E, top_k, code);
+  const Tensor ws = scratch(bytes, x);
+  // A longer batch goes through in pieces of as many rows as a call takes, one behind the other on the stream.
+  for (int64_t m = 0; m < M; m += FEW_ROWS)
+    check(lib.gmlp_moe_fwd((const char*)ptr(x) + m * K * x.element_size(), (const char*)ptr(logits) + m * E * logits.element_size(),
+                           w[0], w[1], w[2], sc[0], sc[1], sc[2], (char*)out_ptr(y) + m * K * y.element_size(),
+                           std::min(M - m, FEW_ROWS), K, N, E, top_k, normalize, group, code, logits_code, (int)act, out_ptr(ws),
+                           bytes, stream_of(x)));
+  return y;
+}
+int check_logits(const Tensor& x, const Tensor& logits, int64_t top_k) {
+  const int code = require_gpu({logits});
+  TORCH_CHECK(logits.device() == x.device(), "tensors on different devices: ", x.device(), " and ", logits.device());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && logits.dim() == x.dim() &&
+                        std::equal(x.sizes().begin(), x.sizes().end() - 1, logits.sizes().begin()),
+                    "x ", x.sizes(), " and logits ", logits.sizes(), " are of different token rows");
+  TORCH_CHECK_VALUE(top_k >= 1 && top_k <= logits.size(-1), "top_k = ", top_k, " of ", logits.size(-1), " experts");
+  return code;
+}
+Tensor moe_mlp(const Tensor& x, const Tensor& logits, const Tensor& gate, const Tensor& up, const Tensor& down, int64_t top_k,
+               bool normalize, int64_t act) {
+  inference_only("moe_mlp_fwd", {x, logits, gate, up, down});
+  const int code = require_half("moe_mlp_fwd", {x, gate, up, down}), logits_code = check_logits(x, logits, top_k);
+  const int64_t K = x.size(-1), E = logits.size(-1);
+  TORCH_CHECK_VALUE(gate.dim() == 3 && gate.size(0) == E && gate.size(2) == K, "dimension mismatch in W_gate ", gate.sizes(), ": ", E,
+                    " experts, hidden size ", K);
+  const int64_t N = gate.size(1);
+  TORCH_CHECK_VALUE(up.sizes() == gate.sizes(), "dimension mismatch in W_up ", up.sizes(), " or W_gate ", gate.sizes());
+  TORCH_CHECK_VALUE(down.dim() == 3 && down.size(0) == E && down.size(1) == K && down.size(2) == N, "dimension mismatch in W_down ",
+                    down.sizes());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  const Tensor g = gate.contiguous(), u = up.contiguous(), d = down.contiguous();
+  return moe_rows(x, logits, code, logits_code, {ptr(g), ptr(u), ptr(d)}, {nullptr, nullptr, nullptr}, N, E, top_k, normalize, 0, act);
+}
+Tensor moe_mlp_q4(const Tensor& x, const Tensor& logits, const Q4& gate, const Q4& up, const Q4& down, int64_t top_k, bool normalize,
+                  int64_t act) {
+  inference_only("moe_mlp_fwd", {x, logits, std::get<1>(gate), std::get<1>(up), std::get<1>(down)});
+  const int code = require_half("moe_mlp_fwd", {x}), logits_code = check_logits(x, logits, top_k);
+  const int64_t K = x.size(-1), E = logits.size(-1), N = std::get<2>(gate);
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x.device());
+  const Q4Matrix g("W_gate", gate, x, E, N, K), u("W_up", up, x, E, N, K), d("W_down", down, x, E, K, N);
+  TORCH_CHECK_VALUE(g.group == u.group && g.group == d.group, "the matrices have different group sizes");
+  return moe_rows(x, logits, code, logits_code, {ptr(g.codes), ptr(u.codes), ptr(d.codes)}, {ptr(g.scales), ptr(u.scales), ptr(d.scales)},
+                  N, E, top_k, normalize, g.group, act);
+}
+
 // ------------------------------------------------------------------ torch.jit.trace
 // While a trace is being recorded a call goes through torch's dispatcher, as an operator with a schema: the
 // tracer then records the call itself.  Called directly it would record the only torch operation that it
@@ -533,4 +746,11 @@ PYBIND11_MODULE(_gmlp_torch, m) {
   m.def("mlp_infer", torch::wrap_pybind_function_no_gil(mlp_infer));
   m.def("mlp_train", torch::wrap_pybind_function_no_gil(call_mlp_train));
   m.def("hidden", torch::wrap_pybind_function_no_gil(call_hidden));
+  m.def("q4_linear", torch::wrap_pybind_function_no_gil(q4_linear));
+  m.def("q4_mlp", torch::wrap_pybind_function_no_gil(q4_mlp));
+  m.def("q4_quantize", torch::wrap_pybind_function_no_gil(q4_quantize));
+  m.def("q4_dequantize", torch::wrap_pybind_function_no_gil(q4_dequantize));
+  m.def("moe_route", torch::wrap_pybind_function_no_gil(moe_route));
+  m.def("moe_mlp", torch::wrap_pybind_function_no_gil(moe_mlp));
+  m.def("moe_mlp_q4", torch::wrap_pybind_function_no_gil(moe_mlp_q4));
 }
