@@ -336,16 +336,20 @@ int gmlp_hidden_bwd(const void* dh, const void* x, const void* w_gate, const voi
  * gmlp_q4_linear_fwd: y[M,C] = x[M,R]·Wᵀ + bias, W [C,R] 4-bit; bias may be NULL.  The products are of scale·n itself, not
  *   of its rounding.
  * gmlp_q4_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) in dtype [M,N] (scratch), y = h·W_downᵀ + b_down.
+ * workspace: partial sums of a reduction that is split over workgroups, gmlp_q4_workspace_bytes(M, R, C, ...) bytes for the
+ *   linear layer and (M, R = N, C = K, ...) for the MLP.  NULL, 0 or fewer bytes are accepted and only slower.
  */
 int gmlp_q4_quantize(const void* w, void* codes, void* scales, int64_t count, int64_t rows, int64_t cols, int group, int dtype,
                      void* stream);
 int gmlp_q4_dequantize(const void* codes, const void* scales, void* w, int64_t count, int64_t rows, int64_t cols, int group,
                        int dtype, void* stream);
+size_t gmlp_q4_workspace_bytes(int64_t M, int64_t R, int64_t C, int group, int dtype);
 int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, const void* bias, void* y, int64_t M, int64_t R,
-                       int64_t C, int group, int dtype, void* stream);
+                       int64_t C, int group, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_gate, const void* codes_up, const void* scales_up,
                     const void* codes_down, const void* scales_down, const void* b_gate, const void* b_up, const void* b_down,
-                    void* h, void* y, int64_t M, int64_t K, int64_t N, int group, int dtype, int act, void* stream);
+                    void* h, void* y, int64_t M, int64_t K, int64_t N, int group, int dtype, int act, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 /*
  * gmlp_moe_route: p = softmax(logits[m, 0..E)) in fp32; experts [M, top_k] are the numbers of the top_k largest logits in
@@ -360,7 +364,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
  */
 int gmlp_moe_route(const void* logits, float* weights, int64_t* experts, int64_t M, int64_t E, int64_t top_k, int normalize, int dtype,
                    void* stream);
-size_t gmlp_moe_workspace_bytes(int64_t M, int64_t N, int64_t E, int64_t top_k, int dtype);
+size_t gmlp_moe_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group, int dtype);
 int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const void* w_up, const void* w_down, const void* s_gate,
                  const void* s_up, const void* s_down, void* y, int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k,
                  int normalize, int group, int dtype, int logits_dtype, int act, void* workspace, size_t workspace_bytes,

@@ -148,17 +148,17 @@ def test_refusals_of_the_c_interface():
     a = (ctypes.addressof(raw) + 63) & ~63
     err = lambda: lib.gmlp_last_error().decode()
     # NULL, group size, dtype, widths, rows, alignment
-    assert lib.gmlp_q4_linear_fwd(None, a, a, None, a, 1, 64, 64, 128, 0, None) == -1 and "NULL" in err()
-    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 48, 0, None) == -1 and "group" in err()
-    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 128, 2, None) == -2
-    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 128, 9, None) == -1
-    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 60, 64, 128, 0, None) == -2 and "multiple of 8" in err()
-    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 60, 128, 0, None) == -2
-    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 65, 64, 64, 128, 0, None) == -2 and "64" in err()
-    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 0, 64, 64, 128, 0, None) == -2
-    assert lib.gmlp_q4_linear_fwd(a + 8, a, a, None, a, 1, 64, 64, 128, 0, None) == -3
-    assert lib.gmlp_q4_linear_fwd(a, a, a, a + 2, a, 1, 64, 64, 128, 0, None) == -3
-    mlp = lambda x, M, K, N, group, dtype, act: lib.gmlp_q4_mlp_fwd(x, a, a, a, a, a, a, None, None, None, a, a, M, K, N, group, dtype, act, None)
+    assert lib.gmlp_q4_linear_fwd(None, a, a, None, a, 1, 64, 64, 128, 0, None, 0, None) == -1 and "NULL" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 48, 0, None, 0, None) == -1 and "group" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 128, 2, None, 0, None) == -2
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 64, 128, 9, None, 0, None) == -1
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 60, 64, 128, 0, None, 0, None) == -2 and "multiple of 8" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 1, 64, 60, 128, 0, None, 0, None) == -2
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 65, 64, 64, 128, 0, None, 0, None) == -2 and "64" in err()
+    assert lib.gmlp_q4_linear_fwd(a, a, a, None, a, 0, 64, 64, 128, 0, None, 0, None) == -2
+    assert lib.gmlp_q4_linear_fwd(a + 8, a, a, None, a, 1, 64, 64, 128, 0, None, 0, None) == -3
+    assert lib.gmlp_q4_linear_fwd(a, a, a, a + 2, a, 1, 64, 64, 128, 0, None, 0, None) == -3
+    mlp = lambda x, M, K, N, group, dtype, act: lib.gmlp_q4_mlp_fwd(x, a, a, a, a, a, a, None, None, None, a, a, M, K, N, group, dtype, act, None, 0, None)
     assert mlp(None, 1, 64, 64, 32, 0, 0) == -1 and mlp(a, 1, 64, 64, 32, 0, 7) == -1 and "act" in err()
     assert mlp(a, 1, 64, 68, 32, 0, 0) == -2 and mlp(a, 65, 64, 64, 32, 0, 0) == -2 and mlp(a, 1, 64, 64, 16, 0, 0) == -1
     for quantize in (lib.gmlp_q4_quantize, lib.gmlp_q4_dequantize):
@@ -175,9 +175,9 @@ def test_refusals_of_the_c_interface():
     assert lib.gmlp_moe_route(a, a, a, 1, 64, 17, 1, 2, None) == -2
     assert lib.gmlp_moe_route(a, a, a, 0, 8, 2, 1, 2, None) == -2
     assert lib.gmlp_moe_route(a, a, a, 1, 8, 2, 1, 5, None) == -1
-    need = lib.gmlp_moe_workspace_bytes(4, 64, 8, 2, 0)
+    need = lib.gmlp_moe_workspace_bytes(4, 64, 64, 8, 2, 0, 0)
     assert need >= 4 * 2 * 64 * 2
-    assert lib.gmlp_moe_workspace_bytes(65, 64, 8, 2, 0) == 0
+    assert lib.gmlp_moe_workspace_bytes(65, 64, 64, 8, 2, 0, 0) == 0
 
     def layer(x=a, logits=a, s=None, y=a, M=4, K=64, N=64, E=8, k=2, group=0, dtype=0, ld=2, act=0, ws=a, n=need):
         return lib.gmlp_moe_fwd(x, logits, a, a, a, s, s, s, y, M, K, N, E, k, 1, group, dtype, ld, act, ws, n, None)

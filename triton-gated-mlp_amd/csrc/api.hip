@@ -1445,11 +1445,11 @@ int check_rows(const char* fn, int64_t M) {
     return fail(GMLP_ESHAPE, "%s: M = %lld exceeds the %d token rows of a call", fn, (long long)M, gmlp::EXPERTS_MAX_M);
   return 0;
 }
-// The kernels address a tile of weights, the token rows and the hidden states with 32-bit byte offsets, and a grid
+// The kernels address four tiles of weights, the token rows and the hidden states with 32-bit byte offsets, and a grid
 // has a workgroup per tile.
 int check_expert_sizes(const char* fn, int64_t M, int64_t K, int64_t N, int64_t experts, int64_t pairs) {
-  const int64_t limit = (int64_t)1 << 31, most = K > N ? K : N;
-  if (most * 32 >= limit || M * K * 2 >= limit || pairs * N * 2 >= limit || experts * cdiv(most, 16) >= limit)
+  const int64_t limit = gmlp::EXPERTS_MAX_BYTES, most = K > N ? K : N;
+  if (most * 2 * 16 * 4 >= limit || M * K * 2 >= limit || pairs * N * 2 >= limit || experts * cdiv(most, 16) >= limit)
     return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
   return 0;
 }
@@ -1467,14 +1467,25 @@ int check_routing(const char* fn, int64_t E, int64_t top_k) {
                 gmlp::EXPERTS_MAX_E, (long long)top_k, (long long)E);
   return 0;
 }
+// The workspace is for partial sums: too small a one, or none, and the reduction is not split.
+void use_partial(gmlp::ExpertArgs& a, int group, void* workspace, size_t workspace_bytes) {
+  const size_t n = gmlp::experts_partial_bytes(a, group);
+  if (n > 0 && workspace != nullptr && workspace_bytes >= n) a.partial = (float*)workspace;
+}
 template <typename F>
 hipError_t by_half(int dtype, F&& f) {
   return dtype == GMLP_F16 ? f(gmlp::f16{}) : f(gmlp::bf16{});
 }
 // Where the parts of gmlp_moe_fwd's workspace begin.
+gmlp::ExpertArgs expert_sizes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k) {
+  gmlp::ExpertArgs a = {};
+  a.M = (int)M; a.K = (int)K; a.N = (int)N; a.E = (int)E; a.top_k = (int)top_k;
+  a.cus = num_cu();
+  return a;
+}
 struct MoeWorkspace {
-  size_t active, slot, tokens, count, weight, bytes;
-  MoeWorkspace(int64_t M, int64_t N, int64_t E, int64_t top_k) {
+  size_t active, slot, tokens, count, weight, partial, bytes;
+  MoeWorkspace(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group) {
     const size_t pairs = (size_t)(M * top_k), experts = (size_t)E < pairs ? (size_t)E : pairs;
     size_t at = pairs * (size_t)N * 2;
     auto part = [&](size_t n) {
@@ -1487,6 +1498,7 @@ struct MoeWorkspace {
     tokens = part(experts * gmlp::EXPERTS_MAX_M);
     count = part(experts);
     weight = part(pairs * sizeof(float));
+    partial = part(gmlp::experts_partial_bytes(expert_sizes(M, K, N, E, top_k), group));
     bytes = at;
   }
 };
@@ -1519,8 +1531,13 @@ int gmlp_q4_dequantize(const void* codes, const void* scales, void* w, int64_t c
   }));
 }
 
+size_t gmlp_q4_workspace_bytes(int64_t M, int64_t R, int64_t C, int group, int dtype) {
+  if (M < 1 || M > gmlp::EXPERTS_MAX_M || R < 1 || R > kMaxDim || C < 1 || C > kMaxDim || check_q4(__func__, group, dtype) != 0) return 0;
+  return gmlp::experts_partial_bytes(expert_sizes(M, C, R, 1, 1), group);
+}
+
 int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, const void* bias, void* y, int64_t M, int64_t R,
-                       int64_t C, int group, int dtype, void* stream) {
+                       int64_t C, int group, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales); GMLP_REQUIRE_PTR(y);
   if (int rc = check_q4(__func__, group, dtype)) return rc;
   if (int rc = check_dims(__func__, M, R, C)) return rc;
@@ -1529,13 +1546,13 @@ int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, con
   if (int rc = check_mult8(__func__, "C", C)) return rc;
   if (int rc = check_expert_sizes(__func__, M, C, R, 1, M)) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(bias);
-  GMLP_REQUIRE_ALIGNED(y);
-  gmlp::ExpertArgs a = {};
+  GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
+  gmlp::ExpertArgs a = expert_sizes(M, C, R, 1, 1);
   a.h = const_cast<void*>(x);  // read only
   a.y = y;
   a.bias[2] = bias;
   a.down = {codes, scales};
-  a.M = (int)M; a.K = (int)C; a.N = (int)R; a.E = a.top_k = a.dense = 1;
+  use_partial(a, group, workspace, workspace_bytes);
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     return gmlp::launch_experts_down<decltype(tag)>(a, group, (hipStream_t)stream);
   }));
@@ -1543,7 +1560,8 @@ int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, con
 
 int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_gate, const void* codes_up, const void* scales_up,
                     const void* codes_down, const void* scales_down, const void* b_gate, const void* b_up, const void* b_down,
-                    void* h, void* y, int64_t M, int64_t K, int64_t N, int group, int dtype, int act, void* stream) {
+                    void* h, void* y, int64_t M, int64_t K, int64_t N, int group, int dtype, int act, void* workspace,
+                    size_t workspace_bytes, void* stream) {
   GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(codes_gate); GMLP_REQUIRE_PTR(scales_gate); GMLP_REQUIRE_PTR(codes_up);
   GMLP_REQUIRE_PTR(scales_up); GMLP_REQUIRE_PTR(codes_down); GMLP_REQUIRE_PTR(scales_down); GMLP_REQUIRE_PTR(h);
   GMLP_REQUIRE_PTR(y);
@@ -1557,8 +1575,8 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(scales_gate); GMLP_REQUIRE_ALIGNED(codes_up);
   GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(codes_down); GMLP_REQUIRE_ALIGNED(scales_down);
   GMLP_REQUIRE_ALIGNED(b_gate); GMLP_REQUIRE_ALIGNED(b_up); GMLP_REQUIRE_ALIGNED(b_down); GMLP_REQUIRE_ALIGNED(h);
-  GMLP_REQUIRE_ALIGNED(y);
-  gmlp::ExpertArgs a = {};
+  GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
+  gmlp::ExpertArgs a = expert_sizes(M, K, N, 1, 1);
   a.x = x;
   a.h = h;
   a.y = y;
@@ -1566,7 +1584,8 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
   a.gate = {codes_gate, scales_gate};
   a.up = {codes_up, scales_up};
   a.down = {codes_down, scales_down};
-  a.M = (int)M; a.K = (int)K; a.N = (int)N; a.act = act; a.E = a.top_k = a.dense = 1;
+  a.act = act;
+  use_partial(a, group, workspace, workspace_bytes);
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
     if (hipError_t e = gmlp::launch_experts_gateup<T>(a, group, (hipStream_t)stream)) return e;
@@ -1586,11 +1605,11 @@ int gmlp_moe_route(const void* logits, float* weights, int64_t* experts, int64_t
   }));
 }
 
-size_t gmlp_moe_workspace_bytes(int64_t M, int64_t N, int64_t E, int64_t top_k, int dtype) {
-  if (M < 1 || M > gmlp::EXPERTS_MAX_M || N < 1 || N > kMaxDim || E < 1 || E > gmlp::EXPERTS_MAX_E || top_k < 1 ||
-      top_k > gmlp::EXPERTS_MAX_K || (dtype != GMLP_F16 && dtype != GMLP_BF16))
+size_t gmlp_moe_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group, int dtype) {
+  if (M < 1 || M > gmlp::EXPERTS_MAX_M || K < 1 || K > kMaxDim || N < 1 || N > kMaxDim || E < 1 || E > gmlp::EXPERTS_MAX_E || top_k < 1 ||
+      top_k > gmlp::EXPERTS_MAX_K || check_q4(__func__, group == 0 ? 32 : group, dtype) != 0)
     return 0;
-  return MoeWorkspace(M, N, E, top_k).bytes;
+  return MoeWorkspace(M, K, N, E, top_k, group).bytes;
 }
 
 int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const void* w_up, const void* w_down, const void* s_gate,
@@ -1614,26 +1633,33 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(w_gate); GMLP_REQUIRE_ALIGNED(w_up);
   GMLP_REQUIRE_ALIGNED(w_down); GMLP_REQUIRE_ALIGNED(s_gate); GMLP_REQUIRE_ALIGNED(s_up); GMLP_REQUIRE_ALIGNED(s_down);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
-  const MoeWorkspace ws(M, N, E, top_k);
+  const MoeWorkspace ws(M, K, N, E, top_k, group);
   if (workspace_bytes < ws.bytes)
     return fail(GMLP_EINVAL, "%s: workspace of %zu bytes, needs %zu", __func__, workspace_bytes, ws.bytes);
   char* const base = (char*)workspace;
-  gmlp::ExpertArgs a = {};
+  gmlp::ExpertArgs a = expert_sizes(M, K, N, E, top_k);
   a.x = x;
   a.h = base;
   a.y = y;
   a.gate = {w_gate, s_gate};
   a.up = {w_up, s_up};
   a.down = {w_down, s_down};
-  a.M = (int)M; a.K = (int)K; a.N = (int)N; a.E = (int)E; a.top_k = (int)top_k; a.act = act;
+  a.act = act;
+  a.logits = logits;
+  a.logits_dtype = logits_dtype;
+  a.normalize = normalize;
+  a.routing = gmlp::experts_solo(a) ? gmlp::ROUTING_SOLO : gmlp::ROUTING_PLAN;
   a.plan = {(int*)(base + ws.active), (uint8_t*)(base + ws.count), (uint8_t*)(base + ws.tokens), (int8_t*)(base + ws.slot),
             (float*)(base + ws.weight)};
+  if (ws.bytes > ws.partial) a.partial = (float*)(base + ws.partial);
   const hipStream_t s = (hipStream_t)stream;
-  const hipError_t planned = by_dtype(logits_dtype, [&](auto tag) {
-    typedef decltype(tag) L;
-    return gmlp::launch_experts_plan<L>((const L*)logits, a.plan, a.M, a.E, a.top_k, normalize, s);
-  });
-  if (planned != hipSuccess) return hip_result(__func__, planned);
+  if (a.routing == gmlp::ROUTING_PLAN) {
+    const hipError_t planned = by_dtype(logits_dtype, [&](auto tag) {
+      typedef decltype(tag) L;
+      return gmlp::launch_experts_plan<L>((const L*)logits, a.plan, a.M, a.E, a.top_k, normalize, s);
+    });
+    if (planned != hipSuccess) return hip_result(__func__, planned);
+  }
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
     if (hipError_t e = gmlp::launch_experts_gateup<T>(a, group, s)) return e;

@@ -14,27 +14,31 @@
 // product in fp32, so what is multiplied is scale·n itself, not its rounding.
 #include "experts.hpp"
 
-#include "gemm.hpp"
+#include "launch.hpp"
 
 namespace gmlp {
 
 typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x2 __attribute__((ext_vector_type(2)));
 
-constexpr uint32_t EX_NOWHERE = 0x80000000u;  // byte offset beyond any descriptor (all are < 2 GiB)
+// Byte offsets beyond any descriptor (all are shorter than EX_PAST): of a lane that loads nothing, and of a stage that does
+// not exist.  Their sum does not wrap.
+constexpr uint32_t EX_NOWHERE = 0x80000000u, EX_PAST = EXPERTS_MAX_BYTES;
 
 typedef __amdgpu_buffer_rsrc_t ex_rsrc;
 __device__ __forceinline__ ex_rsrc ex_make_rsrc(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
+// LDS for the tables of the largest routing (experts_down_kernel).
+constexpr int EX_TABLES = EXPERTS_MAX_E * (4 + EXPERTS_MAX_M) + EXPERTS_MAX_M * EXPERTS_MAX_K * 4;
 constexpr int EX_STREAM = 2;  // cache policy: non-temporal, what is read once
 template <int POLICY = 0>
-__device__ __forceinline__ u32x4 ex_load16(ex_rsrc r, uint32_t off) {
-  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, POLICY));
+__device__ __forceinline__ u32x4 ex_load16(ex_rsrc r, uint32_t lane_off, uint32_t off) {
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)lane_off, (int)off, POLICY));
 }
 template <int POLICY = 0>
-__device__ __forceinline__ u32x2 ex_load8(ex_rsrc r, uint32_t off) {
-  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)off, 0, POLICY));
+__device__ __forceinline__ u32x2 ex_load8(ex_rsrc r, uint32_t lane_off, uint32_t off) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(r, (int)lane_off, (int)off, POLICY));
 }
 
 // ------------------------------------------------------------------ 4-bit integers as 16-bit floats
@@ -45,33 +49,40 @@ struct Int4;
 template <>
 struct Int4<f16> {
   static constexpr float SCALE = 1.f;
-  // 0x6400 | u is 1024 + u in fp16; u = n + 8
-  static __device__ __forceinline__ f16x8 floats(uint32_t w) {
-    u32x4 o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t v = ((w >> (4 * j)) & 0x000f000fu) | 0x64006400u;
-      o[j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, v) - f16x2{(f16)1032.f, (f16)1032.f});
-    }
+  uint32_t magic;
+  __device__ __forceinline__ Int4() : magic(0x64006400u) {
+    asm("" : "+v"(magic));  // (in a register, so that the mask and it go into one instruction)
+  }
+  // 0x6400 | u is 1024 + u in fp16, 0x6400 | 16 u is 1024 + 16 u; u = n + 8
+  __device__ __forceinline__ f16x8 floats(uint32_t w) const {
+    const uint32_t v = w >> 8;
+    const f16x2 low = {(f16)-1032.f, (f16)-1032.f}, high = {(f16)-72.f, (f16)-72.f}, part = {(f16)0.0625f, (f16)0.0625f};
+    const f16x2 o[4] = {pair(w & 0x000f000fu | magic) + low, pair(w & 0x00f000f0u | magic) * part + high,
+                        pair(v & 0x000f000fu | magic) + low, pair(v & 0x00f000f0u | magic) * part + high};
     return __builtin_bit_cast(f16x8, o);
   }
+  static __device__ __forceinline__ f16x2 pair(uint32_t u) { return __builtin_bit_cast(f16x2, u); }
 };
 template <>
 struct Int4<bf16> {
   static constexpr float SCALE = 16.f;
   // v_cvt_off_f32_i4 makes n / 16 of a signed nibble; a bf16 is the upper half of the fp32 number
-  static __device__ __forceinline__ bf16x8 floats(uint32_t w) {
+  template <int BYTE>
+  static __device__ __forceinline__ uint32_t sixteenth(uint32_t v) {
+    float f;
+    if constexpr (BYTE == 0) f = __builtin_amdgcn_cvt_off_f32_i4((int)v);
+    else if constexpr (BYTE == 1) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(v));
+    else if constexpr (BYTE == 2) asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(v));
+    else asm("v_cvt_off_f32_i4_sdwa %0, %1 dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(v));
+    return __builtin_bit_cast(uint32_t, f);
+  }
+  __device__ __forceinline__ bf16x8 floats(uint32_t w) const {
     const uint32_t even = w ^ 0x88888888u, odd = even >> 4;
-    u32x4 o;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t v = j % 2 ? odd : even;
-      const float lo = __builtin_amdgcn_cvt_off_f32_i4((int)((v >> (8 * (j / 2))) & 0xffu));
-      const float hi = __builtin_amdgcn_cvt_off_f32_i4((int)((v >> (8 * (j / 2) + 16)) & 0xffu));
-      o[j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
-    }
+    const u32x4 o = {upper(sixteenth<2>(even), sixteenth<0>(even)), upper(sixteenth<2>(odd), sixteenth<0>(odd)),
+                     upper(sixteenth<3>(even), sixteenth<1>(even)), upper(sixteenth<3>(odd), sixteenth<1>(odd))};
     return __builtin_bit_cast(bf16x8, o);
   }
+  static __device__ __forceinline__ uint32_t upper(uint32_t hi, uint32_t lo) { return __builtin_amdgcn_perm(hi, lo, 0x07060302u); }
 };
 
 template <typename T>
@@ -79,344 +90,7 @@ __device__ __forceinline__ float bits_to_f32(uint32_t u) {
   return (float)__builtin_bit_cast(T, (unsigned short)u);
 }
 
-// ------------------------------------------------------------------ a block of the reduction
-// 16 weight rows of NMAT matrices by 64 columns (16-bit weights) or 128 (4-bit ones), and MT tiles of 16 token
-// rows by the same columns.  16-bit: a lane holds 32 consecutive bytes of its row in two loads, so a row's segment
-// is one 128-byte line; 4-bit: 16 consecutive bytes, a wavefront one KiB.  (The products do not mind which columns share a
-// step, so the token operands follow the weights.)
-template <typename T, int G, int NMAT, int MT>
-struct Block {
-  typedef typename Traits<T>::vec8 vec8;
-  static constexpr int COLS = G ? Q4_BLOCK : 64;
-  static constexpr int STEPS = COLS / 32;
-  static constexpr int GROUPS = G ? Q4_BLOCK / G : 1;
-  static constexpr int WL = G ? 1 : 2;  // weight loads of a lane
-  u32x4 w[NMAT][WL];
-  u32x2 sc[NMAT][GROUPS];
-  u32x4 x[MT][STEPS];
-
-  static __device__ __forceinline__ uint32_t column(int kb, int s, int kg) {
-    return (uint32_t)(kb * COLS + (G ? s * 32 + kg * 8 : kg * 16 + s * 8));
-  }
-  // of tile `tile` of a matrix of `rows` x `cols`
-  static __device__ __forceinline__ ex_rsrc weights_of(const ExpertWeights& m, int expert, int tile, int rows, int cols) {
-    const int tiles = (rows + Q4_TILE - 1) / Q4_TILE, blocks = (cols + Q4_BLOCK - 1) / Q4_BLOCK;
-    if (G) return ex_make_rsrc((const char*)m.w + ((size_t)expert * tiles + tile) * blocks * 1024, (uint32_t)blocks * 1024u);
-    const int first = tile * Q4_TILE, own = rows - first < Q4_TILE ? rows - first : Q4_TILE;
-    return ex_make_rsrc((const T*)m.w + ((size_t)expert * rows + first) * cols, (uint32_t)own * (uint32_t)cols * 2u);
-  }
-  static __device__ __forceinline__ ex_rsrc scales_of(const ExpertWeights& m, int expert, int tile, int rows, int cols) {
-    const int tiles = (rows + Q4_TILE - 1) / Q4_TILE, blocks = (cols + Q4_BLOCK - 1) / Q4_BLOCK;
-    const uint32_t pitch = (uint32_t)blocks * (Q4_TILE * GROUPS * 2);
-    return ex_make_rsrc((const char*)m.scales + ((size_t)expert * tiles + tile) * pitch, G ? pitch : 0u);
-  }
-
-  __device__ __forceinline__ void load_weights(int n, ex_rsrc rw, ex_rsrc rs, int kb, bool ok, int cols, int lane) {
-    const int kg = lane >> 4, r16 = lane & 15;
-    if (G) {
-      w[n][0] = ex_load16<EX_STREAM>(rw, ok ? (uint32_t)kb * 1024u + (uint32_t)lane * 16u : EX_NOWHERE);
-      const uint32_t at = ok ? (uint32_t)(kb * 4 + kg) * (GROUPS * 8u) : EX_NOWHERE;
-      if constexpr (GROUPS == 1) {
-        sc[n][0] = ex_load8<EX_STREAM>(rs, at);
-      } else {
-#pragma unroll
-        for (int g = 0; g < GROUPS; g += 2) {
-          const u32x4 v = ex_load16<EX_STREAM>(rs, at + (uint32_t)g * 8u);
-          sc[n][g] = u32x2{v[0], v[1]};
-          sc[n][g + 1] = u32x2{v[2], v[3]};
-        }
-      }
-    } else {
-#pragma unroll
-      for (int s = 0; s < WL; ++s) {
-        const uint32_t c = column(kb, s, kg);
-        w[n][s] = ex_load16<EX_STREAM>(rw, ok && c < (uint32_t)cols ? ((uint32_t)r16 * (uint32_t)cols + c) * 2u : EX_NOWHERE);
-      }
-    }
-  }
-  // row[m]: byte offset of the lane's token row, or EX_NOWHERE
-  __device__ __forceinline__ void load_tokens(ex_rsrc rx, const uint32_t (&row)[MT], int kb, bool ok, int cols, int lane) {
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      const uint32_t c = column(kb, s, lane >> 4);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) x[m][s] = ex_load16(rx, ok && c < (uint32_t)cols ? row[m] + c * 2u : EX_NOWHERE);
-    }
-  }
-  __device__ __forceinline__ void multiply(f32x4 (&acc)[NMAT][MT]) const {
-#pragma unroll
-    for (int n = 0; n < NMAT; ++n) {
-      if (G) {
-#pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
-          f32x4 part[MT];
-#pragma unroll
-          for (int m = 0; m < MT; ++m) part[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = g * STEPS / GROUPS; s < (g + 1) * STEPS / GROUPS; ++s) {
-            const vec8 a = Int4<T>::floats(w[n][0][s]);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) part[m] = Traits<T>::mfma16(a, __builtin_bit_cast(vec8, x[m][s]), part[m]);
-          }
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float f = bits_to_f32<T>(sc[n][g][r / 2] >> (16 * (r % 2)) & 0xffffu) * Int4<T>::SCALE;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) acc[n][m][r] += f * part[m][r];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int s = 0; s < STEPS; ++s)
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            acc[n][m] = Traits<T>::mfma16(__builtin_bit_cast(vec8, w[n][s]), __builtin_bit_cast(vec8, x[m][s]), acc[n][m]);
-      }
-    }
-  }
-};
-
-// ------------------------------------------------------------------ gate/up
-template <typename T, int G, int MT, int NW, int D>
-__global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
-  typedef Block<T, G, 2, MT> B;
-  __shared__ f32x4 part[NW][2][MT][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r16 = lane & 15, kg = lane >> 4;
-  const int tiles = (a.N + Q4_TILE - 1) / Q4_TILE;
-  const int slot = (int)blockIdx.x / tiles, tile = (int)blockIdx.x - slot * tiles;
-  int expert = 0, count = a.M;
-  if (!a.dense) {
-    if (slot >= a.plan.active[0]) return;
-    expert = a.plan.active[1 + slot];
-    count = a.plan.count[slot];
-  }
-  const ex_rsrc rx = ex_make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 2u);
-  const ExpertWeights* const mats[2] = {&a.gate, &a.up};
-  ex_rsrc rw[2], rs[2];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    rw[n] = B::weights_of(*mats[n], expert, tile, a.N, a.K);
-    rs[n] = B::scales_of(*mats[n], expert, tile, a.N, a.K);
-  }
-  const int blocks = (a.K + B::COLS - 1) / B::COLS;
-  const int b0 = blocks * wave / NW, run = blocks * (wave + 1) / NW - b0;
-
-  for (int base = 0; base < count; base += 16 * MT) {
-    uint32_t row[MT];
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int j = base + 16 * m + r16;
-      const int t = j < count ? (a.dense ? j : a.plan.tokens[slot * EXPERTS_MAX_M + j]) : 0;
-      row[m] = j < count ? (uint32_t)t * (uint32_t)a.K * 2u : EX_NOWHERE;
-    }
-    B st[D];
-    auto load = [&](B& b, int i) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n) b.load_weights(n, rw[n], rs[n], b0 + i, i < run, a.K, lane);
-      b.load_tokens(rx, row, b0 + i, i < run, a.K, lane);
-    };
-    f32x4 acc[2][MT];
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], d);
-    for (int i = 0; i < run; i += D)
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        st[d].multiply(acc);
-        load(st[d], i + d + D);
-      }
-    if (base > 0) __syncthreads();
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int m = 0; m < MT; ++m) part[wave][n][m][lane] = acc[n][m];
-    __syncthreads();
-    if (wave < MT) {
-      const int j = base + 16 * wave + r16, first = tile * Q4_TILE + 4 * kg;
-      if (j < count && first < a.N) {
-        float v[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          f32x4 sum = part[0][n][wave][lane];
-#pragma unroll
-          for (int w = 1; w < NW; ++w) sum += part[w][n][wave][lane];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[n][r] = sum[r];
-          if (a.bias[n]) add_w<T, 4>((const T*)a.bias[n] + first, v[n]);
-        }
-        float h[4];
-        act_fwd_w<4>(a.act, v[0], h);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) h[r] *= v[1][r];
-        int p = j;
-        if (!a.dense) {
-          const int t = a.plan.tokens[slot * EXPERTS_MAX_M + j];
-          p = t * a.top_k + a.plan.slot[slot * EXPERTS_MAX_M + t];
-        }
-        store_w<T, 4>((T*)a.h + (size_t)p * a.N + first, h);
-      }
-    }
-  }
-}
-
-// ------------------------------------------------------------------ down
-// The blocks of all experts in use, one expert behind the other, are shared out evenly over the wavefronts.  What an
-// expert gives is added to a token's sum only where the token chose it (a weight that is not finite in one
-// expert stays out of the others' tokens).
-template <typename T, int G, int MT, int NW, int D>
-__global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
-  typedef Block<T, G, 1, MT> B;
-  extern __shared__ __align__(16) char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r16 = lane & 15, kg = lane >> 4, tile = (int)blockIdx.x;
-  const int pairs = a.M * a.top_k;
-  // tables: the experts' numbers, the pairs' weights, the slots
-  int in_use = 1;
-  int* const numbers = (int*)smem;
-  float* weight = nullptr;
-  int8_t* slots = nullptr;
-  if (!a.dense) {
-    in_use = a.plan.active[0];
-    weight = (float*)(numbers + in_use);
-    slots = (int8_t*)(weight + pairs);
-    for (int i = threadIdx.x; i < in_use; i += NW * 64) numbers[i] = a.plan.active[1 + i];
-    for (int i = threadIdx.x; i < pairs; i += NW * 64) weight[i] = a.plan.weight[i];
-    for (int i = threadIdx.x; i < in_use * (EXPERTS_MAX_M / 4); i += NW * 64)
-      ((int*)slots)[i] = ((const int*)a.plan.slot)[i];
-    __syncthreads();
-  }
-  const ex_rsrc rh = ex_make_rsrc(a.h, (uint32_t)pairs * (uint32_t)a.N * 2u);
-  const int blocks = (a.N + B::COLS - 1) / B::COLS;
-  const int total = in_use * blocks;
-  const int b0 = (int)((int64_t)total * wave / NW), run = (int)((int64_t)total * (wave + 1) / NW) - b0;
-
-  // choice of token row 16 m + r16 that expert e is, or -1
-  auto slot_of = [&](int e, int m) -> int {
-    const int t = 16 * m + r16;
-    if (t >= a.M) return -1;
-    return a.dense ? 0 : slots[e * EXPERTS_MAX_M + t];
-  };
-  // where loads go on: expert, block of it
-  int le = b0 / blocks, lb = b0 - le * blocks;
-  uint32_t row[MT];
-  ex_rsrc rw, rs;
-  auto enter = [&]() {
-    const int e = le < in_use ? le : in_use - 1;
-    const int number = a.dense ? 0 : __builtin_amdgcn_readfirstlane(numbers[e]);
-    rw = B::weights_of(a.down, number, tile, a.K, a.N);
-    rs = B::scales_of(a.down, number, tile, a.K, a.N);
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int s = slot_of(e, m);
-      row[m] = s < 0 ? EX_NOWHERE : (uint32_t)((16 * m + r16) * a.top_k + s) * (uint32_t)a.N * 2u;
-    }
-  };
-  f32x4 acc[1][MT], sum[MT];
-#pragma unroll
-  for (int m = 0; m < MT; ++m) acc[0][m] = sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (run > 0) {
-    enter();
-    B st[D];
-    auto load = [&](B& b, int i) {
-      b.load_weights(0, rw, rs, lb, i < run, a.N, lane);
-      b.load_tokens(rh, row, lb, i < run, a.N, lane);
-      if (++lb == blocks) {
-        lb = 0;
-        ++le;
-        enter();
-      }
-    };
-    int me = le, mb = lb;  // where products are
-    auto fold = [&]() {
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const int s = slot_of(me, m);
-        const float w = s < 0 ? 0.f : a.dense ? 1.f : weight[(16 * m + r16) * a.top_k + s];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (s >= 0) sum[m][r] += w * acc[0][m][r];
-          acc[0][m][r] = 0.f;
-        }
-      }
-    };
-#pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], d);
-    for (int i = 0; i < run; i += D)
-#pragma unroll
-      for (int d = 0; d < D; ++d) {
-        st[d].multiply(acc);
-        load(st[d], i + d + D);
-        if (++mb == blocks || i + d + 1 == run) {
-          if (i + d < run) fold();
-          mb = 0;
-          ++me;
-        }
-      }
-  }
-  if (!a.dense) __syncthreads();  // the tables' last readers
-  f32x4* const part = (f32x4*)smem;  // [NW][MT][64]
-#pragma unroll
-  for (int m = 0; m < MT; ++m) part[(wave * MT + m) * 64 + lane] = sum[m];
-  __syncthreads();
-  if (wave < MT) {
-    const int t = 16 * wave + r16, first = tile * Q4_TILE + 4 * kg;
-    if (t < a.M && first < a.K) {
-      f32x4 v = part[wave * 64 + lane];
-#pragma unroll
-      for (int w = 1; w < NW; ++w) v += part[(w * MT + wave) * 64 + lane];
-      float y[4] = {v[0], v[1], v[2], v[3]};
-      if (a.bias[2]) add_w<T, 4>((const T*)a.bias[2] + first, y);
-      store_w<T, 4>((T*)a.y + (size_t)t * a.K + first, y);
-    }
-  }
-}
-
-template <typename T, int G>
-static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
-  const int tiles = (a.N + Q4_TILE - 1) / Q4_TILE;
-  const int experts = a.dense ? 1 : (a.E < a.M * a.top_k ? a.E : a.M * a.top_k);
-  const dim3 grid((unsigned)(tiles * experts)), block(256);
-  if (a.M <= 16) hipLaunchKernelGGL((experts_gateup_kernel<T, G, 1, 4, 2>), grid, block, 0, s, a);
-  else if (a.M <= 32) hipLaunchKernelGGL((experts_gateup_kernel<T, G, 2, 4, 2>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((experts_gateup_kernel<T, G, 4, 4, 1>), grid, block, 0, s, a);
-  return hipGetLastError();
-}
-template <typename T, int G>
-static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
-  constexpr int NW = 8;
-  const dim3 grid((unsigned)((a.K + Q4_TILE - 1) / Q4_TILE)), block(NW * 64);
-  const int experts = a.dense ? 0 : (a.E < a.M * a.top_k ? a.E : a.M * a.top_k);
-  const size_t tables = (size_t)experts * (4 + EXPERTS_MAX_M) + (size_t)a.M * a.top_k * 4;
-  auto lds = [&](int mt) { return (unsigned)(tables > (size_t)NW * mt * 1024 ? tables : (size_t)NW * mt * 1024); };
-  if (a.M <= 16) hipLaunchKernelGGL((experts_down_kernel<T, G, 1, NW, 2>), grid, block, lds(1), s, a);
-  else if (a.M <= 32) hipLaunchKernelGGL((experts_down_kernel<T, G, 2, NW, 2>), grid, block, lds(2), s, a);
-  else hipLaunchKernelGGL((experts_down_kernel<T, G, 4, NW, 1>), grid, block, lds(4), s, a);
-  return hipGetLastError();
-}
-template <typename T>
-hipError_t launch_experts_gateup(const ExpertArgs& a, int group, hipStream_t s) {
-  switch (group) {
-    case 0: return gateup_of<T, 0>(a, s);
-    case 32: return gateup_of<T, 32>(a, s);
-    case 64: return gateup_of<T, 64>(a, s);
-    default: return gateup_of<T, 128>(a, s);
-  }
-}
-template <typename T>
-hipError_t launch_experts_down(const ExpertArgs& a, int group, hipStream_t s) {
-  switch (group) {
-    case 0: return down_of<T, 0>(a, s);
-    case 32: return down_of<T, 32>(a, s);
-    case 64: return down_of<T, 64>(a, s);
-    default: return down_of<T, 128>(a, s);
-  }
-}
-
-// ------------------------------------------------------------------ routing
+// ------------------------------------------------------------------ choice of experts
 // A logit as an integer of the same order: NaN above everything, -0 equal to 0, and 0 below every logit.
 __device__ __forceinline__ uint32_t logit_key(float v) {
   uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);
@@ -426,31 +100,43 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 __device__ __forceinline__ float key_logit(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
+// Reductions over a wavefront in the vector units: along the rows of 16 lanes, then from row to row; lane 63 has them all.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t from_lane(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
 __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const uint32_t o = (uint32_t)__shfl_xor((int)v, d);
-    v = o > v ? o : v;
-  }
-  return v;
+  auto take = [&](uint32_t o) { v = o > v ? o : v; };
+  take(from_lane<0x111>(v));
+  take(from_lane<0x112>(v));
+  take(from_lane<0x114>(v));
+  take(from_lane<0x118>(v));
+  take(from_lane<0x142>(v));
+  take(from_lane<0x143>(v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+  auto take = [&](uint32_t o) { v += __uint_as_float(o); };
+  take(from_lane<0x111>(__float_as_uint(v)));
+  take(from_lane<0x112>(__float_as_uint(v)));
+  take(from_lane<0x114>(__float_as_uint(v)));
+  take(from_lane<0x118>(__float_as_uint(v)));
+  take(from_lane<0x142, 0xa>(__float_as_uint(v)));
+  take(from_lane<0x143, 0xc>(__float_as_uint(v)));
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
 }
 
 // One wavefront, one token: lane j < top_k gets the token's j-th choice and its weight.  The experts lie in lane order
 // (lane l: VPL l .. VPL l + VPL - 1), so among equal logits the lowest lane holds the lowest number.
 // (-inf: not available, weight 0 and expert -1 - number.)
-template <int VPL, typename L>
-__device__ __forceinline__ void choose(const L* logits, int E, int top_k, bool normalize, int lane, int& expert, float& weight) {
+template <int VPL, typename F>
+__device__ __forceinline__ void choose(F&& logit, int E, int top_k, bool normalize, int lane, int& expert, float& weight) {
   uint32_t key[VPL];
   float value[VPL];
 #pragma unroll
   for (int v = 0; v < VPL; ++v) {
     const int e = lane * VPL + v;
-    value[v] = e < E ? (float)logits[e] : -__builtin_inff();
+    value[v] = e < E ? logit(e) : -__builtin_inff();
     key[v] = e < E ? logit_key(value[v]) : 0u;
   }
   uint32_t mine = 0, top = 0;
@@ -484,6 +170,556 @@ __device__ __forceinline__ void choose(const L* logits, int E, int top_k, bool n
   if (own == -__builtin_inff()) expert = -1 - expert;
 }
 
+// The routing of the only token of a call, in every wavefront of both kernels: a launch less, and 1 us against the 4 that the
+// launch and its kernel take.
+constexpr int SOLO_MAX_E = 256;
+__device__ __forceinline__ void choose_solo(const ExpertArgs& a, int lane, int& expert, float& weight) {
+  auto logit = [&](int i) -> float {
+    if (a.logits_dtype == 0) return (float)((const f16*)a.logits)[i];
+    if (a.logits_dtype == 1) return (float)((const bf16*)a.logits)[i];
+    return ((const float*)a.logits)[i];
+  };
+  if (a.E <= 64) choose<1>(logit, a.E, a.top_k, a.normalize != 0, lane, expert, weight);
+  else choose<SOLO_MAX_E / 64>(logit, a.E, a.top_k, a.normalize != 0, lane, expert, weight);
+}
+
+// ------------------------------------------------------------------ a block of the reduction
+// 16 rows of NT weight tiles by 64 columns (16-bit weights) or 128 (4-bit ones), and MT tiles of 16 token rows by the
+// same columns.  An MFMA wants neighbouring lanes on different rows; a load of that kind takes a cycle of the address unit per
+// lane (16-bit down projections stood at 8 bytes a clock and CU, 5 TB/s, whatever the number of loads in flight).  So rows
+// are loaded as they lie, 128 or 256 bytes of a row by neighbouring lanes, and change lanes through a piece of LDS of
+// the wavefront's own (in order, so without a barrier).  4-bit weights are stored as the MFMA takes them.
+// XR: loads per token tile; a load brings 8 (16-bit weights) or 4 token rows.
+template <typename T, int G, int NT, int MT, int XR>
+struct Block {
+  typedef typename Traits<T>::vec8 vec8;
+  static constexpr int COLS = G ? Q4_BLOCK : 64;
+  static constexpr int STEPS = COLS / 32;
+  static constexpr int GROUPS = G ? Q4_BLOCK / G : 1;
+  static constexpr int PIECES = COLS / 8;       // 16-byte pieces of a row
+  static constexpr int ROWS = 64 / PIECES;      // rows of a load
+  static constexpr int WL = G ? 1 : 16 / ROWS;  // loads of a weight tile
+  static constexpr int TILE = 16 * COLS * 2;    // bytes of a tile in LDS
+  static constexpr int XB = MT < 2 ? MT : 2, WB = G ? 0 : NT < 4 ? NT : 4;  // tiles in LDS at a time
+  static constexpr int LDS = (XB + WB) * TILE;  // of a wavefront
+  static_assert(XR * ROWS <= 16, "a token tile has 16 rows");
+  u32x4 w[NT][WL];
+  u32x2 sc[NT][GROUPS];
+  u32x4 x[MT][XR];
+
+  // from tile `tile` of an expert's matrix on, of `rows` x `cols`: `tiles` of them
+  static __device__ __forceinline__ ex_rsrc weights_of(const ExpertWeights& m, int expert, int tile, int tiles, int rows, int cols) {
+    const int all = (rows + Q4_TILE - 1) / Q4_TILE, blocks = (cols + Q4_BLOCK - 1) / Q4_BLOCK;
+    const int own = all - tile < tiles ? all - tile : tiles;
+    if (G) return ex_make_rsrc((const char*)m.w + ((size_t)expert * all + tile) * blocks * 1024, (uint32_t)(own * blocks) * 1024u);
+    const int first = tile * Q4_TILE, r = rows - first < tiles * Q4_TILE ? rows - first : tiles * Q4_TILE;
+    return ex_make_rsrc((const T*)m.w + ((size_t)expert * rows + first) * cols, (uint32_t)r * (uint32_t)cols * 2u);
+  }
+  static __device__ __forceinline__ ex_rsrc scales_of(const ExpertWeights& m, int expert, int tile, int tiles, int rows, int cols) {
+    const int all = (rows + Q4_TILE - 1) / Q4_TILE, blocks = (cols + Q4_BLOCK - 1) / Q4_BLOCK;
+    const int own = all - tile < tiles ? all - tile : tiles;
+    const uint32_t pitch = (uint32_t)blocks * (Q4_TILE * GROUPS * 2);
+    return ex_make_rsrc((const char*)m.scales + ((size_t)expert * all + tile) * pitch, G ? (uint32_t)own * pitch : 0u);
+  }
+  // Row of a tile and byte in the row's segment that a lane loads.
+  static __device__ __forceinline__ int load_row(int i, int lane) { return i * ROWS + lane / PIECES; }
+  static __device__ __forceinline__ uint32_t load_byte(int lane) { return (uint32_t)(lane % PIECES) * 16u; }
+  // Byte in LDS of a row's piece.  256-byte rows reach all banks, 128-byte ones two by two.
+  static __device__ __forceinline__ uint32_t at(int row, int piece) {
+    return (uint32_t)(row * PIECES + (piece ^ (PIECES == 16 ? row : row >> 1))) * 16u;
+  }
+
+  // Tile n: tile r behind the descriptors' first one.  `ok`: the block exists; `tail`: it may reach past the last column.
+  __device__ __forceinline__ void load_weights(int n, int r, ex_rsrc rw, ex_rsrc rs, int kb, bool ok, bool tail, int cols, int lane) {
+    if (G) {
+      const uint32_t unit = (uint32_t)(r * ((cols + Q4_BLOCK - 1) / Q4_BLOCK) + kb);
+      w[n][0] = ex_load16<EX_STREAM>(rw, (uint32_t)lane * 16u, ok ? unit * 1024u : EX_PAST);
+      const uint32_t from = ok ? unit * (GROUPS * 32u) : EX_PAST, own = (uint32_t)(lane >> 4) * (GROUPS * 8u);
+      if constexpr (GROUPS == 1) {
+        sc[n][0] = ex_load8<EX_STREAM>(rs, own, from);
+      } else {
+#pragma unroll
+        for (int g = 0; g < GROUPS; g += 2) {
+          const u32x4 v = ex_load16<EX_STREAM>(rs, own + (uint32_t)g * 8u, from);
+          sc[n][g] = u32x2{v[0], v[1]};
+          sc[n][g + 1] = u32x2{v[2], v[3]};
+        }
+      }
+    } else {
+      const uint32_t lane_off = tail && beyond(kb, cols, lane) ? EX_NOWHERE : (uint32_t)load_row(0, lane) * (uint32_t)cols * 2u + load_byte(lane);
+#pragma unroll
+      for (int i = 0; i < WL; ++i)
+        w[n][i] = ex_load16<EX_STREAM>(rw, lane_off, ok ? ((uint32_t)(r * Q4_TILE + i * ROWS) * (uint32_t)cols + (uint32_t)(kb * COLS)) * 2u : EX_PAST);
+    }
+  }
+  static __device__ __forceinline__ bool beyond(int kb, int cols, int lane) { return kb * COLS + lane % PIECES * 8 >= cols; }
+  // row[m][i]: byte offset of the lane's piece of its token row, or EX_NOWHERE
+  __device__ __forceinline__ void load_tokens(ex_rsrc rx, const uint32_t (&row)[MT][XR], int kb, bool ok, bool tail, int cols, int lane) {
+    const bool skip = tail && beyond(kb, cols, lane);
+    const uint32_t from = ok ? (uint32_t)(kb * COLS) * 2u : EX_PAST;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < XR; ++i) x[m][i] = ex_load16(rx, skip ? EX_NOWHERE : row[m][i], from);
+  }
+
+  // Columns of a tile: step s takes 32 s + 8 (lane / 16) + 0..7.  (Token rows that XR leaves out are whatever LDS holds: their
+  // columns of the product are not used.)
+  static __device__ __forceinline__ vec8 operand(const char* tile, int s, int lane) {
+    return *(const vec8*)(tile + at(lane & 15, s * 4 + (lane >> 4)));
+  }
+  template <int L>
+  static __device__ __forceinline__ void to_lds(char* tile, const u32x4 (&v)[L], int lane) {
+#pragma unroll
+    for (int i = 0; i < L; ++i) *(u32x4*)(tile + at(load_row(i, lane), lane % PIECES)) = v[i];
+  }
+  __device__ __forceinline__ void multiply(const Int4<T>& int4, char* lds, int lane, f32x4 (&acc)[NT][MT]) const {
+    vec8 xf[MT][STEPS];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      char* const tile = lds + (m % XB) * TILE;
+      to_lds(tile, x[m], lane);
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) xf[m][s] = operand(tile, s, lane);
+      __builtin_amdgcn_wave_barrier();
+    }
+    if (!G)
+#pragma unroll
+      for (int n = 0; n < WB; ++n) to_lds(lds + (XB + n) * TILE, w[n], lane);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (G) {
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+          f32x4 part[MT];
+#pragma unroll
+          for (int m = 0; m < MT; ++m) part[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = g * STEPS / GROUPS; s < (g + 1) * STEPS / GROUPS; ++s) {
+            const vec8 a = int4.floats(w[n][0][s]);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) part[m] = Traits<T>::mfma16(a, xf[m][s], part[m]);
+          }
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float f = bits_to_f32<T>(sc[n][g][r / 2] >> (16 * (r % 2)) & 0xffffu) * Int4<T>::SCALE;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) acc[n][m][r] += f * part[m][r];
+          }
+        }
+      } else {
+        char* const tile = lds + (XB + n % (WB ? WB : 1)) * TILE;
+        if (n >= WB) to_lds(tile, w[n], lane);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < STEPS; ++s) {
+          const vec8 a = operand(tile, s, lane);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) acc[n][m] = Traits<T>::mfma16(a, xf[m][s], acc[n][m]);
+        }
+        __builtin_amdgcn_wave_barrier();
+      }
+    }
+  }
+};
+
+// Adds up the wavefronts' sums, a few units of U vectors at a time through LDS, and calls done(unit, sums) for each in one
+// wavefront.
+template <int NW, int NU, int U>
+constexpr int units_at_a_time() {
+  return NW * NU * U <= 32 ? NU : 32 / (NW * U);  // 32 KiB
+}
+template <int NW, int NU, int U, typename F>
+__device__ __forceinline__ void sum_wavefronts(const f32x4 (&acc)[NU][U], char* smem, int wave, int lane, F&& done) {
+  constexpr int EACH = units_at_a_time<NW, NU, U>();
+  static_assert(EACH > 0, "a unit of every wavefront fits");
+  f32x4* const part = (f32x4*)smem;  // [NW][EACH][U][64]
+#pragma unroll
+  for (int first = 0; first < NU; first += EACH) {
+    __syncthreads();  // the readers of what LDS held before
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (first + i < NU) part[((wave * EACH + i) * U + u) * 64 + lane] = acc[first + i][u];
+    __syncthreads();
+    for (int i = wave; i < EACH && first + i < NU; i += NW) {
+      f32x4 sum[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        sum[u] = part[(i * U + u) * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) sum[u] += part[((w * EACH + i) * U + u) * 64 + lane];
+      }
+      done(first + i, sum);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ gate/up
+template <typename T, int G, int MT, int XR, int R, int NW>
+constexpr int gateup_lds() {
+  constexpr int ring = NW * Block<T, G, 2 * R, MT, XR>::LDS, part = NW * units_at_a_time<NW, R * MT, 2>() * 2 * 1024;
+  return ring > part ? ring : part;
+}
+template <typename T, int G, int MT, int XR, int R, int NW, int D>
+__global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
+  typedef Block<T, G, 2 * R, MT, XR> B;
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, kg = lane >> 4;
+  const int strips = (a.N + R * Q4_TILE - 1) / (R * Q4_TILE);
+  const int slot = (int)blockIdx.x / strips, tile = ((int)blockIdx.x - slot * strips) * R;
+  int expert = 0, count = a.M;
+  if (a.routing == ROUTING_SOLO) {
+    int e;
+    float w;
+    choose_solo(a, lane, e, w);
+    expert = __builtin_amdgcn_readlane(e, slot);
+    if (expert < 0) return;
+  } else if (a.routing == ROUTING_PLAN) {
+    if (slot >= a.plan.active[0]) return;
+    expert = a.plan.active[1 + slot];
+    count = a.plan.count[slot];
+  }
+  const ex_rsrc rx = ex_make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 2u);
+  const ex_rsrc rw[2] = {B::weights_of(a.gate, expert, tile, R, a.N, a.K), B::weights_of(a.up, expert, tile, R, a.N, a.K)};
+  const ex_rsrc rs[2] = {B::scales_of(a.gate, expert, tile, R, a.N, a.K), B::scales_of(a.up, expert, tile, R, a.N, a.K)};
+  const int blocks = (a.K + B::COLS - 1) / B::COLS;
+  const int b0 = blocks * wave / NW, run = blocks * (wave + 1) / NW - b0;
+  const int rot = run > 1 ? (int)blockIdx.x % run : 0;
+  const bool ragged = a.K % B::COLS != 0;
+  const Int4<T> int4;
+  char* const lds = smem + wave * B::LDS;
+
+  for (int base = 0; base < count; base += 16 * MT) {
+    uint32_t row[MT][XR];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < XR; ++i) {
+        const int j = base + 16 * m + B::load_row(i, lane);
+        const int t = j >= count ? 0 : a.routing == ROUTING_PLAN ? a.plan.tokens[slot * EXPERTS_MAX_M + j] : j;
+        row[m][i] = j < count ? (uint32_t)t * (uint32_t)a.K * 2u + B::load_byte(lane) : EX_NOWHERE;
+      }
+    B st[D];
+    auto load_block = [&](B& b, int kb, bool ok, bool tail) {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int n = 0; n < 2; ++n) b.load_weights(2 * r + n, r, rw[n], rs[n], kb, ok, tail, a.K, lane);
+      b.load_tokens(rx, row, kb, ok, tail, a.K, lane);
+    };
+    auto load = [&](B& b, int i) {
+      const int kb = b0 + (i + rot < run ? i + rot : i + rot - run);
+      if (ragged && kb + 1 == blocks) load_block(b, kb, i < run, true);
+      else load_block(b, kb, i < run, false);
+    };
+    f32x4 acc[2 * R][MT];
+#pragma unroll
+    for (int n = 0; n < 2 * R; ++n)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (base > 0) __syncthreads();  // the readers of the sums before
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(st[d], d);
+    for (int i = 0; i < run; i += D)
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        st[d].multiply(int4, lds, lane, acc);
+        load(st[d], i + d + D);
+      }
+    f32x4 both[R * MT][2];
+#pragma unroll
+    for (int i = 0; i < R * MT; ++i)
+#pragma unroll
+      for (int n = 0; n < 2; ++n) both[i][n] = acc[i / MT * 2 + n][i % MT];
+    sum_wavefronts<NW>(both, smem, wave, lane, [&](int unit, const f32x4 (&sum)[2]) {
+      const int r = unit / MT, j = base + 16 * (unit - r * MT) + r16, first = (tile + r) * Q4_TILE + 4 * kg;
+      if (j >= count || first >= a.N) return;
+      float v[2][4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[n][q] = sum[n][q];
+        if (a.bias[n]) add_w<T, 4>((const T*)a.bias[n] + first, v[n]);
+      }
+      float h[4];
+      act_fwd_w<4>(a.act, v[0], h);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) h[q] *= v[1][q];
+      int p = a.routing == ROUTING_SOLO ? slot : j;
+      if (a.routing == ROUTING_PLAN) {
+        const int t = a.plan.tokens[slot * EXPERTS_MAX_M + j];
+        p = t * a.top_k + a.plan.slot[slot * EXPERTS_MAX_M + t];
+      }
+      store_w<T, 4>((T*)a.h + (size_t)p * a.N + first, h);
+    });
+  }
+}
+
+// ------------------------------------------------------------------ down
+// The blocks of all experts in use, one expert behind the other, are shared out evenly over the wavefronts.  What an
+// expert gives is added to a token's sum only where the token chose it (a weight that is not finite in one
+// expert stays out of the others' tokens).
+template <typename T, int G, int MT, int XR, int R, int NW>
+constexpr int down_lds() {
+  constexpr int ring = NW * Block<T, G, R, MT, XR>::LDS, part = NW * units_at_a_time<NW, R * MT, 1>() * 1024;
+  return ring > part ? ring : part;
+}
+template <typename T, int G, int MT, int XR, int R, int NW, int D>
+__global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
+  typedef Block<T, G, R, MT, XR> B;
+  extern __shared__ __align__(16) char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r16 = lane & 15, kg = lane >> 4, tile = (int)blockIdx.x * R;
+  const int pairs = a.M * a.top_k;
+  // tables: the experts' numbers, the pairs' weights, the slots
+  int in_use = 1;
+  int* const numbers = (int*)(smem + down_lds<T, G, MT, XR, R, NW>());
+  float* weight = nullptr;
+  int8_t* slots = nullptr;
+  if (a.routing == ROUTING_SOLO) {
+    int e;
+    float w;
+    choose_solo(a, lane, e, w);
+    const uint64_t chosen = __ballot(lane < pairs && e >= 0);
+    in_use = __popcll(chosen);
+    weight = (float*)(numbers + in_use);
+    slots = (int8_t*)(weight + pairs);
+    if (wave == 0 && lane < pairs) {
+      const int i = __popcll(chosen & ((1ull << lane) - 1));
+      weight[lane] = w;
+      if (e >= 0) numbers[i] = e, slots[i * EXPERTS_MAX_M] = (int8_t)lane;
+    }
+    __syncthreads();
+  } else if (a.routing == ROUTING_PLAN) {
+    in_use = a.plan.active[0];
+    weight = (float*)(numbers + in_use);
+    slots = (int8_t*)(weight + pairs);
+    for (int i = threadIdx.x; i < in_use; i += NW * 64) numbers[i] = a.plan.active[1 + i];
+    for (int i = threadIdx.x; i < pairs; i += NW * 64) weight[i] = a.plan.weight[i];
+    for (int i = threadIdx.x; i < in_use * (EXPERTS_MAX_M / 4); i += NW * 64)
+      ((int*)slots)[i] = ((const int*)a.plan.slot)[i];
+    __syncthreads();
+  }
+  const ex_rsrc rh = ex_make_rsrc(a.h, (uint32_t)pairs * (uint32_t)a.N * 2u);
+  const int blocks = (a.N + B::COLS - 1) / B::COLS;
+  const int total = in_use * blocks;
+  const int parts = NW * (int)gridDim.y, me_part = (int)blockIdx.y * NW + wave;
+  const int b0 = (int)((int64_t)total * me_part / parts), run = (int)((int64_t)total * (me_part + 1) / parts) - b0;
+  const int rot = run > 1 ? (int)blockIdx.x % run : 0;
+  const bool ragged = a.N % B::COLS != 0;
+  const Int4<T> int4;
+  char* const lds = smem + wave * B::LDS;
+
+  // choice of token row t that expert e is, or -1
+  auto slot_of = [&](int e, int t) -> int {
+    if (t >= a.M) return -1;
+    return a.routing == ROUTING_DENSE ? 0 : slots[e * EXPERTS_MAX_M + t];
+  };
+  // where loads go on: expert, block of it
+  const int first_e = b0 / blocks, first_b = b0 - first_e * blocks;
+  int le = (b0 + rot) / blocks, lb = b0 + rot - le * blocks;
+  uint32_t row[MT][XR];
+  ex_rsrc rw, rs;
+  auto enter = [&]() {
+    const int e = le < in_use ? le : in_use - 1;
+    const int number = a.routing == ROUTING_DENSE ? 0 : __builtin_amdgcn_readfirstlane(numbers[e]);
+    rw = B::weights_of(a.down, number, tile, R, a.K, a.N);
+    rs = B::scales_of(a.down, number, tile, R, a.K, a.N);
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int i = 0; i < XR; ++i) {
+        const int t = 16 * m + B::load_row(i, lane), s = slot_of(e, t);
+        row[m][i] = s < 0 ? EX_NOWHERE : (uint32_t)(t * a.top_k + s) * (uint32_t)a.N * 2u + B::load_byte(lane);
+      }
+  };
+  f32x4 acc[R][MT], sum[R * MT][1];
+#pragma unroll
+  for (int n = 0; n < R; ++n)
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[n][m] = sum[n * MT + m][0] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (run > 0) {
+    enter();
+    B st[D];
+    auto load_block = [&](B& b, bool ok, bool tail) {
+#pragma unroll
+      for (int n = 0; n < R; ++n) b.load_weights(n, n, rw, rs, lb, ok, tail, a.N, lane);
+      b.load_tokens(rh, row, lb, ok, tail, a.N, lane);
+    };
+    auto load = [&](B& b, int i) {
+      if (ragged && lb + 1 == blocks) load_block(b, i < run, true);
+      else load_block(b, i < run, false);
+      const bool wrap = i + 1 == run - rot;
+      if (++lb == blocks || wrap) {
+        lb = wrap ? first_b : 0;
+        le = wrap ? first_e : le + 1;
+        enter();
+      }
+    };
+    int me = le, mb = lb;  // where products are
+    auto fold = [&]() {
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const int t = 16 * m + r16, s = slot_of(me, t);
+        const float w = s < 0 ? 0.f : a.routing == ROUTING_DENSE ? 1.f : weight[t * a.top_k + s];
+#pragma unroll
+        for (int n = 0; n < R; ++n)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (s >= 0) sum[n * MT + m][0][r] += w * acc[n][m][r];
+            acc[n][m][r] = 0.f;
+          }
+      }
+    };
+#pragma unroll
+    for (int d = 0; d < D; ++d) load(st[d], d);
+    for (int i = 0; i < run; i += D)
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        st[d].multiply(int4, lds, lane, acc);
+        load(st[d], i + d + D);
+        const bool wrap = i + d + 1 == run - rot;
+        if (++mb == blocks || wrap || i + d + 1 == run) {
+          if (i + d < run) fold();
+          mb = wrap ? first_b : 0;
+          me = wrap ? first_e : me + 1;
+        }
+      }
+  }
+  sum_wavefronts<NW>(sum, smem, wave, lane, [&](int unit, const f32x4 (&v)[1]) {
+    const int n = unit / MT, t = 16 * (unit - n * MT) + r16, first = (tile + n) * Q4_TILE + 4 * kg;
+    if (t >= a.M || first >= a.K) return;
+    if (gridDim.y > 1) {
+      *(f32x4*)(a.partial + ((size_t)blockIdx.y * a.M + t) * a.K + first) = v[0];
+      return;
+    }
+    float y[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+    if (a.bias[2]) add_w<T, 4>((const T*)a.bias[2] + first, y);
+    store_w<T, 4>((T*)a.y + (size_t)t * a.K + first, y);
+  });
+}
+
+// Second stage of a down projection whose reduction was split over workgroups: the parts' sums, in their order.
+template <typename T>
+__global__ void __launch_bounds__(256) experts_join_kernel(ExpertArgs a, int parts) {
+  const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)a.M * a.K;
+  if (i >= all) return;
+  f32x4 v = *(const f32x4*)(a.partial + i);
+  for (int p = 1; p < parts; ++p) v += *(const f32x4*)(a.partial + p * all + i);
+  float y[4] = {v[0], v[1], v[2], v[3]};
+  if (a.bias[2]) add_w<T, 4>((const T*)a.bias[2] + i % a.K, y);
+  store_w<T, 4>((T*)a.y + i, y);
+}
+
+// Experts that a call can use.
+static int experts_at_most(const ExpertArgs& a) { return a.E < a.M * a.top_k ? a.E : a.M * a.top_k; }
+static double weight_bytes(const ExpertArgs& a, int group) {
+  return (double)experts_at_most(a) * a.K * a.N * (group ? 0.5 + 2.0 / group : 2.0);
+}
+
+template <typename T, int G, int MT, int XR, int R, int NW, int D>
+static hipError_t run_gateup(const ExpertArgs& a, hipStream_t s) {
+  constexpr int LDS = gateup_lds<T, G, MT, XR, R, NW>();
+  static_assert(LDS <= 64 * 1024, "what a launch may ask for without ado");
+  const int strips = (a.N + R * Q4_TILE - 1) / (R * Q4_TILE);
+  hipLaunchKernelGGL((experts_gateup_kernel<T, G, MT, XR, R, NW, D>), dim3((unsigned)(strips * experts_at_most(a))), dim3(NW * 64), LDS, s,
+                     a);
+  return hipGetLastError();
+}
+template <typename T, int G, int MT, int XR, int R, int NW, int D>
+static hipError_t run_down(const ExpertArgs& a, int parts, hipStream_t s) {
+  constexpr int LDS = down_lds<T, G, MT, XR, R, NW>();
+  const int tables = a.routing == ROUTING_DENSE ? 0 : experts_at_most(a) * (4 + EXPERTS_MAX_M) + a.M * a.top_k * 4;
+  constexpr auto kern = experts_down_kernel<T, G, MT, XR, R, NW, D>;
+  if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, LDS + EX_TABLES>, s)) return e;
+  const dim3 grid((unsigned)((a.K + R * Q4_TILE - 1) / (R * Q4_TILE)), (unsigned)parts);
+  hipLaunchKernelGGL(kern, grid, dim3(NW * 64), (unsigned)(LDS + tables), s, a);
+  if (hipError_t e = hipGetLastError()) return e;
+  if (parts > 1) hipLaunchKernelGGL(experts_join_kernel<T>, dim3((unsigned)(((int64_t)a.M * a.K / 4 + 255) / 256)), dim3(256), 0, s, a, parts);
+  return hipGetLastError();
+}
+
+// Gate/up.
+template <typename T, int G>
+static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
+  if constexpr (G == 0) {
+    if (a.M <= 8) return run_gateup<T, 0, 1, 1, 1, 4, 2>(a, s);
+    if (a.M <= 16) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
+    return run_gateup<T, 0, 2, 2, 2, 4, 1>(a, s);
+  } else {
+  const bool few = (a.N + Q4_TILE - 1) / Q4_TILE * experts_at_most(a) <= 4 * a.cus;
+  if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 1>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 1>(a, s);
+  if (a.M <= 16) return few ? run_gateup<T, G, 1, 4, 1, 4, 1>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
+  if (a.M <= 32) return run_gateup<T, G, 2, 4, 2, 4, 1>(a, s);
+  if (a.M <= 48) return run_gateup<T, G, 3, 4, 1, 4, 1>(a, s);
+  return run_gateup<T, G, 4, 4, 1, 4, 1>(a, s);
+  }
+}
+
+// Down: tiles of a workgroup, and workgroups that share a strip of them.
+constexpr int DOWN_MAX_PARTS = 8;
+struct DownPlan {
+  int tiles, parts;
+};
+static DownPlan plan_down(const ExpertArgs& a, int group) {
+  const bool large = weight_bytes(a, group) >= 48e6;
+  const int tiles = (a.K + Q4_TILE - 1) / Q4_TILE;
+  DownPlan p = {a.M > 48 && group == 32 ? 1 : a.M > 16 ? 2 : large ? (group && a.M > 4 ? 4 : 2) : group && tiles > 2 * a.cus ? 2 : 1, 1};
+  const int strips = (tiles + p.tiles - 1) / p.tiles;
+  if (a.M > 16 || large) {
+    p.parts = a.cus / strips < 1 ? 1 : a.cus / strips;
+    if (p.parts > DOWN_MAX_PARTS) p.parts = DOWN_MAX_PARTS;
+  }
+  return p;
+}
+size_t experts_partial_bytes(const ExpertArgs& a, int group) {
+  const int parts = plan_down(a, group).parts;
+  return parts > 1 ? (size_t)parts * a.M * a.K * sizeof(float) : 0;
+}
+template <typename T, int G>
+static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
+  const DownPlan p = plan_down(a, G);
+  const int parts = a.partial ? p.parts : 1;
+  constexpr int FEW = G ? 4 : 8, ALL = 16 / FEW;
+  const bool few = a.M <= FEW;
+  if (a.M > 48) return run_down<T, G, 4, ALL, G == 32 ? 1 : 2, 4, 1>(a, parts, s);  // (two tiles of the finest groups would spill)
+  if (a.M > 32) return run_down<T, G, 3, ALL, 2, 4, 1>(a, parts, s);
+  if (a.M > 16) return run_down<T, G, 2, ALL, 2, 8, 1>(a, parts, s);
+  if (p.tiles == 1) {
+    const int blocks = (a.N + Block<T, G, 1, 1, 1>::COLS - 1) / Block<T, G, 1, 1, 1>::COLS * experts_at_most(a);
+    if (blocks >= 32) return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
+    return few ? run_down<T, G, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s);
+  }
+  if constexpr (G != 0)
+    if (p.tiles == 4) return run_down<T, G, 1, ALL, 4, 8, 1>(a, parts, s);
+  return few ? run_down<T, G, 1, 1, 2, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 2, 8, 1>(a, parts, s);
+}
+bool experts_solo(const ExpertArgs& a) { return a.M == 1 && a.E <= SOLO_MAX_E; }
+
+template <typename T>
+hipError_t launch_experts_gateup(const ExpertArgs& a, int group, hipStream_t s) {
+  switch (group) {
+    case 0: return gateup_of<T, 0>(a, s);
+    case 32: return gateup_of<T, 32>(a, s);
+    case 64: return gateup_of<T, 64>(a, s);
+    default: return gateup_of<T, 128>(a, s);
+  }
+}
+template <typename T>
+hipError_t launch_experts_down(const ExpertArgs& a, int group, hipStream_t s) {
+  switch (group) {
+    case 0: return down_of<T, 0>(a, s);
+    case 32: return down_of<T, 32>(a, s);
+    case 64: return down_of<T, 64>(a, s);
+    default: return down_of<T, 128>(a, s);
+  }
+}
+
+// ------------------------------------------------------------------ routing
 template <int VPL, typename L>
 __global__ void __launch_bounds__(256) route_kernel(const L* logits, float* weights, int64_t* experts, int64_t M, int E, int top_k,
                                                     int normalize) {
@@ -492,7 +728,7 @@ __global__ void __launch_bounds__(256) route_kernel(const L* logits, float* weig
   if (t >= M) return;
   int e;
   float w;
-  choose<VPL>(logits + t * E, E, top_k, normalize != 0, lane, e, w);
+  choose<VPL>([&](int i) { return (float)logits[t * E + i]; }, E, top_k, normalize != 0, lane, e, w);
   if (lane < top_k) {
     weights[t * top_k + lane] = w;
     experts[t * top_k + lane] = e < 0 ? -1 - e : e;
@@ -512,7 +748,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const L* logits, ExpertPlan 
   for (int t = wave; t < M; t += 16) {
     int e;
     float w;
-    choose<VPL>(logits + (size_t)t * E, E, top_k, normalize != 0, lane, e, w);
+    choose<VPL>([&](int i) { return (float)logits[(size_t)t * E + i]; }, E, top_k, normalize != 0, lane, e, w);
     if (lane < top_k) {
       p.weight[t * top_k + lane] = w;
       chosen[t * top_k + lane] = (short)e;

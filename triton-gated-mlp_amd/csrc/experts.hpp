@@ -6,6 +6,7 @@ namespace gmlp {
 
 constexpr int Q4_TILE = 16;          // weight rows of a tile
 constexpr int Q4_BLOCK = 128;        // weight columns of a block
+constexpr uint32_t EXPERTS_MAX_BYTES = 0x7fff0000u;  // a buffer descriptor of these kernels is shorter
 constexpr int EXPERTS_MAX_M = 64;    // token rows of a call
 constexpr int EXPERTS_MAX_E = 512;   // experts
 constexpr int EXPERTS_MAX_K = 16;    // experts of a token
@@ -25,16 +26,28 @@ struct ExpertPlan {
   float* weight;    // [M * top_k]
 };
 
+// Who runs through which expert: every token through the only one, with weight 1; as the plan says; or, of one token, as each
+// kernel finds from the logits itself.
+enum Routing : int { ROUTING_DENSE = 0, ROUTING_PLAN = 1, ROUTING_SOLO = 2 };
+
 struct ExpertArgs {
   const void* x;      // [M, K]
   const void* bias[3];
   ExpertWeights gate, up, down;
   void* h;            // [M * top_k, N]
   void* y;            // [M, K]
+  float* partial;     // [parts][M, K], where the down projection's reduction is split
   int M, K, N, E, top_k, act;
-  int dense;          // one expert, every token's, with weight 1: plan is not read
+  int routing;        // Routing
+  int cus;            // compute units of the device
+  const void* logits; // [M, E] of a GMLP_* type
+  int logits_dtype, normalize;
   ExpertPlan plan;
 };
+
+// Whether ROUTING_SOLO takes the call, and the bytes of `partial` that launch_experts_down asks for (it does with none).
+bool experts_solo(const ExpertArgs& a);
+size_t experts_partial_bytes(const ExpertArgs& a, int group);
 
 // Gate/up, then down, on 16-bit (group = 0) or 4-bit weights (group = 32, 64 or 128).
 template <typename T>

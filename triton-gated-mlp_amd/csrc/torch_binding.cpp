@@ -42,7 +42,7 @@ typedef std::optional<Tensor> OptTensor;
 #define GMLP_ENTRY_POINTS(X)                                                                     \
   X(gmlp_last_error) X(gmlp_workspace_bytes) X(gmlp_mlp_workspace_bytes) X(gmlp_mlp_fwd)         \
   X(gmlp_mlp_bwd) X(gmlp_gateup_fwd) X(gmlp_decode_fwd) X(gmlp_decode_stream_fwd) X(gmlp_hidden_bwd) \
-  X(gmlp_grads_workspace_bytes) X(gmlp_linear_fwd) X(gmlp_q4_quantize) X(gmlp_q4_dequantize) X(gmlp_q4_linear_fwd) \
+  X(gmlp_grads_workspace_bytes) X(gmlp_linear_fwd) X(gmlp_q4_quantize) X(gmlp_q4_dequantize) X(gmlp_q4_workspace_bytes) X(gmlp_q4_linear_fwd) \
   X(gmlp_q4_mlp_fwd) X(gmlp_moe_route) X(gmlp_moe_workspace_bytes) X(gmlp_moe_fwd)
 struct Library {
 #define GMLP_MEMBER(name) decltype(&::name) name = nullptr;
@@ -547,7 +547,10 @@ Tensor q4_linear(const Tensor& x_in, const Q4& q, const OptTensor& bias_in) {
   const Tensor y = at::empty(sizes, x.options());
   if (M == 0) return y;
   if (M <= FEW_ROWS) {
-    check(lib.gmlp_q4_linear_fwd(ptr(x), ptr(w.codes), ptr(w.scales), ptr(b), out_ptr(y), M, R, C, w.group, code, stream_of(x)));
+    const size_t bytes = lib.gmlp_q4_workspace_bytes(M, R, C, w.group, code);
+    const Tensor ws = scratch(bytes, x);
+    check(lib.gmlp_q4_linear_fwd(ptr(x), ptr(w.codes), ptr(w.scales), ptr(b), out_ptr(y), M, R, C, w.group, code, out_ptr(ws), bytes,
+                                 stream_of(x)));
     return y;
   }
   const Tensor dense = w.dense(code);
@@ -575,9 +578,14 @@ Tensor q4_mlp(const Tensor& x_in, const Q4& gate, const OptTensor& bg_in, const 
   const Tensor y = at::empty(x.sizes(), x.options());
   if (M == 0) return y;
   if (M <= FEW_ROWS) {
-    const Tensor h = at::empty({M, N}, x.options());
+    // the hidden states and the workspace in one allocation
+    const size_t plane = ((size_t)(M * N) * x.element_size() + 255) / 256 * 256;
+    const size_t bytes = lib.gmlp_q4_workspace_bytes(M, N, K, wg.group, code);
+    const Tensor arena = scratch(plane + bytes, x);
+    char* const h = (char*)out_ptr(arena);
     check(lib.gmlp_q4_mlp_fwd(ptr(x), ptr(wg.codes), ptr(wg.scales), ptr(wu.codes), ptr(wu.scales), ptr(wd.codes), ptr(wd.scales),
-                              ptr(bg), ptr(bu), ptr(bd), out_ptr(h), out_ptr(y), M, K, N, wg.group, code, (int)act, stream_of(x)));
+                              ptr(bg), ptr(bu), ptr(bd), h, out_ptr(y), M, K, N, wg.group, code, (int)act, bytes ? h + plane : nullptr,
+                              bytes, stream_of(x)));
     return y;
   }
   return mlp_infer(x, wg.dense(code), bg.defined() ? OptTensor(bg) : OptTensor(), wu.dense(code),
@@ -635,6 +643,13 @@ std::tuple<Tensor, Tensor> moe_route(const Tensor& logits_in, int64_t top_k, boo
   return {weights, experts};
 }
 
+// (The last piece of a batch may ask for more than the others: fewer experts in use, another split.)
+size_t moe_workspace(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group, int code) {
+  size_t bytes = lib.gmlp_moe_workspace_bytes(std::min(M, FEW_ROWS), K, N, E, top_k, group, code);
+  if (M > FEW_ROWS && M % FEW_ROWS != 0)
+    bytes = std::max(bytes, lib.gmlp_moe_workspace_bytes(M % FEW_ROWS, K, N, E, top_k, group, code));
+  return bytes;
+}
 // gate, up, down: pointers to the experts' weights, and to their scales
 Tensor moe_rows(const Tensor& x_in, const Tensor& logits_in, int code, int logits_code, const void* const (&w)[3],
                 const void* const (&sc)[3], int64_t N, int64_t E, int64_t top_k, bool normalize, int group, int64_t act) {
@@ -642,7 +657,7 @@ Tensor moe_rows(const Tensor& x_in, const Tensor& logits_in, int code, int logit
   const int64_t K = x.size(-1), M = K > 0 ? x.numel() / K : 0;
   const Tensor y = at::empty(x.sizes(), x.options());
   if (M == 0) return y;
-  const size_t bytes = lib.gmlp_moe_workspace_bytes(std::min(M, FEW_ROWS), N, E, top_k, code);
+  const size_t bytes = moe_workspace(M, K, N, E, top_k, group, code);
   const Tensor ws = scratch(bytes, x);
   // A longer batch goes through in pieces of as many rows as a call takes, one behind the other on the stream.
   for (int64_t m = 0; m < M; m += FEW_ROWS)
