@@ -1663,6 +1663,7 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
     if (hipError_t e = gmlp::launch_experts_gateup<T>(a, group, s)) return e;
+    if (a.routing == gmlp::ROUTING_SOLO) a.routing = gmlp::ROUTING_PLAN;  // which gate/up has left
     return gmlp::launch_experts_down<T>(a, group, s);
   }));
 }

@@ -15,6 +15,7 @@
 #include "experts.hpp"
 
 #include "launch.hpp"
+#include "lds_dma.hpp"
 
 namespace gmlp {
 
@@ -170,8 +171,8 @@ __device__ __forceinline__ void choose(F&& logit, int E, int top_k, bool normali
   if (own == -__builtin_inff()) expert = -1 - expert;
 }
 
-// The routing of the only token of a call, in every wavefront of both kernels: a launch less, and 1 us against the 4 that the
-// launch and its kernel take.
+// The routing of the only token of a call: every wavefront of gate/up finds it from the logits, and one leaves the plan for
+// down.  A launch less, and 1 us in the place of 4.
 constexpr int SOLO_MAX_E = 256;
 __device__ __forceinline__ void choose_solo(const ExpertArgs& a, int lane, int& expert, float& weight) {
   auto logit = [&](int i) -> float {
@@ -181,6 +182,18 @@ __device__ __forceinline__ void choose_solo(const ExpertArgs& a, int lane, int& 
   };
   if (a.E <= 64) choose<1>(logit, a.E, a.top_k, a.normalize != 0, lane, expert, weight);
   else choose<SOLO_MAX_E / 64>(logit, a.E, a.top_k, a.normalize != 0, lane, expert, weight);
+}
+
+__device__ __forceinline__ void leave_plan(const ExpertArgs& a, int lane, int expert, float weight) {
+  const uint64_t chosen = __ballot(lane < a.top_k && expert >= 0);
+  if (lane == 0) a.plan.active[0] = __popcll(chosen);
+  if (lane >= a.top_k) return;
+  a.plan.weight[lane] = weight;
+  if (expert >= 0) {
+    const int i = __popcll(chosen & ((1ull << lane) - 1));
+    a.plan.active[1 + i] = expert;
+    a.plan.slot[i * EXPERTS_MAX_M] = (int8_t)lane;
+  }
 }
 
 // ------------------------------------------------------------------ a block of the reduction
@@ -200,12 +213,16 @@ struct Block {
   static constexpr int ROWS = 64 / PIECES;      // rows of a load
   static constexpr int WL = G ? 1 : 16 / ROWS;  // loads of a weight tile
   static constexpr int TILE = 16 * COLS * 2;    // bytes of a tile in LDS
-  static constexpr int XB = MT < 2 ? MT : 2, WB = G ? 0 : NT < 4 ? NT : 4;  // tiles in LDS at a time
-  static constexpr int LDS = (XB + WB) * TILE;  // of a wavefront
+  static constexpr int WB = G ? 0 : NT < 4 ? NT : 4;  // weight tiles in LDS at a time
+  // 4-bit weights: token rows go to LDS without passing through registers (buffer_load ... lds), a slot for each stage; two
+  // stages of the weights then fit where one of both did.  16-bit: one slot for what the wavefront multiplies.
+  static constexpr bool DMA = G != 0;
+  static constexpr int SLOT = (MT + WB) * TILE;
+  static constexpr int lds_bytes(int depth) { return (DMA ? depth : 1) * SLOT; }  // of a wavefront
   static_assert(XR * ROWS <= 16, "a token tile has 16 rows");
   u32x4 w[NT][WL];
   u32x2 sc[NT][GROUPS];
-  u32x4 x[MT][XR];
+  u32x4 x[DMA ? 1 : MT][DMA ? 1 : XR];
 
   // from tile `tile` of an expert's matrix on, of `rows` x `cols`: `tiles` of them
   static __device__ __forceinline__ ex_rsrc weights_of(const ExpertWeights& m, int expert, int tile, int tiles, int rows, int cols) {
@@ -223,7 +240,9 @@ struct Block {
   }
   // Row of a tile and byte in the row's segment that a lane loads.
   static __device__ __forceinline__ int load_row(int i, int lane) { return i * ROWS + lane / PIECES; }
-  static __device__ __forceinline__ uint32_t load_byte(int lane) { return (uint32_t)(lane % PIECES) * 16u; }
+  // (DMA fills LDS in the order of the lanes: the lane loads the piece that `at` has in its place)
+  static __device__ __forceinline__ int load_piece(int i, int lane) { return DMA ? lane % PIECES ^ load_row(i, lane) : lane % PIECES; }
+  static __device__ __forceinline__ uint32_t load_byte(int i, int lane) { return (uint32_t)load_piece(i, lane) * 16u; }
   // Byte in LDS of a row's piece.  256-byte rows reach all banks, 128-byte ones two by two.
   static __device__ __forceinline__ uint32_t at(int row, int piece) {
     return (uint32_t)(row * PIECES + (piece ^ (PIECES == 16 ? row : row >> 1))) * 16u;
@@ -236,31 +255,43 @@ struct Block {
       w[n][0] = ex_load16<EX_STREAM>(rw, (uint32_t)lane * 16u, ok ? unit * 1024u : EX_PAST);
       const uint32_t from = ok ? unit * (GROUPS * 32u) : EX_PAST, own = (uint32_t)(lane >> 4) * (GROUPS * 8u);
       if constexpr (GROUPS == 1) {
-        sc[n][0] = ex_load8<EX_STREAM>(rs, own, from);
+        sc[n][0] = ex_load8(rs, own, from);
       } else {
 #pragma unroll
         for (int g = 0; g < GROUPS; g += 2) {
-          const u32x4 v = ex_load16<EX_STREAM>(rs, own + (uint32_t)g * 8u, from);
+          const u32x4 v = ex_load16(rs, own + (uint32_t)g * 8u, from);
           sc[n][g] = u32x2{v[0], v[1]};
           sc[n][g + 1] = u32x2{v[2], v[3]};
         }
       }
     } else {
-      const uint32_t lane_off = tail && beyond(kb, cols, lane) ? EX_NOWHERE : (uint32_t)load_row(0, lane) * (uint32_t)cols * 2u + load_byte(lane);
+      const uint32_t lane_off = tail && beyond(kb, cols, 0, lane) ? EX_NOWHERE : (uint32_t)load_row(0, lane) * (uint32_t)cols * 2u + load_byte(0, lane);
 #pragma unroll
       for (int i = 0; i < WL; ++i)
         w[n][i] = ex_load16<EX_STREAM>(rw, lane_off, ok ? ((uint32_t)(r * Q4_TILE + i * ROWS) * (uint32_t)cols + (uint32_t)(kb * COLS)) * 2u : EX_PAST);
     }
   }
-  static __device__ __forceinline__ bool beyond(int kb, int cols, int lane) { return kb * COLS + lane % PIECES * 8 >= cols; }
-  // row[m][i]: byte offset of the lane's piece of its token row, or EX_NOWHERE
-  __device__ __forceinline__ void load_tokens(ex_rsrc rx, const uint32_t (&row)[MT][XR], int kb, bool ok, bool tail, int cols, int lane) {
-    const bool skip = tail && beyond(kb, cols, lane);
+  // (What goes into scalar operands of inline assembly has to be known to be uniform.)
+  static __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+  static __device__ __forceinline__ buffer_rsrc uniform_rsrc(const void* p, uint32_t bytes) {
+    buffer_rsrc r = make_rsrc(p, bytes);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) r[i] = __builtin_amdgcn_readfirstlane(r[i]);
+    return r;
+  }
+  static __device__ __forceinline__ bool beyond(int kb, int cols, int i, int lane) { return kb * COLS + load_piece(i, lane) * 8 >= cols; }
+  // row[m][i]: byte offset of the lane's piece of its token row, or EX_NOWHERE; slot: LDS of the stage (DMA)
+  __device__ __forceinline__ void load_tokens(const void* tokens, uint32_t bytes, const uint32_t (&row)[MT][XR], int kb, bool ok, bool tail,
+                                              int cols, int lane, uint32_t slot) {
     const uint32_t from = ok ? (uint32_t)(kb * COLS) * 2u : EX_PAST;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int i = 0; i < XR; ++i) x[m][i] = ex_load16(rx, skip ? EX_NOWHERE : row[m][i], from);
+      for (int i = 0; i < XR; ++i) {
+        const uint32_t lane_off = tail && beyond(kb, cols, i, lane) ? EX_NOWHERE : row[m][i];
+        if constexpr (DMA) load16_to_lds(uniform_rsrc(tokens, bytes), lane_off, uniform(from), uniform(slot + (uint32_t)(m * TILE + i * 1024)));
+        else x[m][i] = ex_load16(ex_make_rsrc(tokens, bytes), lane_off, from);
+      }
   }
 
   // Columns of a tile: step s takes 32 s + 8 (lane / 16) + 0..7.  (Token rows that XR leaves out are whatever LDS holds: their
@@ -273,23 +304,26 @@ struct Block {
 #pragma unroll
     for (int i = 0; i < L; ++i) *(u32x4*)(tile + at(load_row(i, lane), lane % PIECES)) = v[i];
   }
-  __device__ __forceinline__ void multiply(const Int4<T>& int4, char* lds, int lane, f32x4 (&acc)[NT][MT]) const {
+  __device__ __forceinline__ void multiply(const Int4<T>& int4, char* slot, int lane, f32x4 (&acc)[NT][MT]) {
     vec8 xf[MT][STEPS];
+    if constexpr (DMA) {
+      // The token rows were asked for ahead of the weights and scales, and loads return in order: once the last scale is there
+      // (the compiler waits for it here, it goes into the statement), they are in LDS.
+      asm volatile("" : "+v"(sc[NT - 1][GROUPS - 1]) : : "memory");
+    } else {
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      char* const tile = lds + (m % XB) * TILE;
-      to_lds(tile, x[m], lane);
-      __builtin_amdgcn_wave_barrier();
+      for (int m = 0; m < MT; ++m) to_lds(slot + m * TILE, x[m], lane);
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) xf[m][s] = operand(tile, s, lane);
+      for (int n = 0; n < WB; ++n) to_lds(slot + (MT + n) * TILE, w[n], lane);
       __builtin_amdgcn_wave_barrier();
     }
-    if (!G)
 #pragma unroll
-      for (int n = 0; n < WB; ++n) to_lds(lds + (XB + n) * TILE, w[n], lane);
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) xf[m][s] = operand(slot + m * TILE, s, lane);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      if (G) {
+      if constexpr (G != 0) {
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
           f32x4 part[MT];
@@ -309,20 +343,33 @@ struct Block {
           }
         }
       } else {
-        char* const tile = lds + (XB + n % (WB ? WB : 1)) * TILE;
-        if (n >= WB) to_lds(tile, w[n], lane);
-        __builtin_amdgcn_wave_barrier();
+        char* const tile = slot + (MT + n % WB) * TILE;
+        if (n >= WB) {
+          __builtin_amdgcn_wave_barrier();
+          to_lds(tile, w[n], lane);
+          __builtin_amdgcn_wave_barrier();
+        }
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) {
           const vec8 a = operand(tile, s, lane);
 #pragma unroll
           for (int m = 0; m < MT; ++m) acc[n][m] = Traits<T>::mfma16(a, xf[m][s], acc[n][m]);
         }
-        __builtin_amdgcn_wave_barrier();
       }
     }
+    if constexpr (DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
+    else __builtin_amdgcn_wave_barrier();
   }
 };
+
+// f(0), f(1), ... f(D - 1), each a constant
+template <int D, int AT = 0, typename F>
+__device__ __forceinline__ void each_stage(F&& f) {
+  if constexpr (AT < D) {
+    f(std::integral_constant<int, AT>{});
+    each_stage<D, AT + 1>(f);
+  }
+}
 
 // Adds up the wavefronts' sums, a few units of U vectors at a time through LDS, and calls done(unit, sums) for each in one
 // wavefront.
@@ -358,9 +405,9 @@ __device__ __forceinline__ void sum_wavefronts(const f32x4 (&acc)[NU][U], char* 
 }
 
 // ------------------------------------------------------------------ gate/up
-template <typename T, int G, int MT, int XR, int R, int NW>
+template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int gateup_lds() {
-  constexpr int ring = NW * Block<T, G, 2 * R, MT, XR>::LDS, part = NW * units_at_a_time<NW, R * MT, 2>() * 2 * 1024;
+  constexpr int ring = NW * Block<T, G, 2 * R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 2>() * 2 * 1024;
   return ring > part ? ring : part;
 }
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
@@ -377,13 +424,13 @@ __global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
     float w;
     choose_solo(a, lane, e, w);
     expert = __builtin_amdgcn_readlane(e, slot);
+    if (blockIdx.x == 0 && wave == 0) leave_plan(a, lane, e, w);
     if (expert < 0) return;
   } else if (a.routing == ROUTING_PLAN) {
     if (slot >= a.plan.active[0]) return;
     expert = a.plan.active[1 + slot];
     count = a.plan.count[slot];
   }
-  const ex_rsrc rx = ex_make_rsrc(a.x, (uint32_t)a.M * (uint32_t)a.K * 2u);
   const ex_rsrc rw[2] = {B::weights_of(a.gate, expert, tile, R, a.N, a.K), B::weights_of(a.up, expert, tile, R, a.N, a.K)};
   const ex_rsrc rs[2] = {B::scales_of(a.gate, expert, tile, R, a.N, a.K), B::scales_of(a.up, expert, tile, R, a.N, a.K)};
   const int blocks = (a.K + B::COLS - 1) / B::COLS;
@@ -391,7 +438,8 @@ __global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
   const int rot = run > 1 ? (int)blockIdx.x % run : 0;
   const bool ragged = a.K % B::COLS != 0;
   const Int4<T> int4;
-  char* const lds = smem + wave * B::LDS;
+  char* const lds = smem + wave * B::lds_bytes(D);
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void*)lds;
 
   for (int base = 0; base < count; base += 16 * MT) {
     uint32_t row[MT][XR];
@@ -401,20 +449,20 @@ __global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
       for (int i = 0; i < XR; ++i) {
         const int j = base + 16 * m + B::load_row(i, lane);
         const int t = j >= count ? 0 : a.routing == ROUTING_PLAN ? a.plan.tokens[slot * EXPERTS_MAX_M + j] : j;
-        row[m][i] = j < count ? (uint32_t)t * (uint32_t)a.K * 2u + B::load_byte(lane) : EX_NOWHERE;
+        row[m][i] = j < count ? (uint32_t)t * (uint32_t)a.K * 2u + B::load_byte(i, lane) : EX_NOWHERE;
       }
     B st[D];
-    auto load_block = [&](B& b, int kb, bool ok, bool tail) {
+    auto load_block = [&](B& b, int kb, bool ok, bool tail, int d) {
+      b.load_tokens(a.x, (uint32_t)a.M * (uint32_t)a.K * 2u, row, kb, ok, tail, a.K, lane, lds_at + (uint32_t)(d * B::SLOT));
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int n = 0; n < 2; ++n) b.load_weights(2 * r + n, r, rw[n], rs[n], kb, ok, tail, a.K, lane);
-      b.load_tokens(rx, row, kb, ok, tail, a.K, lane);
     };
-    auto load = [&](B& b, int i) {
+    auto load = [&](B& b, int i, int d) {
       const int kb = b0 + (i + rot < run ? i + rot : i + rot - run);
-      if (ragged && kb + 1 == blocks) load_block(b, kb, i < run, true);
-      else load_block(b, kb, i < run, false);
+      if (ragged && kb + 1 == blocks) load_block(b, kb, i < run, true, d);
+      else load_block(b, kb, i < run, false, d);
     };
     f32x4 acc[2 * R][MT];
 #pragma unroll
@@ -423,13 +471,17 @@ __global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
       for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
     if (base > 0) __syncthreads();  // the readers of the sums before
 #pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], d);
-    for (int i = 0; i < run; i += D)
+    for (int d = 0; d < D; ++d) load(st[d], d, d);
+    int i = 0;
+    for (; i + D < run; i += D)
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        st[d].multiply(int4, lds, lane, acc);
-        load(st[d], i + d + D);
+        st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
+        load(st[d], i + d + D, d);
       }
+    each_stage<D>([&](auto d) {
+      if (i + d < run) st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
+    });
     f32x4 both[R * MT][2];
 #pragma unroll
     for (int i = 0; i < R * MT; ++i)
@@ -463,9 +515,9 @@ __global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
 // The blocks of all experts in use, one expert behind the other, are shared out evenly over the wavefronts.  What an
 // expert gives is added to a token's sum only where the token chose it (a weight that is not finite in one
 // expert stays out of the others' tokens).
-template <typename T, int G, int MT, int XR, int R, int NW>
+template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int down_lds() {
-  constexpr int ring = NW * Block<T, G, R, MT, XR>::LDS, part = NW * units_at_a_time<NW, R * MT, 1>() * 1024;
+  constexpr int ring = NW * Block<T, G, R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 1>() * 1024;
   return ring > part ? ring : part;
 }
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
@@ -477,34 +529,20 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
   const int pairs = a.M * a.top_k;
   // tables: the experts' numbers, the pairs' weights, the slots
   int in_use = 1;
-  int* const numbers = (int*)(smem + down_lds<T, G, MT, XR, R, NW>());
+  int* const numbers = (int*)(smem + down_lds<T, G, MT, XR, R, NW, D>());
   float* weight = nullptr;
   int8_t* slots = nullptr;
-  if (a.routing == ROUTING_SOLO) {
-    int e;
-    float w;
-    choose_solo(a, lane, e, w);
-    const uint64_t chosen = __ballot(lane < pairs && e >= 0);
-    in_use = __popcll(chosen);
-    weight = (float*)(numbers + in_use);
-    slots = (int8_t*)(weight + pairs);
-    if (wave == 0 && lane < pairs) {
-      const int i = __popcll(chosen & ((1ull << lane) - 1));
-      weight[lane] = w;
-      if (e >= 0) numbers[i] = e, slots[i * EXPERTS_MAX_M] = (int8_t)lane;
-    }
-    __syncthreads();
-  } else if (a.routing == ROUTING_PLAN) {
+  if (a.routing == ROUTING_PLAN) {
     in_use = a.plan.active[0];
-    weight = (float*)(numbers + in_use);
+    const int rows = a.M == 1 ? pairs : in_use;  // (all there can be: their loads do not wait for the number)
+    weight = (float*)(numbers + rows);
     slots = (int8_t*)(weight + pairs);
-    for (int i = threadIdx.x; i < in_use; i += NW * 64) numbers[i] = a.plan.active[1 + i];
+    for (int i = threadIdx.x; i < rows; i += NW * 64) numbers[i] = a.plan.active[1 + i];
     for (int i = threadIdx.x; i < pairs; i += NW * 64) weight[i] = a.plan.weight[i];
-    for (int i = threadIdx.x; i < in_use * (EXPERTS_MAX_M / 4); i += NW * 64)
+    for (int i = threadIdx.x; i < rows * (EXPERTS_MAX_M / 4); i += NW * 64)
       ((int*)slots)[i] = ((const int*)a.plan.slot)[i];
     __syncthreads();
   }
-  const ex_rsrc rh = ex_make_rsrc(a.h, (uint32_t)pairs * (uint32_t)a.N * 2u);
   const int blocks = (a.N + B::COLS - 1) / B::COLS;
   const int total = in_use * blocks;
   const int parts = NW * (int)gridDim.y, me_part = (int)blockIdx.y * NW + wave;
@@ -512,7 +550,8 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
   const int rot = run > 1 ? (int)blockIdx.x % run : 0;
   const bool ragged = a.N % B::COLS != 0;
   const Int4<T> int4;
-  char* const lds = smem + wave * B::LDS;
+  char* const lds = smem + wave * B::lds_bytes(D);
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void*)lds;
 
   // choice of token row t that expert e is, or -1
   auto slot_of = [&](int e, int t) -> int {
@@ -534,7 +573,7 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
 #pragma unroll
       for (int i = 0; i < XR; ++i) {
         const int t = 16 * m + B::load_row(i, lane), s = slot_of(e, t);
-        row[m][i] = s < 0 ? EX_NOWHERE : (uint32_t)(t * a.top_k + s) * (uint32_t)a.N * 2u + B::load_byte(lane);
+        row[m][i] = s < 0 ? EX_NOWHERE : (uint32_t)(t * a.top_k + s) * (uint32_t)a.N * 2u + B::load_byte(i, lane);
       }
   };
   f32x4 acc[R][MT], sum[R * MT][1];
@@ -545,14 +584,14 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
   if (run > 0) {
     enter();
     B st[D];
-    auto load_block = [&](B& b, bool ok, bool tail) {
+    auto load_block = [&](B& b, bool ok, bool tail, int d) {
+      b.load_tokens(a.h, (uint32_t)pairs * (uint32_t)a.N * 2u, row, lb, ok, tail, a.N, lane, lds_at + (uint32_t)(d * B::SLOT));
 #pragma unroll
       for (int n = 0; n < R; ++n) b.load_weights(n, n, rw, rs, lb, ok, tail, a.N, lane);
-      b.load_tokens(rh, row, lb, ok, tail, a.N, lane);
     };
-    auto load = [&](B& b, int i) {
-      if (ragged && lb + 1 == blocks) load_block(b, i < run, true);
-      else load_block(b, i < run, false);
+    auto load = [&](B& b, int i, int d) {
+      if (ragged && lb + 1 == blocks) load_block(b, i < run, true, d);
+      else load_block(b, i < run, false, d);
       const bool wrap = i + 1 == run - rot;
       if (++lb == blocks || wrap) {
         lb = wrap ? first_b : 0;
@@ -576,19 +615,29 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
       }
     };
 #pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], d);
-    for (int i = 0; i < run; i += D)
+    for (int d = 0; d < D; ++d) load(st[d], d, d);
+    auto leave = [&](int i) {  // behind the products of block i
+      const bool wrap = i + 1 == run - rot;
+      if (++mb == blocks || wrap || i + 1 == run) {
+        fold();
+        mb = wrap ? first_b : 0;
+        me = wrap ? first_e : me + 1;
+      }
+    };
+    int i = 0;
+    for (; i + D < run; i += D)
 #pragma unroll
       for (int d = 0; d < D; ++d) {
-        st[d].multiply(int4, lds, lane, acc);
-        load(st[d], i + d + D);
-        const bool wrap = i + d + 1 == run - rot;
-        if (++mb == blocks || wrap || i + d + 1 == run) {
-          if (i + d < run) fold();
-          mb = wrap ? first_b : 0;
-          me = wrap ? first_e : me + 1;
-        }
+        st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
+        load(st[d], i + d + D, d);
+        leave(i + d);
       }
+    each_stage<D>([&](auto d) {
+      if (i + d < run) {
+        st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
+        leave(i + d);
+      }
+    });
   }
   sum_wavefronts<NW>(sum, smem, wave, lane, [&](int unit, const f32x4 (&v)[1]) {
     const int n = unit / MT, t = 16 * (unit - n * MT) + r16, first = (tile + n) * Q4_TILE + 4 * kg;
@@ -623,16 +672,17 @@ static double weight_bytes(const ExpertArgs& a, int group) {
 
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 static hipError_t run_gateup(const ExpertArgs& a, hipStream_t s) {
-  constexpr int LDS = gateup_lds<T, G, MT, XR, R, NW>();
-  static_assert(LDS <= 64 * 1024, "what a launch may ask for without ado");
+  constexpr int LDS = gateup_lds<T, G, MT, XR, R, NW, D>();
+  constexpr auto kern = experts_gateup_kernel<T, G, MT, XR, R, NW, D>;
+  if constexpr (LDS > 64 * 1024)
+    if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, LDS>, s)) return e;
   const int strips = (a.N + R * Q4_TILE - 1) / (R * Q4_TILE);
-  hipLaunchKernelGGL((experts_gateup_kernel<T, G, MT, XR, R, NW, D>), dim3((unsigned)(strips * experts_at_most(a))), dim3(NW * 64), LDS, s,
-                     a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(strips * experts_at_most(a))), dim3(NW * 64), LDS, s, a);
   return hipGetLastError();
 }
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 static hipError_t run_down(const ExpertArgs& a, int parts, hipStream_t s) {
-  constexpr int LDS = down_lds<T, G, MT, XR, R, NW>();
+  constexpr int LDS = down_lds<T, G, MT, XR, R, NW, D>();
   const int tables = a.routing == ROUTING_DENSE ? 0 : experts_at_most(a) * (4 + EXPERTS_MAX_M) + a.M * a.top_k * 4;
   constexpr auto kern = experts_down_kernel<T, G, MT, XR, R, NW, D>;
   if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, LDS + EX_TABLES>, s)) return e;
@@ -646,17 +696,19 @@ static hipError_t run_down(const ExpertArgs& a, int parts, hipStream_t s) {
 // Gate/up.
 template <typename T, int G>
 static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
+  const bool few = (a.N + Q4_TILE - 1) / Q4_TILE * experts_at_most(a) <= (a.M <= 16 ? 4 : 2) * a.cus;
   if constexpr (G == 0) {
     if (a.M <= 8) return run_gateup<T, 0, 1, 1, 1, 4, 2>(a, s);
     if (a.M <= 16) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
     return run_gateup<T, 0, 2, 2, 2, 4, 1>(a, s);
   } else {
-  const bool few = (a.N + Q4_TILE - 1) / Q4_TILE * experts_at_most(a) <= 4 * a.cus;
-  if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 1>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 1>(a, s);
-  if (a.M <= 16) return few ? run_gateup<T, G, 1, 4, 1, 4, 1>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
-  if (a.M <= 32) return run_gateup<T, G, 2, 4, 2, 4, 1>(a, s);
-  if (a.M <= 48) return run_gateup<T, G, 3, 4, 1, 4, 1>(a, s);
-  return run_gateup<T, G, 4, 4, 1, 4, 1>(a, s);
+    if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 1>(a, s);
+    if (a.M <= 16) return few ? run_gateup<T, G, 1, 4, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
+    // More than one token tile: as many tiles and wavefronts as the registers hold, fewer with finer groups.
+    constexpr bool coarse = G == 128, fine = G == 32;
+    if (a.M <= 32) return few ? run_gateup<T, G, 2, 4, 2, 8, 1>(a, s) : run_gateup<T, G, 2, 4, 3, coarse ? 8 : 4, 1>(a, s);
+    if (a.M <= 48) return few ? run_gateup<T, G, 3, 4, coarse ? 2 : 1, coarse ? 8 : 4, 1>(a, s) : run_gateup<T, G, 3, 4, fine ? 2 : 3, 4, 1>(a, s);
+    return few ? run_gateup<T, G, 4, 4, coarse ? 2 : 1, 4, 1>(a, s) : run_gateup<T, G, 4, 4, fine ? 2 : 3, 4, 1>(a, s);
   }
 }
 
@@ -668,11 +720,13 @@ struct DownPlan {
 static DownPlan plan_down(const ExpertArgs& a, int group) {
   const bool large = weight_bytes(a, group) >= 48e6;
   const int tiles = (a.K + Q4_TILE - 1) / Q4_TILE;
-  DownPlan p = {a.M > 48 && group == 32 ? 1 : a.M > 16 ? 2 : large ? (group && a.M > 4 ? 4 : 2) : group && tiles > 2 * a.cus ? 2 : 1, 1};
-  const int strips = (tiles + p.tiles - 1) / p.tiles;
+  DownPlan p = {1, 1};
+  if (a.M > 16) p.tiles = a.M > 48 && group == 32 ? 1 : 2;  // (two of the finest groups would spill)
+  else if (large) p.tiles = group && a.M > 4 ? 4 : 2;
+  else if (group && a.M > 4 && tiles > 2 * a.cus) p.tiles = 4;
   if (a.M > 16 || large) {
-    p.parts = a.cus / strips < 1 ? 1 : a.cus / strips;
-    if (p.parts > DOWN_MAX_PARTS) p.parts = DOWN_MAX_PARTS;
+    p.parts = a.cus / ((tiles + p.tiles - 1) / p.tiles);
+    p.parts = p.parts < 1 ? 1 : p.parts > DOWN_MAX_PARTS ? DOWN_MAX_PARTS : p.parts;
   }
   return p;
 }
@@ -686,12 +740,13 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
   const int parts = a.partial ? p.parts : 1;
   constexpr int FEW = G ? 4 : 8, ALL = 16 / FEW;
   const bool few = a.M <= FEW;
-  if (a.M > 48) return run_down<T, G, 4, ALL, G == 32 ? 1 : 2, 4, 1>(a, parts, s);  // (two tiles of the finest groups would spill)
-  if (a.M > 32) return run_down<T, G, 3, ALL, 2, 4, 1>(a, parts, s);
+  if (a.M > 48) return run_down<T, G, 4, ALL, G == 32 ? 1 : 2, 4, 1>(a, parts, s);
+  if (a.M > 32) return run_down<T, G, 3, ALL, 2, G == 32 ? 4 : 8, 1>(a, parts, s);
   if (a.M > 16) return run_down<T, G, 2, ALL, 2, 8, 1>(a, parts, s);
   if (p.tiles == 1) {
-    const int blocks = (a.N + Block<T, G, 1, 1, 1>::COLS - 1) / Block<T, G, 1, 1, 1>::COLS * experts_at_most(a);
-    if (blocks >= 32) return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
+    constexpr int COLS = Block<T, G, 1, 1, 1>::COLS;
+    if ((a.N + COLS - 1) / COLS * experts_at_most(a) >= 32)
+      return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
     return few ? run_down<T, G, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s);
   }
   if constexpr (G != 0)

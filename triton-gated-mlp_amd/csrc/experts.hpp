@@ -26,8 +26,8 @@ struct ExpertPlan {
   float* weight;    // [M * top_k]
 };
 
-// Who runs through which expert: every token through the only one, with weight 1; as the plan says; or, of one token, as each
-// kernel finds from the logits itself.
+// Who runs through which expert: every token through the only one, with weight 1; as the plan says; or (gate/up), of one token,
+// as the kernel finds from the logits itself, which then leaves the plan.
 enum Routing : int { ROUTING_DENSE = 0, ROUTING_PLAN = 1, ROUTING_SOLO = 2 };
 
 struct ExpertArgs {
