@@ -653,13 +653,17 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
 }
 
 // Second stage of a down projection whose reduction was split over workgroups: the parts' sums, in their order.
+constexpr int DOWN_MAX_PARTS = 8;
 template <typename T>
 __global__ void __launch_bounds__(256) experts_join_kernel(ExpertArgs a, int parts) {
   const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4, all = (int64_t)a.M * a.K;
   if (i >= all) return;
-  f32x4 v = *(const f32x4*)(a.partial + i);
-  for (int p = 1; p < parts; ++p) v += *(const f32x4*)(a.partial + p * all + i);
-  float y[4] = {v[0], v[1], v[2], v[3]};
+  f32x4 v[DOWN_MAX_PARTS];
+#pragma unroll
+  for (int p = 0; p < DOWN_MAX_PARTS; ++p) v[p] = p < parts ? *(const f32x4*)(a.partial + p * all + i) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int p = 1; p < DOWN_MAX_PARTS; ++p) v[0] += v[p];
+  float y[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
   if (a.bias[2]) add_w<T, 4>((const T*)a.bias[2] + i % a.K, y);
   store_w<T, 4>((T*)a.y + i, y);
 }
@@ -713,7 +717,6 @@ static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
 }
 
 // Down: tiles of a workgroup, and workgroups that share a strip of them.
-constexpr int DOWN_MAX_PARTS = 8;
 struct DownPlan {
   int tiles, parts;
 };
@@ -722,7 +725,7 @@ static DownPlan plan_down(const ExpertArgs& a, int group) {
   const int tiles = (a.K + Q4_TILE - 1) / Q4_TILE;
   DownPlan p = {1, 1};
   if (a.M > 16) p.tiles = a.M > 48 && group == 32 ? 1 : 2;  // (two of the finest groups would spill)
-  else if (large) p.tiles = group && a.M > 4 ? 4 : 2;
+  else if (large) p.tiles = group == 0 ? 1 : a.M > 4 ? 4 : 2;
   else if (group && a.M > 4 && tiles > 2 * a.cus) p.tiles = 4;
   if (a.M > 16 || large) {
     p.parts = a.cus / ((tiles + p.tiles - 1) / p.tiles);
@@ -749,9 +752,8 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
       return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
     return few ? run_down<T, G, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s);
   }
-  if constexpr (G != 0)
-    if (p.tiles == 4) return run_down<T, G, 1, ALL, 4, 8, 1>(a, parts, s);
-  return few ? run_down<T, G, 1, 1, 2, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 2, 8, 1>(a, parts, s);
+  if constexpr (G != 0) return p.tiles == 4 ? run_down<T, G, 1, ALL, 4, 8, 1>(a, parts, s) : run_down<T, G, 1, 1, 2, 8, 1>(a, parts, s);
+  return hipErrorInvalidValue;  // (one tile with 16-bit weights)
 }
 bool experts_solo(const ExpertArgs& a) { return a.M == 1 && a.E <= SOLO_MAX_E; }
 
@@ -775,6 +777,102 @@ hipError_t launch_experts_down(const ExpertArgs& a, int group, hipStream_t s) {
 }
 
 // ------------------------------------------------------------------ routing
+// Four tokens to a wavefront, a row of 16 lanes each; lane l of a row has VPL experts from VPL l on.  What bounds routing many
+// tokens is the instructions of its rounds, and a round of four tokens takes little more than one of one: 16384 tokens, 8 of
+// 128 experts, bf16, 8.8 us with a token per wavefront, 7.0 with four, 6.4 with a lane's logits in one load,
+// 5.5 with the number in the key.
+template <typename F>
+__device__ __forceinline__ uint32_t across_row(uint32_t v, F&& f) {
+  v = f(v, from_lane<0x121>(v));
+  v = f(v, from_lane<0x122>(v));
+  v = f(v, from_lane<0x124>(v));
+  return f(v, from_lane<0x128>(v));
+}
+__device__ __forceinline__ float row_sum(float v, int lane) {
+  const uint32_t s = across_row(__float_as_uint(v), [](uint32_t x, uint32_t y) { return __float_as_uint(__uint_as_float(x) + __uint_as_float(y)); });
+  return __shfl(__uint_as_float(s), lane & 48);  // (the lanes' own sums are of other orders)
+}
+template <int VPL, typename L>
+__global__ void __launch_bounds__(256) route_rows_kernel(const L* logits, float* weights, int64_t* experts, int64_t M, int E, int top_k,
+                                                         int normalize) {
+  const int lane = threadIdx.x & 63, l = lane & 15;
+  const int64_t token = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), t = token < M ? token : M - 1;
+  // A lane's logits in one load where they all exist and lie as the load wants them (VPL divides E: all or none exist).
+  typedef L vec __attribute__((ext_vector_type(VPL)));
+  L raw[VPL] = {};
+  if (VPL > 1 && E % VPL == 0 && ((uintptr_t)logits & (sizeof(vec) - 1)) == 0) {
+    if (l * VPL < E) {
+      const vec packed = *(const vec*)(logits + t * E + l * VPL);
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) raw[v] = packed[v];
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if (l * VPL + v < E) raw[v] = logits[t * E + l * VPL + v];
+  }
+  uint32_t key[VPL];
+  float value[VPL];
+  float first = 0.f, own = 0.f;  // the token's largest logit, and that of the lane's choice
+  int expert = 0;
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) value[v] = (float)raw[v];
+  if constexpr (sizeof(L) == 2) {
+    // 16-bit logits leave room for the number in the key, the lower ones larger: one maximum finds both.
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) {
+      const int e = l * VPL + v;
+      uint32_t u = __builtin_bit_cast(unsigned short, raw[v]);
+      u = value[v] != value[v] ? 0x7fffu : value[v] == 0.f ? 0u : u;
+      u = u & 0x8000u ? ~u & 0xffffu : u | 0x8000u;
+      key[v] = e < E ? u << 16 | (uint32_t)(0xffff - e) : 0u;
+    }
+    for (int j = 0; j < top_k; ++j) {
+      uint32_t best = key[0];
+#pragma unroll
+      for (int v = 1; v < VPL; ++v) best = key[v] > best ? key[v] : best;
+      const uint32_t most = across_row(best, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) key[v] = key[v] == most ? 0u : key[v];
+      const uint32_t u = most >> 16, bits = u & 0x8000u ? u & 0x7fffu : ~u & 0xffffu;
+      const float logit = (float)__builtin_bit_cast(L, (unsigned short)bits);
+      if (j == 0) first = logit;
+      if (l == j) own = logit, expert = (int)(0xffffu - (most & 0xffffu));
+    }
+  } else {
+#pragma unroll
+    for (int v = 0; v < VPL; ++v) key[v] = l * VPL + v < E ? logit_key(value[v]) : 0u;
+    for (int j = 0; j < top_k; ++j) {
+      uint32_t best = key[0];
+      int at = 0;
+#pragma unroll
+      for (int v = 1; v < VPL; ++v)
+        if (key[v] > best) best = key[v], at = v;
+      const uint32_t most = across_row(best, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+      const uint32_t e = across_row(best == most ? (uint32_t)(l * VPL + at) : ~0u, [](uint32_t x, uint32_t y) { return x < y ? x : y; });
+      const int gone = (int)e - l * VPL;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v) key[v] = v == gone ? 0u : key[v];
+      if (j == 0) first = key_logit(most);
+      if (l == j) own = key_logit(most), expert = (int)e;
+    }
+  }
+  const bool none = first == -__builtin_inff();
+  const float e = l < top_k && !none ? expf(own - first) : 0.f;
+  float all = e;
+  if (!normalize) {
+    all = 0.f;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if (l * VPL + v < E && !none) all += expf(value[v] - first);
+  }
+  all = row_sum(all, lane);
+  if (token < M && l < top_k) {
+    weights[t * top_k + l] = none ? 0.f : e / all;
+    experts[t * top_k + l] = expert;
+  }
+}
+
 template <int VPL, typename L>
 __global__ void __launch_bounds__(256) route_kernel(const L* logits, float* weights, int64_t* experts, int64_t M, int E, int top_k,
                                                     int normalize) {
@@ -847,10 +945,15 @@ __global__ void __launch_bounds__(1024) plan_kernel(const L* logits, ExpertPlan 
 
 template <typename L>
 hipError_t launch_route(const L* logits, float* weights, int64_t* experts, int64_t M, int E, int top_k, int normalize, hipStream_t s) {
-#define CALL(V) \
-  hipLaunchKernelGGL((route_kernel<V, L>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, logits, weights, experts, M, E, top_k, normalize)
-  GMLP_BY_EXPERTS(E, CALL);
-#undef CALL
+#define ROWS(V) \
+  hipLaunchKernelGGL((route_rows_kernel<V, L>), dim3((unsigned)((M + 15) / 16)), dim3(256), 0, s, logits, weights, experts, M, E, top_k, normalize)
+  if (E <= 16) ROWS(1);
+  else if (E <= 64) ROWS(4);
+  else if (E <= 128) ROWS(8);
+  else if (E <= 256) ROWS(16);
+  else
+    hipLaunchKernelGGL((route_kernel<8, L>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, logits, weights, experts, M, E, top_k, normalize);
+#undef ROWS
   return hipGetLastError();
 }
 template <typename L>
