@@ -352,6 +352,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
                     size_t workspace_bytes, void* stream);
 
 /*
+ * gmlp_moe_logits: logits [M,E] = x·W_routerᵀ in float, W_router [E,K] in dtype; M <= 64, E a multiple of 4.
  * gmlp_moe_route: p = softmax(logits[m, 0..E)) in fp32; experts [M, top_k] are the numbers of the top_k largest logits in
  *   descending order (the lowest number first among equals, NaN above everything), weights [M, top_k] their p, divided
  *   by their sum if `normalize`.  dtype: of the logits (any GMLP_* one); weights are float, experts int64_t.  A logit of -inf
@@ -362,6 +363,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
  *   dtype, the sum over experts is fp32.  Experts that no token chose are not read; one with weight 0 through -inf is not
  *   run.  M <= 64.  workspace: gmlp_moe_workspace_bytes.
  */
+int gmlp_moe_logits(const void* x, const void* w_router, float* logits, int64_t M, int64_t K, int64_t E, int dtype, void* stream);
 int gmlp_moe_route(const void* logits, float* weights, int64_t* experts, int64_t M, int64_t E, int64_t top_k, int normalize, int dtype,
                    void* stream);
 size_t gmlp_moe_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group, int dtype);

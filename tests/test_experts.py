@@ -624,3 +624,131 @@ def test_operators_replay_in_a_graph(bits):
         ref = call()
         assert all(torch.equal(a, b) for a, b in zip(ref, out))
         torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ modules
+def test_modules_on_the_cpu():
+    from triton_gated_mlp import FusedGatedMLP, GatedMoE, Q4GatedMLP
+
+    m = GatedMoE(64, 72, 12, 3, hidden_act="gelu")
+    assert {n: tuple(p.shape) for n, p in m.named_parameters()} == {
+        "gate_proj": (12, 72, 64), "up_proj": (12, 72, 64), "down_proj": (12, 64, 72), "router.weight": (12, 64)}
+    assert not m.quantized and "top_k=3" in repr(m)
+    for bad in (0, 13):
+        with pytest.raises(ValueError, match="top_k"):
+            GatedMoE(64, 72, 12, bad)
+    with pytest.raises(KeyError):
+        GatedMoE(64, 72, 12, 3, hidden_act="softsign")
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        with torch.no_grad():
+            m(torch.zeros(2, 64))
+    with pytest.raises(RuntimeError, match="AMD GPU"):
+        Q4GatedMLP.from_float(FusedGatedMLP(64, 72).half())
+    # the batch from which experts run one by one, by their size
+    assert GatedMoE(8, 8, 2, 1).long_batch() > 10**7
+    with torch.device("meta"):
+        assert GatedMoE(4096, 14336, 8, 2).long_batch() == 113 and GatedMoE(8192, 28672, 8, 2).long_batch() == 65
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,K,E", [(1, 8, 4), (1, 2048, 64), (5, 264, 60), (16, 136, 8), (33, 1000, 128), (64, 264, 12), (100, 136, 16)])
+def test_moe_logits(M, K, E, dtype):
+    dev, g = device(), gen(M + K)
+    x, w = normal((M, K), 1.0, dtype, g), normal((E, K), 0.1, dtype, g)
+    out = moe.moe_logits(x.to(dev), w.to(dev))
+    assert out.dtype == torch.float32
+    y, mass = x.double() @ w.double().T, x.double().abs() @ w.double().abs().T
+    assert ((out.cpu().double() - y).abs() <= (K + 16) * 2.0**-23 * mass).all()
+    assert moe.moe_logits(x.to(dev)[:0], w.to(dev)).shape == (0, E)
+
+
+@gpu
+def test_moe_logits_refusals():
+    dev = device()
+    x, w = torch.zeros(2, 64, dtype=torch.float16, device=dev), torch.zeros(8, 64, dtype=torch.float16, device=dev)
+    with pytest.raises(ValueError, match="W_router"):
+        moe.moe_logits(x, w[:, :56])
+    with pytest.raises(NotImplementedError):
+        moe.moe_logits(x, w[:6])
+    with pytest.raises(TypeError):
+        moe.moe_logits(x, w.float())
+    with pytest.raises(RuntimeError, match="no backward"):
+        moe.moe_logits(x, w.clone().requires_grad_(True))
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("E,router", [(12, torch.bfloat16), (6, torch.float32)])
+def test_gated_moe_module(E, router, bits):
+    """Few tokens, the same tokens through the experts one by one, and a saved and loaded copy."""
+    from triton_gated_mlp import GatedMoE
+
+    dev, dtype, K, N, k = device(), torch.bfloat16, 136, 264, 2
+    torch.manual_seed(3)
+    m = GatedMoE(K, N, E, k, hidden_act="gelu").to(dev, dtype)
+    m.router.to(router)
+    x = torch.randn(2, 9, K, device=dev).to(dtype)
+    with pytest.raises(RuntimeError, match="no backward"):
+        m(x)
+    with torch.no_grad():
+        if bits == 4:
+            m.quantize_(64)
+            one = lambda e: tuple(weights_of(p.of(e)) for p in (m.gate_proj, m.up_proj, m.down_proj))
+        else:
+            one = lambda e: tuple(p[e].cpu().double() for p in (m.gate_proj, m.up_proj, m.down_proj))
+        assert m.quantized == (bits == 4)
+        y = m(x)
+        rows = x.reshape(-1, K)
+        logits = m.route_logits(rows)
+        assert torch.allclose(logits.cpu().double(), rows.cpu().double() @ m.router.weight.cpu().double().T, atol=1e-4, rtol=0)
+        ref, bound = moe64(rows.cpu().double(), logits.cpu(), k, True, "gelu", dtype, one)
+        hold(y, ref, bound, dtype, 2)
+        # each expert's output is rounded as well: three roundings, u in the mean square, and the weights' 1e-6
+        out = m._one_by_one(rows, logits).cpu().double()
+        assert ((out - ref).norm() / ref.norm()).item() <= 1.02 * U[dtype]
+        m.long_batch = lambda: 1
+        assert torch.equal(m(x).cpu().double().reshape(out.shape), out)
+        other = GatedMoE(K, N, E, k, hidden_act="gelu").to(dev, dtype)
+        other.router.to(router)
+        if bits == 4:
+            other.quantize_(64)
+        other.load_state_dict(m.state_dict())
+        assert torch.equal(other(x), y)
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 70])
+def test_q4_gated_mlp_module(rows):
+    from triton_gated_mlp import FusedGatedMLP, Q4GatedMLP
+
+    dev, dtype = device(), torch.float16
+    torch.manual_seed(5)
+    mlp = FusedGatedMLP(136, 264, bias=True, hidden_act="relu").to(dev, dtype).eval()
+    q = Q4GatedMLP.from_float(mlp, 32)
+    x = torch.randn(rows, 136, device=dev).to(dtype)
+    with torch.no_grad():
+        y = q(x)
+    ws = [weights_of(p.weight()) for p in (q.gate_proj, q.up_proj, q.down_proj)]
+    if rows > 64:
+        ws = [w.to(dtype).double() for w in ws]
+    bs = [layer.bias.detach().cpu().double() for layer in (mlp.gate_proj, mlp.up_proj, mlp.down_proj)]
+    ref, bound = mlp64(x.cpu().double(), ws[0], bs[0], ws[1], bs[1], ws[2], bs[2], "relu", dtype)
+    hold(y, ref, bound + U[dtype] * ref.abs() + SUB[dtype], dtype, 2)
+    assert y.requires_grad is False and len(list(q.parameters())) == 0
+    q2 = Q4GatedMLP.from_float(FusedGatedMLP(136, 264, bias=True, hidden_act="relu").to(dev, dtype), 32)
+    q2.load_state_dict(q.state_dict())
+    assert torch.equal(q2(x), y)
+    # within the quantisation's error of the module it came from: at most half a step of 1/7 of a group's largest weight
+    with torch.no_grad():
+        assert ((mlp(x) - y).norm() / mlp(x).norm()).item() < 0.25
+
+
+@gpu
+@pytest.mark.parametrize("bits", ["4", "16"])
+def test_the_decode_example_runs(bits):
+    from triton_gated_mlp import decode_example
+
+    us = decode_example.main(["--tokens", "2", "--layers", "2", "--hidden", "1024", "--intermediate", "1408", "--expert", "512",
+                              "--experts", "16", "--top-k", "4", "--bits", bits, "--steps", "5"])
+    assert us > 0

@@ -1605,6 +1605,25 @@ int gmlp_moe_route(const void* logits, float* weights, int64_t* experts, int64_t
   }));
 }
 
+int gmlp_moe_logits(const void* x, const void* w_router, float* logits, int64_t M, int64_t K, int64_t E, int dtype, void* stream) {
+  GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(w_router); GMLP_REQUIRE_PTR(logits);
+  if (int rc = check_q4(__func__, 32, dtype)) return rc;
+  if (int rc = check_dims(__func__, M, K, E)) return rc;
+  if (int rc = check_rows(__func__, M)) return rc;
+  if (int rc = check_mult8(__func__, "K", K)) return rc;
+  if (E % 4 != 0) return fail(GMLP_ESHAPE, "%s: E = %lld must be a multiple of 4", __func__, (long long)E);
+  if (int rc = check_expert_sizes(__func__, M, E, K, 1, M)) return rc;
+  GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(w_router); GMLP_REQUIRE_ALIGNED(logits);
+  gmlp::ExpertArgs a = expert_sizes(M, E, K, 1, 1);
+  a.h = const_cast<void*>(x);  // read only
+  a.y = logits;
+  a.y_f32 = 1;
+  a.down = {w_router, nullptr};
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    return gmlp::launch_experts_down<decltype(tag)>(a, 0, (hipStream_t)stream);
+  }));
+}
+
 size_t gmlp_moe_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group, int dtype) {
   if (M < 1 || M > gmlp::EXPERTS_MAX_M || K < 1 || K > kMaxDim || N < 1 || N > kMaxDim || E < 1 || E > gmlp::EXPERTS_MAX_E || top_k < 1 ||
       top_k > gmlp::EXPERTS_MAX_K || check_q4(__func__, group == 0 ? 32 : group, dtype) != 0)

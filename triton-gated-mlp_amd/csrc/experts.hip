@@ -647,6 +647,10 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
       return;
     }
     float y[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
+    if (a.y_f32) {  // (router logits: rows of whole fours)
+      *(f32x4*)((float*)a.y + (size_t)t * a.K + first) = v[0];
+      return;
+    }
     if (a.bias[2]) add_w<T, 4>((const T*)a.bias[2] + first, y);
     store_w<T, 4>((T*)a.y + (size_t)t * a.K + first, y);
   });

@@ -35,9 +35,10 @@ struct ExpertArgs {
   const void* bias[3];
   ExpertWeights gate, up, down;
   void* h;            // [M * top_k, N]
-  void* y;            // [M, K]
+  void* y;            // [M, K], of the activations' type or (y_f32, without partial) float
   float* partial;     // [parts][M, K], where the down projection's reduction is split
   int M, K, N, E, top_k, act;
+  int y_f32;
   int routing;        // Routing
   int cus;            // compute units of the device
   const void* logits; // [M, E] of a GMLP_* type

@@ -43,7 +43,7 @@ typedef std::optional<Tensor> OptTensor;
   X(gmlp_last_error) X(gmlp_workspace_bytes) X(gmlp_mlp_workspace_bytes) X(gmlp_mlp_fwd)         \
   X(gmlp_mlp_bwd) X(gmlp_gateup_fwd) X(gmlp_decode_fwd) X(gmlp_decode_stream_fwd) X(gmlp_hidden_bwd) \
   X(gmlp_grads_workspace_bytes) X(gmlp_linear_fwd) X(gmlp_q4_quantize) X(gmlp_q4_dequantize) X(gmlp_q4_workspace_bytes) X(gmlp_q4_linear_fwd) \
-  X(gmlp_q4_mlp_fwd) X(gmlp_moe_route) X(gmlp_moe_workspace_bytes) X(gmlp_moe_fwd)
+  X(gmlp_q4_mlp_fwd) X(gmlp_moe_logits) X(gmlp_moe_route) X(gmlp_moe_workspace_bytes) X(gmlp_moe_fwd)
 struct Library {
 #define GMLP_MEMBER(name) decltype(&::name) name = nullptr;
   GMLP_ENTRY_POINTS(GMLP_MEMBER)
@@ -643,6 +643,24 @@ std::tuple<Tensor, Tensor> moe_route(const Tensor& logits_in, int64_t top_k, boo
   return {weights, experts};
 }
 
+Tensor moe_logits(const Tensor& x_in, const Tensor& w_in) {
+  inference_only("moe_logits", {x_in, w_in});
+  const int code = require_half("moe_logits", {x_in, w_in});
+  TORCH_CHECK_VALUE(x_in.dim() >= 1 && w_in.dim() == 2 && w_in.size(1) == x_in.size(-1), "dimension mismatch: x ", x_in.sizes(),
+                    ", W_router ", w_in.sizes());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x_in.device());
+  const Tensor x = x_in.contiguous(), w = w_in.contiguous();
+  const int64_t K = x.size(-1), E = w.size(0), M = K > 0 ? x.numel() / K : 0;
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = E;
+  const Tensor out = at::empty(sizes, x.options().dtype(at::kFloat));
+  for (int64_t m = 0; m < M; m += FEW_ROWS)
+    check(lib.gmlp_moe_logits((const char*)ptr(x) + m * K * x.element_size(), ptr(w), (float*)out_ptr(out) + m * E,
+                              std::min(M - m, FEW_ROWS), K, E, code, stream_of(x)));
+  return out;
+}
+
 // (The last piece of a batch may ask for more than the others: fewer experts in use, another split.)
 size_t moe_workspace(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group, int code) {
   size_t bytes = lib.gmlp_moe_workspace_bytes(std::min(M, FEW_ROWS), K, N, E, top_k, group, code);
@@ -765,6 +783,7 @@ PYBIND11_MODULE(_gmlp_torch, m) {
   m.def("q4_mlp", torch::wrap_pybind_function_no_gil(q4_mlp));
   m.def("q4_quantize", torch::wrap_pybind_function_no_gil(q4_quantize));
   m.def("q4_dequantize", torch::wrap_pybind_function_no_gil(q4_dequantize));
+  m.def("moe_logits", torch::wrap_pybind_function_no_gil(moe_logits));
   m.def("moe_route", torch::wrap_pybind_function_no_gil(moe_route));
   m.def("moe_mlp", torch::wrap_pybind_function_no_gil(moe_mlp));
   m.def("moe_mlp_q4", torch::wrap_pybind_function_no_gil(moe_mlp_q4));

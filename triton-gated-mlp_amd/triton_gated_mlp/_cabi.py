@@ -93,6 +93,7 @@ _SIGNATURES = {
     "gmlp_q4_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int, _int]),
     "gmlp_q4_linear_fwd": (_int, [_c_ptr] * 5 + [_i64, _i64, _i64, _int, _int, _c_ptr, ctypes.c_size_t, _c_ptr]),
     "gmlp_q4_mlp_fwd": (_int, [_c_ptr] * 12 + [_i64, _i64, _i64, _int, _int, _int, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "gmlp_moe_logits": (_int, [_c_ptr] * 3 + [_i64, _i64, _i64, _int, _c_ptr]),
     "gmlp_moe_route": (_int, [_c_ptr] * 3 + [_i64, _i64, _i64, _int, _int, _c_ptr]),
     "gmlp_moe_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _int, _int]),
     "gmlp_moe_fwd": (

@@ -1,1 +1,1 @@
-from . import bwd, fwd  # noqa: F401
+from . import bwd, fwd, moe, quant  # noqa: F401

@@ -19,6 +19,12 @@ class Routing(NamedTuple):
     experts: Tensor  # int64 [..., top_k], in descending order of the logits
 
 
+def moe_logits(x: Tensor, W_router: Tensor) -> Tensor:
+    """float32 x [..., hidden]·W_routerᵀ, W_router [experts, hidden] in x's dtype; experts a multiple of 4.  Made for a few
+    tokens: 64 rows at a time."""
+    return _cabi.torch_binding().moe_logits(x, W_router)
+
+
 def moe_route(logits: Tensor, top_k: int, normalize: bool = True) -> Routing:
     """Softmax over the last dimension of `logits` (float32, float16 or bfloat16; at most 512 experts) and the top_k
     (at most 16) largest of each token, the lowest number first among equals; with `normalize` their weights are divided by
