@@ -215,8 +215,9 @@ struct Block {
   static constexpr int TILE = 16 * COLS * 2;    // bytes of a tile in LDS
   static constexpr int WB = G ? 0 : NT < 4 ? NT : 4;  // weight tiles in LDS at a time
   // 4-bit weights: token rows go to LDS without passing through registers (buffer_load ... lds), a slot for each stage; two
-  // stages of the weights then fit where one of both did.  16-bit: one slot for what the wavefront multiplies.
-  static constexpr bool DMA = G != 0;
+  // stages of the weights then fit where one of both did.  16-bit weights, and a single load of token rows, whose four
+  // registers are no matter: one slot for what the wavefront multiplies.
+  static constexpr bool DMA = G != 0 && MT * XR > 1;
   static constexpr int SLOT = (MT + WB) * TILE;
   static constexpr int lds_bytes(int depth) { return (DMA ? depth : 1) * SLOT; }  // of a wavefront
   static_assert(XR * ROWS <= 16, "a token tile has 16 rows");
@@ -294,6 +295,13 @@ struct Block {
       }
   }
 
+  // Between a wavefront's writes to LDS and its other lanes' reads: the LDS takes them in order, the compiler has to leave them so.
+  static __device__ __forceinline__ void turn() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
+  }
+
   // Columns of a tile: step s takes 32 s + 8 (lane / 16) + 0..7.  (Token rows that XR leaves out are whatever LDS holds: their
   // columns of the product are not used.)
   static __device__ __forceinline__ vec8 operand(const char* tile, int s, int lane) {
@@ -305,7 +313,6 @@ struct Block {
     for (int i = 0; i < L; ++i) *(u32x4*)(tile + at(load_row(i, lane), lane % PIECES)) = v[i];
   }
   __device__ __forceinline__ void multiply(const Int4<T>& int4, char* slot, int lane, f32x4 (&acc)[NT][MT]) {
-    vec8 xf[MT][STEPS];
     if constexpr (DMA) {
       // The token rows were asked for ahead of the weights and scales, and loads return in order: once the last scale is there
       // (the compiler waits for it here, it goes into the statement), they are in LDS.
@@ -315,23 +322,25 @@ struct Block {
       for (int m = 0; m < MT; ++m) to_lds(slot + m * TILE, x[m], lane);
 #pragma unroll
       for (int n = 0; n < WB; ++n) to_lds(slot + (MT + n) * TILE, w[n], lane);
-      __builtin_amdgcn_wave_barrier();
+      turn();
     }
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int g = 0; g < GROUPS; ++g) {
+      constexpr int SG = STEPS / GROUPS;  // steps of a group
+      vec8 xf[MT][SG];
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) xf[m][s] = operand(slot + m * TILE, s, lane);
+      for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if constexpr (G != 0) {
+        for (int s = 0; s < SG; ++s) xf[m][s] = operand(slot + m * TILE, g * SG + s, lane);
 #pragma unroll
-        for (int g = 0; g < GROUPS; ++g) {
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (G != 0) {
           f32x4 part[MT];
 #pragma unroll
           for (int m = 0; m < MT; ++m) part[m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int s = g * STEPS / GROUPS; s < (g + 1) * STEPS / GROUPS; ++s) {
-            const vec8 a = int4.floats(w[n][0][s]);
+          for (int s = 0; s < SG; ++s) {
+            const vec8 a = int4.floats(w[n][0][g * SG + s]);
 #pragma unroll
             for (int m = 0; m < MT; ++m) part[m] = Traits<T>::mfma16(a, xf[m][s], part[m]);
           }
@@ -341,24 +350,26 @@ struct Block {
 #pragma unroll
             for (int m = 0; m < MT; ++m) acc[n][m][r] += f * part[m][r];
           }
-        }
-      } else {
-        char* const tile = slot + (MT + n % WB) * TILE;
-        if (n >= WB) {
-          __builtin_amdgcn_wave_barrier();
-          to_lds(tile, w[n], lane);
-          __builtin_amdgcn_wave_barrier();
-        }
+        } else {
+          char* const tile = slot + (MT + n % WB) * TILE;
+          if (n >= WB) {
+            turn();
+            to_lds(tile, w[n], lane);
+            turn();
+          }
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s) {
-          const vec8 a = operand(tile, s, lane);
+          for (int s = 0; s < SG; ++s) {
+            const vec8 a = operand(tile, s, lane);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) acc[n][m] = Traits<T>::mfma16(a, xf[m][s], acc[n][m]);
+            for (int m = 0; m < MT; ++m) acc[n][m] = Traits<T>::mfma16(a, xf[m][s], acc[n][m]);
+          }
         }
       }
+      // A group at a time: the scheduler would fetch the next one's token operands ahead, and pay in registers.
+      if constexpr (MT > 1 && GROUPS > 1) __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (DMA) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the slot has been read
-    else __builtin_amdgcn_wave_barrier();
+    else turn();
   }
 };
 
@@ -410,8 +421,10 @@ constexpr int gateup_lds() {
   constexpr int ring = NW * Block<T, G, 2 * R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 2>() * 2 * 1024;
   return ring > part ? ring : part;
 }
+// (Two or three token tiles: 256 registers, so that a CU holds two workgroups of four wavefronts.  M=48, K=4096, N=11008, groups of
+// 64 36.7 -> 25.5 us.  Four tiles do not fit.)
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
-__global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
+__global__ void __launch_bounds__(NW * 64, MT > 1 && MT < 4 && R <= 2 ? 2 : 1) experts_gateup_kernel(ExpertArgs a) {
   typedef Block<T, G, 2 * R, MT, XR> B;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -482,6 +495,7 @@ __global__ void __launch_bounds__(NW * 64) experts_gateup_kernel(ExpertArgs a) {
     each_stage<D>([&](auto d) {
       if (i + d < run) st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
     });
+    if constexpr (B::DMA) wait_vmem<0>();  // stages past the end bring nothing, but they write: not into the sums
     f32x4 both[R * MT][2];
 #pragma unroll
     for (int i = 0; i < R * MT; ++i)
@@ -639,6 +653,7 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
       }
     });
   }
+  if constexpr (B::DMA) wait_vmem<0>();  // (as in gate/up)
   sum_wavefronts<NW>(sum, smem, wave, lane, [&](int unit, const f32x4 (&v)[1]) {
     const int n = unit / MT, t = 16 * (unit - n * MT) + r16, first = (tile + n) * Q4_TILE + 4 * kg;
     if (t >= a.M || first >= a.K) return;
@@ -693,7 +708,8 @@ static hipError_t run_down(const ExpertArgs& a, int parts, hipStream_t s) {
   constexpr int LDS = down_lds<T, G, MT, XR, R, NW, D>();
   const int tables = a.routing == ROUTING_DENSE ? 0 : experts_at_most(a) * (4 + EXPERTS_MAX_M) + a.M * a.top_k * 4;
   constexpr auto kern = experts_down_kernel<T, G, MT, XR, R, NW, D>;
-  if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, LDS + EX_TABLES>, s)) return e;
+  if (LDS + tables > 64 * 1024)
+    if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, LDS + EX_TABLES>, s)) return e;
   const dim3 grid((unsigned)((a.K + R * Q4_TILE - 1) / (R * Q4_TILE)), (unsigned)parts);
   hipLaunchKernelGGL(kern, grid, dim3(NW * 64), (unsigned)(LDS + tables), s, a);
   if (hipError_t e = hipGetLastError()) return e;
@@ -710,13 +726,13 @@ static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
     if (a.M <= 16) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
     return run_gateup<T, 0, 2, 2, 2, 4, 1>(a, s);
   } else {
-    if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 1>(a, s);
+    if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 2>(a, s);
     if (a.M <= 16) return few ? run_gateup<T, G, 1, 4, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
     // More than one token tile: as many tiles and wavefronts as the registers hold, fewer with finer groups.
     constexpr bool coarse = G == 128, fine = G == 32;
-    if (a.M <= 32) return few ? run_gateup<T, G, 2, 4, 2, 8, 1>(a, s) : run_gateup<T, G, 2, 4, 3, coarse ? 8 : 4, 1>(a, s);
-    if (a.M <= 48) return few ? run_gateup<T, G, 3, 4, coarse ? 2 : 1, coarse ? 8 : 4, 1>(a, s) : run_gateup<T, G, 3, 4, fine ? 2 : 3, 4, 1>(a, s);
-    return few ? run_gateup<T, G, 4, 4, coarse ? 2 : 1, 4, 1>(a, s) : run_gateup<T, G, 4, 4, fine ? 2 : 3, 4, 1>(a, s);
+    if (a.M <= 32) return few ? run_gateup<T, G, 2, 4, fine ? 1 : 2, 8, 1>(a, s) : run_gateup<T, G, 2, 4, 3, coarse ? 8 : 4, 1>(a, s);
+    if (a.M <= 48) return run_gateup<T, G, 3, 4, fine ? 1 : 2, 4, 1>(a, s);
+    return few ? run_gateup<T, G, 4, 4, 1, 4, 1>(a, s) : run_gateup<T, G, 4, 4, fine ? 2 : 3, 4, 1>(a, s);
   }
 }
 
@@ -729,8 +745,7 @@ static DownPlan plan_down(const ExpertArgs& a, int group) {
   const int tiles = (a.K + Q4_TILE - 1) / Q4_TILE;
   DownPlan p = {1, 1};
   if (a.M > 16) p.tiles = a.M > 48 && group == 32 ? 1 : 2;  // (two of the finest groups would spill)
-  else if (large) p.tiles = group == 0 ? 1 : a.M > 4 ? 4 : 2;
-  else if (group && a.M > 4 && tiles > 2 * a.cus) p.tiles = 4;
+  else if (group && a.M > 4 && (large || tiles > 2 * a.cus)) p.tiles = 4;
   if (a.M > 16 || large) {
     p.parts = a.cus / ((tiles + p.tiles - 1) / p.tiles);
     p.parts = p.parts < 1 ? 1 : p.parts > DOWN_MAX_PARTS ? DOWN_MAX_PARTS : p.parts;
@@ -750,14 +765,17 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
   if (a.M > 48) return run_down<T, G, 4, ALL, G == 32 ? 1 : 2, 4, 1>(a, parts, s);
   if (a.M > 32) return run_down<T, G, 3, ALL, 2, G == 32 ? 4 : 8, 1>(a, parts, s);
   if (a.M > 16) return run_down<T, G, 2, ALL, 2, 8, 1>(a, parts, s);
-  if (p.tiles == 1) {
-    constexpr int COLS = Block<T, G, 1, 1, 1>::COLS;
-    if ((a.N + COLS - 1) / COLS * experts_at_most(a) >= 32)
-      return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
-    return few ? run_down<T, G, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s);
+  if constexpr (G != 0)
+    if (p.tiles == 4) return run_down<T, G, 1, ALL, 4, 8, 1>(a, parts, s);
+  // One tile.  Enough wavefronts, and stages of them, for a share of the blocks that is in flight at once.
+  constexpr int COLS = Block<T, G, 1, 1, 1>::COLS;
+  const int blocks = (a.N + COLS - 1) / COLS * experts_at_most(a);
+  if (few && G != 0) {
+    if (blocks <= 16) return run_down<T, G, 1, 1, 1, 8, 2>(a, parts, s);
+    return blocks < 128 ? run_down<T, G, 1, 1, 1, 8, 4>(a, parts, s) : run_down<T, G, 1, 1, 1, 16, 2>(a, parts, s);
   }
-  if constexpr (G != 0) return p.tiles == 4 ? run_down<T, G, 1, ALL, 4, 8, 1>(a, parts, s) : run_down<T, G, 1, 1, 2, 8, 1>(a, parts, s);
-  return hipErrorInvalidValue;  // (one tile with 16-bit weights)
+  if (blocks < 32) return few ? run_down<T, G, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s);
+  return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
 }
 bool experts_solo(const ExpertArgs& a) { return a.M == 1 && a.E <= SOLO_MAX_E; }
 
