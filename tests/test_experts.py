@@ -453,6 +453,7 @@ def experts_of(E, K, N, bits, group, dtype, g):
         (2, 136, 72, 4, 4, 16, 0, "relu", False), (7, 200, 328, 16, 4, 4, 64, "silu", False), (16, 264, 136, 60, 6, 16, 0, "silu", True),
         (16, 392, 264, 8, 2, 4, 128, "silu", True), (17, 72, 200, 4, 2, 16, 0, "tanh", True), (33, 136, 264, 128, 8, 16, 0, "silu", False),
         (40, 264, 136, 8, 3, 4, 32, "silu", True), (64, 128, 64, 512, 16, 16, 0, "silu", True), (64, 136, 72, 2, 1, 4, 64, "gelu", True),
+        (64, 8, 8, 1, 1, 16, 0, "silu", False), (64, 136, 1032, 1, 1, 4, 32, "silu", True),
         (100, 72, 136, 8, 2, 16, 0, "silu", True), (130, 72, 136, 8, 2, 4, 128, "silu", True),
     ],
 )
@@ -490,8 +491,25 @@ def test_moe_mlp_with_masked_experts(M, bits):
 
 
 @gpu
-def test_what_is_not_finite_stays_with_its_token_and_its_expert():
-    dev, dtype, E, K, N, M = device(), torch.float16, 4, 136, 72, 16
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("M,E,k", [(17, 40, 2), (64, 64, 2), (64, 512, 3), (48, 6, 2)])
+def test_moe_mlp_with_one_crowded_expert(M, E, k, bits):
+    """An expert that every token chose beside many that one or two did: its tokens are more than the kernels take at once."""
+    dev, dtype, K, N = device(), torch.float16, 72, 136
+    g = gen(M + E)
+    x, logits = normal((M, K), 1.0, dtype, g), normal((M, E), 1.0, torch.float32, g)
+    logits[:, 3] += 20
+    logits[5, 3] = -math.inf
+    ws, one = experts_of(E, K, N, bits, 128, dtype, g)
+    y = moe.moe_mlp_fwd(x.to(dev), logits.to(dev), *ws, k, normalize=False)
+    ref, bound = moe64(x.double(), logits, k, False, "silu", dtype, one)
+    hold(y, ref, bound, dtype, 2)
+
+
+@gpu
+@pytest.mark.parametrize("M,E", [(16, 4), (40, 4), (40, 20)])
+def test_what_is_not_finite_stays_with_its_token_and_its_expert(M, E):
+    dev, dtype, K, N = device(), torch.float16, 136, 72
     g = gen(0)
     x, logits = normal((M, K), 1.0, dtype, g).to(dev), normal((M, E), 1.5, torch.float32, g).to(dev)
     (gate, up, down), _ = experts_of(E, K, N, 16, 0, dtype, g)

@@ -1477,28 +1477,29 @@ hipError_t by_half(int dtype, F&& f) {
   return dtype == GMLP_F16 ? f(gmlp::f16{}) : f(gmlp::bf16{});
 }
 // Where the parts of gmlp_moe_fwd's workspace begin.
-gmlp::ExpertArgs expert_sizes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k) {
+gmlp::ExpertArgs expert_sizes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, gmlp::Routing routing) {
   gmlp::ExpertArgs a = {};
   a.M = (int)M; a.K = (int)K; a.N = (int)N; a.E = (int)E; a.top_k = (int)top_k;
   a.cus = num_cu();
+  a.routing = routing;
   return a;
 }
 struct MoeWorkspace {
-  size_t active, slot, tokens, count, weight, partial, bytes;
+  size_t active, slot, which, count, weight, partial, bytes;
   MoeWorkspace(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group) {
-    const size_t pairs = (size_t)(M * top_k), experts = (size_t)E < pairs ? (size_t)E : pairs;
+    const size_t pairs = (size_t)(M * top_k), entries = (size_t)gmlp::expert_entries((int)M, (int)E, (int)top_k);
     size_t at = pairs * (size_t)N * 2;
     auto part = [&](size_t n) {
       const size_t begin = (at + 255) / 256 * 256;
       at = begin + n;
       return begin;
     };
-    active = part((1 + experts) * sizeof(int));
-    slot = part(experts * gmlp::EXPERTS_MAX_M);
-    tokens = part(experts * gmlp::EXPERTS_MAX_M);
-    count = part(experts);
+    active = part((1 + entries) * sizeof(int));
+    slot = part(entries * gmlp::EXPERTS_MAX_M);
+    which = part(entries * gmlp::EXPERTS_MAX_M * sizeof(uint16_t));
+    count = part(entries);
     weight = part(pairs * sizeof(float));
-    partial = part(gmlp::experts_partial_bytes(expert_sizes(M, K, N, E, top_k), group));
+    partial = part(gmlp::experts_partial_bytes(expert_sizes(M, K, N, E, top_k, gmlp::ROUTING_PLAN), group));
     bytes = at;
   }
 };
@@ -1533,7 +1534,7 @@ int gmlp_q4_dequantize(const void* codes, const void* scales, void* w, int64_t c
 
 size_t gmlp_q4_workspace_bytes(int64_t M, int64_t R, int64_t C, int group, int dtype) {
   if (M < 1 || M > gmlp::EXPERTS_MAX_M || R < 1 || R > kMaxDim || C < 1 || C > kMaxDim || check_q4(__func__, group, dtype) != 0) return 0;
-  return gmlp::experts_partial_bytes(expert_sizes(M, C, R, 1, 1), group);
+  return gmlp::experts_partial_bytes(expert_sizes(M, C, R, 1, 1, gmlp::ROUTING_DENSE), group);
 }
 
 int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, const void* bias, void* y, int64_t M, int64_t R,
@@ -1547,7 +1548,7 @@ int gmlp_q4_linear_fwd(const void* x, const void* codes, const void* scales, con
   if (int rc = check_expert_sizes(__func__, M, C, R, 1, M)) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(bias);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
-  gmlp::ExpertArgs a = expert_sizes(M, C, R, 1, 1);
+  gmlp::ExpertArgs a = expert_sizes(M, C, R, 1, 1, gmlp::ROUTING_DENSE);
   a.h = const_cast<void*>(x);  // read only
   a.y = y;
   a.bias[2] = bias;
@@ -1576,7 +1577,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
   GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(codes_down); GMLP_REQUIRE_ALIGNED(scales_down);
   GMLP_REQUIRE_ALIGNED(b_gate); GMLP_REQUIRE_ALIGNED(b_up); GMLP_REQUIRE_ALIGNED(b_down); GMLP_REQUIRE_ALIGNED(h);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
-  gmlp::ExpertArgs a = expert_sizes(M, K, N, 1, 1);
+  gmlp::ExpertArgs a = expert_sizes(M, K, N, 1, 1, gmlp::ROUTING_DENSE);
   a.x = x;
   a.h = h;
   a.y = y;
@@ -1614,7 +1615,7 @@ int gmlp_moe_logits(const void* x, const void* w_router, float* logits, int64_t 
   if (E % 4 != 0) return fail(GMLP_ESHAPE, "%s: E = %lld must be a multiple of 4", __func__, (long long)E);
   if (int rc = check_expert_sizes(__func__, M, E, K, 1, M)) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(w_router); GMLP_REQUIRE_ALIGNED(logits);
-  gmlp::ExpertArgs a = expert_sizes(M, E, K, 1, 1);
+  gmlp::ExpertArgs a = expert_sizes(M, E, K, 1, 1, gmlp::ROUTING_DENSE);
   a.h = const_cast<void*>(x);  // read only
   a.y = logits;
   a.y_f32 = 1;
@@ -1656,7 +1657,8 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   if (workspace_bytes < ws.bytes)
     return fail(GMLP_EINVAL, "%s: workspace of %zu bytes, needs %zu", __func__, workspace_bytes, ws.bytes);
   char* const base = (char*)workspace;
-  gmlp::ExpertArgs a = expert_sizes(M, K, N, E, top_k);
+  const gmlp::Routing routing = gmlp::experts_solo((int)M, (int)E) ? gmlp::ROUTING_SOLO : gmlp::ROUTING_PLAN;
+  gmlp::ExpertArgs a = expert_sizes(M, K, N, E, top_k, routing);
   a.x = x;
   a.h = base;
   a.y = y;
@@ -1667,15 +1669,14 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   a.logits = logits;
   a.logits_dtype = logits_dtype;
   a.normalize = normalize;
-  a.routing = gmlp::experts_solo(a) ? gmlp::ROUTING_SOLO : gmlp::ROUTING_PLAN;
-  a.plan = {(int*)(base + ws.active), (uint8_t*)(base + ws.count), (uint8_t*)(base + ws.tokens), (int8_t*)(base + ws.slot),
+  a.plan = {(int*)(base + ws.active), (uint8_t*)(base + ws.count), (uint16_t*)(base + ws.which), (int8_t*)(base + ws.slot),
             (float*)(base + ws.weight)};
   if (ws.bytes > ws.partial) a.partial = (float*)(base + ws.partial);
   const hipStream_t s = (hipStream_t)stream;
   if (a.routing == gmlp::ROUTING_PLAN) {
     const hipError_t planned = by_dtype(logits_dtype, [&](auto tag) {
       typedef decltype(tag) L;
-      return gmlp::launch_experts_plan<L>((const L*)logits, a.plan, a.M, a.E, a.top_k, normalize, s);
+      return gmlp::launch_experts_plan<L>((const L*)logits, a, s);
     });
     if (planned != hipSuccess) return hip_result(__func__, planned);
   }

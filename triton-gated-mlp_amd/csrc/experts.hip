@@ -30,8 +30,16 @@ typedef __amdgpu_buffer_rsrc_t ex_rsrc;
 __device__ __forceinline__ ex_rsrc ex_make_rsrc(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
-// LDS for the tables of the largest routing (experts_down_kernel).
-constexpr int EX_TABLES = EXPERTS_MAX_E * (4 + EXPERTS_MAX_M) + EXPERTS_MAX_M * EXPERTS_MAX_K * 4;
+// LDS of experts_down_kernel for the tables of the largest routing: without GATHER 16 tokens; with it one token tile an entry or,
+// beyond ten tokens for each expert (token_tiles), two.
+constexpr int ex_tables(int entries, bool gather, int token_tiles, int pairs) {
+  return entries * (gather ? 4 + 1 + 16 * token_tiles * 2 : 4 + EXPERTS_MAX_M) + pairs * 4;
+}
+constexpr int ex_tables_at_most(bool gather, int token_tiles) {
+  constexpr int pairs = EXPERTS_MAX_M * EXPERTS_MAX_K;
+  return !gather ? ex_tables(16 * EXPERTS_MAX_K, false, 1, 16 * EXPERTS_MAX_K)
+                 : ex_tables((token_tiles == 1 ? EXPERTS_MAX_E : pairs / 10) + pairs / 16, true, token_tiles, pairs);
+}
 constexpr int EX_STREAM = 2;  // cache policy: non-temporal, what is read once
 template <int POLICY = 0>
 __device__ __forceinline__ u32x4 ex_load16(ex_rsrc r, uint32_t lane_off, uint32_t off) {
@@ -454,107 +462,120 @@ __global__ void __launch_bounds__(NW * 64, MT > 1 && MT < 4 && R <= 2 ? 2 : 1) e
   char* const lds = smem + wave * B::lds_bytes(D);
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void*)lds;
 
-  for (int base = 0; base < count; base += 16 * MT) {
-    uint32_t row[MT][XR];
+  uint32_t row[MT][XR];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+  for (int m = 0; m < MT; ++m)
 #pragma unroll
-      for (int i = 0; i < XR; ++i) {
-        const int j = base + 16 * m + B::load_row(i, lane);
-        const int t = j >= count ? 0 : a.routing == ROUTING_PLAN ? a.plan.tokens[slot * EXPERTS_MAX_M + j] : j;
-        row[m][i] = j < count ? (uint32_t)t * (uint32_t)a.K * 2u + B::load_byte(i, lane) : EX_NOWHERE;
-      }
-    B st[D];
-    auto load_block = [&](B& b, int kb, bool ok, bool tail, int d) {
-      b.load_tokens(a.x, (uint32_t)a.M * (uint32_t)a.K * 2u, row, kb, ok, tail, a.K, lane, lds_at + (uint32_t)(d * B::SLOT));
+    for (int i = 0; i < XR; ++i) {
+      const int j = 16 * m + B::load_row(i, lane);
+      const int t = j >= count ? 0 : a.routing == ROUTING_PLAN ? a.plan.pairs[slot * EXPERTS_MAX_M + j] / a.top_k : j;
+      row[m][i] = j < count ? (uint32_t)t * (uint32_t)a.K * 2u + B::load_byte(i, lane) : EX_NOWHERE;
+    }
+  B st[D];
+  auto load_block = [&](B& b, int kb, bool ok, bool tail, int d) {
+    b.load_tokens(a.x, (uint32_t)a.M * (uint32_t)a.K * 2u, row, kb, ok, tail, a.K, lane, lds_at + (uint32_t)(d * B::SLOT));
 #pragma unroll
-      for (int r = 0; r < R; ++r)
+    for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int n = 0; n < 2; ++n) b.load_weights(2 * r + n, r, rw[n], rs[n], kb, ok, tail, a.K, lane);
-    };
-    auto load = [&](B& b, int i, int d) {
-      const int kb = b0 + (i + rot < run ? i + rot : i + rot - run);
-      if (ragged && kb + 1 == blocks) load_block(b, kb, i < run, true, d);
-      else load_block(b, kb, i < run, false, d);
-    };
-    f32x4 acc[2 * R][MT];
+      for (int n = 0; n < 2; ++n) b.load_weights(2 * r + n, r, rw[n], rs[n], kb, ok, tail, a.K, lane);
+  };
+  auto load = [&](B& b, int i, int d) {
+    const int kb = b0 + (i + rot < run ? i + rot : i + rot - run);
+    if (ragged && kb + 1 == blocks) load_block(b, kb, i < run, true, d);
+    else load_block(b, kb, i < run, false, d);
+  };
+  f32x4 acc[2 * R][MT];
 #pragma unroll
-    for (int n = 0; n < 2 * R; ++n)
+  for (int n = 0; n < 2 * R; ++n)
 #pragma unroll
-      for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (base > 0) __syncthreads();  // the readers of the sums before
+    for (int m = 0; m < MT; ++m) acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int d = 0; d < D; ++d) load(st[d], d, d);
-    int i = 0;
-    for (; i + D < run; i += D)
+  for (int d = 0; d < D; ++d) load(st[d], d, d);
+  int i = 0;
+  for (; i + D < run; i += D)
 #pragma unroll
-      for (int d = 0; d < D; ++d) {
-        st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
-        load(st[d], i + d + D, d);
-      }
-    each_stage<D>([&](auto d) {
-      if (i + d < run) st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
-    });
-    if constexpr (B::DMA) wait_vmem<0>();  // stages past the end bring nothing, but they write: not into the sums
-    f32x4 both[R * MT][2];
+    for (int d = 0; d < D; ++d) {
+      st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
+      load(st[d], i + d + D, d);
+    }
+  each_stage<D>([&](auto d) {
+    if (i + d < run) st[d].multiply(int4, lds + (B::DMA ? d * B::SLOT : 0), lane, acc);
+  });
+  if constexpr (B::DMA) wait_vmem<0>();  // stages past the end bring nothing, but they write: not into the sums
+  f32x4 both[R * MT][2];
 #pragma unroll
-    for (int i = 0; i < R * MT; ++i)
+  for (int i = 0; i < R * MT; ++i)
 #pragma unroll
-      for (int n = 0; n < 2; ++n) both[i][n] = acc[i / MT * 2 + n][i % MT];
-    sum_wavefronts<NW>(both, smem, wave, lane, [&](int unit, const f32x4 (&sum)[2]) {
-      const int r = unit / MT, j = base + 16 * (unit - r * MT) + r16, first = (tile + r) * Q4_TILE + 4 * kg;
-      if (j >= count || first >= a.N) return;
-      float v[2][4];
+    for (int n = 0; n < 2; ++n) both[i][n] = acc[i / MT * 2 + n][i % MT];
+  sum_wavefronts<NW>(both, smem, wave, lane, [&](int unit, const f32x4 (&sum)[2]) {
+    const int r = unit / MT, j = 16 * (unit - r * MT) + r16, first = (tile + r) * Q4_TILE + 4 * kg;
+    if (j >= count || first >= a.N) return;
+    float v[2][4];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < 2; ++n) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[n][q] = sum[n][q];
-        if (a.bias[n]) add_w<T, 4>((const T*)a.bias[n] + first, v[n]);
-      }
-      float h[4];
-      act_fwd_w<4>(a.act, v[0], h);
+      for (int q = 0; q < 4; ++q) v[n][q] = sum[n][q];
+      if (a.bias[n]) add_w<T, 4>((const T*)a.bias[n] + first, v[n]);
+    }
+    float h[4];
+    act_fwd_w<4>(a.act, v[0], h);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) h[q] *= v[1][q];
-      int p = a.routing == ROUTING_SOLO ? slot : j;
-      if (a.routing == ROUTING_PLAN) {
-        const int t = a.plan.tokens[slot * EXPERTS_MAX_M + j];
-        p = t * a.top_k + a.plan.slot[slot * EXPERTS_MAX_M + t];
-      }
-      store_w<T, 4>((T*)a.h + (size_t)p * a.N + first, h);
-    });
-  }
+    for (int q = 0; q < 4; ++q) h[q] *= v[1][q];
+    const int p = a.routing == ROUTING_SOLO ? slot : a.routing == ROUTING_PLAN ? a.plan.pairs[slot * EXPERTS_MAX_M + j] : j;
+    store_w<T, 4>((T*)a.h + (size_t)p * a.N + first, h);
+  });
 }
 
 // ------------------------------------------------------------------ down
 // The blocks of all experts in use, one expert behind the other, are shared out evenly over the wavefronts.  What an
 // expert gives is added to a token's sum only where the token chose it (a weight that is not finite in one
 // expert stays out of the others' tokens).
+// GATHER: token tiles are an entry's tokens, as many as its expert has, and its products are added to the tokens' sums in LDS;
+// without, they are the call's tokens (M <= 16 * MT), whose sums are registers.  With more tokens than one tile holds and
+// few of them for each expert, most columns would be empty: M=50, K=2816, N=5136, 32 experts, 4 bits, one of them a
+// token, the whole layer 348 us without, 143 with.
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int down_lds() {
   constexpr int ring = NW * Block<T, G, R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 1>() * 1024;
   return ring > part ? ring : part;
 }
-template <typename T, int G, int MT, int XR, int R, int NW, int D>
+template <typename T, int G, int MT, int XR, int R, int NW, int D, bool GATHER>
 __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
   typedef Block<T, G, R, MT, XR> B;
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, kg = lane >> 4, tile = (int)blockIdx.x * R;
   const int pairs = a.M * a.top_k;
-  // tables: the experts' numbers, the pairs' weights, the slots
+  // tables: the entries' experts, the pairs' weights, the slots or (GATHER) the pairs of each entry and their number
   int in_use = 1;
-  int* const numbers = (int*)(smem + down_lds<T, G, MT, XR, R, NW, D>());
+  char* at = smem + down_lds<T, G, MT, XR, R, NW, D>();
+  float* const own = (float*)at + wave * (R * Q4_TILE) * a.M;  // GATHER: the wavefront's sums, [M][R * 16]
+  if constexpr (GATHER) {
+    for (int i = lane; i < a.M * R * Q4_TILE; i += 64) own[i] = 0.f;
+    at += (size_t)NW * a.M * R * Q4_TILE * sizeof(float);
+  }
+  int* const numbers = (int*)at;
   float* weight = nullptr;
   int8_t* slots = nullptr;
+  uint16_t* which = nullptr;
+  uint8_t* counts = nullptr;
   if (a.routing == ROUTING_PLAN) {
     in_use = a.plan.active[0];
     const int rows = a.M == 1 ? pairs : in_use;  // (all there can be: their loads do not wait for the number)
     weight = (float*)(numbers + rows);
-    slots = (int8_t*)(weight + pairs);
     for (int i = threadIdx.x; i < rows; i += NW * 64) numbers[i] = a.plan.active[1 + i];
     for (int i = threadIdx.x; i < pairs; i += NW * 64) weight[i] = a.plan.weight[i];
-    for (int i = threadIdx.x; i < rows * (EXPERTS_MAX_M / 4); i += NW * 64)
-      ((int*)slots)[i] = ((const int*)a.plan.slot)[i];
+    if constexpr (GATHER) {
+      which = (uint16_t*)(weight + pairs);
+      counts = (uint8_t*)(which + rows * 16 * MT);
+      for (int i = threadIdx.x; i < rows * 16 * MT; i += NW * 64)
+        which[i] = a.plan.pairs[i / (16 * MT) * EXPERTS_MAX_M + i % (16 * MT)];
+      for (int i = threadIdx.x; i < rows; i += NW * 64) counts[i] = a.plan.count[i];
+    } else {
+      slots = (int8_t*)(weight + pairs);
+      for (int i = threadIdx.x; i < rows * (EXPERTS_MAX_M / 4); i += NW * 64)
+        ((int*)slots)[i] = ((const int*)a.plan.slot)[i];
+    }
     __syncthreads();
   }
   const int blocks = (a.N + B::COLS - 1) / B::COLS;
@@ -567,10 +588,12 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
   char* const lds = smem + wave * B::lds_bytes(D);
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_void*)lds;
 
-  // choice of token row t that expert e is, or -1
-  auto slot_of = [&](int e, int t) -> int {
-    if (t >= a.M) return -1;
-    return a.routing == ROUTING_DENSE ? 0 : slots[e * EXPERTS_MAX_M + t];
+  // row of h behind column j of entry e, or -1
+  auto pair_of = [&](int e, int j) -> int {
+    if constexpr (GATHER) return j < counts[e] ? which[e * (16 * MT) + j] : -1;
+    if (j >= a.M || a.routing == ROUTING_DENSE) return j < a.M ? j : -1;
+    const int s = slots[e * EXPERTS_MAX_M + j];
+    return s < 0 ? -1 : j * a.top_k + s;
   };
   // where loads go on: expert, block of it
   const int first_e = b0 / blocks, first_b = b0 - first_e * blocks;
@@ -586,8 +609,8 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < XR; ++i) {
-        const int t = 16 * m + B::load_row(i, lane), s = slot_of(e, t);
-        row[m][i] = s < 0 ? EX_NOWHERE : (uint32_t)(t * a.top_k + s) * (uint32_t)a.N * 2u + B::load_byte(i, lane);
+        const int p = pair_of(e, 16 * m + B::load_row(i, lane));
+        row[m][i] = p < 0 ? EX_NOWHERE : (uint32_t)p * (uint32_t)a.N * 2u + B::load_byte(i, lane);
       }
   };
   f32x4 acc[R][MT], sum[R * MT][1];
@@ -617,15 +640,25 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
     auto fold = [&]() {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const int t = 16 * m + r16, s = slot_of(me, t);
-        const float w = s < 0 ? 0.f : a.routing == ROUTING_DENSE ? 1.f : weight[t * a.top_k + s];
+        const int p = pair_of(me, 16 * m + r16);
+        const float w = p < 0 ? 0.f : a.routing == ROUTING_DENSE ? 1.f : weight[p];
 #pragma unroll
-        for (int n = 0; n < R; ++n)
+        for (int n = 0; n < R; ++n) {
+          if constexpr (GATHER) {
+            if (p >= 0) {
+              f32x4* const to = (f32x4*)(own + (p / a.top_k * R + n) * Q4_TILE + 4 * kg);
+              f32x4 v = *to;
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            if (s >= 0) sum[n * MT + m][0][r] += w * acc[n][m][r];
-            acc[n][m][r] = 0.f;
+              for (int r = 0; r < 4; ++r) v[r] += w * acc[n][m][r];
+              *to = v;
+            }
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (p >= 0) sum[n * MT + m][0][r] += w * acc[n][m][r];
           }
+          acc[n][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
       }
     };
 #pragma unroll
@@ -653,22 +686,35 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
       }
     });
   }
-  if constexpr (B::DMA) wait_vmem<0>();  // (as in gate/up)
-  sum_wavefronts<NW>(sum, smem, wave, lane, [&](int unit, const f32x4 (&v)[1]) {
-    const int n = unit / MT, t = 16 * (unit - n * MT) + r16, first = (tile + n) * Q4_TILE + 4 * kg;
+  auto done = [&](int t, int first, f32x4 v) {
     if (t >= a.M || first >= a.K) return;
     if (gridDim.y > 1) {
-      *(f32x4*)(a.partial + ((size_t)blockIdx.y * a.M + t) * a.K + first) = v[0];
+      *(f32x4*)(a.partial + ((size_t)blockIdx.y * a.M + t) * a.K + first) = v;
       return;
     }
-    float y[4] = {v[0][0], v[0][1], v[0][2], v[0][3]};
     if (a.y_f32) {  // (router logits: rows of whole fours)
-      *(f32x4*)((float*)a.y + (size_t)t * a.K + first) = v[0];
+      *(f32x4*)((float*)a.y + (size_t)t * a.K + first) = v;
       return;
     }
+    float y[4] = {v[0], v[1], v[2], v[3]};
     if (a.bias[2]) add_w<T, 4>((const T*)a.bias[2] + first, y);
     store_w<T, 4>((T*)a.y + (size_t)t * a.K + first, y);
-  });
+  };
+  if constexpr (B::DMA) wait_vmem<0>();  // (as in gate/up)
+  if constexpr (GATHER) {
+    __syncthreads();
+    const float* const all = own - wave * (R * Q4_TILE) * a.M;
+    for (int i = threadIdx.x; i < a.M * R * 4; i += NW * 64) {
+      f32x4 v = *(const f32x4*)(all + i * 4);
+      for (int w = 1; w < NW; ++w) v += *(const f32x4*)(all + w * (R * Q4_TILE) * a.M + i * 4);
+      done(i / (R * 4), tile * Q4_TILE + i % (R * 4) * 4, v);
+    }
+  } else {
+    sum_wavefronts<NW>(sum, smem, wave, lane, [&](int unit, const f32x4 (&v)[1]) {
+      const int n = unit / MT;
+      done(16 * (unit - n * MT) + r16, (tile + n) * Q4_TILE + 4 * kg, v[0]);
+    });
+  }
 }
 
 // Second stage of a down projection whose reduction was split over workgroups: the parts' sums, in their order.
@@ -687,8 +733,15 @@ __global__ void __launch_bounds__(256) experts_join_kernel(ExpertArgs a, int par
   store_w<T, 4>((T*)a.y + i, y);
 }
 
-// Experts that a call can use.
+// Experts that a call can use, and entries of its plan.
 static int experts_at_most(const ExpertArgs& a) { return a.E < a.M * a.top_k ? a.E : a.M * a.top_k; }
+static int entries_at_most(const ExpertArgs& a) { return a.routing == ROUTING_DENSE ? 1 : expert_entries(a.M, a.E, a.top_k); }
+// Token tiles of an entry.  Experts of a plan: one, which nearly all of them fit in, up to ten tokens for each on average,
+// then two (weights of one with more tokens are read again).
+static int token_tiles(const ExpertArgs& a) {
+  if (a.routing == ROUTING_DENSE || a.M <= 16) return (a.M + 15) / 16;
+  return a.M * a.top_k <= 10 * a.E ? 1 : 2;
+}
 static double weight_bytes(const ExpertArgs& a, int group) {
   return (double)experts_at_most(a) * a.K * a.N * (group ? 0.5 + 2.0 / group : 2.0);
 }
@@ -700,18 +753,20 @@ static hipError_t run_gateup(const ExpertArgs& a, hipStream_t s) {
   if constexpr (LDS > 64 * 1024)
     if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, LDS>, s)) return e;
   const int strips = (a.N + R * Q4_TILE - 1) / (R * Q4_TILE);
-  hipLaunchKernelGGL(kern, dim3((unsigned)(strips * experts_at_most(a))), dim3(NW * 64), LDS, s, a);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(strips * entries_at_most(a))), dim3(NW * 64), LDS, s, a);
   return hipGetLastError();
 }
-template <typename T, int G, int MT, int XR, int R, int NW, int D>
+template <typename T, int G, int MT, int XR, int R, int NW, int D, bool GATHER = false>
 static hipError_t run_down(const ExpertArgs& a, int parts, hipStream_t s) {
-  constexpr int LDS = down_lds<T, G, MT, XR, R, NW, D>();
-  const int tables = a.routing == ROUTING_DENSE ? 0 : experts_at_most(a) * (4 + EXPERTS_MAX_M) + a.M * a.top_k * 4;
-  constexpr auto kern = experts_down_kernel<T, G, MT, XR, R, NW, D>;
-  if (LDS + tables > 64 * 1024)
-    if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, LDS + EX_TABLES>, s)) return e;
+  constexpr int LDS = down_lds<T, G, MT, XR, R, NW, D>(), SUMS = GATHER ? NW * R * Q4_TILE * 4 : 0,
+                MOST = LDS + ex_tables_at_most(GATHER, MT) + SUMS * EXPERTS_MAX_M;
+  static_assert(MOST <= 160 * 1024, "a workgroup has 160 KiB of LDS");
+  const int lds = LDS + (a.routing == ROUTING_DENSE ? 0 : ex_tables(entries_at_most(a), GATHER, MT, a.M * a.top_k)) + SUMS * a.M;
+  constexpr auto kern = experts_down_kernel<T, G, MT, XR, R, NW, D, GATHER>;
+  if (lds > 64 * 1024)
+    if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, MOST>, s)) return e;
   const dim3 grid((unsigned)((a.K + R * Q4_TILE - 1) / (R * Q4_TILE)), (unsigned)parts);
-  hipLaunchKernelGGL(kern, grid, dim3(NW * 64), (unsigned)(LDS + tables), s, a);
+  hipLaunchKernelGGL(kern, grid, dim3(NW * 64), (unsigned)lds, s, a);
   if (hipError_t e = hipGetLastError()) return e;
   if (parts > 1) hipLaunchKernelGGL(experts_join_kernel<T>, dim3((unsigned)(((int64_t)a.M * a.K / 4 + 255) / 256)), dim3(256), 0, s, a, parts);
   return hipGetLastError();
@@ -720,18 +775,19 @@ static hipError_t run_down(const ExpertArgs& a, int parts, hipStream_t s) {
 // Gate/up.
 template <typename T, int G>
 static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
-  const bool few = (a.N + Q4_TILE - 1) / Q4_TILE * experts_at_most(a) <= (a.M <= 16 ? 4 : 2) * a.cus;
+  const int mt = token_tiles(a);
+  const bool few = (a.N + Q4_TILE - 1) / Q4_TILE * entries_at_most(a) <= (mt == 1 ? 4 : 2) * a.cus;
   if constexpr (G == 0) {
     if (a.M <= 8) return run_gateup<T, 0, 1, 1, 1, 4, 2>(a, s);
-    if (a.M <= 16) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
+    if (mt == 1) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
     return run_gateup<T, 0, 2, 2, 2, 4, 1>(a, s);
   } else {
     if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 2>(a, s);
-    if (a.M <= 16) return few ? run_gateup<T, G, 1, 4, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
+    if (mt == 1) return few ? run_gateup<T, G, 1, 4, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
     // More than one token tile: as many tiles and wavefronts as the registers hold, fewer with finer groups.
     constexpr bool coarse = G == 128, fine = G == 32;
-    if (a.M <= 32) return few ? run_gateup<T, G, 2, 4, fine ? 1 : 2, 8, 1>(a, s) : run_gateup<T, G, 2, 4, 3, coarse ? 8 : 4, 1>(a, s);
-    if (a.M <= 48) return run_gateup<T, G, 3, 4, fine ? 1 : 2, 4, 1>(a, s);
+    if (mt == 2) return few ? run_gateup<T, G, 2, 4, fine ? 1 : 2, 8, 1>(a, s) : run_gateup<T, G, 2, 4, 3, coarse ? 8 : 4, 1>(a, s);
+    if (mt == 3) return run_gateup<T, G, 3, 4, fine ? 1 : 2, 4, 1>(a, s);
     return few ? run_gateup<T, G, 4, 4, 1, 4, 1>(a, s) : run_gateup<T, G, 4, 4, fine ? 2 : 3, 4, 1>(a, s);
   }
 }
@@ -744,7 +800,7 @@ static DownPlan plan_down(const ExpertArgs& a, int group) {
   const bool large = weight_bytes(a, group) >= 48e6;
   const int tiles = (a.K + Q4_TILE - 1) / Q4_TILE;
   DownPlan p = {1, 1};
-  if (a.M > 16) p.tiles = a.M > 48 && group == 32 ? 1 : 2;  // (two of the finest groups would spill)
+  if (a.M > 16) p.tiles = a.M > 48 && group == 32 && a.routing == ROUTING_DENSE ? 1 : 2;  // (two of the finest groups would spill)
   else if (group && a.M > 4 && (large || tiles > 2 * a.cus)) p.tiles = 4;
   if (a.M > 16 || large) {
     p.parts = a.cus / ((tiles + p.tiles - 1) / p.tiles);
@@ -762,6 +818,8 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
   const int parts = a.partial ? p.parts : 1;
   constexpr int FEW = G ? 4 : 8, ALL = 16 / FEW;
   const bool few = a.M <= FEW;
+  if (a.M > 16 && a.routing == ROUTING_PLAN)
+    return token_tiles(a) == 1 ? run_down<T, G, 1, ALL, 2, 8, 1, true>(a, parts, s) : run_down<T, G, 2, ALL, 2, 8, 1, true>(a, parts, s);
   if (a.M > 48) return run_down<T, G, 4, ALL, G == 32 ? 1 : 2, 4, 1>(a, parts, s);
   if (a.M > 32) return run_down<T, G, 3, ALL, 2, G == 32 ? 4 : 8, 1>(a, parts, s);
   if (a.M > 16) return run_down<T, G, 2, ALL, 2, 8, 1>(a, parts, s);
@@ -777,7 +835,7 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
   if (blocks < 32) return few ? run_down<T, G, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s);
   return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
 }
-bool experts_solo(const ExpertArgs& a) { return a.M == 1 && a.E <= SOLO_MAX_E; }
+bool experts_solo(int M, int E) { return M == 1 && E <= SOLO_MAX_E; }
 
 template <typename T>
 hipError_t launch_experts_gateup(const ExpertArgs& a, int group, hipStream_t s) {
@@ -910,11 +968,11 @@ __global__ void __launch_bounds__(256) route_kernel(const L* logits, float* weig
   }
 }
 
-// The routing of at most 64 tokens, in one workgroup.
+// The routing of at most 64 tokens, in one workgroup.  cap: tokens of an entry.
 template <int VPL, typename L>
-__global__ void __launch_bounds__(1024) plan_kernel(const L* logits, ExpertPlan p, int M, int E, int top_k, int normalize) {
+__global__ void __launch_bounds__(1024) plan_kernel(const L* logits, ExpertPlan p, int M, int E, int top_k, int normalize, int cap) {
   __shared__ uint32_t who[EXPERTS_MAX_E][2];  // tokens of an expert, a bit each
-  __shared__ int index[EXPERTS_MAX_E];        // of an expert among those in use
+  __shared__ int index[EXPERTS_MAX_E];        // of an expert's first entry
   __shared__ short chosen[EXPERTS_MAX_M * EXPERTS_MAX_K];
   __shared__ int in_wave[16];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -931,31 +989,38 @@ __global__ void __launch_bounds__(1024) plan_kernel(const L* logits, ExpertPlan 
     }
   }
   __syncthreads();
-  const bool used = tid < E && (who[tid][0] | who[tid][1]) != 0;
-  const uint64_t ballot = __ballot(used);
-  if (lane == 0) in_wave[wave] = __popcll(ballot);
+  // entries of the experts before this thread's
+  const int tokens = tid < E ? __popc(who[tid][0]) + __popc(who[tid][1]) : 0;
+  const int entries = (tokens + cap - 1) / cap;
+  int upto = entries;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) in_wave[wave] = upto;
   __syncthreads();
-  int before = 0, total = 0;
+  int before = upto - entries, total = 0;
   for (int w = 0; w < 16; ++w) {
     if (w < wave) before += in_wave[w];
     total += in_wave[w];
   }
-  if (used) {
-    const int i = before + __popcll(ballot & ((1ull << lane) - 1));
-    index[tid] = i;
-    p.active[1 + i] = tid;
-    p.count[i] = (uint8_t)(__popc(who[tid][0]) + __popc(who[tid][1]));
+  if (tid < E) index[tid] = before;
+  for (int q = 0; q < entries; ++q) {
+    p.active[1 + before + q] = tid;
+    p.count[before + q] = (uint8_t)(tokens - q * cap < cap ? tokens - q * cap : cap);
   }
   if (tid == 0) p.active[0] = total;
-  for (int i = tid; i < total * (EXPERTS_MAX_M / 4); i += 1024) ((int*)p.slot)[i] = -1;
+  if (M <= 16)
+    for (int i = tid; i < total * (EXPERTS_MAX_M / 4); i += 1024) ((int*)p.slot)[i] = -1;
   __syncthreads();
   for (int i = tid; i < M * top_k; i += 1024) {
     const int e = chosen[i], t = i / top_k;
     if (e < 0) continue;
     const uint64_t mask = (uint64_t)who[e][1] << 32 | who[e][0];
-    const int at = index[e] * EXPERTS_MAX_M;
-    p.tokens[at + __popcll(mask & ((1ull << t) - 1))] = (uint8_t)t;
-    p.slot[at + t] = (int8_t)(i - t * top_k);
+    const int nth = __popcll(mask & ((1ull << t) - 1)), entry = index[e] + nth / cap;
+    p.pairs[entry * EXPERTS_MAX_M + nth % cap] = (uint16_t)i;
+    if (M <= 16) p.slot[entry * EXPERTS_MAX_M + t] = (int8_t)(i - t * top_k);
   }
 }
 
@@ -979,9 +1044,10 @@ hipError_t launch_route(const L* logits, float* weights, int64_t* experts, int64
   return hipGetLastError();
 }
 template <typename L>
-hipError_t launch_experts_plan(const L* logits, const ExpertPlan& plan, int M, int E, int top_k, int normalize, hipStream_t s) {
-#define CALL(V) hipLaunchKernelGGL((plan_kernel<V, L>), dim3(1), dim3(1024), 0, s, logits, plan, M, E, top_k, normalize)
-  GMLP_BY_EXPERTS(E, CALL);
+hipError_t launch_experts_plan(const L* logits, const ExpertArgs& a, hipStream_t s) {
+#define CALL(V) \
+  hipLaunchKernelGGL((plan_kernel<V, L>), dim3(1), dim3(1024), 0, s, logits, a.plan, a.M, a.E, a.top_k, a.normalize, 16 * token_tiles(a))
+  GMLP_BY_EXPERTS(a.E, CALL);
 #undef CALL
   return hipGetLastError();
 }
@@ -1095,10 +1161,10 @@ hipError_t launch_q4_dequantize(const uint8_t* codes, const T* scales, T* w, int
   template hipError_t launch_q4_quantize<T>(const T*, uint8_t*, T*, int64_t, int64_t, int64_t, int, hipStream_t);             \
   template hipError_t launch_q4_dequantize<T>(const uint8_t*, const T*, T*, int64_t, int64_t, int64_t, int, hipStream_t);     \
   template hipError_t launch_route<T>(const T*, float*, int64_t*, int64_t, int, int, int, hipStream_t);                       \
-  template hipError_t launch_experts_plan<T>(const T*, const ExpertPlan&, int, int, int, int, hipStream_t);
+  template hipError_t launch_experts_plan<T>(const T*, const ExpertArgs&, hipStream_t);
 GMLP_INSTANTIATE(f16)
 GMLP_INSTANTIATE(bf16)
 template hipError_t launch_route<float>(const float*, float*, int64_t*, int64_t, int, int, int, hipStream_t);
-template hipError_t launch_experts_plan<float>(const float*, const ExpertPlan&, int, int, int, int, hipStream_t);
+template hipError_t launch_experts_plan<float>(const float*, const ExpertArgs&, hipStream_t);
 
 }  // namespace gmlp

@@ -17,14 +17,20 @@ struct ExpertWeights {
   const void* scales;  // 4-bit weights only
 };
 
-// The routing of a call, which plan_kernel makes of the logits: device pointers into the caller's workspace.
+// The routing of a call, which plan_kernel makes of the logits: device pointers into the caller's workspace.  An entry is an
+// expert that is in use with some of its tokens, all of them up to the token tiles that the kernels take at once; one
+// with more tokens has several.  Entries are in ascending order of expert and token.
 struct ExpertPlan {
-  int* active;      // [1 + experts]: how many experts any token chose, then their numbers in ascending order
-  uint8_t* count;   // [active experts]: tokens of the expert
-  uint8_t* tokens;  // [active experts][EXPERTS_MAX_M]: which, ascending
-  int8_t* slot;     // [active experts][EXPERTS_MAX_M]: the token's how-manieth choice the expert is, -1: not chosen
+  int* active;      // [1 + entries]: how many, then their experts
+  uint8_t* count;   // [entries]: tokens
+  uint16_t* pairs;  // [entries][EXPERTS_MAX_M]: which, as token * top_k + the choice that the expert is
+  int8_t* slot;     // [entries][EXPERTS_MAX_M], M <= 16: of a token, the choice that the expert is, -1: not chosen
   float* weight;    // [M * top_k]
 };
+inline int expert_entries(int M, int E, int top_k) {  // at most
+  const int pairs = M * top_k, most = M > 16 ? E + pairs / 16 : E;
+  return pairs < most ? pairs : most;
+}
 
 // Who runs through which expert: every token through the only one, with weight 1; as the plan says; or (gate/up), of one token,
 // as the kernel finds from the logits itself, which then leaves the plan.
@@ -47,7 +53,7 @@ struct ExpertArgs {
 };
 
 // Whether ROUTING_SOLO takes the call, and the bytes of `partial` that launch_experts_down asks for (it does with none).
-bool experts_solo(const ExpertArgs& a);
+bool experts_solo(int M, int E);
 size_t experts_partial_bytes(const ExpertArgs& a, int group);
 
 // Gate/up, then down, on 16-bit (group = 0) or 4-bit weights (group = 32, 64 or 128).
@@ -57,7 +63,7 @@ hipError_t launch_experts_gateup(const ExpertArgs& a, int group, hipStream_t s);
 template <typename T>
 hipError_t launch_experts_down(const ExpertArgs& a, int group, hipStream_t s);
 template <typename L>
-hipError_t launch_experts_plan(const L* logits, const ExpertPlan& plan, int M, int E, int top_k, int normalize, hipStream_t s);
+hipError_t launch_experts_plan(const L* logits, const ExpertArgs& a, hipStream_t s);
 template <typename L>
 hipError_t launch_route(const L* logits, float* weights, int64_t* experts, int64_t M, int E, int top_k, int normalize, hipStream_t s);
 
