@@ -335,7 +335,8 @@ int gmlp_hidden_bwd(const void* dh, const void* x, const void* w_gate, const voi
  *   is n = 0, and scale 0 where a whole group is padding.  gmlp_q4_dequantize: w = scale·n rounded to dtype.
  * gmlp_q4_linear_fwd: y[M,C] = x[M,R]·Wᵀ + bias, W [C,R] 4-bit; bias may be NULL.  The products are of scale·n itself, not
  *   of its rounding.
- * gmlp_q4_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) in dtype [M,N] (scratch), y = h·W_downᵀ + b_down.
+ * gmlp_q4_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) in dtype, y = h·W_downᵀ + b_down.  `h` is scratch
+ *   of M·N elements, 2·M·N for M <= 8: of so few tokens h is kept as two 16-bit values, its rounding and the rest.
  * workspace: partial sums of a reduction that is split over workgroups, gmlp_q4_workspace_bytes(M, R, C, ...) bytes for the
  *   linear layer and (M, R = N, C = K, ...) for the MLP.  NULL, 0 or fewer bytes are accepted and only slower.
  */

@@ -467,6 +467,29 @@ def test_moe_mlp(M, K, N, E, k, bits, group, act, normalize, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("M", [1, 2, 3, 5, 8])
+def test_hidden_states_of_a_few_tokens_keep_more_than_16_bits(M, bits, dtype):
+    """Only y is rounded: its 2-norm is off by what one rounding costs (at most 0.6 u), not by two roundings' 0.8 u."""
+    dev, K, N, E = device(), 1032, 392, 4
+    g = gen(M)
+    x, logits = normal((M, K), 1.0, dtype, g), normal((M, E), 1.0, torch.float32, g)
+    ws, one = experts_of(E, K, N, bits, 64, dtype, g)
+    ref, bound = moe64(x.double(), logits, 2, True, "silu", dtype, one)
+    hold(moe.moe_mlp_fwd(x.to(dev), logits.to(dev), *ws, 2), ref, bound, dtype, 1)
+    if bits == 4:
+        y, off = mlp64(x.double(), *(v for w in one(1) for v in (w, None)), "silu", dtype)
+        hold(quant.q4_mlp_fwd(x.to(dev), *(v for w in ws for v in (sliced(w, 1), None))), y, off + U[dtype] * y.abs() + SUB[dtype], dtype, 1)
+    else:
+        ws[2][:, 9, 17] = math.inf  # the rest of a hidden state can be 0: infinite, not NaN
+        y = moe.moe_mlp_fwd(x.to(dev), logits.to(dev), *ws, 1).cpu()
+        assert torch.isinf(y[:, 9]).all()
+        y[:, 9] = 0
+        assert torch.isfinite(y).all()
+
+
+@gpu
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("M", [1, 16, 50])
 def test_moe_mlp_with_masked_experts(M, bits):

@@ -523,6 +523,14 @@ __global__ void __launch_bounds__(NW * 64, MT > 1 && MT < 4 && R <= 2 ? 2 : 1) e
     for (int q = 0; q < 4; ++q) h[q] *= v[1][q];
     const int p = a.routing == ROUTING_SOLO ? slot : a.routing == ROUTING_PLAN ? a.plan.pairs[slot * EXPERTS_MAX_M + j] : j;
     store_w<T, 4>((T*)a.h + (size_t)p * a.N + first, h);
+    if (a.h_low) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float kept = (float)(T)h[q];
+        h[q] = __builtin_isfinite(kept) ? h[q] - kept : 0.f;
+      }
+      store_w<T, 4>((T*)a.h + (size_t)(a.M * a.top_k + p) * a.N + first, h);
+    }
   });
 }
 
@@ -534,6 +542,10 @@ __global__ void __launch_bounds__(NW * 64, MT > 1 && MT < 4 && R <= 2 ? 2 : 1) e
 // without, they are the call's tokens (M <= 16 * MT), whose sums are registers.  With more tokens than one tile holds and
 // few of them for each expert, most columns would be empty: M=50, K=2816, N=5136, 32 experts, 4 bits, one of them a
 // token, the whole layer 348 us without, 143 with.
+// Up to 8 tokens (h_low): half of the product's 16 columns would be empty, so every hidden state comes as two 16-bit values, its
+// rounding and what that left, in columns 2t and 2t + 1.  Rounding h to 16 bits alone costs as much as rounding y does;
+// with more tokens it is rounded, as FusedGatedMLP's is: a second plane would double tokens' loads and products.  bf16, 1 token,
+// K=4096, N=11008, 4 bits: 11.9 -> 12.5 us, y off by 0.0017 of its norm instead of 0.0024.
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int down_lds() {
   constexpr int ring = NW * Block<T, G, R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 1>() * 1024;
@@ -545,7 +557,7 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
   extern __shared__ __align__(16) char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, kg = lane >> 4, tile = (int)blockIdx.x * R;
-  const int pairs = a.M * a.top_k;
+  const int pairs = a.M * a.top_k, low = MT == 1 && !GATHER ? a.h_low : 0;
   // tables: the entries' experts, the pairs' weights, the slots or (GATHER) the pairs of each entry and their number
   int in_use = 1;
   char* at = smem + down_lds<T, G, MT, XR, R, NW, D>();
@@ -609,8 +621,8 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int i = 0; i < XR; ++i) {
-        const int p = pair_of(e, 16 * m + B::load_row(i, lane));
-        row[m][i] = p < 0 ? EX_NOWHERE : (uint32_t)p * (uint32_t)a.N * 2u + B::load_byte(i, lane);
+        const int j = 16 * m + B::load_row(i, lane), p = pair_of(e, j >> low);
+        row[m][i] = p < 0 ? EX_NOWHERE : (uint32_t)(p + (j & low) * pairs) * (uint32_t)a.N * 2u + B::load_byte(i, lane);
       }
   };
   f32x4 acc[R][MT], sum[R * MT][1];
@@ -622,7 +634,7 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
     enter();
     B st[D];
     auto load_block = [&](B& b, bool ok, bool tail, int d) {
-      b.load_tokens(a.h, (uint32_t)pairs * (uint32_t)a.N * 2u, row, lb, ok, tail, a.N, lane, lds_at + (uint32_t)(d * B::SLOT));
+      b.load_tokens(a.h, (uint32_t)(pairs << low) * (uint32_t)a.N * 2u, row, lb, ok, tail, a.N, lane, lds_at + (uint32_t)(d * B::SLOT));
 #pragma unroll
       for (int n = 0; n < R; ++n) b.load_weights(n, n, rw, rs, lb, ok, tail, a.N, lane);
     };
@@ -640,7 +652,7 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
     auto fold = [&]() {
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        const int p = pair_of(me, 16 * m + r16);
+        const int p = pair_of(me, (16 * m + r16) >> low);
         const float w = p < 0 ? 0.f : a.routing == ROUTING_DENSE ? 1.f : weight[p];
 #pragma unroll
         for (int n = 0; n < R; ++n) {
@@ -711,8 +723,16 @@ __global__ void __launch_bounds__(NW * 64) experts_down_kernel(ExpertArgs a) {
     }
   } else {
     sum_wavefronts<NW>(sum, smem, wave, lane, [&](int unit, const f32x4 (&v)[1]) {
-      const int n = unit / MT;
-      done(16 * (unit - n * MT) + r16, (tile + n) * Q4_TILE + 4 * kg, v[0]);
+      const int n = unit / MT, j = 16 * (unit - n * MT) + r16;
+      f32x4 y = v[0];
+      if (low) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float rest = __shfl_xor(y[r], 1);
+          y[r] += __builtin_isfinite(y[r]) ? rest : 0.f;  // (an infinite weight's product with a rest of 0)
+        }
+      }
+      done(j & low ? a.M : j >> low, (tile + n) * Q4_TILE + 4 * kg, y);
     });
   }
 }
@@ -817,7 +837,7 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
   const DownPlan p = plan_down(a, G);
   const int parts = a.partial ? p.parts : 1;
   constexpr int FEW = G ? 4 : 8, ALL = 16 / FEW;
-  const bool few = a.M <= FEW;
+  const bool few = a.M << a.h_low <= FEW;
   if (a.M > 16 && a.routing == ROUTING_PLAN)
     return token_tiles(a) == 1 ? run_down<T, G, 1, ALL, 2, 8, 1, true>(a, parts, s) : run_down<T, G, 2, ALL, 2, 8, 1, true>(a, parts, s);
   if (a.M > 48) return run_down<T, G, 4, ALL, G == 32 ? 1 : 2, 4, 1>(a, parts, s);

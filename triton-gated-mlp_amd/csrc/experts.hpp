@@ -40,11 +40,11 @@ struct ExpertArgs {
   const void* x;      // [M, K]
   const void* bias[3];
   ExpertWeights gate, up, down;
-  void* h;            // [M * top_k, N]
+  void* h;            // [M * top_k, N]; h_low: behind it another one, of what rounding to 16 bits left
   void* y;            // [M, K], of the activations' type or (y_f32, without partial) float
   float* partial;     // [parts][M, K], where the down projection's reduction is split
   int M, K, N, E, top_k, act;
-  int y_f32;
+  int y_f32, h_low;
   int routing;        // Routing
   int cus;            // compute units of the device
   const void* logits; // [M, E] of a GMLP_* type
@@ -52,7 +52,8 @@ struct ExpertArgs {
   ExpertPlan plan;
 };
 
-// Whether ROUTING_SOLO takes the call, and the bytes of `partial` that launch_experts_down asks for (it does with none).
+// Whether the hidden states of M tokens come as two 16-bit values each, whether ROUTING_SOLO takes the call, and the bytes of `partial` that launch_experts_down asks for (it does with none).
+inline int experts_h_low(int64_t M) { return M <= 8; }
 bool experts_solo(int M, int E);
 size_t experts_partial_bytes(const ExpertArgs& a, int group);
 
