@@ -361,7 +361,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
  *   weights NaN, as softmax does.  logits, weights and experts need the alignment of their elements only.  1 <= top_k <= 16, top_k <= E <= 512, any M.
  * gmlp_moe_fwd: y[m] = sum over m's experts e of weight·MLP_e(x[m]), MLP_e the gated MLP with w_gate[e], w_up[e] [N,K] and
  *   w_down[e] [K,N] (group = 0: dtype, s_* NULL; otherwise 4-bit codes with scales s_*); the hidden states are rounded to
- *   dtype, the sum over experts is fp32.  Experts that no token chose are not read; one with weight 0 through -inf is not
+ *   dtype (M > 8; two values each up to 8), the sum over experts is fp32.  Experts that no token chose are not read; one with weight 0 through -inf is not
  *   run.  M <= 64.  workspace: gmlp_moe_workspace_bytes.
  */
 int gmlp_moe_logits(const void* x, const void* w_router, float* logits, int64_t M, int64_t K, int64_t E, int dtype, void* stream);

@@ -424,6 +424,11 @@ __device__ __forceinline__ void sum_wavefronts(const f32x4 (&acc)[NU][U], char* 
 }
 
 // ------------------------------------------------------------------ gate/up
+// A workgroup: 16 * R rows of each matrix of one expert.  What bounds it is the weights' stream: 16 bits, 8 experts of K=4096,
+// N=14336, one token on two of them, 470 MB in 76 us (6.2 TB/s; a device copy moves 5.3); 4 bits, all 8 of them for
+// 16 tokens, 480 MB in 80 us (6.0 TB/s).  One matrix of 4 bits is shorter than its start and end: K=2048, N=5632, one token, 12 MB
+// in 6.5 us.  M=48, K=4096, N=11008, groups of 64, 48 MB in 25 us: there the conversions and the two workgroups that
+// fit a CU bound it.
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int gateup_lds() {
   constexpr int ring = NW * Block<T, G, 2 * R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 2>() * 2 * 1024;
@@ -542,10 +547,13 @@ __global__ void __launch_bounds__(NW * 64, MT > 1 && MT < 4 && R <= 2 ? 2 : 1) e
 // without, they are the call's tokens (M <= 16 * MT), whose sums are registers.  With more tokens than one tile holds and
 // few of them for each expert, most columns would be empty: M=50, K=2816, N=5136, 32 experts, 4 bits, one of them a
 // token, the whole layer 348 us without, 143 with.
+// 16 bits, two experts of K=4096, N=14336 for a token, 235 MB in 40 us (5.9 TB/s); 4 bits, eight for 16 tokens, 240 MB in
+// 45 us (5.3 TB/s) and 4.5 for the parts' sum; one matrix, K=8192, N=28672, 16 tokens, 121 MB in 25 us (4.8 TB/s); K=2048, N=5632,
+// one token, 6 MB in 5.5 us, mostly its start and the join of the wavefronts.
 // Up to 8 tokens (h_low): half of the product's 16 columns would be empty, so every hidden state comes as two 16-bit values, its
 // rounding and what that left, in columns 2t and 2t + 1.  Rounding h to 16 bits alone costs as much as rounding y does;
 // with more tokens it is rounded, as FusedGatedMLP's is: a second plane would double tokens' loads and products.  bf16, 1 token,
-// K=4096, N=11008, 4 bits: 11.9 -> 12.5 us, y off by 0.0017 of its norm instead of 0.0024.
+// K=2048, N=5632, 4 bits: 11.9 -> 12.5 us, y off by 0.0017 of its norm instead of 0.0024.
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int down_lds() {
   constexpr int ring = NW * Block<T, G, R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 1>() * 1024;
