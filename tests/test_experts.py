@@ -249,6 +249,7 @@ def q4(shape, group, dtype, g):
         (1, 8, 8, 128, False), (1, 128, 16, 32, True), (1, 2048, 256, 128, False), (2, 1160, 3096, 32, True), (7, 264, 72, 64, True),
         (16, 4096, 40, 128, False), (17, 1000, 136, 64, False), (32, 136, 1000, 32, False), (33, 520, 264, 32, True),
         (64, 1032, 520, 128, True), (64, 2048, 48, 64, False), (65, 264, 392, 64, True), (300, 1160, 264, 32, False),
+        (18, 4360, 136, 128, True), (33, 2824, 72, 32, True), (64, 2184, 200, 64, False), (64, 2184, 200, 32, True),
     ],
 )
 def test_q4_linear(M, R, C, group, bias, dtype):
@@ -288,6 +289,7 @@ def test_q4_linear_takes_every_code_scale_and_padding(dtype):
         (1, 8, 8, 32, False, "silu"), (1, 2048, 264, 128, False, "silu"), (3, 264, 1032, 32, True, "gelu"), (16, 520, 640, 64, True, "tanh"),
         (17, 136, 392, 128, False, "relu"), (48, 264, 520, 64, True, "gelu"), (64, 1032, 264, 32, False, "leaky_relu"),
         (5, 128, 128, 128, True, "sigmoid"), (9, 256, 384, 32, False, "no_act"), (130, 264, 520, 64, True, "silu"),
+        (48, 72, 2824, 64, True, "gelu"),
     ],
 )
 def test_q4_mlp(M, K, N, group, bias, act, dtype):
@@ -454,6 +456,7 @@ def experts_of(E, K, N, bits, group, dtype, g):
         (16, 392, 264, 8, 2, 4, 128, "silu", True), (17, 72, 200, 4, 2, 16, 0, "tanh", True), (33, 136, 264, 128, 8, 16, 0, "silu", False),
         (40, 264, 136, 8, 3, 4, 32, "silu", True), (64, 128, 64, 512, 16, 16, 0, "silu", True), (64, 136, 72, 2, 1, 4, 64, "gelu", True),
         (64, 8, 8, 1, 1, 16, 0, "silu", False), (64, 136, 1032, 1, 1, 4, 32, "silu", True),
+        (64, 136, 4296, 1, 1, 4, 32, "silu", True), (40, 264, 1160, 8, 3, 4, 32, "silu", True),
         (100, 72, 136, 8, 2, 16, 0, "silu", True), (130, 72, 136, 8, 2, 4, 128, "silu", True),
     ],
 )
