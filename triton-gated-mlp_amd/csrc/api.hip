@@ -1488,7 +1488,7 @@ struct MoeWorkspace {
   size_t active, slot, which, count, weight, partial, bytes;
   MoeWorkspace(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int group) {
     const size_t pairs = (size_t)(M * top_k), entries = (size_t)gmlp::expert_entries((int)M, (int)E, (int)top_k);
-    size_t at = (pairs << gmlp::experts_h_low(M)) * (size_t)N * 2;
+    size_t at = (pairs << gmlp::experts_h_low(M, group)) * (size_t)N * 2;
     auto part = [&](size_t n) {
       const size_t begin = (at + 255) / 256 * 256;
       at = begin + n;
@@ -1572,7 +1572,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
   if (int rc = check_rows(__func__, M)) return rc;
   if (int rc = check_mult8(__func__, "K", K)) return rc;
   if (int rc = check_mult8(__func__, "N", N)) return rc;
-  if (int rc = check_expert_sizes(__func__, M, K, N, 1, M << gmlp::experts_h_low(M))) return rc;
+  if (int rc = check_expert_sizes(__func__, M, K, N, 1, M << gmlp::experts_h_low(M, group))) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(scales_gate); GMLP_REQUIRE_ALIGNED(codes_up);
   GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(codes_down); GMLP_REQUIRE_ALIGNED(scales_down);
   GMLP_REQUIRE_ALIGNED(b_gate); GMLP_REQUIRE_ALIGNED(b_up); GMLP_REQUIRE_ALIGNED(b_down); GMLP_REQUIRE_ALIGNED(h);
@@ -1580,7 +1580,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
   gmlp::ExpertArgs a = expert_sizes(M, K, N, 1, 1, gmlp::ROUTING_DENSE);
   a.x = x;
   a.h = h;
-  a.h_low = gmlp::experts_h_low(M);
+  a.h_low = gmlp::experts_h_low(M, group);
   a.y = y;
   a.bias[0] = b_gate; a.bias[1] = b_up; a.bias[2] = b_down;
   a.gate = {codes_gate, scales_gate};
@@ -1650,7 +1650,7 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   if (int rc = check_rows(__func__, M)) return rc;
   if (int rc = check_mult8(__func__, "K", K)) return rc;
   if (int rc = check_mult8(__func__, "N", N)) return rc;
-  if (int rc = check_expert_sizes(__func__, M, K, N, E, (M * top_k) << gmlp::experts_h_low(M))) return rc;
+  if (int rc = check_expert_sizes(__func__, M, K, N, E, (M * top_k) << gmlp::experts_h_low(M, group))) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(w_gate); GMLP_REQUIRE_ALIGNED(w_up);
   GMLP_REQUIRE_ALIGNED(w_down); GMLP_REQUIRE_ALIGNED(s_gate); GMLP_REQUIRE_ALIGNED(s_up); GMLP_REQUIRE_ALIGNED(s_down);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
@@ -1662,7 +1662,7 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   gmlp::ExpertArgs a = expert_sizes(M, K, N, E, top_k, routing);
   a.x = x;
   a.h = base;
-  a.h_low = gmlp::experts_h_low(M);
+  a.h_low = gmlp::experts_h_low(M, group);
   a.y = y;
   a.gate = {w_gate, s_gate};
   a.up = {w_up, s_up};

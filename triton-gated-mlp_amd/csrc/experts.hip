@@ -550,9 +550,9 @@ __global__ void __launch_bounds__(NW * 64, MT > 1 && MT < 4 && R <= 2 ? 2 : 1) e
 // 16 bits, two experts of K=4096, N=14336 for a token, 235 MB in 40 us (5.9 TB/s); 4 bits, eight for 16 tokens, 240 MB in
 // 45 us (5.3 TB/s) and 4.5 for the parts' sum; one matrix, K=8192, N=28672, 16 tokens, 121 MB in 25 us (4.8 TB/s); K=2048, N=5632,
 // one token, 6 MB in 5.5 us, mostly its start and the join of the wavefronts.
-// Up to 8 tokens (h_low): half of the product's 16 columns would be empty, so every hidden state comes as two 16-bit values, its
-// rounding and what that left, in columns 2t and 2t + 1.  Rounding h to 16 bits alone costs as much as rounding y does;
-// with more tokens it is rounded, as FusedGatedMLP's is: a second plane would double tokens' loads and products.  bf16, 1 token,
+// h_low: of as few tokens as half a load brings (2 with 4-bit weights, 4 with 16-bit ones) every hidden state comes as two 16-bit
+// values, its rounding and what that left, in columns 2t and 2t + 1.  Rounding h to 16 bits alone costs as much as rounding
+// y does; with more tokens it is rounded, as FusedGatedMLP's is: 6 tokens, K=4384, N=18032, 4 bits 54.9 us with both, 48.4 without.  bf16, 1 token,
 // K=2048, N=5632, 4 bits: 11.9 -> 12.5 us, y off by 0.0017 of its norm instead of 0.0024.
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int down_lds() {

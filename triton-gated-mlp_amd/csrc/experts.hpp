@@ -53,7 +53,7 @@ struct ExpertArgs {
 };
 
 // Whether the hidden states of M tokens come as two 16-bit values each, whether ROUTING_SOLO takes the call, and the bytes of `partial` that launch_experts_down asks for (it does with none).
-inline int experts_h_low(int64_t M) { return M <= 8; }
+inline int experts_h_low(int64_t M, int group) { return M <= (group ? 2 : 4); }
 bool experts_solo(int M, int E);
 size_t experts_partial_bytes(const ExpertArgs& a, int group);
 
