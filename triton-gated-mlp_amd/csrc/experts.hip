@@ -800,11 +800,19 @@ static hipError_t run_down(const ExpertArgs& a, int parts, hipStream_t s) {
   return hipGetLastError();
 }
 
+template <typename F>
+static hipError_t by_token_tiles(int mt, F&& f) {
+  if (mt == 2) return f(std::integral_constant<int, 2>{});
+  if (mt == 3) return f(std::integral_constant<int, 3>{});
+  return f(std::integral_constant<int, 4>{});
+}
+
 // Gate/up.
 template <typename T, int G>
 static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
   const int mt = token_tiles(a);
-  const bool few = (a.N + Q4_TILE - 1) / Q4_TILE * entries_at_most(a) <= (mt == 1 ? 4 : 2) * a.cus;
+  const int tiles = (a.N + Q4_TILE - 1) / Q4_TILE * entries_at_most(a);
+  const bool few = tiles <= 4 * a.cus;
   if constexpr (G == 0) {
     if (a.M <= 8) return run_gateup<T, 0, 1, 1, 1, 4, 2>(a, s);
     if (mt == 1) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
@@ -812,11 +820,22 @@ static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
   } else {
     if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 2>(a, s);
     if (mt == 1) return few ? run_gateup<T, G, 1, 4, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
-    // More than one token tile: as many tiles and wavefronts as the registers hold, fewer with finer groups.
-    constexpr bool coarse = G == 128, fine = G == 32;
-    if (mt == 2) return few ? run_gateup<T, G, 2, 4, fine ? 1 : 2, 8, 1>(a, s) : run_gateup<T, G, 2, 4, 3, coarse ? 8 : 4, 1>(a, s);
-    if (mt == 3) return run_gateup<T, G, 3, 4, fine ? 1 : 2, 4, 1>(a, s);
-    return few ? run_gateup<T, G, 4, 4, 1, 4, 1>(a, s) : run_gateup<T, G, 4, 4, fine ? 2 : 3, 4, 1>(a, s);
+    // More than one token tile.  Token rows are read again for every strip, so two tiles of each matrix, where the registers hold
+    // them; but a tile for every CU first, and eight wavefronts where a CU gets one workgroup and each of them two blocks.  us,
+    // groups of 128, as (tiles, wavefronts): 32 tokens, K=7168, N=2424 (1, 8) 12.8 (1, 4) 17.2 (2, 8) 17.4; K=1536, N=4096 5.7
+    // 5.65 7.9; K=4096, N=7168 14.7 14.2 12.8; K=5280, N=13224 35 36 31 and (2, 4) 26.8; 64 tokens, that size, (1, 4) 53
+    // (2, 8) 43 (2, 4) 36.  Two tiles in finer groups, 64 tokens, groups of 64 53.8 against 53.3, 48 tokens, groups of 32 93 against 49.
+    const bool deep = a.K > 12 * Q4_BLOCK;
+    return by_token_tiles(mt, [&](auto m) -> hipError_t {
+      constexpr int MT = decltype(m)::value;
+      constexpr bool wide = MT == 2 || (MT == 3 && G >= 64) || (MT == 4 && G == 128);
+      if (tiles <= a.cus && deep) return run_gateup<T, G, MT, 4, 1, 8, 1>(a, s);
+      if constexpr (wide) {
+        if (tiles > a.cus && tiles <= 2 * a.cus && deep) return run_gateup<T, G, MT, 4, 2, 8, 1>(a, s);
+        if (tiles > a.cus) return run_gateup<T, G, MT, 4, 2, 4, 1>(a, s);
+      }
+      return run_gateup<T, G, MT, 4, 1, 4, 1>(a, s);
+    });
   }
 }
 
@@ -830,9 +849,14 @@ static DownPlan plan_down(const ExpertArgs& a, int group) {
   const bool large = weight_bytes(a, group) >= 48e6;
   const int tiles = (a.K + Q4_TILE - 1) / Q4_TILE;
   DownPlan p = {1, 1};
-  if (a.M > 16) p.tiles = a.M > 48 && group == 32 && a.routing == ROUTING_DENSE ? 1 : 2;  // (two of the finest groups would spill)
-  else if (group && a.M > 4 && (large || tiles > 2 * a.cus)) p.tiles = 4;
   const int cols = group ? 128 : 64, blocks = (a.N + cols - 1) / cols * experts_at_most(a);
+  if (a.M > 16) {
+    // A tile for every CU where the reduction is short (us, 48 tokens, groups of 128, one tile and two: 4096 rows of 4096 columns 10.1, 11.0,
+    // 2048 of 2048 7.0, 7.6, but 4096 of 11008 20.7, 17.8), and of 64 tokens with the finest groups, where two would spill.
+    const bool spill = a.M > 48 && group == 32, shallow = group && tiles <= a.cus && blocks <= 32;
+    p.tiles = a.routing == ROUTING_DENSE && (spill || shallow) ? 1 : 2;
+  }
+  else if (group && a.M > 4 && (large || tiles > 2 * a.cus)) p.tiles = 4;
   if (a.M > 16 ? blocks * token_tiles(a) > 64 : large) {
     p.parts = a.cus / ((tiles + p.tiles - 1) / p.tiles);
     p.parts = p.parts < 1 ? 1 : p.parts > DOWN_MAX_PARTS ? DOWN_MAX_PARTS : p.parts;
@@ -851,6 +875,11 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
   const bool few = a.M << a.h_low <= FEW;
   if (a.M > 16 && a.routing == ROUTING_PLAN)
     return token_tiles(a) == 1 ? run_down<T, G, 1, ALL, 2, 8, 1, true>(a, parts, s) : run_down<T, G, 2, ALL, 2, 8, 1, true>(a, parts, s);
+  if constexpr (G != 0) {
+    const bool wide = G == 32 && a.K > Q4_TILE * a.cus;  // (more tiles than CUs: 8192 rows of 1024 columns 9.3 us, with eight wavefronts 12.9)
+    if (a.M > 16 && p.tiles == 1 && !wide)
+      return by_token_tiles(token_tiles(a), [&](auto m) { return run_down<T, G, decltype(m)::value, ALL, 1, 8, 1>(a, parts, s); });
+  }
   if (a.M > 48) return run_down<T, G, 4, ALL, G == 32 ? 1 : 2, 4, 1>(a, parts, s);
   if (a.M > 32) return run_down<T, G, 3, ALL, 2, G == 32 ? 4 : 8, 1>(a, parts, s);
   if (a.M > 16) return run_down<T, G, 2, ALL, 2, 8, 1>(a, parts, s);
