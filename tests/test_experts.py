@@ -249,6 +249,8 @@ def q4(shape, group, dtype, g):
         (1, 8, 8, 128, False), (1, 128, 16, 32, True), (1, 2048, 256, 128, False), (2, 1160, 3096, 32, True), (7, 264, 72, 64, True),
         (16, 4096, 40, 128, False), (17, 1000, 136, 64, False), (32, 136, 1000, 32, False), (33, 520, 264, 32, True),
         (64, 1032, 520, 128, True), (64, 2048, 48, 64, False), (65, 264, 392, 64, True), (300, 1160, 264, 32, False),
+        (1, 136, 4360, 32, True), (3, 1160, 4120, 128, False), (4, 1160, 4120, 32, False), (9, 392, 4360, 64, True),
+        (16, 1160, 4360, 32, False), (5, 264, 8456, 128, False), (7, 1160, 8456, 64, False), (20, 136, 4360, 128, True), (60, 136, 4360, 32, False),
         (18, 4360, 136, 128, True), (33, 2824, 72, 32, True), (64, 2184, 200, 64, False), (64, 2184, 200, 32, True),
     ],
 )
@@ -290,6 +292,7 @@ def test_q4_linear_takes_every_code_scale_and_padding(dtype):
         (17, 136, 392, 128, False, "relu"), (48, 264, 520, 64, True, "gelu"), (64, 1032, 264, 32, False, "leaky_relu"),
         (5, 128, 128, 128, True, "sigmoid"), (9, 256, 384, 32, False, "no_act"), (130, 264, 520, 64, True, "silu"),
         (48, 72, 2824, 64, True, "gelu"),
+        (20, 1672, 72, 32, True, "silu"), (40, 72, 4360, 64, False, "silu"), (64, 1672, 4360, 128, False, "relu"), (60, 136, 8456, 128, True, "silu"),
     ],
 )
 def test_q4_mlp(M, K, N, group, bias, act, dtype):

@@ -855,8 +855,8 @@ static DownPlan plan_down(const ExpertArgs& a, int group) {
     // 2048 of 2048 7.0, 7.6, but 4096 of 11008 20.7, 17.8), and of 64 tokens with the finest groups, where two would spill.
     const bool spill = a.M > 48 && group == 32, shallow = group && tiles <= a.cus && blocks <= 32;
     p.tiles = a.routing == ROUTING_DENSE && (spill || shallow) ? 1 : 2;
-  }
-  else if (group && a.M > 4 && (large || tiles > 2 * a.cus)) p.tiles = 4;
+  } else if (group && a.M <= 4) p.tiles = tiles > a.cus ? 2 : 1;
+  else if (group) p.tiles = large ? 4 : tiles <= a.cus ? 1 : tiles <= 2 * a.cus || blocks <= 8 ? 2 : 4;
   if (a.M > 16 ? blocks * token_tiles(a) > 64 : large) {
     p.parts = a.cus / ((tiles + p.tiles - 1) / p.tiles);
     p.parts = p.parts < 1 ? 1 : p.parts > DOWN_MAX_PARTS ? DOWN_MAX_PARTS : p.parts;
@@ -888,6 +888,15 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
   // One tile.  Enough wavefronts, and stages of them, for a share of the blocks that is in flight at once.
   constexpr int COLS = Block<T, G, 1, 1, 1>::COLS;
   const int blocks = (a.N + COLS - 1) / COLS * experts_at_most(a);
+  // More than a tile for every CU: two each.  us, one token, groups of 128: 12312 rows of 7168 columns 13.5, one tile with stages
+  // four deep 15.7 (groups of 32 17.1, 24.1), 21496 of 952 with four wavefronts 5.7, with eight 6.8, one tile 11.3 (groups of 32
+  // 7.2, 7.4, 16.8).  16 tokens, groups of 128: 6144 of 6144 9.9 with two tiles, 12.1 with one, 13.5 with four; 12312 of 7168
+  // 18.1 with two, 15.5 with four.
+  if constexpr (G != 0)
+    if (p.tiles == 2) {
+      if (!few) return blocks <= 8 ? run_down<T, G, 1, ALL, 2, 4, 1>(a, parts, s) : run_down<T, G, 1, ALL, 2, 8, 1>(a, parts, s);
+      return blocks <= 8 ? run_down<T, G, 1, 1, 2, 4, G == 32 ? 1 : 2>(a, parts, s) : run_down<T, G, 1, 1, 2, 8, G == 32 ? 1 : 2>(a, parts, s);
+    }
   if (few && G != 0) {
     if (blocks <= 16) return run_down<T, G, 1, 1, 1, 8, 2>(a, parts, s);
     return blocks < 128 ? run_down<T, G, 1, 1, 1, 8, 4>(a, parts, s) : run_down<T, G, 1, 1, 1, 16, 2>(a, parts, s);
