@@ -459,6 +459,7 @@ def experts_of(E, K, N, bits, group, dtype, g):
         (16, 392, 264, 8, 2, 4, 128, "silu", True), (17, 72, 200, 4, 2, 16, 0, "tanh", True), (33, 136, 264, 128, 8, 16, 0, "silu", False),
         (40, 264, 136, 8, 3, 4, 32, "silu", True), (64, 128, 64, 512, 16, 16, 0, "silu", True), (64, 136, 72, 2, 1, 4, 64, "gelu", True),
         (64, 8, 8, 1, 1, 16, 0, "silu", False), (64, 136, 1032, 1, 1, 4, 32, "silu", True),
+        (1, 72, 4264, 4, 4, 16, 0, "silu", True), (12, 136, 1032, 32, 2, 4, 64, "silu", False), (2, 200, 1544, 16, 8, 4, 32, "gelu", True),
         (64, 136, 4296, 1, 1, 4, 32, "silu", True), (40, 264, 1160, 8, 3, 4, 32, "silu", True),
         (100, 72, 136, 8, 2, 16, 0, "silu", True), (130, 72, 136, 8, 2, 4, 128, "silu", True),
     ],

@@ -842,6 +842,8 @@ static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
 // Down: tiles of a workgroup, and workgroups that share a strip of them.  The parts' sum is a launch more, 2 us behind others and
 // more from an idle queue.  With more than one token tile it pays beyond 64 blocks (of all experts, times token tiles), even
 // where the weights would not: M=48, 4 bits, 768 rows of 2048 columns 7.7 us whole, 8.4 in four parts; of 4096 10.8 and 8.7.
+// Up to 16 tokens: large weights, which take as long anyway, and long reductions of all experts together in few rows, which would leave CUs
+// idle: 12 tokens, 1 of 32 experts of K=512, N=6144, 4 bits, the layer 51.8 us whole, 30.4 split.
 struct DownPlan {
   int tiles, parts;
 };
@@ -857,7 +859,7 @@ static DownPlan plan_down(const ExpertArgs& a, int group) {
     p.tiles = a.routing == ROUTING_DENSE && (spill || shallow) ? 1 : 2;
   } else if (group && a.M <= 4) p.tiles = tiles > a.cus ? 2 : 1;
   else if (group) p.tiles = large ? 4 : tiles <= a.cus ? 1 : tiles <= 2 * a.cus || blocks <= 8 ? 2 : 4;
-  if (a.M > 16 ? blocks * token_tiles(a) > 64 : large) {
+  if (a.M > 16 ? blocks * token_tiles(a) > 64 : large || (2 * tiles <= a.cus && blocks > 128)) {
     p.parts = a.cus / ((tiles + p.tiles - 1) / p.tiles);
     p.parts = p.parts < 1 ? 1 : p.parts > DOWN_MAX_PARTS ? DOWN_MAX_PARTS : p.parts;
   }
