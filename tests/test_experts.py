@@ -764,6 +764,69 @@ def test_gated_moe_module(E, router, bits):
         assert torch.equal(other(x), y)
 
 
+def _on_four_bits(E, K, N, dtype):
+    """A GatedMoE as quantize_ leaves it, without a GPU."""
+    from triton_gated_mlp import GatedMoE
+    from triton_gated_mlp.experts import _Q4Buffers
+
+    m = GatedMoE(K, N, E, 2).to(dtype)
+    for name, rows, cols in (("gate_proj", N, K), ("up_proj", N, K), ("down_proj", K, N)):
+        tiles, blocks = -(-rows // 16), -(-cols // 128)
+        codes = torch.randint(0, 256, (E, tiles, blocks, 4, 16, 4, 4), generator=gen(rows), dtype=torch.uint8)
+        scales = torch.full((E, tiles, blocks, 4, 2, 4), 0.01, dtype=dtype)
+        delattr(m, name)
+        setattr(m, name, _Q4Buffers(quant.Q4Weight(codes, scales, rows, cols, 64)))
+    return m
+
+
+# (70 rows: the float32 GEMM's logits; 3 rows: that of a float32 router, of a number of experts that is no multiple of 4, and moe_logits)
+ROUTERS = [(70, 8, None), (3, 8, torch.float32), (3, 6, None), (3, 8, None)]
+
+
+@pytest.mark.parametrize("rows,E,router", ROUTERS)
+def test_layers_of_four_bit_experts_refuse_what_autograd_would_record(rows, E, router):
+    """The router's weight and x are the tensors that are left to differentiate for."""
+    import torch.autograd.forward_ad as fw
+
+    m = _on_four_bits(E, 64, 72, torch.float16)
+    if router is not None:
+        m.router.to(router)
+    x = torch.zeros(rows, 64, dtype=torch.float16)
+    for one_by_one in (False, True):
+        if one_by_one:
+            m.long_batch = lambda: 1
+        m.router.requires_grad_(True)
+        with pytest.raises(RuntimeError, match="no backward"):
+            m(x)
+        with pytest.raises(RuntimeError, match="no backward"):
+            m.route_logits(x)
+        m.router.requires_grad_(False)
+        with pytest.raises(RuntimeError, match="no backward"):
+            m(x.clone().requires_grad_(True))
+        with fw.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            m(fw.make_dual(x, x))
+        with torch.no_grad(), pytest.raises(RuntimeError, match="functorch"):
+            torch.vmap(m)(x[None])
+        with pytest.raises(RuntimeError, match="AMD GPU"):  # nothing to record: it gets as far as the kernels
+            m(x)
+
+
+@gpu
+@pytest.mark.parametrize("rows,E,router", ROUTERS)
+def test_layers_of_four_bit_experts_run_where_autograd_records_nothing(rows, E, router):
+    m = _on_four_bits(E, 64, 72, torch.float16)
+    if router is not None:
+        m.router.to(router)
+    m = m.to(device())
+    x = normal((rows, 64), 1.0, torch.float16, gen(rows)).to(device())
+    with pytest.raises(RuntimeError, match="no backward"):
+        m(x)
+    with torch.no_grad():
+        y = m(x)
+    m.router.requires_grad_(False)
+    assert torch.equal(m(x), y) and not m(x).requires_grad
+
+
 @gpu
 @pytest.mark.parametrize("rows", [3, 70])
 def test_q4_gated_mlp_module(rows):

@@ -488,6 +488,10 @@ void inference_only(const char* name, std::initializer_list<std::reference_wrapp
   TORCH_CHECK(!(graph && at::GradMode::is_enabled()), name, " has no backward pass: call it under torch.no_grad()");
   TORCH_CHECK(!torch::jit::tracer::isTracing(), name, " cannot be traced");
 }
+// the same for a Python function that is made of operators without checks of their own
+void inference_only_of(const std::string& name, const std::vector<Tensor>& tensors) {
+  for (const Tensor& t : tensors) inference_only(name.c_str(), {t});
+}
 constexpr int64_t FEW_ROWS = 64;  // token rows of the weight-streaming kernels
 
 // triton_gated_mlp.ops.quant.Q4Weight: codes, scales, rows, cols, group size
@@ -779,6 +783,7 @@ PYBIND11_MODULE(_gmlp_torch, m) {
   m.def("mlp_infer", torch::wrap_pybind_function_no_gil(mlp_infer));
   m.def("mlp_train", torch::wrap_pybind_function_no_gil(call_mlp_train));
   m.def("hidden", torch::wrap_pybind_function_no_gil(call_hidden));
+  m.def("inference_only", torch::wrap_pybind_function_no_gil(inference_only_of));
   m.def("q4_linear", torch::wrap_pybind_function_no_gil(q4_linear));
   m.def("q4_mlp", torch::wrap_pybind_function_no_gil(q4_mlp));
   m.def("q4_quantize", torch::wrap_pybind_function_no_gil(q4_quantize));

@@ -15,6 +15,7 @@ from typing import Optional
 import torch
 from torch import Tensor, nn
 
+from . import _cabi
 from .gated_mlp import ACT_FWD
 from .ops import fwd as _fwd
 from .ops import moe as _moe
@@ -115,7 +116,8 @@ class GatedMoE(nn.Module):
         w, E = self.router.weight, self.num_experts
         if x.shape[0] <= 64 and w.dtype == x.dtype and E % 4 == 0:
             return _moe.moe_logits(x, w)
-        # a router kept in float32, or many rows: the float32 GEMM (which takes whole rows of 8)
+        # a router kept in float32, or many rows: the float32 GEMM (which takes whole rows of 8, and looks at no gradients)
+        _cabi.torch_binding().inference_only("GatedMoE", [x, w])
         w = w.float()
         if E % 8:
             w = nn.functional.pad(w, (0, 0, 0, 8 - E % 8))
@@ -138,8 +140,7 @@ class GatedMoE(nn.Module):
         return y.reshape(x.shape)
 
     def _one_by_one(self, x: Tensor, logits: Tensor) -> Tensor:
-        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
-            raise RuntimeError("GatedMoE has no backward pass: call it under torch.no_grad()")
+        _cabi.torch_binding().inference_only("GatedMoE", [x, *self.parameters()])
         weights, experts = _moe.moe_route(logits, self.top_k, normalize=self.normalize)
         order = experts.reshape(-1).argsort(stable=True)
         counts = torch.bincount(experts.reshape(-1), minlength=self.num_experts).tolist()
