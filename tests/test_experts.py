@@ -439,6 +439,22 @@ def test_route_strides_leading_dimensions_and_refusals():
         moe.moe_route(torch.zeros(2, 8, device=dev, requires_grad=True), 2)
 
 
+@gpu
+@pytest.mark.parametrize("M,E", [(2**28 + 9, 2), (2**26 + 5, 257)])
+def test_route_of_more_rows_than_a_launch_has_threads_for(M, E):
+    """(16 threads a row up to 256 experts, 64 beyond, and less than 2^32 in a launch.)"""
+    dev = device()
+    logits = torch.zeros((M, E), dtype=torch.float16, device=dev)
+    best = torch.arange(M, device=dev) % E
+    logits.scatter_(1, best[:, None], 1.0)
+    w, e = moe.moe_route(logits, 1, normalize=False)
+    assert torch.equal(e[:, 0], best)
+    p = math.e / (math.e + E - 1)
+    assert (w - p).abs().max().item() <= 5e-6 * p
+    del logits, best, w, e
+    torch.cuda.empty_cache()
+
+
 # ------------------------------------------------------------------ expert layers
 def experts_of(E, K, N, bits, group, dtype, g):
     """(gate, up, down) for the operator, and a function that gives one expert's in float64."""

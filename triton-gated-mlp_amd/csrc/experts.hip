@@ -1101,18 +1101,29 @@ __global__ void __launch_bounds__(1024) plan_kernel(const L* logits, ExpertPlan 
   else if ((E) <= 256) CALL(4);    \
   else CALL(8)
 
+// Rows of a launch: it has fewer than 2^32 threads, 16 or 64 for a row.  (Past that the runtime starts fewer than asked for, and
+// reports no error: 2^28 + 9 rows of two experts came back in part.)
+constexpr int64_t ROUTE_ROWS = (int64_t)1 << 24;
+
 template <typename L>
 hipError_t launch_route(const L* logits, float* weights, int64_t* experts, int64_t M, int E, int top_k, int normalize, hipStream_t s) {
 #define ROWS(V) \
-  hipLaunchKernelGGL((route_rows_kernel<V, L>), dim3((unsigned)((M + 15) / 16)), dim3(256), 0, s, logits, weights, experts, M, E, top_k, normalize)
-  if (E <= 16) ROWS(1);
-  else if (E <= 64) ROWS(4);
-  else if (E <= 128) ROWS(8);
-  else if (E <= 256) ROWS(16);
-  else
-    hipLaunchKernelGGL((route_kernel<8, L>), dim3((unsigned)((M + 3) / 4)), dim3(256), 0, s, logits, weights, experts, M, E, top_k, normalize);
+  hipLaunchKernelGGL((route_rows_kernel<V, L>), dim3((unsigned)((m + 15) / 16)), dim3(256), 0, s, logits, weights, experts, m, E, top_k, normalize)
+  for (int64_t m; M > 0; M -= m) {
+    m = M < ROUTE_ROWS ? M : ROUTE_ROWS;
+    if (E <= 16) ROWS(1);
+    else if (E <= 64) ROWS(4);
+    else if (E <= 128) ROWS(8);
+    else if (E <= 256) ROWS(16);
+    else
+      hipLaunchKernelGGL((route_kernel<8, L>), dim3((unsigned)((m + 3) / 4)), dim3(256), 0, s, logits, weights, experts, m, E, top_k, normalize);
+    if (hipError_t e = hipGetLastError()) return e;
+    logits += m * E;
+    weights += m * top_k;
+    experts += m * top_k;
+  }
 #undef ROWS
-  return hipGetLastError();
+  return hipSuccess;
 }
 template <typename L>
 hipError_t launch_experts_plan(const L* logits, const ExpertArgs& a, hipStream_t s) {
