@@ -333,6 +333,7 @@ int gmlp_hidden_bwd(const void* dh, const void* x, const void* w_gate, const voi
  *
  * gmlp_q4_quantize: scale = (largest magnitude of the group) / 7 rounded to dtype, n = w / scale rounded to nearest (even); padding
  *   is n = 0, and scale 0 where a whole group is padding.  gmlp_q4_dequantize: w = scale·n rounded to dtype.
+ *   count * tiles * blocks of both at most 2^26 - 4.
  * gmlp_q4_linear_fwd: y[M,C] = x[M,R]·Wᵀ + bias, W [C,R] 4-bit; bias may be NULL.  The products are of scale·n itself, not
  *   of its rounding.
  * gmlp_q4_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) in dtype, y = h·W_downᵀ + b_down.  `h` is scratch

@@ -189,6 +189,18 @@ def test_refusals_of_the_c_interface():
     assert layer(x=a + 4) == -3 and layer(ws=a + 8) == -3
 
 
+def test_storage_that_a_launch_has_no_threads_for_is_refused():
+    """A wavefront of 64 threads per 1 KiB of codes, and less than 2^32 in a launch: 2^26 of them are too many."""
+    import ctypes
+
+    lib = _cabi.lib()
+    raw = ctypes.create_string_buffer(64 + 64)
+    a = (ctypes.addressof(raw) + 63) & ~63
+    for call in (lib.gmlp_q4_quantize, lib.gmlp_q4_dequantize):
+        for count, rows, cols in ((1 << 26, 8, 8), (1 << 20, 1024, 72), (1, 1 << 20, 1 << 17), (1 << 31, 16, 128)):
+            assert call(a, a, a, count, rows, cols, 32, 0, None) == -2 and "too large" in lib.gmlp_last_error().decode()
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 64, dtype=torch.float16)
     with pytest.raises(RuntimeError, match="AMD GPU"):

@@ -1453,9 +1453,11 @@ int check_expert_sizes(const char* fn, int64_t M, int64_t K, int64_t N, int64_t 
     return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
   return 0;
 }
+// (A wavefront per tile and block, four to a workgroup, and fewer than 2^32 threads in a launch: of more the runtime starts
+// a part only, without an error.  2^26 of them are 2^37 weights where no padding is among them.)
 int check_storage(const char* fn, int64_t count, int64_t rows, int64_t cols) {
   if (count < 1 || rows < 1 || cols < 1 || rows > kMaxDim || cols > kMaxDim ||
-      count > ((int64_t)1 << 32) / cdiv(rows, 16) / cdiv(cols, 128))
+      count > (((int64_t)1 << 26) - 4) / cdiv(rows, 16) / cdiv(cols, 128))
     return fail(GMLP_ESHAPE, "%s: count, rows, cols must be >= 1 and not too large (got %lld, %lld, %lld)", fn, (long long)count,
                 (long long)rows, (long long)cols);
   if (int rc = check_mult8(fn, "rows", rows)) return rc;
