@@ -201,6 +201,22 @@ def test_storage_that_a_launch_has_no_threads_for_is_refused():
             assert call(a, a, a, count, rows, cols, 32, 0, None) == -2 and "too large" in lib.gmlp_last_error().decode()
 
 
+def test_expert_layers_that_a_launch_has_no_threads_for_are_refused():
+    """256 experts in use times 2^20 / 16 tiles of gate/up, 256 threads each, are 2^32 threads."""
+    import ctypes
+
+    lib = _cabi.lib()
+    raw = ctypes.create_string_buffer(64 + 64)
+    a = (ctypes.addressof(raw) + 63) & ~63
+
+    def layer(N, group, s):  # (a workspace of no bytes: what the sizes leave is refused behind them)
+        return lib.gmlp_moe_fwd(a, a, a, a, a, s, s, s, a, 16, 8, N, 256, 16, 1, group, 0, 2, 0, a, 0, None)
+
+    for group, s in ((0, None), (128, a)):
+        assert layer(1 << 20, group, s) == -2 and "too large" in lib.gmlp_last_error().decode()
+        assert layer((1 << 20) - 16, group, s) == -1 and "workspace" in lib.gmlp_last_error().decode()
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 64, dtype=torch.float16)
     with pytest.raises(RuntimeError, match="AMD GPU"):

@@ -1445,11 +1445,12 @@ int check_rows(const char* fn, int64_t M) {
     return fail(GMLP_ESHAPE, "%s: M = %lld exceeds the %d token rows of a call", fn, (long long)M, gmlp::EXPERTS_MAX_M);
   return 0;
 }
-// The kernels address four tiles of weights, the token rows and the hidden states with 32-bit byte offsets, and a grid
-// has a workgroup per tile.
-int check_expert_sizes(const char* fn, int64_t M, int64_t K, int64_t N, int64_t experts, int64_t pairs) {
+// The kernels address four tiles of weights, the token rows and the hidden states with 32-bit byte offsets, and gate/up has
+// a workgroup of 256 threads per tile and entry of the plan (eight wavefronts only where that is no more than a few for each
+// CU), down one of at most 1024 per tile: fewer than 2^32 threads, of more the runtime starts a part only, without an error.
+int check_expert_sizes(const char* fn, int64_t M, int64_t K, int64_t N, int64_t entries, int64_t pairs) {
   const int64_t limit = gmlp::EXPERTS_MAX_BYTES, most = K > N ? K : N;
-  if (most * 2 * 16 * 4 >= limit || M * K * 2 >= limit || pairs * N * 2 >= limit || experts * cdiv(most, 16) >= limit)
+  if (most * 2 * 16 * 4 >= limit || M * K * 2 >= limit || pairs * N * 2 >= limit || entries * cdiv(N, 16) >= ((int64_t)1 << 32) / 256)
     return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
   return 0;
 }
@@ -1652,7 +1653,7 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   if (int rc = check_rows(__func__, M)) return rc;
   if (int rc = check_mult8(__func__, "K", K)) return rc;
   if (int rc = check_mult8(__func__, "N", N)) return rc;
-  if (int rc = check_expert_sizes(__func__, M, K, N, E, (M * top_k) << gmlp::experts_h_low(M, group))) return rc;
+  if (int rc = check_expert_sizes(__func__, M, K, N, gmlp::expert_entries((int)M, (int)E, (int)top_k), (M * top_k) << gmlp::experts_h_low(M, group))) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(w_gate); GMLP_REQUIRE_ALIGNED(w_up);
   GMLP_REQUIRE_ALIGNED(w_down); GMLP_REQUIRE_ALIGNED(s_gate); GMLP_REQUIRE_ALIGNED(s_up); GMLP_REQUIRE_ALIGNED(s_down);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
