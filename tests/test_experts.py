@@ -872,6 +872,47 @@ def test_layers_of_four_bit_experts_run_where_autograd_records_nothing(rows, E, 
 
 
 @gpu
+@pytest.mark.parametrize("bits", [16, 4])
+def test_masked_experts_of_a_long_batch_are_not_run(bits, monkeypatch):
+    """As the streaming kernels have it: an expert that every token's mask leaves out, rows whose mask leaves fewer than top_k
+    and a row whose mask leaves nothing."""
+    from triton_gated_mlp import GatedMoE, experts
+
+    dev, dtype, E, K, N, M, k = device(), torch.bfloat16, 6, 72, 136, 80, 3
+    torch.manual_seed(1)
+    g = gen(1)
+    m = GatedMoE(K, N, E, k).to(dev, dtype)
+    x, logits = normal((M, K), 1.0, dtype, g), normal((M, E), 1.5, torch.float32, g)
+    logits[:, 1:] = logits[:, 1:].masked_fill(torch.rand((M, E - 1), generator=g) < 0.6, -math.inf)
+    logits[:, 4] = -math.inf
+    logits[2] = -math.inf
+    ran = []
+    for module, name in ((experts._fwd, "mlp_fwd"), (experts._quant, "q4_mlp_fwd")):
+        def recorded(rows, *rest, call=getattr(module, name), **named):
+            ran.append(rows.shape[0])
+            return call(rows, *rest, **named)
+        monkeypatch.setattr(module, name, recorded)
+    with torch.no_grad():
+        if bits == 4:
+            m.quantize_(32)
+            one = lambda e: tuple(weights_of(p.of(e)) for p in (m.gate_proj, m.up_proj, m.down_proj))
+        else:
+            one = lambda e: tuple(p[e].cpu().double() for p in (m.gate_proj, m.up_proj, m.down_proj))
+        out = m._one_by_one(x.to(dev), logits.to(dev)).cpu().double()
+        w, experts_of_rows = route64(logits, k, True)
+        assert ran == [int(((experts_of_rows == e) & (w > 0)).sum()) for e in range(E) if e != 4]
+        ref, _ = moe64(x.double(), logits, k, True, "silu", dtype, one)
+        assert (out[2] == 0).all() and ((out - ref).norm() / ref.norm()).item() <= 1.02 * U[dtype]
+        assert (m._one_by_one(x.to(dev), torch.full((M, E), -math.inf, device=dev)) == 0).all()
+        assert len(ran) == E - 1
+        # a token whose logits are not finite, in the way softmax has it, beside rows that stay as they are
+        logits[7, 1] = math.nan
+        wrong = m._one_by_one(x.to(dev), logits.to(dev)).cpu().double()
+        keep = torch.arange(M) != 7
+        assert ((wrong - ref)[keep].norm() / ref[keep].norm()).item() <= 1.02 * U[dtype] and torch.isnan(wrong[7]).all()
+
+
+@gpu
 @pytest.mark.parametrize("rows", [3, 70])
 def test_q4_gated_mlp_module(rows):
     from triton_gated_mlp import FusedGatedMLP, Q4GatedMLP

@@ -142,8 +142,10 @@ class GatedMoE(nn.Module):
     def _one_by_one(self, x: Tensor, logits: Tensor) -> Tensor:
         _cabi.torch_binding().inference_only("GatedMoE", [x, *self.parameters()])
         weights, experts = _moe.moe_route(logits, self.top_k, normalize=self.normalize)
-        order = experts.reshape(-1).argsort(stable=True)
-        counts = torch.bincount(experts.reshape(-1), minlength=self.num_experts).tolist()
+        # (an expert that is not available to the token, logit -inf, is not run for it: behind the others, and not counted)
+        experts = experts.masked_fill(logits.gather(-1, experts) == -math.inf, self.num_experts).reshape(-1)
+        order = experts.argsort(stable=True)
+        counts = torch.bincount(experts, minlength=self.num_experts).tolist()[: self.num_experts]
         y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
         first = 0
         for e, n in enumerate(counts):
@@ -157,9 +159,7 @@ class GatedMoE(nn.Module):
                 out = _quant.q4_mlp_fwd(x[tokens], gate, None, up, None, down, None, act_fn=self.act_fn)
             else:
                 out, _ = _fwd.mlp_fwd(x[tokens], gate, None, up, None, down, None, act_fn=self.act_fn)
-            share = weights.reshape(-1)[pairs, None]
-            # (a token that an expert does not serve, weight 0, gets nothing of it whatever it computes)
-            y.index_add_(0, tokens, torch.where(share == 0, 0.0, out.float() * share))
+            y.index_add_(0, tokens, out.float() * weights.reshape(-1)[pairs, None])
         return y.to(x.dtype)
 
     def extra_repr(self) -> str:
