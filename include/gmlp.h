@@ -337,10 +337,14 @@ int gmlp_hidden_bwd(const void* dh, const void* x, const void* w_gate, const voi
  * gmlp_q4_linear_fwd: y[M,C] = x[M,R]·Wᵀ + bias, W [C,R] 4-bit; bias may be NULL.  The products are of scale·n itself, not
  *   of its rounding.
  * gmlp_q4_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) in dtype, y = h·W_downᵀ + b_down.  `h` is scratch
- *   of M·N elements, 2·M·N for M <= 2: of so few tokens h is kept as two 16-bit values, its rounding and the rest.
+ *   of GMLP_Q4_MLP_H_ELEMENTS(M, N) elements: of up to GMLP_H_PAIR_ROWS_Q4 tokens h is kept as two 16-bit values, its
+ *   rounding and the rest, of more as its rounding (in fp16 one past 65504 is infinite, as gmlp_mlp_fwd's).
  * workspace: partial sums of a reduction that is split over workgroups, gmlp_q4_workspace_bytes(M, R, C, ...) bytes for the
  *   linear layer and (M, R = N, C = K, ...) for the MLP.  NULL, 0 or fewer bytes are accepted and only slower.
  */
+#define GMLP_H_PAIR_ROWS_Q4 2   /* tokens, 4-bit weights */
+#define GMLP_H_PAIR_ROWS_16BIT 4   /* tokens, 16-bit weights (gmlp_moe_fwd, in its workspace) */
+#define GMLP_Q4_MLP_H_ELEMENTS(M, N) (((M) <= GMLP_H_PAIR_ROWS_Q4 ? 2 : 1) * (M) * (N))
 int gmlp_q4_quantize(const void* w, void* codes, void* scales, int64_t count, int64_t rows, int64_t cols, int group, int dtype,
                      void* stream);
 int gmlp_q4_dequantize(const void* codes, const void* scales, void* w, int64_t count, int64_t rows, int64_t cols, int group,
@@ -362,7 +366,7 @@ int gmlp_q4_mlp_fwd(const void* x, const void* codes_gate, const void* scales_ga
  *   weights NaN, as softmax does.  logits, weights and experts need the alignment of their elements only.  1 <= top_k <= 16, top_k <= E <= 512, any M.
  * gmlp_moe_fwd: y[m] = sum over m's experts e of weight·MLP_e(x[m]), MLP_e the gated MLP with w_gate[e], w_up[e] [N,K] and
  *   w_down[e] [K,N] (group = 0: dtype, s_* NULL; otherwise 4-bit codes with scales s_*); the hidden states are rounded to
- *   dtype (two values each for M <= 2, with 16-bit weights M <= 4), the sum over experts is fp32.  Experts that no token chose are not read; one with weight 0 through -inf is not
+ *   dtype (two values each for M <= GMLP_H_PAIR_ROWS_Q4, with 16-bit weights GMLP_H_PAIR_ROWS_16BIT), the sum over experts is fp32.  Experts that no token chose are not read; one with weight 0 through -inf is not
  *   run.  M <= 64.  workspace: gmlp_moe_workspace_bytes.
  */
 int gmlp_moe_logits(const void* x, const void* w_router, float* logits, int64_t M, int64_t K, int64_t E, int dtype, void* stream);

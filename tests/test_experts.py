@@ -339,6 +339,32 @@ def test_q4_mlp(M, K, N, group, bias, act, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("M", [1, 2, 3, 16, 17, 64])
+def test_q4_mlp_writes_as_much_scratch_as_the_header_says(M):
+    """h of GMLP_Q4_MLP_H_ELEMENTS, all of it in use, and nothing behind it."""
+    import re
+    from pathlib import Path
+
+    header = (Path(__file__).resolve().parent.parent / "include" / "gmlp.h").read_text()
+    pairs = int(re.search(r"#define GMLP_H_PAIR_ROWS_Q4 (\d+)", header).group(1))
+    assert re.search(r"GMLP_Q4_MLP_H_ELEMENTS\(M, N\) \(\(\(M\) <= GMLP_H_PAIR_ROWS_Q4 \? 2 : 1\) \* \(M\) \* \(N\)\)", header)
+    dev, dtype, K, N, group = device(), torch.bfloat16, 136, 264, 64
+    g = gen(M)
+    qs = [q4((N, K), group, dtype, g), q4((N, K), group, dtype, g), q4((K, N), group, dtype, g)]
+    x = normal((M, K), 1.0, dtype, g).to(dev)
+    used = (2 if M <= pairs else 1) * M * N
+    h = torch.full((used + 4 * 64 * N,), math.nan, dtype=dtype, device=dev)
+    y = torch.full((M + 1, K), math.nan, dtype=dtype, device=dev)
+    weights = [t.data_ptr() for q in qs for t in (q.codes, q.scales)]
+    rc = _cabi.lib().gmlp_q4_mlp_fwd(x.data_ptr(), *weights, None, None, None, h.data_ptr(), y.data_ptr(), M, K, N, group, 1, 0, None, 0,
+                                     _cabi.stream_ptr(dev))
+    assert rc == 0
+    torch.cuda.synchronize()
+    assert torch.isfinite(h[:used]).all() and torch.isnan(h[used:]).all()
+    assert torch.isfinite(y[:M]).all() and torch.isnan(y[M]).all()
+
+
+@gpu
 def test_q4_operators_take_leading_dimensions_strides_and_no_rows():
     dev, g, dtype = device(), gen(3), torch.bfloat16
     q = q4((72, 136), 64, dtype, g)

@@ -1,6 +1,7 @@
 // 4-bit weights and expert layers: what the kernels of experts.hip and the C entry points share.
 #pragma once
 #include "common.hpp"
+#include "gmlp.h"
 
 namespace gmlp {
 
@@ -53,7 +54,7 @@ struct ExpertArgs {
 };
 
 // Whether the hidden states of M tokens come as two 16-bit values each, whether ROUTING_SOLO takes the call, and the bytes of `partial` that launch_experts_down asks for (it does with none).
-inline int experts_h_low(int64_t M, int group) { return M <= (group ? 2 : 4); }
+inline int experts_h_low(int64_t M, int group) { return M <= (group ? GMLP_H_PAIR_ROWS_Q4 : GMLP_H_PAIR_ROWS_16BIT); }
 bool experts_solo(int M, int E);
 size_t experts_partial_bytes(const ExpertArgs& a, int group);
 

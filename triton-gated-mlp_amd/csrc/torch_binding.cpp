@@ -582,8 +582,8 @@ Tensor q4_mlp(const Tensor& x_in, const Q4& gate, const OptTensor& bg_in, const 
   const Tensor y = at::empty(x.sizes(), x.options());
   if (M == 0) return y;
   if (M <= FEW_ROWS) {
-    // the hidden states (of up to 2 tokens in two halves) and the workspace in one allocation
-    const size_t plane = ((size_t)((M <= 2 ? 2 : 1) * M * N) * x.element_size() + 255) / 256 * 256;
+    // the hidden states and the workspace in one allocation
+    const size_t plane = ((size_t)GMLP_Q4_MLP_H_ELEMENTS(M, N) * x.element_size() + 255) / 256 * 256;
     const size_t bytes = lib.gmlp_q4_workspace_bytes(M, N, K, wg.group, code);
     const Tensor arena = scratch(plane + bytes, x);
     char* const h = (char*)out_ptr(arena);
