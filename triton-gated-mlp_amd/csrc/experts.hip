@@ -4,8 +4,9 @@
 //   gate/up        h[p] = act(W_gate_e x_t + b_gate) * (W_up_e x_t + b_up)   for every pair p = (token t, its choice e)
 //   down           y[t] = sum_e w_te W_down_e h_te + b_down
 //
-// The products are bound by the weights' way from memory: each weight is read once per call and feeds one
-// v_mfma_f32_16x16x32 column per token row.  A workgroup takes 16 weight rows (gate/up: 16 of each matrix); its wavefronts
+// The products are bound by the weights' way from memory: each weight is read once for the tokens of an entry (all of a
+// dense call's, up to 16 or 32 of an expert's) and feeds one v_mfma_f32_16x16x32 column per token row.  A workgroup takes R
+// tiles of 16 weight rows (gate/up: of each matrix), R = 1, 2 or 4; its wavefronts
 // split the reduction and add up through LDS in a fixed order, so results do not depend on timing.  Every load is a
 // buffer load with an exact descriptor: rows past the matrix, columns past its end, tokens that an expert does not have
 // and the stages past the end of a wavefront's run all get an offset beyond it, which reads as zero and moves no data.
@@ -221,7 +222,7 @@ struct Block {
   static constexpr int ROWS = 64 / PIECES;      // rows of a load
   static constexpr int WL = G ? 1 : 16 / ROWS;  // loads of a weight tile
   static constexpr int TILE = 16 * COLS * 2;    // bytes of a tile in LDS
-  static constexpr int WB = G ? 0 : NT < 4 ? NT : 4;  // weight tiles in LDS at a time
+  static constexpr int WB = G ? 0 : NT;         // weight tiles in LDS
   // 4-bit weights: token rows go to LDS without passing through registers (buffer_load ... lds), a slot for each stage; two
   // stages of the weights then fit where one of both did.  16-bit weights, and a single load of token rows, whose four
   // registers are no matter: one slot for what the wavefront multiplies.
@@ -359,12 +360,7 @@ struct Block {
             for (int m = 0; m < MT; ++m) acc[n][m][r] += f * part[m][r];
           }
         } else {
-          char* const tile = slot + (MT + n % WB) * TILE;
-          if (n >= WB) {
-            turn();
-            to_lds(tile, w[n], lane);
-            turn();
-          }
+          const char* const tile = slot + (MT + n) * TILE;
 #pragma unroll
           for (int s = 0; s < SG; ++s) {
             const vec8 a = operand(tile, s, lane);
