@@ -895,12 +895,15 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
       if (!few) return blocks <= 8 ? run_down<T, G, 1, ALL, 2, 4, 1>(a, parts, s) : run_down<T, G, 1, ALL, 2, 8, 1>(a, parts, s);
       return blocks <= 8 ? run_down<T, G, 1, 1, 2, 4, G == 32 ? 1 : 2>(a, parts, s) : run_down<T, G, 1, 1, 2, 8, G == 32 ? 1 : 2>(a, parts, s);
     }
-  if (few && G != 0) {
-    if (blocks <= 16) return run_down<T, G, 1, 1, 1, 8, 2>(a, parts, s);
-    return blocks < 128 ? run_down<T, G, 1, 1, 1, 8, 4>(a, parts, s) : run_down<T, G, 1, 1, 1, 16, 2>(a, parts, s);
+  if constexpr (G != 0) {
+    if (few) {
+      if (blocks <= 16) return run_down<T, G, 1, 1, 1, 8, 2>(a, parts, s);
+      return blocks < 128 ? run_down<T, G, 1, 1, 1, 8, 4>(a, parts, s) : run_down<T, G, 1, 1, 1, 16, 2>(a, parts, s);
+    }
+  } else {
+    if (few) return blocks < 32 ? run_down<T, 0, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, 0, 1, 1, 1, 16, 1>(a, parts, s);
   }
-  if (blocks < 32) return few ? run_down<T, G, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s);
-  return few ? run_down<T, G, 1, 1, 1, 16, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
+  return blocks < 32 ? run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
 }
 bool experts_solo(int M, int E) { return M == 1 && E <= SOLO_MAX_E; }
 
