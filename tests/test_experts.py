@@ -694,6 +694,154 @@ def test_moe_refusals():
         torch.jit.trace(lambda t: call(t, logits, *ws, 2), (x,))
 
 
+# ------------------------------------------------------------------ every kernel that the rules on sizes can choose
+# The shapes below were picked from the rules in csrc/experts.hip for 256 CUs: a tile is 16 rows, a block 128 columns of the reduction
+# (64 of 16-bit weights).  The references are computed on the GPU, in float64.
+def weights64(q):
+    """weights_of, looked up where the codes are."""
+    codes, scales = q.codes.reshape(-1), q.scales.reshape(-1).double()
+    KB, g = q.codes.shape[-5], q.group_size
+    r = torch.arange(q.rows, device=codes.device).unsqueeze(1)
+    c = torch.arange(q.cols, device=codes.device).unsqueeze(0)
+    block = (r // 16) * KB + c // 128
+    nibble = torch.where(c % 2 == 0, (c % 8) // 2, 4 + (c % 8) // 2)
+    byte = block * 1024 + ((c % 32) // 8) * 256 + (r % 16) * 16 + ((c % 128) // 32) * 4 + nibble // 2
+    n = ((codes[byte].int() >> (4 * (nibble % 2))) & 15) - 8
+    at = block * (16 * 128 // g) + ((r % 16) // 4) * (4 * 128 // g) + ((c % 128) // g) * 4 + r % 4
+    return n.double() * scales[at]
+
+
+def drawn(shape, std, dtype, g):
+    return torch.empty(shape, device=g.device).normal_(0.0, std, generator=g).to(dtype)
+
+
+def on_gpu(seed):
+    return torch.Generator(device=device()).manual_seed(seed)
+
+
+def hold_on_gpu(got, y, bound, dtype, roundings):
+    hold(got, y.cpu(), bound.cpu(), dtype, roundings)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize(
+    "M,R,C",
+    [
+        # up to four tokens: one tile and up to 16, 17 to 127, 128 or more blocks (there split over workgroups too); more tiles
+        # than CUs and up to 8 blocks, more
+        (1, 1544, 264), (1, 2824, 264), (4, 4360, 136), (3, 16392, 72), (2, 520, 4360), (4, 1160, 4120),
+        # 5 to 16: one tile and fewer than 32 blocks, 32 or more; two tiles and up to 8 blocks, more; four tiles
+        (7, 1160, 264), (9, 4360, 136), (16, 1000, 4360), (12, 1160, 4360), (5, 1160, 8200),
+        # 17 to 64, two, three and four token tiles: a short reduction in no more tiles than CUs, more tiles, a long reduction in parts
+        (20, 520, 264), (40, 520, 264), (60, 520, 264), (20, 520, 4360), (40, 520, 4360), (60, 520, 4360), (20, 4360, 264), (40, 4360, 264),
+        (60, 4360, 264),
+    ],
+)
+def test_q4_linear_on_every_kernel(M, R, C, group, dtype):
+    g = on_gpu(M + R)
+    x, q, b = drawn((M, R), 1.0, dtype, g), quant.quantize_q4(drawn((C, R), 0.02, dtype, g), group), drawn((C,), 0.5, dtype, g)
+    ref, bound = linear64(x.double(), weights64(q), b.double(), dtype)
+    hold_on_gpu(quant.q4_linear_fwd(x, q, b), ref, bound, dtype, 1)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize(
+    "M,K,N",
+    [
+        # up to four tokens and 5 to 16, up to four tiles a CU and more
+        (2, 72, 264), (3, 72, 16424), (11, 72, 264), (9, 72, 16424),
+        # 17 to 64: no more tiles than CUs, up to 12 blocks and more; up to two a CU, up to 12 blocks and more; more still
+        *((M, K, N) for M in (20, 40, 60) for K, N in ((136, 264), (1672, 264), (136, 4360), (1672, 4360), (1672, 8200))),
+    ],
+)
+def test_q4_mlp_on_every_kernel(M, K, N, group, dtype):
+    g = on_gpu(M + K)
+    x = drawn((M, K), 1.0, dtype, g)
+    qs = [quant.quantize_q4(drawn(shape, 0.02, dtype, g), group) for shape in ((N, K), (N, K), (K, N))]
+    bs = [drawn((n,), 0.1, dtype, g) for n in (N, N, K)]
+    args = [v for pair in zip(qs, bs) for v in pair]
+    ref, bound = mlp64(x.double(), *(weights64(v) if isinstance(v, quant.Q4Weight) else v.double() for v in args), "silu", dtype)
+    hold_on_gpu(quant.q4_mlp_fwd(x, *args), ref, bound + U[dtype] * ref.abs() + SUB[dtype], dtype, 2)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("bits,group", [(16, 0), (4, 32), (4, 64), (4, 128)])
+@pytest.mark.parametrize(
+    "M,K,N,E,k",
+    [
+        # one token, its routing inside gate/up (up to 256 experts) and ahead of it, with few and many blocks of its experts together
+        (1, 136, 520, 8, 8), (1, 72, 136, 200, 6), (1, 72, 136, 300, 6), (1, 136, 2056, 16, 16),
+        # small batches
+        (3, 136, 520, 200, 4), (8, 136, 392, 100, 2), (14, 136, 392, 8, 2), (16, 72, 1032, 32, 8),
+        # 17 to 64 tokens: few for each expert (one token tile an entry), more (two)
+        (50, 136, 264, 40, 2), (50, 136, 264, 4, 2), (64, 72, 1544, 200, 3), (33, 264, 1544, 6, 3),
+    ],
+)
+def test_moe_mlp_on_every_kernel(M, K, N, E, k, bits, group, dtype):
+    g = on_gpu(M + K + N)
+    x, logits = drawn((M, K), 1.0, dtype, g), drawn((M, E), 1.5, torch.float32, g)
+    ws = [drawn(shape, 0.05, dtype, g) for shape in ((E, N, K), (E, N, K), (E, K, N))]
+    if bits == 4:
+        ws = [quant.quantize_q4(w, group) for w in ws]
+        one = lambda e: tuple(weights64(sliced(w, e)).cpu() for w in ws)
+    else:
+        one = lambda e: tuple(w[e].double().cpu() for w in ws)
+    ref, bound = moe64(x.double().cpu(), logits.cpu(), k, True, "silu", dtype, one)
+    hold(moe.moe_mlp_fwd(x, logits, *ws, k), ref, bound, dtype, 2)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+def test_weights_so_large_that_their_reduction_is_split(dtype):
+    """48 MB and more: four tiles a workgroup and three parts (4 bits, 12 tokens), one tile and three parts (16 bits, 9 tokens)."""
+    g = on_gpu(1)
+    M, R, C = 12, 23432, 4104
+    x, q = drawn((M, R), 1.0, dtype, g), quant.quantize_q4(drawn((C, R), 0.02, dtype, g), 128)
+    ref, bound = linear64(x.double(), weights64(q), None, dtype)
+    y = quant.q4_linear_fwd(x, q)
+    hold_on_gpu(y, ref, bound, dtype, 1)
+    # the same without a workspace, in one part
+    whole = torch.empty_like(y)
+    rc = _cabi.lib().gmlp_q4_linear_fwd(x.data_ptr(), q.codes.data_ptr(), q.scales.data_ptr(), None, whole.data_ptr(), M, R, C, 128,
+                                        HALF.index(dtype), None, 0, _cabi.stream_ptr(device()))
+    assert rc == 0
+    hold_on_gpu(whole, ref, bound, dtype, 1)
+    M, K, N, E = 9, 1032, 11656, 2
+    x, logits = drawn((M, K), 1.0, dtype, g), drawn((M, E), 1.5, torch.float32, g)
+    ws = [drawn(shape, 0.02, dtype, g) for shape in ((E, N, K), (E, N, K), (E, K, N))]
+    ref, bound = moe64(x.double().cpu(), logits.cpu(), 2, True, "silu", dtype, lambda e: tuple(w[e].double().cpu() for w in ws))
+    hold(moe.moe_mlp_fwd(x, logits, *ws, 2), ref, bound, dtype, 2)
+
+
+@gpu
+@pytest.mark.parametrize("M", [1, 2, 30])
+@pytest.mark.parametrize("E", [8, 100, 200, 300])
+def test_logits_of_every_type(M, E):
+    """16-bit logits route as their values in float32 do."""
+    dtype, K, N, k = torch.bfloat16, 72, 136, 3
+    g = on_gpu(E)
+    x, logits = drawn((M, K), 1.0, dtype, g), drawn((M, E), 1.5, torch.float32, g)
+    ws = [drawn(shape, 0.05, dtype, g) for shape in ((E, N, K), (E, N, K), (E, K, N))]
+    for kind in HALF:
+        low = logits.to(kind)
+        assert torch.equal(moe.moe_mlp_fwd(x, low, *ws, k), moe.moe_mlp_fwd(x, low.float(), *ws, k))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,K,E", [(2, 4104, 8), (8, 2056, 64), (12, 4104, 256), (20, 1160, 12), (40, 1160, 8), (60, 4104, 128)])
+def test_moe_logits_on_every_kernel(M, K, E, dtype):
+    g = on_gpu(M + K)
+    x, w = drawn((M, K), 1.0, dtype, g), drawn((E, K), 0.1, dtype, g)
+    y, mass = x.double() @ w.double().T, x.double().abs() @ w.double().abs().T
+    assert ((moe.moe_logits(x, w).double() - y).abs() <= (K + 16) * 2.0**-23 * mass).all()
+
+
 # ------------------------------------------------------------------ streams and graphs
 def _calls(bits):
     dev, dtype, g = device(), torch.bfloat16, gen(4)
