@@ -228,6 +228,41 @@ def test_cpu_tensors_are_refused():
         moe.moe_mlp_fwd(x, torch.zeros(2, 8), w, w, w, 2)
 
 
+def test_forward_mode_and_functorch_are_refused():
+    """Each operator for each tensor that a tangent could come with (a result without it would be wrong)."""
+    import torch.autograd.forward_ad as fw
+
+    half = lambda *shape: torch.zeros(shape, dtype=torch.float16)
+    codes = lambda *lead: torch.zeros((*lead, 4, 1, 4, 16, 4, 4), dtype=torch.uint8)
+    q = lambda scales: quant.Q4Weight(codes(), scales, 64, 64, 128)
+    qe = lambda scales: quant.Q4Weight(codes(2), scales, 64, 64, 128)
+    x, b, s, se, w, wr = half(3, 64), half(64), half(4, 1, 4, 1, 4), half(2, 4, 1, 4, 1, 4), half(2, 64, 64), half(4, 64)
+    logits = torch.zeros(3, 2)
+    calls = [
+        (lambda t: quant.quantize_q4(t), x), (lambda t: quant.dequantize_q4(q(t)), s),
+        (lambda t: quant.q4_linear_fwd(t, q(s)), x), (lambda t: quant.q4_linear_fwd(x, q(t)), s), (lambda t: quant.q4_linear_fwd(x, q(s), t), b),
+        *((lambda t, i=i: quant.q4_mlp_fwd(*(t if j == i else v for j, v in enumerate((x, q(s), b, q(s), b, q(s), b)))), x if i == 0 else b)
+          for i in (0, 2, 4, 6)),
+        *((lambda t, i=i: quant.q4_mlp_fwd(x, *(v for j in range(3) for v in (q(t if j == i else s), None))), s) for i in range(3)),
+        (lambda t: moe.moe_logits(t, wr), x), (lambda t: moe.moe_logits(x, t), wr), (lambda t: moe.moe_route(t, 2), logits),
+        *((lambda t, i=i: moe.moe_mlp_fwd(*(t if j == i else v for j, v in enumerate((x, logits, w, w, w))), 2), (x, logits, w, w, w)[i])
+          for i in range(5)),
+        (lambda t: moe.moe_mlp_fwd(t, logits, qe(se), qe(se), qe(se), 2), x),
+        *((lambda t, i=i: moe.moe_mlp_fwd(x, logits, *(qe(t if j == i else se) for j in range(3)), 2), se) for i in range(3)),
+    ]
+    for call, t in calls:
+        with pytest.raises(RuntimeError, match="AMD GPU"):  # without a transform it gets as far as the device
+            call(t)
+        with fw.dual_level(), torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            call(fw.make_dual(t, t))
+        with pytest.raises(RuntimeError, match="functorch"):
+            torch.vmap(call)(t[None])
+        with pytest.raises(RuntimeError, match="functorch"):
+            torch.func.jvp(call, (t,), (t,))
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(t.clone().requires_grad_(True))
+
+
 # ------------------------------------------------------------------ 4-bit weights
 gpu = pytest.mark.gpu
 
@@ -819,6 +854,32 @@ def test_weights_so_large_that_their_reduction_is_split(dtype):
 
 
 @gpu
+@pytest.mark.parametrize("bits,E", [(16, 40), (4, 160)])
+def test_experts_beyond_4_gib(bits, E):
+    """The last expert's weights lie past 32-bit byte offsets; one token and 20, whose plan has entries of 16."""
+    dtype, K, N = torch.bfloat16, 4096, 14336
+    g = on_gpu(2)
+    if bits == 16:
+        ws = [drawn(shape, 0.02, dtype, g) for shape in ((E, N, K), (E, N, K), (E, K, N))]
+        one = [w[E - 1].double() for w in ws]
+    else:
+        ws = []
+        for rows, cols in ((N, K), (N, K), (K, N)):
+            codes = torch.randint(0, 256, (E, rows // 16, cols // 128, 4, 16, 4, 4), generator=g, dtype=torch.uint8, device=g.device)
+            scales = (0.002 + 0.003 * torch.rand((E, rows // 16, cols // 128, 4, 2, 4), generator=g, device=g.device)).to(dtype)
+            ws.append(quant.Q4Weight(codes, scales, rows, cols, 64))
+        one = [weights64(sliced(w, E - 1)) for w in ws]
+    for M in (1, 20):
+        x, logits = drawn((M, K), 1.0, dtype, g), drawn((M, E), 1.5, torch.float32, g)
+        logits[:, E - 1] += 20
+        ref, bound = mlp64(x.double(), *(v for w in one for v in (w, None)), "silu", dtype)
+        y = moe.moe_mlp_fwd(x, logits, *ws, 1)
+        hold_on_gpu(y, ref, bound + (U[dtype] + 1e-6) * ref.abs() + SUB[dtype], dtype, 2)
+    del ws, one
+    torch.cuda.empty_cache()
+
+
+@gpu
 @pytest.mark.parametrize("M", [1, 2, 30])
 @pytest.mark.parametrize("E", [8, 100, 200, 300])
 def test_logits_of_every_type(M, E):
@@ -980,6 +1041,22 @@ def test_gated_moe_module(E, router, bits):
             other.quantize_(64)
         other.load_state_dict(m.state_dict())
         assert torch.equal(other(x), y)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("E,router", [(8, None), (6, None), (8, torch.float32)])
+def test_gated_moe_module_without_rows(E, router, bits):
+    from triton_gated_mlp import GatedMoE
+
+    m = GatedMoE(64, 72, E, 2).to(device(), torch.float16)
+    if router is not None:
+        m.router.to(router)
+    with torch.no_grad():
+        m = m.quantize_(32) if bits == 4 else m
+        for shape in ((0, 64), (2, 0, 64)):
+            y = m(torch.zeros(shape, dtype=torch.float16, device=device()))
+            assert y.shape == shape and y.dtype == torch.float16
 
 
 def _on_four_bits(E, K, N, dtype):
