@@ -1074,6 +1074,28 @@ def _on_four_bits(E, K, N, dtype):
     return m
 
 
+@pytest.mark.parametrize(
+    "K,N,E,bits,streamed,own",
+    [
+        # a number of rows at which streaming measured the faster way, and one at which passes of their own did
+        (4096, 14336, 8, 16, 96, 192), (2048, 5632, 8, 16, 256, 512), (2048, 1024, 64, 16, 1024, 3072), (1024, 2816, 16, 16, 768, 1536),
+        (4096, 14336, 8, 4, 512, 1024), (2048, 5632, 8, 4, 512, 1536), (2048, 1024, 64, 4, 2048, 6144), (1024, 2816, 16, 4, 1536, 3072),
+        (8192, 28672, 4, 4, 256, 512),
+    ],
+)
+def test_the_way_of_a_batch_goes_by_its_experts_size_and_type(K, N, E, bits, streamed, own):
+    from triton_gated_mlp import GatedMoE
+    from triton_gated_mlp.experts import _Q4Buffers
+
+    with torch.device("meta"):
+        m = GatedMoE(K, N, E, 2)
+        if bits == 4:
+            for name, rows, cols in (("gate_proj", N, K), ("up_proj", N, K), ("down_proj", K, N)):
+                delattr(m, name)
+                setattr(m, name, _Q4Buffers(quant.Q4Weight(torch.empty(1, dtype=torch.uint8), torch.empty(1), rows, cols, 128)))
+    assert streamed < m.long_batch() <= own
+
+
 # (70 rows: the float32 GEMM's logits; 3 rows: that of a float32 router, of a number of experts that is no multiple of 4, and moe_logits)
 ROUTERS = [(70, 8, None), (3, 8, torch.float32), (3, 6, None), (3, 8, None)]
 

@@ -124,11 +124,17 @@ class GatedMoE(nn.Module):
         return _fwd.linear_fwd(x.float(), w)[:, :E]
 
     def long_batch(self) -> int:
-        """Token rows from which the experts' own passes are the faster way.  The streaming kernels read the experts once per 64
-        rows, passes of their own cost 0.12 ms an expert on the host: 8 experts of 4096 x 14336, 128 rows 1.10 ms streamed and
-        1.17 one by one, 192 rows 1.64 and 1.16; 64 of 2048 x 1024, 2048 rows 5.6 and 7.5; 4 bits cross at the same
-        rows."""
-        return max(65, int(2e10 / (3 * self.hidden_size * self.intermediate_size)))
+        """Token rows from which the experts' own passes are the faster way.  The streaming kernels read the experts in use once
+        per 64 rows; passes of their own cost 60 to 70 us an expert on the host or, of large experts, their weights' way at
+        half the rate, and 4-bit weights of more than 64 tokens are written out in 16 bits first.  ms, streamed and one by one,
+        experts of hidden x intermediate size: 16 bits, 8 of 4096 x 14336 128 rows 0.91 0.92, 192 rows 1.37 0.95; 8 of 2048 x 5632
+        384 rows 0.66 0.67, 512 rows 0.88 0.67; 64 of 2048 x 1024 1536 rows 3.4 4.0, 2048 rows 4.6 4.0; 4 of 8192 x 28672 65 rows
+        1.9 1.3.  4 bits, 8 of 4096 x 14336 512 rows 1.6 2.0, 768 rows 2.3 2.1; 8 of 2048 x 5632 768 rows 0.75 0.78, 1024 rows 0.99
+        0.83; 64 of 2048 x 1024 2048 rows 2.1 4.5, 6144 rows 6.4 4.8, but 8 of them 1536 rows 0.71 0.70; 4 of 8192 x 28672 256 rows
+        2.4 3.1, 384 rows 3.5 3.3."""
+        size = self.hidden_size * self.intermediate_size
+        rows = min(9e10 / size, 550 + 4e9 / size) if self.quantized else min(2e10 / (3 * size), 95 + 3.4e9 / size)
+        return max(65, int(rows))
 
     def forward(self, x: Tensor) -> Tensor:
         rows = x.reshape(-1, self.hidden_size)
