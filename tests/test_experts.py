@@ -815,6 +815,8 @@ def test_q4_mlp_on_every_kernel(M, K, N, group, dtype):
         (3, 136, 520, 200, 4), (8, 136, 392, 100, 2), (14, 136, 392, 8, 2), (16, 72, 1032, 32, 8),
         # 17 to 64 tokens: few for each expert (one token tile an entry), more (two)
         (50, 136, 264, 40, 2), (50, 136, 264, 4, 2), (64, 72, 1544, 200, 3), (33, 264, 1544, 6, 3),
+        # on either side of 12 tokens for each
+        (64, 72, 136, 85, 16), (64, 72, 136, 86, 16),
     ],
 )
 def test_moe_mlp_on_every_kernel(M, K, N, E, k, bits, group, dtype):

@@ -31,15 +31,17 @@ typedef __amdgpu_buffer_rsrc_t ex_rsrc;
 __device__ __forceinline__ ex_rsrc ex_make_rsrc(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)bytes, 0x00020000);
 }
+// Tokens for each expert on average up to which an entry has one token tile (token_tiles).
+constexpr int ONE_TILE_TOKENS = 12;
 // LDS of experts_down_kernel for the tables of the largest routing: without GATHER 16 tokens; with it one token tile an entry or,
-// beyond ten tokens for each expert (token_tiles), two.
+// beyond ONE_TILE_TOKENS, two.
 constexpr int ex_tables(int entries, bool gather, int token_tiles, int pairs) {
   return entries * (gather ? 4 + 1 + 16 * token_tiles * 2 : 4 + EXPERTS_MAX_M) + pairs * 4;
 }
 constexpr int ex_tables_at_most(bool gather, int token_tiles) {
   constexpr int pairs = EXPERTS_MAX_M * EXPERTS_MAX_K;
   return !gather ? ex_tables(16 * EXPERTS_MAX_K, false, 1, 16 * EXPERTS_MAX_K)
-                 : ex_tables((token_tiles == 1 ? EXPERTS_MAX_E : pairs / 10) + pairs / 16, true, token_tiles, pairs);
+                 : ex_tables((token_tiles == 1 ? EXPERTS_MAX_E : pairs / ONE_TILE_TOKENS) + pairs / 16, true, token_tiles, pairs);
 }
 constexpr int EX_STREAM = 2;  // cache policy: non-temporal, what is read once
 template <int POLICY = 0>
@@ -760,11 +762,13 @@ __global__ void __launch_bounds__(256) experts_join_kernel(ExpertArgs a, int par
 // Experts that a call can use, and entries of its plan.
 static int experts_at_most(const ExpertArgs& a) { return a.E < a.M * a.top_k ? a.E : a.M * a.top_k; }
 static int entries_at_most(const ExpertArgs& a) { return a.routing == ROUTING_DENSE ? 1 : expert_entries(a.M, a.E, a.top_k); }
-// Token tiles of an entry.  Experts of a plan: one, which nearly all of them fit in, up to ten tokens for each on average,
-// then two (weights of one with more tokens are read again).
+// Token tiles of an entry.  Experts of a plan: one, which nearly all of them fit in, up to 12 tokens for each on average,
+// then two (weights of one with more tokens are read again).  us, plan, gate/up and down with one and two: 64 tokens, 32 experts of K=2048, N=1408,
+// 8 tokens for each 105 106, 12 110 108, 14 122 110, 16 136 110; 4 bits 54 60, 57 62, 63 63, 70 64; 8 of K=N=4096, 16 bits, 48 tokens
+// (12) 150 156, 56 tokens (14) 162 156; 4 bits 66 72, 72 73, 64 tokens (16) 79 73.
 static int token_tiles(const ExpertArgs& a) {
   if (a.routing == ROUTING_DENSE || a.M <= 16) return (a.M + 15) / 16;
-  return a.M * a.top_k <= 10 * a.E ? 1 : 2;
+  return a.M * a.top_k <= ONE_TILE_TOKENS * a.E ? 1 : 2;
 }
 static double weight_bytes(const ExpertArgs& a, int group) {
   return (double)experts_at_most(a) * a.K * a.N * (group ? 0.5 + 2.0 / group : 2.0);
@@ -814,6 +818,8 @@ static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
     if (mt == 1) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
     return run_gateup<T, 0, 2, 2, 2, 4, 1>(a, s);
   } else {
+    // Eight wavefronts on a tile of each matrix, or four on two.  us, K=4096, groups of 128: one token, N=11008 (2.7 tiles a CU) 13.9
+    // 16.1, 16384 (4) 17.5 17.1, 20480 22.3 21.9, 28672 29.2 27.4; 12 tokens 16.2 17.0, 21.7 18.2, 26.9 22.6, 34.4 27.8.
     if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 2>(a, s);
     if (mt == 1) return few ? run_gateup<T, G, 1, 4, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
     // More than one token tile.  Token rows are read again for every strip, so two tiles of each matrix, where the registers hold
@@ -838,8 +844,12 @@ static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
 // Down: tiles of a workgroup, and workgroups that share a strip of them.  The parts' sum is a launch more, 2 us behind others and
 // more from an idle queue.  With more than one token tile it pays beyond 64 blocks (of all experts, times token tiles), even
 // where the weights would not: M=48, 4 bits, 768 rows of 2048 columns 7.7 us whole, 8.4 in four parts; of 4096 10.8 and 8.7.
-// Up to 16 tokens: large weights, which take as long anyway, and long reductions of all experts together in few rows, which would leave CUs
-// idle: 12 tokens, 1 of 32 experts of K=512, N=6144, 4 bits, the layer 51.8 us whole, 30.4 split.
+// Up to 16 tokens: large weights, which take as long anyway (us, 12 tokens, groups of 128, the tiles that smaller ones get, whole, and four
+// split: 4096 rows of 14336 columns, 30 MB, 14.1 14.0, of 22528, 48 MB, 19.5 18.0; 8192 rows of 11008, 46 MB, 17.4 17.6, of 14336,
+// 61 MB, 21.0 20.0; 16 bits whole and split, 2048 rows, 16 experts of 1024 columns, 67 MB, 18.2 14.7), and long reductions of all
+// experts together in few rows, which would leave CUs idle: one token, groups of 128, 1024 rows of 64 blocks 7.1 7.1, of 160
+// 11.35 8.9; 2048 rows of 96 8.8 9.0, of 160 12.0 10.9; 12 tokens, 2048 rows of 64 8.8 8.75, of 160 16.5 13.4; 1 of 32 experts of
+// K=512, N=6144, 4 bits, the layer 51.8 us whole, 30.4 split.
 struct DownPlan {
   int tiles, parts;
 };
@@ -896,13 +906,17 @@ static hipError_t down_of(const ExpertArgs& a, hipStream_t s) {
       return blocks <= 8 ? run_down<T, G, 1, 1, 2, 4, G == 32 ? 1 : 2>(a, parts, s) : run_down<T, G, 1, 1, 2, 8, G == 32 ? 1 : 2>(a, parts, s);
     }
   if constexpr (G != 0) {
+    // us as (wavefronts, stages), one token, groups of 128, weights from memory: 2048 rows of 16 blocks (8, 2) 4.4 (8, 4) 4.6 (16, 2)
+    // 5.0; 32 5.4 5.2 5.6; 44 6.3 6.45 6.6; 80 8.2 8.2 7.9; 4096 rows of 17 5.0 4.9 5.3; 32 5.55 5.4 5.7; 64 8.1 7.5 7.5; 80 9.4 8.8 8.1.
     if (few) {
       if (blocks <= 16) return run_down<T, G, 1, 1, 1, 8, 2>(a, parts, s);
-      return blocks < 128 ? run_down<T, G, 1, 1, 1, 8, 4>(a, parts, s) : run_down<T, G, 1, 1, 1, 16, 2>(a, parts, s);
+      return blocks < 64 ? run_down<T, G, 1, 1, 1, 8, 4>(a, parts, s) : run_down<T, G, 1, 1, 1, 16, 2>(a, parts, s);
     }
   } else {
     if (few) return blocks < 32 ? run_down<T, 0, 1, 1, 1, 8, 1>(a, parts, s) : run_down<T, 0, 1, 1, 1, 16, 1>(a, parts, s);
   }
+  // us with 8 and 16 wavefronts, 2048 rows: 12 tokens, groups of 128, 24 blocks 5.8 6.2, 32 6.6 6.4, 64 9.9 8.8; 16 bits, 2 tokens 5.2 5.35,
+  // 5.9 5.5, 8.7 7.3; 12 tokens 5.4 5.6, 6.2 5.8, 9.3 8.6.
   return blocks < 32 ? run_down<T, G, 1, ALL, 1, 8, 1>(a, parts, s) : run_down<T, G, 1, ALL, 1, 16, 1>(a, parts, s);
 }
 bool experts_solo(int M, int E) { return M == 1 && E <= SOLO_MAX_E; }
