@@ -425,8 +425,8 @@ __device__ __forceinline__ void sum_wavefronts(const f32x4 (&acc)[NU][U], char* 
 // A workgroup: 16 * R rows of each matrix of one expert.  What bounds it is the weights' stream: 16 bits, 8 experts of K=4096,
 // N=14336, one token on two of them, 470 MB in 76 us (6.2 TB/s; a device copy moves 5.3); 4 bits, all 8 of them for
 // 16 tokens, 480 MB in 80 us (6.0 TB/s).  One matrix of 4 bits is shorter than its start and end: K=2048, N=5632, one token, 12 MB
-// in 6.5 us.  M=48, K=4096, N=11008, groups of 64, 48 MB in 25 us: there the conversions and the two workgroups that
-// fit a CU bound it.
+// in 6.5 us.  M=48, K=4096, N=11008, groups of 64, 48 MB in 25 us: there the grid (344 workgroups on two
+// places a CU: 88 CUs hold two of them) and the conversions bound it.
 template <typename T, int G, int MT, int XR, int R, int NW, int D>
 constexpr int gateup_lds() {
   constexpr int ring = NW * Block<T, G, 2 * R, MT, XR>::lds_bytes(D), part = NW * units_at_a_time<NW, R * MT, 2>() * 2 * 1024;

@@ -46,7 +46,8 @@ def moe_mlp_fwd(
 
     x [..., K]; logits [..., E]; W_gate, W_up [E, N, K] and W_down [E, K, N] in x's dtype, or all three as Q4Weight.  Made for a
     few tokens: the weights of every expert that any of 64 token rows chose are read once, and of no other; a longer
-    batch runs 64 rows at a time.  Nothing is copied to the host."""
+    batch runs 64 rows at a time.  Nothing is copied to the host.  Beyond 4 token rows (2 with Q4Weight) the hidden
+    states are rounded to x's dtype, as FusedGatedMLP does; the sum over experts is rounded once."""
     binding = _cabi.torch_binding()
     quantized = [isinstance(w, Q4Weight) for w in (W_gate, W_up, W_down)]
     if any(quantized) and not all(quantized):

@@ -59,5 +59,6 @@ def q4_mlp_fwd(
     act_fn: str = "silu",
 ) -> Tensor:
     """A whole gated MLP on 4-bit weights: two kernels up to 64 token rows, beyond as q4_linear_fwd.  Beyond
-    2 token rows the hidden states are rounded to x's dtype between the two, as FusedGatedMLP does."""
+    2 token rows the hidden states are rounded to x's dtype between the two, as FusedGatedMLP does (in float16 one past
+    65504 is infinite)."""
     return _cabi.torch_binding().q4_mlp(x, W_gate, b_gate, W_up, b_up, W_down, b_down, _cabi.act_code(act_fn))
