@@ -1653,7 +1653,9 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
   if (int rc = check_rows(__func__, M)) return rc;
   if (int rc = check_mult8(__func__, "K", K)) return rc;
   if (int rc = check_mult8(__func__, "N", N)) return rc;
-  if (int rc = check_expert_sizes(__func__, M, K, N, gmlp::expert_entries((int)M, (int)E, (int)top_k), (M * top_k) << gmlp::experts_h_low(M, group))) return rc;
+  if (int rc = check_expert_sizes(__func__, M, K, N, gmlp::expert_entries((int)M, (int)E, (int)top_k),
+                                  (M * top_k) << gmlp::experts_h_low(M, group)))
+    return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(w_gate); GMLP_REQUIRE_ALIGNED(w_up);
   GMLP_REQUIRE_ALIGNED(w_down); GMLP_REQUIRE_ALIGNED(s_gate); GMLP_REQUIRE_ALIGNED(s_up); GMLP_REQUIRE_ALIGNED(s_down);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);

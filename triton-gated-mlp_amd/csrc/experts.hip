@@ -6,10 +6,10 @@
 //
 // The products are bound by the weights' way from memory: each weight is read once for the tokens of an entry (all of a
 // dense call's, up to 16 or 32 of an expert's) and feeds one v_mfma_f32_16x16x32 column per token row.  A workgroup takes R
-// tiles of 16 weight rows (gate/up: of each matrix), R = 1, 2 or 4; its wavefronts
-// split the reduction and add up through LDS in a fixed order, so results do not depend on timing.  Every load is a
-// buffer load with an exact descriptor: rows past the matrix, columns past its end, tokens that an expert does not have
-// and the stages past the end of a wavefront's run all get an offset beyond it, which reads as zero and moves no data.
+// tiles of 16 weight rows (gate/up: of each matrix), R = 1, 2 or 4; its wavefronts split the reduction and add up through LDS
+// in a fixed order, so results do not depend on timing.  Every load is a buffer load with an exact descriptor: rows past
+// the matrix, columns past its end, tokens that an expert does not have and the stages past the end of a wavefront's run all
+// get an offset beyond it, which reads as zero and moves no data.
 //
 // 4-bit weights keep their integers for the matrix product (exact in 16 bits); a group's scale is applied to the
 // product in fp32, so what is multiplied is scale·n itself, not its rounding.
@@ -812,14 +812,15 @@ template <typename T, int G>
 static hipError_t gateup_of(const ExpertArgs& a, hipStream_t s) {
   const int mt = token_tiles(a);
   const int tiles = (a.N + Q4_TILE - 1) / Q4_TILE * entries_at_most(a);
-  const bool few = tiles <= 4 * a.cus;
+  const bool few = tiles <= 3 * a.cus;
   if constexpr (G == 0) {
     if (a.M <= 8) return run_gateup<T, 0, 1, 1, 1, 4, 2>(a, s);
     if (mt == 1) return run_gateup<T, 0, 1, 2, 1, 4, 2>(a, s);
     return run_gateup<T, 0, 2, 2, 2, 4, 1>(a, s);
   } else {
-    // Eight wavefronts on a tile of each matrix, or four on two.  us, K=4096, groups of 128: one token, N=11008 (2.7 tiles a CU) 13.9
-    // 16.1, 16384 (4) 17.5 17.1, 20480 22.3 21.9, 28672 29.2 27.4; 12 tokens 16.2 17.0, 21.7 18.2, 26.9 22.6, 34.4 27.8.
+    // Eight wavefronts on a tile of each matrix, or four on two.  us, groups of 128, K=4096: one token, N=11008 (2.7 tiles a CU) 13.9
+    // 16.1, 14336 (3.5) 16.9 16.5, 28672 (7) 29.2 27.4; 12 tokens 16.2 17.0, 20.2 17.6, 34.4 27.8; K=2048: 9.2 10.1, 10.7 10.3, 18.1 16.4;
+    // 9.7 10.4, 12.0 10.6, 20.5 17.1.
     if (a.M <= 4) return few ? run_gateup<T, G, 1, 1, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 1, 2, 4, 2>(a, s);
     if (mt == 1) return few ? run_gateup<T, G, 1, 4, 1, 8, 2>(a, s) : run_gateup<T, G, 1, 4, 2, 4, 1>(a, s);
     // More than one token tile.  Token rows are read again for every strip, so two tiles of each matrix, where the registers hold

@@ -73,7 +73,8 @@ class GatedMoE(nn.Module):
     `router` [experts, hidden] gives float32 logits, from weights of x's type or float32; gate_proj, up_proj [experts, intermediate,
     hidden] and down_proj [experts, hidden, intermediate] have x's type.  Few tokens run on the weight-streaming
     kernels, nothing goes to the host, and the call can be captured into a HIP graph; from `long_batch` token rows on
-    the experts run one after the other on the dense kernels, which needs the number of each expert's tokens on the host.
+    the experts run one after the other on the dense kernels, which needs the number of each expert's tokens on the host
+    and rounds each expert's output to x's type ahead of the sum over experts.
     """
 
     def __init__(self, hidden_size: int, intermediate_size: int, num_experts: int, top_k: int, normalize: bool = True,
