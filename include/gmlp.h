@@ -378,6 +378,64 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
                  int normalize, int group, int dtype, int logits_dtype, int act, void* workspace, size_t workspace_bytes,
                  void* stream);
 
+/*
+ * Routing that is trained: gmlp_moe_route's weights and experts, the number of tokens of each expert, the balance loss, and the
+ * gradient of the logits.  The reference has none of it.
+ *
+ * gmlp_moe_balance_fwd: weights [M, top_k] and experts [M, top_k] are gmlp_moe_route's (up to 256 experts bit for bit; beyond, the
+ *   sums of the weights have another order).  counts [E]: choices of each
+ *   expert by the tokens that count: those that `mask` [M] (bytes, NULL: all) has not at 0 and to which at least one expert is
+ *   available; a choice of an expert that is not (-inf) does not count.  loss [1] = E sum_e f_e P_e, f_e = counts_e / sum of
+ *   counts, P_e = mean of the softmax probability of e over the tokens that count: 1 where all experts get as much, 0 where
+ *   no token counts.  slope [E]: f_e E / number of tokens that count, for the backward pass.
+ * gmlp_moe_balance_bwd: d_logits [M, E] in dtype from d_weights [M, top_k] and d_loss [1] (either may be NULL: zero); counts
+ *   are constants.  The others are what the forward pass read and wrote.
+ * dtype: of the logits (any GMLP_* one).  1 <= top_k <= 16, top_k <= E <= 512, any M; pointers need the alignment of their
+ * elements only, workspace (gmlp_moe_balance_workspace_bytes) 16 bytes.
+ */
+size_t gmlp_moe_balance_workspace_bytes(int64_t M, int64_t E);
+int gmlp_moe_balance_fwd(const void* logits, const uint8_t* mask, float* weights, int64_t* experts, int64_t* counts, float* loss,
+                         float* slope, int64_t M, int64_t E, int64_t top_k, int normalize, int dtype, void* workspace,
+                         size_t workspace_bytes, void* stream);
+int gmlp_moe_balance_bwd(const void* logits, const uint8_t* mask, const float* weights, const int64_t* experts, const float* slope,
+                         const float* d_weights, const float* d_loss, void* d_logits, int64_t M, int64_t E, int64_t top_k,
+                         int normalize, int dtype, void* stream);
+
+/*
+ * 8-bit integer weights and activations, inference only, fp16 and bf16, any number of token rows.  A row of numbers v becomes
+ * n = 127 v / max|v| rounded to nearest (even) and the scale max|v| / 127 (float): a row of a weight, once, or of token
+ * rows, in each call.  A row with a number that is not finite has scale NaN and n = 0.  Products are sums of n, exact in
+ * 32-bit integers, times both scales in fp32.
+ *
+ * Storage of a matrix [rows, cols] (multiples of 8, cols at most 131072), padded with zeros to tiles of 16 rows and blocks of 128
+ * columns: codes int8 [tiles][blocks][2 s][4 q][16 r][16]: columns 64 s + 16 q + 0..15 of the block, row r of the tile;
+ * scales float [rows].  Several matrices of one size (experts) follow each other.
+ *
+ * gmlp_q8_quantize, gmlp_q8_dequantize (w = scale·n rounded to dtype): `count` matrices (at most 65535).
+ * gmlp_q8_linear_fwd: y[M,C] = x[M,R]·Wᵀ + bias, W [C,R]; bias may be NULL.
+ * gmlp_q8_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) rounded to dtype (in fp16 one past 65504 is infinite, and the
+ *   token's outputs NaN), y = h·W_downᵀ + b_down, h in 8 bits again.
+ * gmlp_q8_moe_fwd: y[m] = sum over m's experts e of weight·MLP_e(x[m]), routed as gmlp_moe_route does, the sum over experts in
+ *   fp32; experts without tokens are not read, and a choice of weight 0 is not run.  M * top_k <= GMLP_Q8_MOE_MAX_PAIRS.
+ * workspace: as many bytes as the function beside each says.
+ */
+#define GMLP_Q8_MOE_MAX_PAIRS 65536
+int gmlp_q8_quantize(const void* w, void* codes, float* scales, int64_t count, int64_t rows, int64_t cols, int dtype, void* stream);
+int gmlp_q8_dequantize(const void* codes, const float* scales, void* w, int64_t count, int64_t rows, int64_t cols, int dtype,
+                       void* stream);
+size_t gmlp_q8_linear_workspace_bytes(int64_t M, int64_t R, int64_t C, int dtype);
+int gmlp_q8_linear_fwd(const void* x, const void* codes, const float* scales, const void* bias, void* y, int64_t M, int64_t R,
+                       int64_t C, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t gmlp_q8_mlp_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype);
+int gmlp_q8_mlp_fwd(const void* x, const void* codes_gate, const float* scales_gate, const void* codes_up, const float* scales_up,
+                    const void* codes_down, const float* scales_down, const void* b_gate, const void* b_up, const void* b_down, void* y,
+                    int64_t M, int64_t K, int64_t N, int dtype, int act, void* workspace, size_t workspace_bytes, void* stream);
+size_t gmlp_q8_moe_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int dtype);
+int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, const void* codes_up, const void* codes_down,
+                    const float* scales_gate, const float* scales_up, const float* scales_down, void* y, int64_t M, int64_t K, int64_t N,
+                    int64_t E, int64_t top_k, int normalize, int dtype, int logits_dtype, int act, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* Writes the dropout keep mask (1 = keep) for an [M,N] tensor; the test oracle of the generator. */
 int gmlp_dropout_mask(uint8_t* mask, int64_t M, int64_t N, float dropout_p, uint64_t seed,
                       uint64_t offset, void* stream);

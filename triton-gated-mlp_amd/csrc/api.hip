@@ -11,8 +11,10 @@
 #include <mutex>
 #include <vector>
 
+#include "balance.hpp"
 #include "experts.hpp"
 #include "launch.hpp"
+#include "q8.hpp"
 
 namespace {
 
@@ -1692,6 +1694,371 @@ int gmlp_moe_fwd(const void* x, const void* logits, const void* w_gate, const vo
     if (hipError_t e = gmlp::launch_experts_gateup<T>(a, group, s)) return e;
     if (a.routing == gmlp::ROUTING_SOLO) a.routing = gmlp::ROUTING_PLAN;  // which gate/up has left
     return gmlp::launch_experts_down<T>(a, group, s);
+  }));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ routing that is trained
+extern "C" {
+
+size_t gmlp_moe_balance_workspace_bytes(int64_t M, int64_t E) {
+  if (M < 1 || M > kMaxDim || E < 1 || E > gmlp::EXPERTS_MAX_E) return 0;
+  return (size_t)gmlp::balance_workgroups(M) * gmlp::balance_partial((int)E) * sizeof(float);
+}
+
+int gmlp_moe_balance_fwd(const void* logits, const uint8_t* mask, float* weights, int64_t* experts, int64_t* counts, float* loss,
+                         float* slope, int64_t M, int64_t E, int64_t top_k, int normalize, int dtype, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  GMLP_REQUIRE_PTR(logits); GMLP_REQUIRE_PTR(weights); GMLP_REQUIRE_PTR(experts); GMLP_REQUIRE_PTR(counts);
+  GMLP_REQUIRE_PTR(loss); GMLP_REQUIRE_PTR(slope); GMLP_REQUIRE_PTR(workspace);
+  GMLP_REQUIRE_DTYPE(dtype);
+  if (int rc = check_routing(__func__, E, top_k)) return rc;
+  if (M < 1 || M > kMaxDim) return fail(GMLP_ESHAPE, "%s: M = %lld must be in [1, 2^30]", __func__, (long long)M);
+  GMLP_REQUIRE_ALIGNED(workspace);
+  const size_t needs = gmlp_moe_balance_workspace_bytes(M, E);
+  if (workspace_bytes < needs) return fail(GMLP_EINVAL, "%s: workspace of %zu bytes, needs %zu", __func__, workspace_bytes, needs);
+  gmlp::BalanceArgs a = {};
+  a.logits = logits; a.mask = mask; a.weights = weights; a.experts = experts; a.counts = counts; a.loss = loss; a.slope = slope;
+  a.partial = (float*)workspace;
+  a.M = M; a.E = (int)E; a.top_k = (int)top_k; a.normalize = normalize;
+  return hip_result(__func__, by_dtype(dtype, [&](auto tag) { return gmlp::launch_balance_fwd<decltype(tag)>(a, (hipStream_t)stream); }));
+}
+
+int gmlp_moe_balance_bwd(const void* logits, const uint8_t* mask, const float* weights, const int64_t* experts, const float* slope,
+                         const float* d_weights, const float* d_loss, void* d_logits, int64_t M, int64_t E, int64_t top_k,
+                         int normalize, int dtype, void* stream) {
+  GMLP_REQUIRE_PTR(logits); GMLP_REQUIRE_PTR(weights); GMLP_REQUIRE_PTR(experts); GMLP_REQUIRE_PTR(slope); GMLP_REQUIRE_PTR(d_logits);
+  GMLP_REQUIRE_DTYPE(dtype);
+  if (int rc = check_routing(__func__, E, top_k)) return rc;
+  if (M < 1 || M > kMaxDim) return fail(GMLP_ESHAPE, "%s: M = %lld must be in [1, 2^30]", __func__, (long long)M);
+  gmlp::BalanceArgs a = {};
+  a.logits = logits; a.mask = mask; a.weights = const_cast<float*>(weights); a.experts = const_cast<int64_t*>(experts);  // read only
+  a.slope = const_cast<float*>(slope);
+  a.d_weights = d_weights; a.d_loss = d_loss; a.d_logits = d_logits;
+  a.M = M; a.E = (int)E; a.top_k = (int)top_k; a.normalize = normalize;
+  return hip_result(__func__, by_dtype(dtype, [&](auto tag) { return gmlp::launch_balance_bwd<decltype(tag)>(a, (hipStream_t)stream); }));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ 8-bit integers
+namespace {
+
+int check_q8_type(const char* fn, int dtype) {
+  if (dtype != GMLP_F16 && dtype != GMLP_BF16)
+    return fail(dtype == GMLP_F32 ? GMLP_ESHAPE : GMLP_EINVAL, "%s: dtype %d is not GMLP_F16/GMLP_BF16", fn, dtype);
+  return 0;
+}
+int check_q8_cols(const char* fn, const char* name, int64_t cols) {
+  if (int rc = check_mult8(fn, name, cols)) return rc;
+  if (cols > gmlp::Q8_MAX_COLS)
+    return fail(GMLP_ESHAPE, "%s: %s = %lld exceeds the %d columns whose sums fit 32 bits", fn, name, (long long)cols, gmlp::Q8_MAX_COLS);
+  return 0;
+}
+// Launches have fewer than 2^32 threads: a workgroup of 512 per tile of weight rows and 16 token rows at most, and of 256 per
+// 16 rows of integers.
+int check_q8_sizes(const char* fn, int64_t rows, int64_t K, int64_t N, int64_t tiles) {
+  const int64_t most = K > N ? K : N;
+  if (cdiv(rows, 16) >= ((int64_t)1 << 24) || tiles * cdiv(most, 16) >= ((int64_t)1 << 32) / 512 ||
+      rows * cdiv(most, 8) >= ((int64_t)1 << 40))
+    return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
+  return 0;
+}
+int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
+// Parts of a workspace, one behind the other.
+struct Arena {
+  size_t at = 0;
+  size_t part(int64_t bytes) {
+    const size_t begin = at;
+    at += (size_t)round256(bytes);
+    return begin;
+  }
+};
+
+int q8_token_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+
+// How a dense product of more rows than the streaming kernels take runs.  A reduction tile of 128 integers costs what one of 64
+// 16-bit elements does (the same bytes and as many matrix instructions), so the estimates are theirs.
+GemmPlan plan_q8(int kind, int64_t M, int64_t N, int64_t padded) {
+  return cheapest(kind, tiles_of(kLarge, kind, M, N), tiles_of(kWide, kind, M, N), 0, tiles_of(kMedium, kind, M, N), padded / 128,
+                  (double)M * (double)N * (kind == GATEUP ? 2 : 1), kMaxSplits);
+}
+size_t q8_split_bytes(int kind, int64_t M, int64_t N, int64_t padded) {
+  if (M <= gmlp::Q8_FEW_ROWS) return 0;
+  return split_workspace_bytes(plan_q8(kind, M, N, padded).splits, M, N, kind == GATEUP ? 2 : 1);
+}
+
+gmlp::Q8Product q8_product(const int8_t* x, const float* sx, int64_t M, int64_t N, int64_t cols) {
+  gmlp::Q8Product p = {};
+  p.x = x; p.sx = sx;
+  p.M = (int)M; p.N = (int)N; p.K = (int)gmlp::q8_padded(cols);
+  p.nxcd = num_xcd(); p.cus = num_cu();
+  p.splits = 1;
+  return p;
+}
+template <typename T>
+hipError_t run_q8_dense(gmlp::Q8Product& p, int sets, float* partial, hipStream_t s) {
+  if (p.M <= gmlp::Q8_FEW_ROWS) return gmlp::launch_q8_few<T>(p, sets, q8_token_tiles(p.M), s);
+  const GemmPlan plan = plan_q8(sets == 2 ? GATEUP : LINEAR, p.M, p.N, p.K);
+  p.tile_class = plan.tile_class;
+  p.splits = plan.splits;
+  p.rotate = p.M <= 512;
+  p.group_m = pick_group(p.M, p.N, sets);
+  p.partial = partial;
+  return gmlp::launch_q8_gemm<T>(p, sets, s);
+}
+
+struct Q8LinearWorkspace {
+  size_t x, sx, partial, bytes;
+  Q8LinearWorkspace(int64_t M, int64_t R, int64_t C) {
+    Arena a;
+    const int64_t padded = gmlp::q8_padded(R);
+    x = a.part(gmlp::q8_tiled_rows(M) * padded);
+    sx = a.part(M * 4);
+    partial = a.part((int64_t)q8_split_bytes(LINEAR, M, C, padded));
+    bytes = a.at;
+  }
+};
+struct Q8MlpWorkspace {
+  size_t x, sx, h, q, sq, partial, bytes;
+  Q8MlpWorkspace(int64_t M, int64_t K, int64_t N) {
+    Arena a;
+    const int64_t kp = gmlp::q8_padded(K), np = gmlp::q8_padded(N);
+    x = a.part(gmlp::q8_tiled_rows(M) * kp);
+    sx = a.part(M * 4);
+    h = a.part(M * N * 2);
+    q = a.part(gmlp::q8_tiled_rows(M) * np);
+    sq = a.part(M * 4);
+    partial = a.part((int64_t)std::max(q8_split_bytes(GATEUP, M, N, kp), q8_split_bytes(LINEAR, M, K, np)));
+    bytes = a.at;
+  }
+};
+
+// An expert layer: rows of a tile, and with it which kernels: 16, 32 or 64 the streaming ones, 128 and 256 the GEMM.
+struct Q8MoePlan {
+  int cap, tile_class[2];
+  int64_t rows, tiles;
+};
+Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
+  Q8MoePlan p = {};
+  const int64_t each = cdiv(pairs, E);
+  if (each <= 12) p.cap = 16;
+  else if (each <= 24) p.cap = 32;
+  else if (each <= 48) p.cap = 64;
+  else {
+    p.cap = each >= 512 ? 256 : 128;
+    p.tile_class[0] = p.tile_class[1] = each >= 512 ? gmlp::TILE_LARGE : gmlp::TILE_WIDE;
+  }
+  p.rows = gmlp::q8_plan_rows(pairs, E);
+  p.tiles = gmlp::q8_plan_tiles(pairs, E, p.cap);
+  return p;
+}
+struct Q8MoeWorkspace {
+  size_t weights, experts, total, tiles, row_of, token_of, x, sx, h, q, sq, parts, bytes;
+  Q8MoeWorkspace(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k) {
+    Arena a;
+    const int64_t pairs = M * top_k;
+    const Q8MoePlan p = plan_q8_moe(pairs, K, N, E);
+    weights = a.part(pairs * 4);
+    experts = a.part(pairs * 8);
+    total = a.part(8);
+    tiles = a.part(p.tiles * (int64_t)sizeof(gmlp::Q8Tile));
+    row_of = a.part(pairs * 4);
+    token_of = a.part(p.rows * 4);
+    x = a.part(p.rows * gmlp::q8_padded(K));
+    sx = a.part(p.rows * 4);
+    h = a.part(p.rows * N * 2);
+    q = a.part(p.rows * gmlp::q8_padded(N));
+    sq = a.part(p.rows * 4);
+    parts = a.part(p.rows * K * 4);
+    bytes = a.at;
+  }
+};
+
+}  // namespace
+
+namespace gmlp {
+template <typename T>
+hipError_t launch_q8_gateup(const Q8Product& p, hipStream_t s);
+template <typename T>
+hipError_t launch_q8_single(const Q8Product& p, hipStream_t s);
+template <typename T>
+hipError_t launch_q8_gemm(const Q8Product& p, int sets, hipStream_t s) {
+  if (sets == 2) return launch_q8_gateup<T>(p, s);
+  return p.out_f32 ? launch_q8_single<f16>(p, s) : launch_q8_single<T>(p, s);
+}
+}  // namespace gmlp
+
+extern "C" {
+
+int gmlp_q8_quantize(const void* w, void* codes, float* scales, int64_t count, int64_t rows, int64_t cols, int dtype, void* stream) {
+  GMLP_REQUIRE_PTR(w); GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales);
+  if (int rc = check_q8_type(__func__, dtype)) return rc;
+  if (int rc = check_storage(__func__, count, rows, cols)) return rc;
+  if (int rc = check_q8_cols(__func__, "cols", cols)) return rc;
+  if (count > 65535) return fail(GMLP_ESHAPE, "%s: count = %lld exceeds 65535", __func__, (long long)count);
+  GMLP_REQUIRE_ALIGNED(w); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales);
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    return gmlp::launch_q8_rows<T>((const T*)w, (int8_t*)codes, scales, count, rows, cols, nullptr, nullptr, (hipStream_t)stream);
+  }));
+}
+
+int gmlp_q8_dequantize(const void* codes, const float* scales, void* w, int64_t count, int64_t rows, int64_t cols, int dtype,
+                       void* stream) {
+  GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales); GMLP_REQUIRE_PTR(w);
+  if (int rc = check_q8_type(__func__, dtype)) return rc;
+  if (int rc = check_storage(__func__, count, rows, cols)) return rc;
+  if (int rc = check_q8_cols(__func__, "cols", cols)) return rc;
+  if (count > 65535) return fail(GMLP_ESHAPE, "%s: count = %lld exceeds 65535", __func__, (long long)count);
+  GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(w);
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    return gmlp::launch_q8_dequantize<T>((const int8_t*)codes, scales, (T*)w, count, rows, cols, (hipStream_t)stream);
+  }));
+}
+
+size_t gmlp_q8_linear_workspace_bytes(int64_t M, int64_t R, int64_t C, int dtype) {
+  if (M < 1 || M > kMaxDim || R < 1 || R > gmlp::Q8_MAX_COLS || C < 1 || C > kMaxDim || check_q8_type(__func__, dtype) != 0) return 0;
+  return Q8LinearWorkspace(M, R, C).bytes;
+}
+
+int gmlp_q8_linear_fwd(const void* x, const void* codes, const float* scales, const void* bias, void* y, int64_t M, int64_t R,
+                       int64_t C, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales); GMLP_REQUIRE_PTR(y); GMLP_REQUIRE_PTR(workspace);
+  if (int rc = check_q8_type(__func__, dtype)) return rc;
+  if (int rc = check_dims(__func__, M, R, C)) return rc;
+  if (int rc = check_q8_cols(__func__, "R", R)) return rc;
+  if (int rc = check_mult8(__func__, "C", C)) return rc;
+  if (int rc = check_q8_sizes(__func__, M, R, C, cdiv(M, 128))) return rc;
+  GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(bias);
+  GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
+  const Q8LinearWorkspace ws(M, R, C);
+  if (workspace_bytes < ws.bytes) return fail(GMLP_EINVAL, "%s: workspace of %zu bytes, needs %zu", __func__, workspace_bytes, ws.bytes);
+  char* const base = (char*)workspace;
+  const hipStream_t s = (hipStream_t)stream;
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), M, C, R);
+    p.w[0] = (const int8_t*)codes; p.sw[0] = scales; p.bias[0] = bias; p.out = y;
+    if (hipError_t e = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, M, R, nullptr, nullptr, s))
+      return e;
+    return run_q8_dense<T>(p, 1, (float*)(base + ws.partial), s);
+  }));
+}
+
+size_t gmlp_q8_mlp_workspace_bytes(int64_t M, int64_t K, int64_t N, int dtype) {
+  if (M < 1 || M > kMaxDim || K < 1 || K > gmlp::Q8_MAX_COLS || N < 1 || N > gmlp::Q8_MAX_COLS || check_q8_type(__func__, dtype) != 0)
+    return 0;
+  return Q8MlpWorkspace(M, K, N).bytes;
+}
+
+int gmlp_q8_mlp_fwd(const void* x, const void* codes_gate, const float* scales_gate, const void* codes_up, const float* scales_up,
+                    const void* codes_down, const float* scales_down, const void* b_gate, const void* b_up, const void* b_down, void* y,
+                    int64_t M, int64_t K, int64_t N, int dtype, int act, void* workspace, size_t workspace_bytes, void* stream) {
+  GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(codes_gate); GMLP_REQUIRE_PTR(scales_gate); GMLP_REQUIRE_PTR(codes_up);
+  GMLP_REQUIRE_PTR(scales_up); GMLP_REQUIRE_PTR(codes_down); GMLP_REQUIRE_PTR(scales_down); GMLP_REQUIRE_PTR(y);
+  GMLP_REQUIRE_PTR(workspace);
+  if (int rc = check_q8_type(__func__, dtype)) return rc;
+  GMLP_REQUIRE_ACT(act);
+  if (int rc = check_dims(__func__, M, K, N)) return rc;
+  if (int rc = check_q8_cols(__func__, "K", K)) return rc;
+  if (int rc = check_q8_cols(__func__, "N", N)) return rc;
+  if (int rc = check_q8_sizes(__func__, M, K, N, cdiv(M, 128))) return rc;
+  GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(scales_gate); GMLP_REQUIRE_ALIGNED(codes_up);
+  GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(codes_down); GMLP_REQUIRE_ALIGNED(scales_down);
+  GMLP_REQUIRE_ALIGNED(b_gate); GMLP_REQUIRE_ALIGNED(b_up); GMLP_REQUIRE_ALIGNED(b_down);
+  GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
+  const Q8MlpWorkspace ws(M, K, N);
+  if (workspace_bytes < ws.bytes) return fail(GMLP_EINVAL, "%s: workspace of %zu bytes, needs %zu", __func__, workspace_bytes, ws.bytes);
+  char* const base = (char*)workspace;
+  const hipStream_t s = (hipStream_t)stream;
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    T* const h = (T*)(base + ws.h);
+    float* const partial = (float*)(base + ws.partial);
+    if (hipError_t e = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, M, K, nullptr, nullptr, s))
+      return e;
+    gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), M, N, K);
+    p.w[0] = (const int8_t*)codes_gate; p.sw[0] = scales_gate; p.bias[0] = b_gate;
+    p.w[1] = (const int8_t*)codes_up; p.sw[1] = scales_up; p.bias[1] = b_up;
+    p.out = h; p.act = act;
+    if (hipError_t e = run_q8_dense<T>(p, 2, partial, s)) return e;
+    if (hipError_t e = gmlp::launch_q8_rows<T>(h, (int8_t*)(base + ws.q), (float*)(base + ws.sq), 1, M, N, nullptr, nullptr, s)) return e;
+    p = q8_product((const int8_t*)(base + ws.q), (const float*)(base + ws.sq), M, K, N);
+    p.w[0] = (const int8_t*)codes_down; p.sw[0] = scales_down; p.bias[0] = b_down; p.out = y;
+    return run_q8_dense<T>(p, 1, partial, s);
+  }));
+}
+
+size_t gmlp_q8_moe_workspace_bytes(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k, int dtype) {
+  if (M < 1 || E < 1 || E > gmlp::EXPERTS_MAX_E || top_k < 1 || top_k > gmlp::EXPERTS_MAX_K || M > GMLP_Q8_MOE_MAX_PAIRS / top_k ||
+      K < 1 || K > gmlp::Q8_MAX_COLS || N < 1 || N > gmlp::Q8_MAX_COLS || check_q8_type(__func__, dtype) != 0)
+    return 0;
+  return Q8MoeWorkspace(M, K, N, E, top_k).bytes;
+}
+
+int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, const void* codes_up, const void* codes_down,
+                    const float* scales_gate, const float* scales_up, const float* scales_down, void* y, int64_t M, int64_t K, int64_t N,
+                    int64_t E, int64_t top_k, int normalize, int dtype, int logits_dtype, int act, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  GMLP_REQUIRE_PTR(x); GMLP_REQUIRE_PTR(logits); GMLP_REQUIRE_PTR(codes_gate); GMLP_REQUIRE_PTR(codes_up); GMLP_REQUIRE_PTR(codes_down);
+  GMLP_REQUIRE_PTR(scales_gate); GMLP_REQUIRE_PTR(scales_up); GMLP_REQUIRE_PTR(scales_down); GMLP_REQUIRE_PTR(y);
+  GMLP_REQUIRE_PTR(workspace);
+  if (int rc = check_q8_type(__func__, dtype)) return rc;
+  GMLP_REQUIRE_DTYPE(logits_dtype);
+  GMLP_REQUIRE_ACT(act);
+  if (int rc = check_routing(__func__, E, top_k)) return rc;
+  if (int rc = check_dims(__func__, M, K, N)) return rc;
+  if (int rc = check_q8_cols(__func__, "K", K)) return rc;
+  if (int rc = check_q8_cols(__func__, "N", N)) return rc;
+  if (M > GMLP_Q8_MOE_MAX_PAIRS / top_k)
+    return fail(GMLP_ESHAPE, "%s: M * top_k = %lld exceeds the %d choices of a call", __func__, (long long)(M * top_k), GMLP_Q8_MOE_MAX_PAIRS);
+  const Q8MoePlan plan = plan_q8_moe(M * top_k, K, N, E);
+  if (int rc = check_q8_sizes(__func__, plan.rows, K, N, plan.tiles)) return rc;
+  GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(codes_up); GMLP_REQUIRE_ALIGNED(codes_down);
+  GMLP_REQUIRE_ALIGNED(scales_gate); GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(scales_down);
+  GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
+  const Q8MoeWorkspace ws(M, K, N, E, top_k);
+  if (workspace_bytes < ws.bytes) return fail(GMLP_EINVAL, "%s: workspace of %zu bytes, needs %zu", __func__, workspace_bytes, ws.bytes);
+  char* const base = (char*)workspace;
+  const hipStream_t s = (hipStream_t)stream;
+  float* const weights = (float*)(base + ws.weights);
+  int64_t* const experts = (int64_t*)(base + ws.experts);
+  const gmlp::Q8Plan routed = {(int*)(base + ws.total), (gmlp::Q8Tile*)(base + ws.tiles), (int*)(base + ws.row_of), (int*)(base + ws.token_of)};
+  hipError_t e = by_dtype(logits_dtype, [&](auto tag) {
+    typedef decltype(tag) L;
+    return gmlp::launch_route<L>((const L*)logits, weights, experts, M, (int)E, (int)top_k, normalize, s);
+  });
+  if (e == hipSuccess) e = gmlp::launch_q8_plan(experts, weights, routed, (int)M, (int)E, (int)top_k, plan.cap, s);
+  if (e != hipSuccess) return hip_result(__func__, e);
+  return hip_result(__func__, by_half(dtype, [&](auto tag) {
+    typedef decltype(tag) T;
+    auto product = [&](gmlp::Q8Product& p, int sets) {
+      p.tiles = routed.tiles; p.total = routed.total; p.most_tiles = (int)plan.tiles;
+      if (plan.cap <= gmlp::Q8_FEW_ROWS) return gmlp::launch_q8_few<T>(p, sets, plan.cap / 16, s);
+      p.tile_class = plan.tile_class[sets == 2 ? 0 : 1];
+      p.group_m = 8;
+      return gmlp::launch_q8_gemm<T>(p, sets, s);
+    };
+    T* const h = (T*)(base + ws.h);
+    float* const parts = (float*)(base + ws.parts);
+    if (hipError_t err = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, plan.rows, K,
+                                                 routed.token_of, routed.total + 1, s))
+      return err;
+    gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), plan.rows, N, K);
+    p.w[0] = (const int8_t*)codes_gate; p.sw[0] = scales_gate;
+    p.w[1] = (const int8_t*)codes_up; p.sw[1] = scales_up;
+    p.out = h; p.act = act;
+    if (hipError_t err = product(p, 2)) return err;
+    if (hipError_t err = gmlp::launch_q8_rows<T>(h, (int8_t*)(base + ws.q), (float*)(base + ws.sq), 1, plan.rows, N, nullptr,
+                                                 routed.total + 1, s))
+      return err;
+    p = q8_product((const int8_t*)(base + ws.q), (const float*)(base + ws.sq), plan.rows, K, N);
+    p.w[0] = (const int8_t*)codes_down; p.sw[0] = scales_down; p.out = parts; p.out_f32 = 1;
+    if (hipError_t err = product(p, 1)) return err;
+    return gmlp::launch_q8_combine<T>(parts, weights, routed.row_of, (T*)y, M, K, (int)top_k, s);
   }));
 }
 

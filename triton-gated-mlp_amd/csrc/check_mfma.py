@@ -88,7 +88,7 @@ def follow(code, labels, start, budget, visit):
 
 # instructions that write both of their operands
 SWAPS = re.compile(r"v_(swap_|permlane(16|32)_swap_)")
-PIPELINED = re.compile(r"gemm_(group_|dx_dw_)?kernel_pipelined")
+PIPELINED = re.compile(r"gemm_(group_|dx_dw_|q8_)?kernel_pipelined")
 STREAM_K = re.compile(r"gemm_kernel_pipelined.*Lb1ELb[01]EEEv")
 
 

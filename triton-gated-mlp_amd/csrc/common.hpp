@@ -63,6 +63,26 @@ struct Traits<bf16> {
   static __device__ __forceinline__ bf16 from_f32(float v) { return (bf16)v; }
 };
 
+// 8-bit integers: a unit of two stands where the kernels have a 16-bit element, 16 integers where they have 8, so that loads,
+// LDS and loops are those of the 16-bit types, and a matrix instruction of the same length does twice the products.
+// Sums are 32-bit integers in the registers of the floats (bit patterns, until an epilogue converts them).
+struct I8Pair;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+template <>
+struct Traits<I8Pair> {
+  typedef i32x4 vec8;
+  typedef u32x2 vec4;  // of an epilogue's results: four 16-bit values
+  static __device__ __forceinline__ i32x4 mfma16(vec8 a, vec8 b, i32x4 c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(vec8 a, vec8 b, f32x4 c) {
+    return __builtin_bit_cast(f32x4, mfma16(a, b, __builtin_bit_cast(i32x4, c)));
+  }
+  static __device__ __forceinline__ void mfma16_inplace(vec8 a, vec8 b, f32x4& c) {
+    asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+  }
+};
+
 // Until the results of mfma16_inplace may be read by anything else (7 wait states for the 16x16x32 shape).
 __device__ __forceinline__ void mfma_settle() {
   asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");

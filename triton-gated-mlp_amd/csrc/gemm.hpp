@@ -39,7 +39,8 @@ struct GemmArgs {
                      // otherwise all read the same offset along their rows at the same time, which
                      // for the usual power-of-two row pitches crowds onto a few memory channels.
                      // Workgroups that share B rows keep the same order, so they still share them
-                     // in L2.
+                     // in L2.  (rotate - 1 is added to the column: launches that hand over one tile
+                     // at a time)
   // Stream-K (pipelined kernel, non-split epilogues): the last sk_tiles output tiles (in workgroup
   // order) are not computed one per workgroup; their reduction tiles are shared out evenly over
   // sk_wgs extra workgroups at the end of the grid, which leave partial sums in sk_ws

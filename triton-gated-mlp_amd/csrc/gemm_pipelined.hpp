@@ -182,11 +182,10 @@ __device__ __forceinline__ void gemm_pipelined_body(const GemmArgs& ga, const ty
 #pragma unroll
   for (int i = 0; i < BTile::PER_WAVE; ++i)
     boff[i] = BTile::lane_offset(i, ga.ldb, wave, lane) + DMA_BIAS - (i & 3) * 1024;
-  const uint32_t a_step = A_KS ? (uint32_t)BK * ga.lda * 2 : (uint32_t)BK * 2;
-  const uint32_t b_step = B_KS ? (uint32_t)BK * ga.ldb * 2 : (uint32_t)BK * 2;
+  const uint32_t a_step = ATile::k_step(ga.lda), b_step = BTile::k_step(ga.ldb);
   const uint32_t lds_base = (uint32_t)(uintptr_t)(lds_void*)smem;
-  const uint32_t a_bytes = (uint32_t)(A_KS ? ga.K : ga.M) * ga.lda * 2 + DMA_BIAS - (uint32_t)ga.a_trim;
-  const uint32_t b_bytes = (uint32_t)(B_KS ? ga.K : ga.N) * ga.ldb * 2 + DMA_BIAS - (uint32_t)ga.b_trim;
+  const uint32_t a_bytes = (A_KS ? (uint32_t)ga.K : ATile::stored_rows(ga.M)) * ga.lda * 2 + DMA_BIAS - (uint32_t)ga.a_trim;
+  const uint32_t b_bytes = (B_KS ? (uint32_t)ga.K : BTile::stored_rows(ga.N)) * ga.ldb * 2 + DMA_BIAS - (uint32_t)ga.b_trim;
   const buffer_rsrc ra[2] = {make_rsrc((const char*)ga.A[0] - DMA_BIAS, a_bytes),
                              make_rsrc((const char*)ga.A[1] - DMA_BIAS, a_bytes)};
   const buffer_rsrc rb[2] = {make_rsrc((const char*)ga.B[0] - DMA_BIAS, b_bytes),
@@ -575,7 +574,7 @@ __device__ __forceinline__ void gemm_pipelined_body(const GemmArgs& ga, const ty
     kt_first = __builtin_amdgcn_readfirstlane(kt_first);
     kt_total = __builtin_amdgcn_readfirstlane(kt_total);
     kt_len = kt_total - kt_first;
-    rot = ga.rotate && kt_len > 0 ? tn_i % kt_len : 0;
+    rot = ga.rotate && kt_len > 0 ? (tn_i + ga.rotate - 1) % kt_len : 0;
     a_org = A_KS ? (uint32_t)m0 * 2 : (uint32_t)m0 * ga.lda * 2;
     b_org = B_KS ? (uint32_t)n0 * 2 : (uint32_t)n0 * ga.ldb * 2;
   }

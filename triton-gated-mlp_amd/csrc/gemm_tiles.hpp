@@ -55,6 +55,10 @@ struct LdsTile {
     }
   }
 
+  // Bytes from one reduction tile to the next, and rows that a KC operand of `rows` has in memory.
+  static __device__ __forceinline__ uint32_t k_step(int ld) { return KS ? (uint32_t)BK * ld * 2 : (uint32_t)BK * 2; }
+  static __device__ __forceinline__ uint32_t stored_rows(int rows) { return (uint32_t)rows; }
+
   // MFMA operand fragment (8 reduction elements per lane) for a 16 x 16 x 32 instruction: rows
   // row0 .. row0+15, reduction step ks (32 elements).  Lane l carries row l % 16 and reduction
   // slots 8*(l / 16) .. +7.
@@ -83,6 +87,31 @@ struct LdsTile {
       i16x8 both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
       return __builtin_bit_cast(vec8, both);
     }
+  }
+};
+
+// An operand in 8-bit integers (q8.hpp), whose units of two integers stand in the place of the 16-bit elements: ld and BK count
+// them.  It is stored in tiles of 16 rows, [64 integers][quarter of them][row][16 integers], which is the order in which a
+// wavefront's lanes want the fragments of v_mfma_i32_16x16x64_i8: LDS holds the same KiB blocks, written and read 16 bytes
+// a lane in lane order, without bank conflicts or swizzles.
+template <int ROWS, int BK, bool KS, int NWAVES>
+struct LdsTile<I8Pair, ROWS, BK, KS, NWAVES> {
+  typedef i32x4 vec8;
+  static_assert(BK == 64 && !KS, "8-bit operands are reduction-contiguous, 128 integers a tile");
+  static constexpr int BYTES = ROWS * BK * 2;
+  static constexpr int INSTR = BYTES / 1024;
+  static constexpr int PER_WAVE = INSTR / NWAVES;
+  static_assert(INSTR % NWAVES == 0 && PER_WAVE >= 1, "tile must split evenly over the wavefronts");
+  static __device__ __forceinline__ uint32_t lane_offset(int i, int ld, int wave, int lane) {
+    const int I = wave * PER_WAVE + i;  // block I: row tile I / 2, half I % 2 of the reduction tile
+    return (uint32_t)(I / 2 * 16 * ld) * 2u + (uint32_t)(I % 2 * 1024 + lane * 16);
+  }
+  static __device__ __forceinline__ uint32_t k_step(int) { return 2048u; }
+  static __device__ __forceinline__ uint32_t stored_rows(int rows) { return (uint32_t)(rows + 15) / 16u * 16u; }
+  template <int MI>
+  static __device__ __forceinline__ vec8 frag_mi(const char* lds_tile, int row0, int ks, int lane) {
+    static_assert(MI == 16, "MFMA tile is 16x16x64");
+    return *(const vec8*)(lds_tile + (row0 / 16 * 2 + ks) * 1024 + lane * 16);
   }
 };
 

@@ -43,7 +43,10 @@ typedef std::optional<Tensor> OptTensor;
   X(gmlp_last_error) X(gmlp_workspace_bytes) X(gmlp_mlp_workspace_bytes) X(gmlp_mlp_fwd)         \
   X(gmlp_mlp_bwd) X(gmlp_gateup_fwd) X(gmlp_decode_fwd) X(gmlp_decode_stream_fwd) X(gmlp_hidden_bwd) \
   X(gmlp_grads_workspace_bytes) X(gmlp_linear_fwd) X(gmlp_q4_quantize) X(gmlp_q4_dequantize) X(gmlp_q4_workspace_bytes) X(gmlp_q4_linear_fwd) \
-  X(gmlp_q4_mlp_fwd) X(gmlp_moe_logits) X(gmlp_moe_route) X(gmlp_moe_workspace_bytes) X(gmlp_moe_fwd)
+  X(gmlp_q4_mlp_fwd) X(gmlp_moe_logits) X(gmlp_moe_route) X(gmlp_moe_workspace_bytes) X(gmlp_moe_fwd) \
+  X(gmlp_moe_balance_workspace_bytes) X(gmlp_moe_balance_fwd) X(gmlp_moe_balance_bwd) X(gmlp_q8_quantize) X(gmlp_q8_dequantize) \
+  X(gmlp_q8_linear_workspace_bytes) X(gmlp_q8_linear_fwd) X(gmlp_q8_mlp_workspace_bytes) X(gmlp_q8_mlp_fwd) \
+  X(gmlp_q8_moe_workspace_bytes) X(gmlp_q8_moe_fwd)
 struct Library {
 #define GMLP_MEMBER(name) decltype(&::name) name = nullptr;
   GMLP_ENTRY_POINTS(GMLP_MEMBER)
@@ -160,7 +163,7 @@ Tensor readable(const Tensor& t, int64_t numel, const Tensor& grad) {
 void refuse_second_derivative(const ag::Node& backward, const Tensor& grad, ag::variable_list& out) {
   if (!at::GradMode::is_enabled()) return;
   ag::edge_list next = backward.next_edges();
-  if (grad.requires_grad()) next.push_back(ag::impl::gradient_edge(grad));
+  if (grad.defined() && grad.requires_grad()) next.push_back(ag::impl::gradient_edge(grad));
   const auto node = std::shared_ptr<ag::Error>(
       new ag::Error("the fused gated-MLP operators have no second derivative", std::move(next)), ag::deleteNode);
   for (Tensor& t : out)
@@ -727,6 +730,259 @@ Tensor moe_mlp_q4(const Tensor& x, const Tensor& logits, const Q4& gate, const Q
                   N, E, top_k, normalize, g.group, act);
 }
 
+// ------------------------------------------------------------------ 8-bit integers
+// triton_gated_mlp.ops.quant.Q8Weight: codes, scales, rows, cols
+typedef std::tuple<Tensor, Tensor, int64_t, int64_t> Q8;
+struct Q8Matrix {
+  Tensor codes, scales;
+  int64_t rows, cols, count = 1;
+  // `experts`: 0 for a single matrix; `like`: what it has to be on the device of
+  Q8Matrix(const char* name, const Q8& q, const Tensor& like, int64_t experts, int64_t rows_, int64_t cols_)
+      : codes(std::get<0>(q)), scales(std::get<1>(q)), rows(std::get<2>(q)), cols(std::get<3>(q)) {
+    TORCH_CHECK_VALUE(rows == rows_ && cols == cols_, name, " is [", rows, ", ", cols, "], expected [", rows_, ", ", cols_, "]");
+    std::vector<int64_t> c, s;
+    if (experts > 0) c.push_back(experts), s.push_back(experts), count = experts;
+    c.insert(c.end(), {(rows + 15) / 16, (cols + 127) / 128, 2, 4, 16, 16});
+    s.push_back(rows);
+    TORCH_CHECK_VALUE(codes.sizes() == at::IntArrayRef(c), name, ": codes of size ", codes.sizes(), ", expected ", c);
+    TORCH_CHECK_VALUE(scales.sizes() == at::IntArrayRef(s), name, ": scales of size ", scales.sizes(), ", expected ", s);
+    TORCH_CHECK_TYPE(codes.scalar_type() == at::kChar, name, ": codes are ", codes.scalar_type(), ", expected int8");
+    TORCH_CHECK_TYPE(scales.scalar_type() == at::kFloat, name, ": scales are ", scales.scalar_type(), ", expected float32");
+    TORCH_CHECK(codes.device() == like.device() && scales.device() == like.device(), name, " is on another device than the input");
+    codes = aligned(codes.contiguous());
+    scales = aligned(scales.contiguous());
+  }
+  // (a view may begin anywhere)
+  static Tensor aligned(const Tensor& t) { return (uintptr_t)ptr(t) % 16 == 0 ? t : t.clone(); }
+  const float* s() const { return (const float*)ptr(scales); }
+};
+
+std::tuple<Tensor, Tensor> q8_quantize(const Tensor& w_in) {
+  inference_only("quantize_q8", {w_in});
+  const int code = require_half("quantize_q8", {w_in});
+  TORCH_CHECK_VALUE(w_in.dim() == 2 || w_in.dim() == 3, "quantize_q8 takes [rows, cols] or [experts, rows, cols], got ", w_in.sizes());
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(w_in.device());
+  const Tensor w = Q8Matrix::aligned(w_in.contiguous());
+  const int64_t rows = w.size(-2), cols = w.size(-1), count = w.dim() == 3 ? w.size(0) : 1;
+  std::vector<int64_t> c, s;
+  if (w.dim() == 3) c.push_back(count), s.push_back(count);
+  c.insert(c.end(), {(rows + 15) / 16, (cols + 127) / 128, 2, 4, 16, 16});
+  s.push_back(rows);
+  const Tensor codes = at::empty(c, w.options().dtype(at::kChar)), scales = at::empty(s, w.options().dtype(at::kFloat));
+  check(lib.gmlp_q8_quantize(ptr(w), out_ptr(codes), (float*)out_ptr(scales), count, rows, cols, code, stream_of(w)));
+  return {codes, scales};
+}
+Tensor q8_dequantize(const Q8& q, at::ScalarType dtype) {
+  const Tensor& s = std::get<1>(q);
+  inference_only("dequantize_q8", {s});
+  require_gpu({s});
+  TORCH_CHECK_TYPE(dtype == at::kHalf || dtype == at::kBFloat16, "dequantize_q8 gives float16 or bfloat16");
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(s.device());
+  const int64_t experts = s.dim() == 2 ? s.size(0) : 0;
+  const Q8Matrix w("weight", q, s, experts, std::get<2>(q), std::get<3>(q));
+  std::vector<int64_t> sizes;
+  if (experts > 0) sizes.push_back(experts);
+  sizes.insert(sizes.end(), {w.rows, w.cols});
+  const Tensor out = at::empty(sizes, s.options().dtype(dtype));
+  check(lib.gmlp_q8_dequantize(ptr(w.codes), w.s(), out_ptr(out), w.count, w.rows, w.cols, dtype == at::kHalf ? GMLP_F16 : GMLP_BF16,
+                               stream_of(out)));
+  return out;
+}
+
+// Token rows of a piece of a long batch: what its scratch grows with.  (Rows are independent, and sums of integers exact.)
+constexpr int64_t Q8_PIECE = 65536;
+
+Tensor q8_linear(const Tensor& x_in, const Q8& q, const OptTensor& bias_in) {
+  const Tensor& b_in = or_undefined(bias_in);
+  inference_only("q8_linear_fwd", {x_in, std::get<1>(q), b_in});
+  const int code = require_half("q8_linear_fwd", {x_in, b_in});
+  TORCH_CHECK_VALUE(x_in.dim() >= 1, "x needs at least one dimension");
+  const int64_t R = x_in.size(-1), C = std::get<2>(q), M = R > 0 ? x_in.numel() / R : 0;
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x_in.device());
+  const Q8Matrix w("weight", q, x_in, 0, C, R);
+  check_bias("bias", b_in, C);
+  const Tensor x = Q8Matrix::aligned(x_in.contiguous()), b = b_in.defined() ? Q8Matrix::aligned(b_in.contiguous()) : b_in;
+  std::vector<int64_t> sizes = x.sizes().vec();
+  sizes.back() = C;
+  const Tensor y = at::empty(sizes, x.options());
+  if (M == 0) return y;
+  size_t bytes = lib.gmlp_q8_linear_workspace_bytes(std::min(M, Q8_PIECE), R, C, code);
+  if (M > Q8_PIECE && M % Q8_PIECE) bytes = std::max(bytes, lib.gmlp_q8_linear_workspace_bytes(M % Q8_PIECE, R, C, code));
+  const Tensor ws = scratch(bytes, x);
+  for (int64_t m = 0; m < M; m += Q8_PIECE)
+    check(lib.gmlp_q8_linear_fwd((const char*)ptr(x) + m * R * 2, ptr(w.codes), w.s(), ptr(b), (char*)out_ptr(y) + m * C * 2,
+                                 std::min(M - m, Q8_PIECE), R, C, code, out_ptr(ws), bytes, stream_of(x)));
+  return y;
+}
+
+Tensor q8_mlp(const Tensor& x_in, const Q8& gate, const OptTensor& bg_in, const Q8& up, const OptTensor& bu_in, const Q8& down,
+              const OptTensor& bd_in, int64_t act) {
+  const Tensor &bg_o = or_undefined(bg_in), &bu_o = or_undefined(bu_in), &bd_o = or_undefined(bd_in);
+  inference_only("q8_mlp_fwd", {x_in, std::get<1>(gate), std::get<1>(up), std::get<1>(down), bg_o, bu_o, bd_o});
+  const int code = require_half("q8_mlp_fwd", {x_in, bg_o, bu_o, bd_o});
+  TORCH_CHECK_VALUE(x_in.dim() >= 1, "x needs at least one dimension");
+  const int64_t K = x_in.size(-1), N = std::get<2>(gate), M = K > 0 ? x_in.numel() / K : 0;
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x_in.device());
+  const Q8Matrix wg("W_gate", gate, x_in, 0, N, K), wu("W_up", up, x_in, 0, N, K), wd("W_down", down, x_in, 0, K, N);
+  check_bias("b_gate", bg_o, N);
+  check_bias("b_up", bu_o, N);
+  check_bias("b_down", bd_o, K);
+  auto bias = [](const Tensor& b) { return b.defined() ? Q8Matrix::aligned(b.contiguous()) : b; };
+  const Tensor x = Q8Matrix::aligned(x_in.contiguous()), bg = bias(bg_o), bu = bias(bu_o), bd = bias(bd_o);
+  const Tensor y = at::empty(x.sizes(), x.options());
+  if (M == 0) return y;
+  size_t bytes = lib.gmlp_q8_mlp_workspace_bytes(std::min(M, Q8_PIECE), K, N, code);
+  if (M > Q8_PIECE && M % Q8_PIECE) bytes = std::max(bytes, lib.gmlp_q8_mlp_workspace_bytes(M % Q8_PIECE, K, N, code));
+  const Tensor ws = scratch(bytes, x);
+  for (int64_t m = 0; m < M; m += Q8_PIECE)
+    check(lib.gmlp_q8_mlp_fwd((const char*)ptr(x) + m * K * 2, ptr(wg.codes), wg.s(), ptr(wu.codes), wu.s(), ptr(wd.codes), wd.s(), ptr(bg),
+                              ptr(bu), ptr(bd), (char*)out_ptr(y) + m * K * 2, std::min(M - m, Q8_PIECE), K, N, code, (int)act,
+                              out_ptr(ws), bytes, stream_of(x)));
+  return y;
+}
+
+Tensor moe_mlp_q8(const Tensor& x_in, const Tensor& logits_in, const Q8& gate, const Q8& up, const Q8& down, int64_t top_k, bool normalize,
+                  int64_t act) {
+  inference_only("moe_mlp_fwd", {x_in, logits_in, std::get<1>(gate), std::get<1>(up), std::get<1>(down)});
+  const int code = require_half("moe_mlp_fwd", {x_in}), logits_code = check_logits(x_in, logits_in, top_k);
+  const int64_t K = x_in.size(-1), E = logits_in.size(-1), N = std::get<2>(gate), M = K > 0 ? x_in.numel() / K : 0;
+  at::AutoDispatchBelowADInplaceOrView below;
+  const c10::DeviceGuard guard(x_in.device());
+  const Q8Matrix g("W_gate", gate, x_in, E, N, K), u("W_up", up, x_in, E, N, K), d("W_down", down, x_in, E, K, N);
+  const Tensor x = Q8Matrix::aligned(x_in.contiguous()), logits = logits_in.contiguous();
+  const Tensor y = at::empty(x.sizes(), x.options());
+  if (M == 0) return y;
+  const int64_t piece = std::max<int64_t>(1, GMLP_Q8_MOE_MAX_PAIRS / top_k);
+  size_t bytes = lib.gmlp_q8_moe_workspace_bytes(std::min(M, piece), K, N, E, top_k, code);
+  if (M > piece && M % piece) bytes = std::max(bytes, lib.gmlp_q8_moe_workspace_bytes(M % piece, K, N, E, top_k, code));
+  const Tensor ws = scratch(bytes > 0 ? bytes : 16, x);  // (0: what the call below refuses)
+  for (int64_t m = 0; m < M; m += piece)
+    check(lib.gmlp_q8_moe_fwd((const char*)ptr(x) + m * K * 2, (const char*)ptr(logits) + m * E * logits.element_size(), ptr(g.codes),
+                              ptr(u.codes), ptr(d.codes), g.s(), u.s(), d.s(), (char*)out_ptr(y) + m * K * 2, std::min(M - m, piece), K, N,
+                              E, top_k, normalize, code, logits_code, (int)act, out_ptr(ws), bytes, stream_of(x)));
+  return y;
+}
+
+// ------------------------------------------------------------------ routing that is trained
+// d weights, d loss -> d logits
+struct RouteBackward : public ag::Node {
+  int64_t M = 0, E = 0, top_k = 0;
+  bool normalize = true;
+  int code = 0;
+  std::vector<int64_t> sizes, weights_sizes;
+  at::TensorOptions options;  // of the logits
+  ag::SavedVariable logits_, weights_, experts_, slope_, mask_;
+
+  std::string name() const override { return "RouteBalancedBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (ag::SavedVariable* v : {&logits_, &weights_, &experts_, &slope_, &mask_}) v->reset_data();
+  }
+  static Tensor readable_as(const Tensor& t, int64_t numel, at::ScalarType type, const at::Device& device) {
+    TORCH_CHECK(t.defined() && t.device() == device && t.scalar_type() == type && t.numel() == numel, "a tensor came back as ",
+                t.defined() ? c10::str(t.sizes(), " ", t.scalar_type(), " on ", t.device()) : "undefined", ", expected ", numel,
+                " elements of ", type, " on ", device);
+    return t.contiguous();
+  }
+  ag::variable_list apply(ag::variable_list&& grads) override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    ag::variable_list out(1);
+    const Tensor logits_saved = logits_.unpack(), weights_saved = weights_.unpack(shared_from_this()), experts_saved = experts_.unpack();
+    const Tensor slope_saved = slope_.unpack(), mask_saved = mask_.unpack();
+    if (!task_should_compute_output(0)) return out;
+    at::AutoDispatchBelowADInplaceOrView below;
+    const at::Device device = options.device();
+    const c10::DeviceGuard guard(device);
+    if (M == 0 || (!grads[0].defined() && !grads[1].defined())) {
+      out[0] = at::zeros(sizes, options);
+    } else {
+      const Tensor logits = readable_as(logits_saved, M * E, options.dtype().toScalarType(), device);
+      const Tensor weights = readable_as(weights_saved, M * top_k, at::kFloat, device);
+      const Tensor experts = readable_as(experts_saved, M * top_k, at::kLong, device);
+      const Tensor slope = readable_as(slope_saved, E, at::kFloat, device);
+      const Tensor mask = mask_saved.defined() ? readable_as(mask_saved, M, at::kBool, device) : Tensor();
+      const Tensor d_weights = grads[0].defined() ? readable_as(grads[0], M * top_k, at::kFloat, device) : Tensor();
+      const Tensor d_loss = grads[1].defined() ? readable_as(grads[1], 1, at::kFloat, device) : Tensor();
+      out[0] = at::empty(sizes, options);
+      check(lib.gmlp_moe_balance_bwd(ptr(logits), (const uint8_t*)ptr(mask), (const float*)ptr(weights), (const int64_t*)ptr(experts),
+                                     (const float*)ptr(slope), (const float*)ptr(d_weights), (const float*)ptr(d_loss), out_ptr(out[0]), M,
+                                     E, top_k, normalize, code, stream_of(out[0])));
+    }
+    for (const Tensor& grad : grads)
+      if (grad.defined() && grad.requires_grad()) {
+        refuse_second_derivative(*this, grad, out);
+        return out;
+      }
+    refuse_second_derivative(*this, Tensor(), out);
+    return out;
+  }
+};
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> moe_route_balanced(const Tensor& logits_in, int64_t top_k, bool normalize,
+                                                              const OptTensor& mask_in) {
+  const Tensor& mask_o = or_undefined(mask_in);
+  refuse_transforms("moe_route_balanced", {logits_in});
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), "moe_route_balanced cannot be traced");
+  const int code = require_gpu({logits_in});
+  TORCH_CHECK_VALUE(logits_in.dim() >= 1, "logits need at least one dimension");
+  const int64_t E = logits_in.size(-1), M = E > 0 ? logits_in.numel() / E : 0;
+  TORCH_CHECK_VALUE(top_k >= 1 && top_k <= E, "top_k = ", top_k, " of ", E, " experts");
+  if (mask_o.defined()) {
+    TORCH_CHECK_TYPE(mask_o.scalar_type() == at::kBool, "token_mask is ", mask_o.scalar_type(), ", expected bool");
+    TORCH_CHECK(mask_o.device() == logits_in.device(), "tensors on different devices: ", logits_in.device(), " and ", mask_o.device());
+    TORCH_CHECK_VALUE(mask_o.dim() == logits_in.dim() - 1 && std::equal(mask_o.sizes().begin(), mask_o.sizes().end(), logits_in.sizes().begin()),
+                      "token_mask ", mask_o.sizes(), " and logits ", logits_in.sizes(), " are of different token rows");
+  }
+  const bool graph = ag::compute_requires_grad(logits_in);
+  Tensor weights, experts, counts, loss, slope, mask;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard guard(logits_in.device());
+    const Tensor logits = logits_in.contiguous();
+    mask = contiguous(mask_o);
+    std::vector<int64_t> sizes = logits.sizes().vec();
+    sizes.back() = top_k;
+    const at::TensorOptions f32 = logits.options().dtype(at::kFloat), i64 = logits.options().dtype(at::kLong);
+    weights = at::empty(sizes, f32);
+    experts = at::empty(sizes, i64);
+    if (M > 0) {
+      counts = at::empty({E}, i64);
+      loss = at::empty({}, f32);
+      const size_t bytes = lib.gmlp_moe_balance_workspace_bytes(M, E), room = ((size_t)E * 4 + 15) / 16 * 16;
+      // (the slopes and the workspace in one allocation where the slopes are dropped with it)
+      slope = graph ? at::empty({E}, f32) : Tensor();
+      const Tensor ws = scratch((bytes + 15) / 16 * 16 + (graph ? 0 : room), logits);
+      float* const to = graph ? (float*)out_ptr(slope) : (float*)((char*)out_ptr(ws) + (bytes + 15) / 16 * 16);
+      check(lib.gmlp_moe_balance_fwd(ptr(logits), (const uint8_t*)ptr(mask), (float*)out_ptr(weights), (int64_t*)out_ptr(experts),
+                                     (int64_t*)out_ptr(counts), (float*)out_ptr(loss), to, M, E, top_k, normalize, code, out_ptr(ws), bytes,
+                                     stream_of(logits)));
+    } else {
+      counts = at::zeros({E}, i64);
+      loss = at::zeros({}, f32);
+      slope = graph ? at::zeros({E}, f32) : Tensor();
+    }
+  }
+  if (graph) {
+    auto node = std::shared_ptr<RouteBackward>(new RouteBackward(), ag::deleteNode);
+    node->set_next_edges(ag::collect_next_edges(logits_in));
+    node->M = M; node->E = E; node->top_k = top_k; node->normalize = normalize; node->code = code;
+    node->sizes = logits_in.sizes().vec();
+    node->options = logits_in.options();
+    node->logits_ = ag::SavedVariable(logits_in, false);
+    node->experts_ = ag::SavedVariable(experts, false);
+    node->slope_ = ag::SavedVariable(slope, false);
+    node->mask_ = ag::SavedVariable(mask, false);
+    ag::set_history(weights, node);
+    ag::set_history(loss, node);
+    node->weights_ = ag::SavedVariable(weights, true);
+  }
+  return {weights, experts, counts, loss};
+}
+
 // ------------------------------------------------------------------ torch.jit.trace
 // While a trace is being recorded a call goes through torch's dispatcher, as an operator with a schema: the
 // tracer then records the call itself.  Called directly it would record the only torch operation that it
@@ -792,4 +1048,10 @@ PYBIND11_MODULE(_gmlp_torch, m) {
   m.def("moe_route", torch::wrap_pybind_function_no_gil(moe_route));
   m.def("moe_mlp", torch::wrap_pybind_function_no_gil(moe_mlp));
   m.def("moe_mlp_q4", torch::wrap_pybind_function_no_gil(moe_mlp_q4));
+  m.def("moe_mlp_q8", torch::wrap_pybind_function_no_gil(moe_mlp_q8));
+  m.def("moe_route_balanced", torch::wrap_pybind_function_no_gil(moe_route_balanced));
+  m.def("q8_quantize", torch::wrap_pybind_function_no_gil(q8_quantize));
+  m.def("q8_dequantize", torch::wrap_pybind_function_no_gil(q8_dequantize));
+  m.def("q8_linear", torch::wrap_pybind_function_no_gil(q8_linear));
+  m.def("q8_mlp", torch::wrap_pybind_function_no_gil(q8_mlp));
 }

@@ -12,5 +12,5 @@ from .gated_mlp import (  # noqa: F401
     mlp_hidden_states_bwd,
     mlp_hidden_states_fwd,
 )
-from .experts import GatedMoE, Q4GatedMLP  # noqa: F401
+from .experts import GatedMoE, Q4GatedMLP, Q8GatedMLP  # noqa: F401
 from .utils import copy_weights, get_device  # noqa: F401

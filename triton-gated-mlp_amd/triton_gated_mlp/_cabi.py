@@ -100,6 +100,17 @@ _SIGNATURES = {
         _int,
         [_c_ptr] * 9 + [_i64] * 5 + [_int] * 5 + [_c_ptr, ctypes.c_size_t, _c_ptr],
     ),
+    "gmlp_moe_balance_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "gmlp_moe_balance_fwd": (_int, [_c_ptr] * 7 + [_i64] * 3 + [_int, _int, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "gmlp_moe_balance_bwd": (_int, [_c_ptr] * 8 + [_i64] * 3 + [_int, _int, _c_ptr]),
+    "gmlp_q8_quantize": (_int, [_c_ptr] * 3 + [_i64] * 3 + [_int, _c_ptr]),
+    "gmlp_q8_dequantize": (_int, [_c_ptr] * 3 + [_i64] * 3 + [_int, _c_ptr]),
+    "gmlp_q8_linear_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
+    "gmlp_q8_linear_fwd": (_int, [_c_ptr] * 5 + [_i64] * 3 + [_int, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "gmlp_q8_mlp_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _int]),
+    "gmlp_q8_mlp_fwd": (_int, [_c_ptr] * 11 + [_i64] * 3 + [_int, _int, _c_ptr, ctypes.c_size_t, _c_ptr]),
+    "gmlp_q8_moe_workspace_bytes": (ctypes.c_size_t, [_i64] * 5 + [_int]),
+    "gmlp_q8_moe_fwd": (_int, [_c_ptr] * 9 + [_i64] * 5 + [_int] * 4 + [_c_ptr, ctypes.c_size_t, _c_ptr]),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -1,4 +1,4 @@
-"""Decoding through a stack of serving layers, in one HIP graph: tokens go through alternating 4-bit gated MLPs and layers of
+"""Decoding through a stack of serving layers, in one HIP graph: tokens go through alternating 4-bit (8-bit, 16-bit) gated MLPs and layers of
 experts, each behind a normalisation and added to the residual, as a language model's feed-forward halves do.
 
     PYTHONPATH=triton-gated-mlp_amd python -m triton_gated_mlp.decode_example [--tokens 1] [--layers 8] [--bits 4]
@@ -12,7 +12,7 @@ import time
 import torch
 from torch import Tensor, nn
 
-from .experts import GatedMoE, Q4GatedMLP
+from .experts import GatedMoE, Q4GatedMLP, Q8GatedMLP
 from .gated_mlp import FusedGatedMLP
 
 
@@ -25,10 +25,11 @@ class DecodeStack(nn.Module):
             with torch.device(device):
                 if i % 2 == 0:
                     layer = FusedGatedMLP(hidden_size, intermediate_size, bias=False).to(dtype).eval()
-                    layer = Q4GatedMLP.from_float(layer, group_size) if bits == 4 else layer
+                    if bits < 16:
+                        layer = Q4GatedMLP.from_float(layer, group_size) if bits == 4 else Q8GatedMLP.from_float(layer)
                 else:
                     layer = GatedMoE(hidden_size, expert_size, num_experts, top_k).to(dtype)
-                    layer = layer.quantize_(group_size) if bits == 4 else layer
+                    layer = layer.quantize_(group_size, bits) if bits < 16 else layer
             self.blocks.append(layer)
 
     def forward(self, x: Tensor) -> Tensor:
@@ -46,7 +47,7 @@ def main(argv=None) -> float:
     ap.add_argument("--expert", type=int, default=1024, help="intermediate size of an expert")
     ap.add_argument("--experts", type=int, default=64)
     ap.add_argument("--top-k", type=int, default=8)
-    ap.add_argument("--bits", type=int, default=4, choices=(4, 16))
+    ap.add_argument("--bits", type=int, default=4, choices=(4, 8, 16))
     ap.add_argument("--group", type=int, default=128, choices=(32, 64, 128))
     ap.add_argument("--steps", type=int, default=200)
     a = ap.parse_args(argv)

@@ -1,17 +1,19 @@
-"""Mixture-of-experts layers of gated MLPs, for serving (host wrappers over libgmlp.so).
+"""Mixture-of-experts layers of gated MLPs (host wrappers over libgmlp.so): routing, for serving and for training, and whole layers, for
+serving.
 
-Inference only: no operator here has a backward pass.  The reference has no such operators; an expert is its EagerGatedMLP
+Inference only, but for moe_route_balanced: no other operator here has a backward pass.  The reference has no such operators; an expert is its EagerGatedMLP
 (src/triton_gated_mlp/gated_mlp.py:73-98) without biases.
 """
 
 from __future__ import annotations
 
-from typing import NamedTuple, Union
+from typing import NamedTuple, Optional, Union
 
+import torch
 from torch import Tensor
 
 from .. import _cabi
-from .quant import Q4Weight
+from .quant import Q4Weight, Q8Weight
 
 
 class Routing(NamedTuple):
@@ -32,25 +34,54 @@ def moe_route(logits: Tensor, top_k: int, normalize: bool = True) -> Routing:
     return Routing(*_cabi.torch_binding().moe_route(logits, int(top_k), bool(normalize)))
 
 
+class BalancedRouting(NamedTuple):
+    weights: Tensor  # float32 [..., top_k]
+    experts: Tensor  # int64 [..., top_k], in descending order of the logits
+    counts: Tensor  # int64 [experts]
+    loss: Tensor  # float32, a scalar
+
+
+def moe_route_balanced(logits: Tensor, top_k: int, normalize: bool = True, token_mask: Optional[Tensor] = None) -> BalancedRouting:
+    """moe_route for training: the same weights and experts, the number of choices that fell on each expert, and the balance loss
+    E · sum_e f_e·P_e, f_e being the expert's share of all choices and P_e the mean of its softmax probability over the tokens.  It is 1
+    where every expert gets as much.
+
+    `weights` and `loss` have gradients for the logits (any of the two may be left unused); f counts as a constant.  `token_mask`
+    (bool [...], the logits' leading dimensions) is False for tokens, padding for instance, that are in neither counts nor
+    loss; they are routed like the others.  Tokens to which no expert is available (logits -inf) are in neither either, nor
+    choices of an expert that is not.  Without a token that counts the loss is 0."""
+    if logits.requires_grad and torch.is_grad_enabled() and logits.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(
+            "moe_route_balanced: capturing a step that records an autograd graph into a HIP graph is not supported (as with "
+            "FusedGatedMLP); capture it under torch.no_grad() only"
+        )
+    return BalancedRouting(*_cabi.torch_binding().moe_route_balanced(logits, int(top_k), bool(normalize), token_mask))
+
+
 def moe_mlp_fwd(
     x: Tensor,
     logits: Tensor,
-    W_gate: Union[Tensor, Q4Weight],
-    W_up: Union[Tensor, Q4Weight],
-    W_down: Union[Tensor, Q4Weight],
+    W_gate: Union[Tensor, Q4Weight, Q8Weight],
+    W_up: Union[Tensor, Q4Weight, Q8Weight],
+    W_down: Union[Tensor, Q4Weight, Q8Weight],
     top_k: int,
     normalize: bool = True,
     act_fn: str = "silu",
 ) -> Tensor:
     """y[t] = sum over t's experts e of weight·down_e(act_fn(gate_e(x[t])) * up_e(x[t])), routed as moe_route does.
 
-    x [..., K]; logits [..., E]; W_gate, W_up [E, N, K] and W_down [E, K, N] in x's dtype, or all three as Q4Weight.  Made for a
-    few tokens: the weights of every expert that any of 64 token rows chose are read once, and of no other; a longer
-    batch runs 64 rows at a time.  Nothing is copied to the host.  Beyond 4 token rows (2 with Q4Weight) the hidden
+    x [..., K]; logits [..., E]; W_gate, W_up [E, N, K] and W_down [E, K, N] in x's dtype, or all three as Q4Weight or Q8Weight.
+    Nothing is copied to the host.
+
+    Q8Weight: for any number of tokens.  The hidden states are rounded to x's dtype and become 8-bit integers as q8_mlp_fwd's
+    do, the sum over experts is rounded once.  An expert is not run for a token whose weight for it is 0.
+
+    Others: made for a few tokens: the weights of every expert that any of 64 token rows chose are read once, and of no other; a longer
+    batch runs 64 rows at a time.  Beyond 4 token rows (2 with Q4Weight) the hidden
     states are rounded to x's dtype, as FusedGatedMLP does; the sum over experts is rounded once."""
     binding = _cabi.torch_binding()
-    quantized = [isinstance(w, Q4Weight) for w in (W_gate, W_up, W_down)]
-    if any(quantized) and not all(quantized):
-        raise TypeError("W_gate, W_up and W_down are either all tensors or all Q4Weight")
-    call = binding.moe_mlp_q4 if quantized[0] else binding.moe_mlp
+    kinds = {Q4Weight if isinstance(w, Q4Weight) else Q8Weight if isinstance(w, Q8Weight) else Tensor for w in (W_gate, W_up, W_down)}
+    if len(kinds) > 1:
+        raise TypeError("W_gate, W_up and W_down are either all tensors or all Q4Weight or all Q8Weight")
+    call = binding.moe_mlp if Tensor in kinds else binding.moe_mlp_q4 if Q4Weight in kinds else binding.moe_mlp_q8
     return call(x, logits, W_gate, W_up, W_down, int(top_k), bool(normalize), _cabi.act_code(act_fn))

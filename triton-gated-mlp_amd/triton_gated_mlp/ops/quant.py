@@ -1,8 +1,9 @@
-"""4-bit weights with group scales, for serving: storage, and the linear layer and gated MLP on it (host wrappers over
-libgmlp.so).
+"""4-bit weights with group scales and 8-bit integers with a scale for each row, for serving: storage, and the linear layer and
+gated MLP on it (host wrappers over libgmlp.so).
 
-A weight is scale·n with -8 <= n <= 7 and one scale per row and group of 32, 64 or 128 columns.  The products are of scale·n
-itself, accumulated in fp32.  Inference only: no operator here has a backward pass.  The reference has no such operators; the
+A 4-bit weight is scale·n with -8 <= n <= 7 and one scale per row and group of 32, 64 or 128 columns.  The products are of scale·n
+itself, accumulated in fp32.  In 8 bits the token rows are integers too, each with a scale of its own that is found in the call,
+and the products run on the matrix cores' integer instructions.  Inference only: no operator here has a backward pass.  The reference has no such operators; the
 math is that of its nn.Linear and EagerGatedMLP (src/triton_gated_mlp/gated_mlp.py:73-98).
 """
 
@@ -10,6 +11,7 @@ from __future__ import annotations
 
 from typing import NamedTuple, Optional
 
+import torch
 from torch import Tensor
 
 from .. import _cabi
@@ -62,3 +64,50 @@ def q4_mlp_fwd(
     2 token rows the hidden states are rounded to x's dtype between the two, as FusedGatedMLP does (in float16 one past
     65504 is infinite)."""
     return _cabi.torch_binding().q4_mlp(x, W_gate, b_gate, W_up, b_up, W_down, b_down, _cabi.act_code(act_fn))
+
+
+class Q8Weight(NamedTuple):
+    """An 8-bit weight matrix [rows, cols], or one per expert with a leading dimension of codes and scales.
+
+    Rows are padded to tiles of 16, columns to blocks of 128, with zeros.  codes: int8 [tiles, blocks, 2 s, 4 q, 16 r, 16], the
+    columns 64 s + 16 q + 0..15 of the block in row r of the tile.  scales: float32 [rows].  The weight is
+    scale·n, -127 <= n <= 127.  (include/gmlp.h defines the same storage.)
+    """
+
+    codes: Tensor
+    scales: Tensor
+    rows: int
+    cols: int
+
+
+def quantize_q8(W: Tensor) -> Q8Weight:
+    """W [rows, cols] or [experts, rows, cols], float16 or bfloat16, in 8 bits: n = 127 w / (largest magnitude of the row), to the
+    nearest, halves to the even one.  A row with a number that is not finite has scale NaN."""
+    codes, scales = _cabi.torch_binding().q8_quantize(W)
+    return Q8Weight(codes, scales, W.shape[-2], W.shape[-1])
+
+
+def dequantize_q8(weight: Q8Weight, dtype: torch.dtype) -> Tensor:
+    """scale·n rounded to `dtype` (float16 or bfloat16), [rows, cols] or [experts, rows, cols]."""
+    return _cabi.torch_binding().q8_dequantize(weight, dtype)
+
+
+def q8_linear_fwd(x: Tensor, weight: Q8Weight, bias: Optional[Tensor] = None) -> Tensor:
+    """x [..., cols]·Wᵀ + bias, any number of token rows.  Each row of x becomes 8-bit integers as quantize_q8 makes them of a weight's; the
+    products' sums are exact integers, multiplied by both scales in fp32.  A row with a number that is not finite gives NaN."""
+    return _cabi.torch_binding().q8_linear(x, weight, bias)
+
+
+def q8_mlp_fwd(
+    x: Tensor,
+    W_gate: Q8Weight,
+    b_gate: Optional[Tensor],
+    W_up: Q8Weight,
+    b_up: Optional[Tensor],
+    W_down: Q8Weight,
+    b_down: Optional[Tensor],
+    act_fn: str = "silu",
+) -> Tensor:
+    """A whole gated MLP in 8 bits, any number of token rows: the hidden states are rounded to x's dtype, as FusedGatedMLP does, and become
+    8-bit integers row by row (in float16 one past 65504 is infinite, and its token's outputs are NaN)."""
+    return _cabi.torch_binding().q8_mlp(x, W_gate, b_gate, W_up, b_up, W_down, b_down, _cabi.act_code(act_fn))
