@@ -25,74 +25,115 @@ __device__ __forceinline__ uint32_t max_bits(uint32_t most, uint32_t two) {
   const u16x2 a = __builtin_bit_cast(u16x2, most), b = __builtin_bit_cast(u16x2, two & 0x7fff7fffu);
   return __builtin_bit_cast(uint32_t, (u16x2)__builtin_elementwise_max(a, b));
 }
-// n = 127 v / top rounded half to even.  127 v and top have few bits, so that the quotient rounded to fp32 is a half only where the
-// exact one is: 1 / (2 top) at least lies between them otherwise, 2^-12 in units of n, and fp32 rounds by 2^-18.
+// n = 127 v / top rounded half to even: a product of 127 v with fl(1 / top), one step of correction, and the addition of 1.5 2^23, whose
+// result has n in its low bits.  127 v and top have few bits: a quotient that is no half is 1 / (2 top) from one at least, 2^-12 in
+// units of n, far more than the two roundings; one that is a half is a number of fp32, and the corrected quotient is it (what
+// the first product is off by is exact in the fused multiply-add).  8 instructions a number in the place of the division's 15.
 template <typename T>
 struct RowScale {
-  float top, pre, scale;
+  float top, pre, by, scale;
   bool finite;
   __device__ __forceinline__ explicit RowScale(uint32_t bits) {
     const float raw = Traits<T>::to_f32(__builtin_bit_cast(T, (unsigned short)bits));
     finite = raw < __builtin_inff();
-    // 127 v stays finite, and its quotient out of the subnormals (powers of two: exact)
+    // powers of two, exact, that keep 127 v finite and its quotient out of the subnormals
     pre = raw > 0x1p64f ? 0x1p-64f : raw < 0x1p-64f ? 0x1p64f : 1.f;
-    top = raw > 0.f ? raw * pre : 1.f;
+    top = finite && raw > 0.f ? raw * pre : 1.f;
+    by = 1.f / top;
     scale = finite ? raw / 127.f : __builtin_nanf("");
+    if (!finite) pre = 0.f;
   }
-  __device__ __forceinline__ int of(T v) const {
-    return finite ? (int)rintf(127.f * (Traits<T>::to_f32(v) * pre) / top) : 0;
+  // the low byte is n
+  __device__ __forceinline__ uint32_t of(float v) const {
+    const float u = 127.f * (v * pre), first = u * by;
+    const float n = __builtin_fmaf(__builtin_fmaf(-first, top, u), by, first);
+    return __float_as_uint(n + 12582912.f);
+  }
+  // four of them
+  __device__ __forceinline__ uint32_t four(const T* v) const {
+    const uint32_t a = __builtin_amdgcn_perm(of(Traits<T>::to_f32(v[1])), of(Traits<T>::to_f32(v[0])), 0x0c0c0400u);
+    const uint32_t b = __builtin_amdgcn_perm(of(Traits<T>::to_f32(v[3])), of(Traits<T>::to_f32(v[2])), 0x04000c0cu);
+    return finite ? a | b : 0u;
   }
 };
+template <typename T>
+__device__ __forceinline__ i32x4 q8_sixteen(const RowScale<T>& scale, const u32x4 (&v)[2]) {
+  i32x4 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const u32x2 four = {v[i / 2][i % 2 * 2], v[i / 2][i % 2 * 2 + 1]};
+    typedef typename Traits<T>::vec4 vec4;
+    const vec4 x = __builtin_bit_cast(vec4, four);
+    const T y[4] = {x[0], x[1], x[2], x[3]};
+    out[i] = (int)scale.four(y);
+  }
+  return out;
+}
 
-// A workgroup: ROWS rows of a tile; a thread takes 16 integers of a row at a time (32 bytes in, 16 out), neighbours first
-// the rows, then the 16 integers behind.
-template <typename T, int ROWS>
-__global__ void __launch_bounds__(256) q8_rows_kernel(const T* x, int8_t* codes, float* scales, int64_t rows, int cols, int padded,
-                                                      int tiles, const int* token_of, const int* rows_at) {
-  typedef typename Traits<T>::vec8 vec8;
-  constexpr int LANES = 256 / ROWS;  // threads of a row
-  __shared__ uint32_t part[256];
+// A workgroup of NT threads: ROWS rows of a tile.  A thread takes 16 numbers of a row at a time (32 bytes in, 16 out), PER times, and
+// keeps them while the row's largest is found; PER = 0: rows of any length, read twice.  Neighbouring threads take the ROWS
+// rows first, which lie together in the result.
+template <typename T, int NT, int ROWS, int PER>
+__global__ void __launch_bounds__(NT) q8_rows_kernel(const T* x, int8_t* codes, float* scales, int64_t rows, int cols, int padded,
+                                                     int tiles, const int* token_of, const int* rows_at) {
+  constexpr int LANES = NT / ROWS, NW = NT / 64, PARTS = 16 / ROWS;  // threads of a row
+  __shared__ uint32_t part[NW][ROWS];
   const int r = threadIdx.x % ROWS, l = threadIdx.x / ROWS;
-  const int64_t at = (int64_t)blockIdx.x * ROWS + r, matrix = blockIdx.y;
+  // The workgroups of a tile are 8 apart: on the same die, whose cache joins what they write to a line.
+  const int64_t b = blockIdx.x, whole = (int64_t)tiles / 8 * 8 * PARTS;
+  const int64_t tile = b < whole ? b / (8 * PARTS) * 8 + b % 8 : b / PARTS, sub = b < whole ? b / 8 % PARTS : b % PARTS;
+  const int64_t at = tile * 16 + sub * ROWS + r, matrix = blockIdx.y;
   int64_t from = at;
   bool there = at < rows;
-  if (rows_at != nullptr && (int64_t)blockIdx.x * ROWS >= rows_at[0]) return;
+  if (rows_at != nullptr && tile * 16 >= rows_at[0]) return;
   if (token_of != nullptr) {
     from = token_of[at];
     there = from >= 0;
   }
   const T* const src = x + (matrix * rows + from) * cols;
+  auto read = [&](u32x4 (&v)[2], int c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) v[h] = there && c + 8 * h < cols ? *(const u32x4*)(src + c + 8 * h) : u32x4{0, 0, 0, 0};
+  };
   uint32_t most = 0;
-  if (there)
-    for (int c = l * 16; c < cols; c += LANES * 16)
+  auto look = [&](const u32x4 (&v)[2]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (c + 8 * h < cols) {
-          const u32x4 v = *(const u32x4*)(src + c + 8 * h);
+    for (int i = 0; i < 8; ++i) most = max_bits(most, v[i / 4][i % 4]);
+  };
+  u32x4 kept[PER > 0 ? PER : 1][2];
+  if constexpr (PER > 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) most = max_bits(most, v[i]);
-        }
-  most = max(most & 0xffffu, most >> 16);
-  part[threadIdx.x] = most;
-  __syncthreads();
-  for (int d = LANES / 2; d > 0; d >>= 1) {
-    if (l < d) part[threadIdx.x] = max(part[threadIdx.x], part[threadIdx.x + d * ROWS]);
-    __syncthreads();
+    for (int i = 0; i < PER; ++i) read(kept[i], (l + i * LANES) * 16);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) look(kept[i]);
+  } else {
+    for (int c = l * 16; c < cols; c += LANES * 16) {
+      read(kept[0], c);
+      look(kept[0]);
+    }
   }
-  const RowScale<T> scale(part[r]);
+  most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+  for (int d = ROWS; d < 64; d <<= 1) most = max(most, (uint32_t)__shfl_xor((int)most, d));
+  if ((threadIdx.x & 63) < ROWS) part[threadIdx.x >> 6][r] = most;
+  __syncthreads();
+  most = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) most = max(most, part[w][r]);
+  const RowScale<T> scale(most);
   if (l == 0 && at < rows) scales[matrix * rows + at] = there ? scale.scale : 0.f;
-  int8_t* const dst = codes + ((matrix * tiles + at / 16) * (int64_t)padded) * 16 + (at % 16) * 16;
-  if (at >= (int64_t)tiles * 16) return;
-  for (int c = l * 16; c < padded; c += LANES * 16) {
-    i32x4 out = {0, 0, 0, 0};
+  int8_t* const dst = codes + ((matrix * tiles + tile) * (int64_t)padded) * 16 + (at % 16) * 16;
+  auto write = [&](const u32x4 (&v)[2], int c) __attribute__((always_inline)) {
+    if (c < padded) *(i32x4*)(dst + (int64_t)(c / 16) * 256) = q8_sixteen<T>(scale, v);
+  };
+  if constexpr (PER > 0) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (there && c + 8 * h < cols) {
-        const vec8 v = *(const vec8*)(src + c + 8 * h);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) out[2 * h + i / 4] |= (scale.of(v[i]) & 0xff) << (8 * (i % 4));
-      }
-    *(i32x4*)(dst + (int64_t)(c / 16) * 256) = out;
+    for (int i = 0; i < PER; ++i) write(kept[i], (l + i * LANES) * 16);
+  } else {
+    for (int c = l * 16; c < padded; c += LANES * 16) {
+      read(kept[0], c);
+      write(kept[0], c);
+    }
   }
 }
 
@@ -101,12 +142,18 @@ hipError_t launch_q8_rows(const T* x, int8_t* codes, float* scales, int64_t coun
                           const int* rows_at, hipStream_t s) {
   const int64_t tiles = (rows + 15) / 16;
   const int padded = (int)q8_padded(cols);
-#define CALL(R)                                                                                                         \
-  hipLaunchKernelGGL((q8_rows_kernel<T, R>), dim3((unsigned)(tiles * (16 / R)), (unsigned)count), dim3(256), 0, s, x, codes, scales, rows, \
-                     (int)cols, padded, (int)tiles, token_of, rows_at)
-  if (tiles * count >= 512) CALL(16);
-  else if (tiles * count >= 64) CALL(4);
-  else CALL(1);
+#define CALL(NT, R, PER)                                                                                                  \
+  hipLaunchKernelGGL((q8_rows_kernel<T, NT, R, PER>), dim3((unsigned)(tiles * (16 / R)), (unsigned)count), dim3(NT), 0, s, x, codes, scales, \
+                     rows, (int)cols, padded, (int)tiles, token_of, rows_at)
+  if (padded > 32768) CALL(1024, 4, 0);
+  else if (tiles * count >= 64) {
+    if (padded <= 4096) CALL(256, 4, 4);
+    else if (padded <= 16384) CALL(1024, 4, 4);
+    else CALL(1024, 4, 8);
+  } else {
+    if (padded <= 4096) CALL(256, 1, 1);
+    else CALL(1024, 1, 2);
+  }
 #undef CALL
   return hipGetLastError();
 }
