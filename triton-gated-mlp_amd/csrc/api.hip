@@ -1776,7 +1776,7 @@ struct Arena {
   }
 };
 
-int q8_token_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+int q8_token_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
 
 // How a dense product of more rows than the streaming kernels take runs.  A reduction tile of 128 integers costs what one of 64
 // 16-bit elements does (the same bytes and as many matrix instructions), so the estimates are theirs.
@@ -1835,9 +1835,11 @@ struct Q8MlpWorkspace {
   }
 };
 
-// An expert layer: rows of a tile, and with it which kernels: 16, 32 or 64 the streaming ones, 128 and 256 the GEMM.
+// An expert layer: rows of a tile (the GEMM's 128 or 256, the streaming kernels' 16 to 128).
 struct Q8MoePlan {
-  int cap, tile_class[2];
+  int cap;
+  bool gemm;
+  int tile_class[2];
   int64_t rows, tiles;
 };
 Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
@@ -1846,7 +1848,9 @@ Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
   if (each <= 12) p.cap = 16;
   else if (each <= 24) p.cap = 32;
   else if (each <= 48) p.cap = 64;
+  else if (each <= 96) p.cap = 128;
   else {
+    p.gemm = true;
     p.cap = each >= 512 ? 256 : 128;
     p.tile_class[0] = p.tile_class[1] = each >= 512 ? gmlp::TILE_LARGE : gmlp::TILE_WIDE;
   }
@@ -1942,6 +1946,7 @@ int gmlp_q8_linear_fwd(const void* x, const void* codes, const float* scales, co
     typedef decltype(tag) T;
     gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), M, C, R);
     p.w[0] = (const int8_t*)codes; p.sw[0] = scales; p.bias[0] = bias; p.out = y;
+    if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, (const T*)x, (int)R, 1, nullptr, s);
     if (hipError_t e = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, M, R, nullptr, nullptr, s))
       return e;
     return run_q8_dense<T>(p, 1, (float*)(base + ws.partial), s);
@@ -1978,17 +1983,20 @@ int gmlp_q8_mlp_fwd(const void* x, const void* codes_gate, const float* scales_g
     typedef decltype(tag) T;
     T* const h = (T*)(base + ws.h);
     float* const partial = (float*)(base + ws.partial);
-    if (hipError_t e = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, M, K, nullptr, nullptr, s))
-      return e;
+    // a product of rows [M][cols]; `at`, `scales`: where they become integers if that takes a launch of its own
+    auto product = [&](gmlp::Q8Product& p, const T* rows, int64_t cols, size_t at, size_t scales, int sets) -> hipError_t {
+      if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
+      if (hipError_t e = gmlp::launch_q8_rows<T>(rows, (int8_t*)(base + at), (float*)(base + scales), 1, M, cols, nullptr, nullptr, s)) return e;
+      return run_q8_dense<T>(p, sets, partial, s);
+    };
     gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), M, N, K);
     p.w[0] = (const int8_t*)codes_gate; p.sw[0] = scales_gate; p.bias[0] = b_gate;
     p.w[1] = (const int8_t*)codes_up; p.sw[1] = scales_up; p.bias[1] = b_up;
     p.out = h; p.act = act;
-    if (hipError_t e = run_q8_dense<T>(p, 2, partial, s)) return e;
-    if (hipError_t e = gmlp::launch_q8_rows<T>(h, (int8_t*)(base + ws.q), (float*)(base + ws.sq), 1, M, N, nullptr, nullptr, s)) return e;
+    if (hipError_t e = product(p, (const T*)x, K, ws.x, ws.sx, 2)) return e;
     p = q8_product((const int8_t*)(base + ws.q), (const float*)(base + ws.sq), M, K, N);
     p.w[0] = (const int8_t*)codes_down; p.sw[0] = scales_down; p.bias[0] = b_down; p.out = y;
-    return run_q8_dense<T>(p, 1, partial, s);
+    return product(p, h, N, ws.q, ws.sq, 1);
   }));
 }
 
@@ -2026,6 +2034,17 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
   const hipStream_t s = (hipStream_t)stream;
   float* const weights = (float*)(base + ws.weights);
   int64_t* const experts = (int64_t*)(base + ws.experts);
+  if (gmlp::q8_solo(M, E, top_k, gmlp::q8_padded(K), gmlp::q8_padded(N)))
+    return hip_result(__func__, by_half(dtype, [&](auto tag) {
+      typedef decltype(tag) T;
+      const gmlp::Q8Solo solo = {logits, logits_dtype, (int)E, (int)top_k, normalize, (int*)(base + ws.row_of), weights};
+      gmlp::Q8Product p = q8_product(nullptr, nullptr, 1, N, K);
+      p.w[0] = (const int8_t*)codes_gate; p.sw[0] = scales_gate;
+      p.w[1] = (const int8_t*)codes_up; p.sw[1] = scales_up;
+      p.out = base + ws.h; p.act = act;
+      if (hipError_t err = gmlp::launch_q8_few_rows<T>(p, (const T*)x, (int)K, 2, &solo, s)) return err;
+      return gmlp::launch_q8_solo_down<T>(solo, (const T*)(base + ws.h), (const int8_t*)codes_down, scales_down, (T*)y, (int)K, (int)N, s);
+    }));
   const gmlp::Q8Plan routed = {(int*)(base + ws.total), (gmlp::Q8Tile*)(base + ws.tiles), (int*)(base + ws.row_of), (int*)(base + ws.token_of)};
   hipError_t e = by_dtype(logits_dtype, [&](auto tag) {
     typedef decltype(tag) L;
@@ -2037,7 +2056,7 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
     typedef decltype(tag) T;
     auto product = [&](gmlp::Q8Product& p, int sets) {
       p.tiles = routed.tiles; p.total = routed.total; p.most_tiles = (int)plan.tiles;
-      if (plan.cap <= gmlp::Q8_FEW_ROWS) return gmlp::launch_q8_few<T>(p, sets, plan.cap / 16, s);
+      if (!plan.gemm) return gmlp::launch_q8_few<T>(p, sets, plan.cap / 16, s);
       p.tile_class = plan.tile_class[sets == 2 ? 0 : 1];
       p.group_m = 8;
       return gmlp::launch_q8_gemm<T>(p, sets, s);

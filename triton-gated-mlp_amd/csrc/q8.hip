@@ -3,6 +3,7 @@
 
 #include "launch.hpp"
 #include "lds_dma.hpp"
+#include "routing.hpp"
 
 namespace gmlp {
 
@@ -185,25 +186,113 @@ hipError_t launch_q8_dequantize(const int8_t* codes, const float* scales, T* w, 
 // A workgroup: R tiles of 16 weight rows (of each matrix) and the token rows of a tile, up to 16 * MT.  Its wavefronts split the
 // reduction and add up through LDS (integers: in any order).  Bound by the weights' way from memory: a load is one KiB as it
 // lies, D of each kind in flight for a wavefront; tokens come from the caches, and past the end a load moves nothing.
+// Q: the token rows, 4 at most, come as they are and every workgroup makes integers of them for itself, in LDS, while its first
+// weights are on their way: a launch less, and for one row no more time (one row of 4096 through two matrices of 14336 rows 20.3 us,
+// of integers 20.9; four rows of 2048 through 8192 7.9, 5.0 and 3 us of a launch).
+constexpr int Q8_OWN_ROWS = 4;
 struct Q8Few {
   Q8Product p;
-  int strips;  // workgroups side by side, R tiles of weight rows each
+  const void* rows;  // Q: [M][cols]
+  int cols;
+  int strips;        // workgroups side by side, R tiles of weight rows each
+  Q8Solo solo;       // Q and solo.logits: the only token of an expert layer
 };
-template <int SETS, int R, int MT>
+
+// `count` rows [cols] as integers in LDS, [count][padded], by NT threads, 16 numbers of a row at a time; a thread's first AHEAD
+// pieces are loaded by read_ahead, for the caller to have other loads behind them.
+template <typename T, int NT, int AHEAD>
+struct Q8RowsToLds {
+  u32x4 ahead[AHEAD][2];
+  __device__ __forceinline__ void read(u32x4 (&v)[2], const T* rows, int cols, int padded, int count, int i) {
+    const int pieces = padded / 16, row = i / pieces, c = (i - row * pieces) * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      v[h] = row < count && c + 8 * h < cols ? *(const u32x4*)(rows + (int64_t)row * cols + c + 8 * h) : u32x4{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void read_ahead(const T* rows, int cols, int padded, int count) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) read(ahead[i], rows, cols, padded, count, threadIdx.x + i * NT);
+  }
+  // most[count], zeros on entry and behind a barrier: the rows' largest magnitudes (max_bits); `to` is there behind the next barrier
+  __device__ __forceinline__ void finish(const T* rows, int cols, int padded, int count, uint32_t* most, char* to) {
+    const int pieces = padded / 16, all = pieces * count;
+    auto look = [&](const u32x4 (&v)[2], int i) __attribute__((always_inline)) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = max_bits(m, v[k / 4][k % 4]);
+      m = max(m & 0xffffu, m >> 16);
+      const int row = i < all ? i / pieces : 0;
+      if (i >= all) m = 0;
+      // (most wavefronts have one row)
+      const int one = __builtin_amdgcn_readfirstlane(row);
+      if (__all(row == one)) {
+        m = wave_max(m);
+        if ((threadIdx.x & 63) == 0) atomicMax(&most[one], m);
+      } else {
+        atomicMax(&most[row], m);
+      }
+    };
+    u32x4 v[2];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if ((int)((threadIdx.x & ~63u) + i * NT) < all) look(ahead[i], threadIdx.x + i * NT);
+    for (int i = threadIdx.x + AHEAD * NT; (int)((unsigned)i & ~63u) < all; i += NT) {
+      read(v, rows, cols, padded, count, i);
+      look(v, i);
+    }
+    __syncthreads();
+    auto write = [&](const u32x4 (&v)[2], int i) __attribute__((always_inline)) {
+      if (i < all) *(i32x4*)(to + (size_t)i * 16) = q8_sixteen<T>(RowScale<T>(most[i / pieces]), v);
+    };
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) write(ahead[i], threadIdx.x + i * NT);
+    for (int i = threadIdx.x + AHEAD * NT; i < all; i += NT) {
+      read(v, rows, cols, padded, count, i);
+      write(v, i);
+    }
+  }
+};
+
+// The choices of a call's only token, every wavefront for itself: lane j < top_k has the j-th, expert < 0 where it is not run.
+__device__ __forceinline__ void q8_choose_solo(const Q8Solo& solo, int lane, int& expert, float& weight) {
+  auto logit = [&](int i) -> float {
+    if (solo.logits_dtype == 0) return (float)((const f16*)solo.logits)[i];
+    if (solo.logits_dtype == 1) return (float)((const bf16*)solo.logits)[i];
+    return ((const float*)solo.logits)[i];
+  };
+  if (solo.E <= 64) choose<1>(logit, solo.E, solo.top_k, solo.normalize != 0, lane, expert, weight);
+  else choose<Q8_SOLO_MAX_E / 64>(logit, solo.E, solo.top_k, solo.normalize != 0, lane, expert, weight);
+  if (weight == 0.f && expert >= 0) expert = -1 - expert;
+}
+
+template <int SETS, int R, int MT, bool Q>
 struct Q8Stage {
-  i32x4 w[SETS][R], x[MT];
+  i32x4 w[SETS][R], x[Q ? 1 : MT];
 };
 constexpr int q8_units_at_a_time(int NW, int units, int sets) { return NW * units * sets <= 32 ? units : 32 / (NW * sets); }
 
-template <typename T, int SETS, int R, int MT, int NW, int D, bool F32>
+template <typename T, int SETS, int R, int MT, int NW, int D, bool F32, bool Q>
 __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
   const Q8Product& p = a.p;
   constexpr int UNITS = R * MT, EACH = q8_units_at_a_time(NW, UNITS, SETS);
   __shared__ i32x4 part[NW * EACH * SETS * 64];
+  extern __shared__ __align__(16) char own_rows[];  // Q: [count][K]
+  __shared__ uint32_t own_most[Q8_OWN_ROWS];
+  static_assert(!Q || MT == 1, "a few rows are one tile");
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int entry = (int)blockIdx.x / a.strips, first_tile = ((int)blockIdx.x - entry * a.strips) * R;
   int expert = 0, row = 0, count = p.M;
-  if (p.tiles != nullptr) {
+  if (Q && a.solo.logits != nullptr) {
+    int e;
+    float w;
+    q8_choose_solo(a.solo, lane, e, w);
+    if (blockIdx.x == 0 && wave == 0 && lane < a.solo.top_k) {
+      a.solo.experts[lane] = e;
+      a.solo.weights[lane] = w;
+    }
+    expert = __builtin_amdgcn_readlane(e, entry);
+    if (expert < 0) return;
+  } else if (p.tiles != nullptr) {
     if (entry >= p.total[0]) return;
     const Q8Tile t = p.tiles[entry];
     expert = __builtin_amdgcn_readfirstlane(t.expert);
@@ -220,34 +309,53 @@ __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
   const q8_rsrc rx = q8_make_rsrc(p.x + (int64_t)(row / 16) * pitch, (uint32_t)((count + 15) / 16) * pitch);
   const int s0 = steps * wave / NW, run = steps * (wave + 1) / NW - s0;
   const uint32_t lane_off = (uint32_t)lane * 16u;
-  Q8Stage<SETS, R, MT> st[D];
-  auto load = [&](Q8Stage<SETS, R, MT>& t, int i) __attribute__((always_inline)) {
+  Q8Stage<SETS, R, MT, Q> st[D];
+  auto load = [&](Q8Stage<SETS, R, MT, Q>& t, int i) __attribute__((always_inline)) {
     const uint32_t at = (uint32_t)(s0 + i) * 1024u;
+    if constexpr (!Q)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) t.x[m] = q8_load16<0>(rx, lane_off, i < run ? at + (uint32_t)m * pitch : Q8_PAST);
+      for (int m = 0; m < MT; ++m) t.x[m] = q8_load16<0>(rx, lane_off, i < run ? at + (uint32_t)m * pitch : Q8_PAST);
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int b = 0; b < SETS; ++b) t.w[b][r] = q8_load16<Q8_STREAM>(rw[b], lane_off, i < run ? at + (uint32_t)r * pitch : Q8_PAST);
   };
   i32x4 acc[UNITS][SETS] = {};
-  auto multiply = [&](const Q8Stage<SETS, R, MT>& t) __attribute__((always_inline)) {
+  const int r16 = lane & 15, kg = lane >> 4;
+  // (Q: columns of the product beyond the rows there are repeat the first one, and are not used; past the end, where the weights
+  // are zeros, the last integers are read again)
+  const char* const integers = own_rows + (r16 < count ? r16 : 0) * p.K + kg * 16;
+  auto multiply = [&](const Q8Stage<SETS, R, MT, Q>& t, int i) __attribute__((always_inline)) {
+    i32x4 x[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+      if constexpr (Q) x[m] = *(const i32x4*)(integers + (i < run ? s0 + i : 0) * 64);
+      else x[m] = t.x[m];
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int b = 0; b < SETS; ++b)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[r * MT + m][b] = Traits<I8Pair>::mfma16(t.w[b][r], t.x[m], acc[r * MT + m][b]);
+        for (int m = 0; m < MT; ++m) acc[r * MT + m][b] = Traits<I8Pair>::mfma16(t.w[b][r], x[m], acc[r * MT + m][b]);
   };
+  Q8RowsToLds<T, NW * 64, 2> rows;
+  if constexpr (Q) {
+    rows.read_ahead((const T*)a.rows, a.cols, p.K, count);
+    if (threadIdx.x < Q8_OWN_ROWS) own_most[threadIdx.x] = 0;
+  }
 #pragma unroll
   for (int d = 0; d < D; ++d) load(st[d], d);
+  if constexpr (Q) {
+    __syncthreads();
+    rows.finish((const T*)a.rows, a.cols, p.K, count, own_most, own_rows);
+    __syncthreads();
+  }
   for (int i = 0; i < run; i += D)
 #pragma unroll
     for (int d = 0; d < D; ++d) {
-      multiply(st[d]);  // (zeros past the end)
+      multiply(st[d], i + d);  // (zeros past the end)
       load(st[d], i + d + D);
     }
-  const int r16 = lane & 15, kg = lane >> 4;
 #pragma unroll
   for (int first = 0; first < UNITS; first += EACH) {
     if (first > 0) __syncthreads();
@@ -266,7 +374,7 @@ __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
       // lane: four output columns of one token row
       const int r = (first + i) / MT, j = 16 * ((first + i) % MT) + r16, n = (first_tile + r) * 16 + 4 * kg;
       if (j >= count || n >= p.N) continue;
-      const float sx = p.sx[row + j];
+      const float sx = Q ? RowScale<T>(own_most[Q ? j : 0]).scale : p.sx[row + j];
       float v[SETS][4], o[4];
 #pragma unroll
       for (int b = 0; b < SETS; ++b) {
@@ -283,36 +391,150 @@ __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) o[q] = v[0][q];
       }
-      const size_t to = (size_t)(row + j) * p.N + n;
+      const size_t to = (size_t)((Q && a.solo.logits != nullptr ? entry : row) + j) * p.N + n;
       if constexpr (F32) *(f32x4*)((float*)p.out + to) = f32x4{o[0], o[1], o[2], o[3]};
       else store_w<T, 4>((T*)p.out + to, o);
     }
   }
 }
 
-template <typename T, int SETS, int R, int MT, int NW, int D>
-hipError_t run_q8_few(const Q8Product& p, hipStream_t s) {
-  Q8Few a = {p, 0};
-  a.strips = ((p.N + 15) / 16 + R - 1) / R;
-  const dim3 grid((unsigned)(a.strips * (p.tiles != nullptr ? p.most_tiles : 1))), block(NW * 64);
-  if constexpr (SETS == 1)
-    if (p.out_f32) {
-      hipLaunchKernelGGL((q8_few_kernel<T, SETS, R, MT, NW, D, true>), grid, block, 0, s, a);
-      return hipGetLastError();
-    }
-  hipLaunchKernelGGL((q8_few_kernel<T, SETS, R, MT, NW, D, false>), grid, block, 0, s, a);
+template <typename T, int SETS, int R, int MT, int NW, int D, bool F32, bool Q>
+hipError_t run_q8_few(const Q8Product& p, const void* rows, int cols, const Q8Solo* solo, hipStream_t s) {
+  Q8Few a = {p, rows, cols, ((p.N + 15) / 16 + R - 1) / R, solo != nullptr ? *solo : Q8Solo{}};
+  const dim3 grid((unsigned)(a.strips * (solo != nullptr ? solo->top_k : p.tiles != nullptr ? p.most_tiles : 1))), block(NW * 64);
+  constexpr auto kern = q8_few_kernel<T, SETS, R, MT, NW, D, F32, Q>;
+  const size_t lds = Q ? (size_t)p.M * p.K : 0;
+  hipLaunchKernelGGL(kern, grid, block, lds, s, a);
   return hipGetLastError();
+}
+// What the sizes choose.  Tiles of weight rows a workgroup: one, or two of a single matrix where they are two for every CU and more.
+// Wavefronts: eight for reductions from 8192 on, or from 2048 on where workgroups are few; otherwise four, with
+// stages two deep below 2048 and four deep beyond.  us, weights from memory, as (tiles, wavefronts, stages): 2048 x 2048, one row (1, 8, 4)
+// 3.2, (1, 4, 4) 3.6, (2, 8, 4) 4.3; 16384 x 1024 (2, 4, 2) 5.1, (1, 4, 4) 5.8, (1, 8, 4) 7.3; 131072 x 1024, 16 rows (2, 4, 2) 24.9, (1, 8, 4) 45;
+// 8192 x 28672, 16 rows (2, 8, 4) 37.2, (1, 8, 4) 41.1; gate and up of 14336 x 4096 (1, 4, 4) 20.3, (1, 8, 4) 21.2; of 28672 x 8192, 16 rows
+// (1, 8, 4) 72.0, (1, 4, 4) 74.5, (2, 4, 2) 90; of 65536 x 2048 (1, 4, 4) 43.6, (1, 8, 4) 47.3.  More token tiles: four wavefronts, and two
+// tiles of gate and up for 33 to 64 rows (11008 x 4096, 48 rows (2, 4, 4) 23.4, (1, 4, 4) 24.4, (1, 8, 4) 28.1).
+template <typename T, int SETS, int R, int MT, bool F32, bool Q>
+hipError_t q8_few_depth(const Q8Product& p, const void* rows, int cols, const Q8Solo* solo, int entries, hipStream_t s) {
+  const int steps = p.K / 64;
+  if constexpr (MT <= 2) {
+    const int64_t wgs = (int64_t)((p.N + 16 * R - 1) / (16 * R)) * entries;
+    if (steps >= 128 || (steps >= 32 && wgs <= 2 * p.cus)) return run_q8_few<T, SETS, R, MT, 8, 4, F32, Q>(p, rows, cols, solo, s);
+  }
+  if (steps >= 32) return run_q8_few<T, SETS, R, MT, 4, 4, F32, Q>(p, rows, cols, solo, s);
+  return run_q8_few<T, SETS, R, MT, 4, 2, F32, Q>(p, rows, cols, solo, s);
+}
+template <typename T, int SETS, int MT, bool F32, bool Q>
+hipError_t q8_few_tiles(const Q8Product& p, const void* rows, int cols, const Q8Solo* solo, hipStream_t s) {
+  const int entries = solo != nullptr ? solo->top_k : p.tiles != nullptr ? p.most_tiles : 1;
+  if constexpr (SETS == 1 && MT <= 4) {
+    if ((int64_t)((p.N + 15) / 16) * entries >= 2 * p.cus) return q8_few_depth<T, SETS, 2, MT, F32, Q>(p, rows, cols, solo, entries, s);
+    return q8_few_depth<T, SETS, 1, MT, F32, Q>(p, rows, cols, solo, entries, s);
+  } else {
+    return q8_few_depth<T, SETS, SETS == 2 && MT == 4 ? 2 : 1, MT, F32, Q>(p, rows, cols, solo, entries, s);
+  }
 }
 template <typename T>
 hipError_t launch_q8_few(const Q8Product& p, int sets, int token_tiles, hipStream_t s) {
-  if (sets == 2) {
-    if (token_tiles == 1) return run_q8_few<T, 2, 1, 1, 8, 4>(p, s);
-    if (token_tiles == 2) return run_q8_few<T, 2, 1, 2, 8, 4>(p, s);
-    return run_q8_few<T, 2, 1, 4, 8, 4>(p, s);
+#define CALL(SETS, F32)                                                                    \
+  if (token_tiles == 1) return q8_few_tiles<T, SETS, 1, F32, false>(p, nullptr, 0, nullptr, s); \
+  if (token_tiles == 2) return q8_few_tiles<T, SETS, 2, F32, false>(p, nullptr, 0, nullptr, s); \
+  if (token_tiles == 4) return q8_few_tiles<T, SETS, 4, F32, false>(p, nullptr, 0, nullptr, s); \
+  return q8_few_tiles<T, SETS, 8, F32, false>(p, nullptr, 0, nullptr, s)
+  if (sets == 2) { CALL(2, false); }
+  if (p.out_f32) { CALL(1, true); }
+  CALL(1, false);
+#undef CALL
+}
+// Rows of which every workgroup makes integers itself: 32 KiB of them at most.
+bool q8_own_rows(int64_t M, int64_t padded) { return M <= Q8_OWN_ROWS && M * padded <= 32768; }
+template <typename T>
+hipError_t launch_q8_few_rows(const Q8Product& p, const T* rows, int cols, int sets, const Q8Solo* solo, hipStream_t s) {
+  if (sets == 2) return q8_few_tiles<T, 2, 1, false, true>(p, rows, cols, solo, s);
+  return q8_few_tiles<T, 1, 1, false, true>(p, rows, cols, solo, s);
+}
+
+// ------------------------------------------------------------------ the only token of an expert layer
+// y = sum over the choices of weight * down_e(h): a workgroup has 16 output columns of all choices, whose hidden states it makes
+// integers of for itself.  Its wavefronts are shared out over the choices; sums of a choice are added up as integers, then scaled
+// and weighted, so nothing but the sum over the choices is in floats (in a fixed order).
+struct Q8SoloDown {
+  Q8Solo solo;
+  const void* h;     // [top_k][cols]
+  const int8_t* w;
+  const float* sw;
+  void* y;           // [N]
+  int N, K, cols;
+};
+template <typename T, int NW, int D>
+__global__ void __launch_bounds__(NW * 64) q8_solo_down_kernel(Q8SoloDown a) {
+  __shared__ i32x4 part[NW * 64];
+  __shared__ uint32_t most[16];
+  extern __shared__ __align__(16) char integers[];  // [top_k][K]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), top_k = a.solo.top_k;
+  const int r16 = lane & 15, kg = lane >> 4, tile = (int)blockIdx.x;
+  Q8RowsToLds<T, NW * 64, 4> rows;
+  rows.read_ahead((const T*)a.h, a.cols, a.K, top_k);  // (rows of choices that are not run are whatever memory holds)
+  if (threadIdx.x < 16) most[threadIdx.x] = 0;
+  const int each = NW / top_k, choice = wave / each, me = wave - choice * each;  // NW >= top_k
+  int expert = choice < top_k ? a.solo.experts[choice] : -1;
+  expert = __builtin_amdgcn_readfirstlane(expert);
+  const int steps = a.K / 64, all_tiles = (a.N + 15) / 16;
+  const uint32_t pitch = (uint32_t)a.K * 16u;
+  const int s0 = steps * me / each, run = expert >= 0 ? steps * (me + 1) / each - s0 : 0;
+  const q8_rsrc rw = q8_make_rsrc(a.w + ((int64_t)(expert >= 0 ? expert : 0) * all_tiles + tile) * pitch, pitch);
+  i32x4 st[D];
+  auto load = [&](i32x4& t, int i) __attribute__((always_inline)) {
+    t = q8_load16<Q8_STREAM>(rw, (uint32_t)lane * 16u, i < run ? (uint32_t)(s0 + i) * 1024u : Q8_PAST);
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) load(st[d], d);
+  __syncthreads();
+  rows.finish((const T*)a.h, a.cols, a.K, top_k, most, integers);
+  __syncthreads();
+  i32x4 acc = {0, 0, 0, 0};
+  const char* const mine = integers + (choice < top_k ? choice : 0) * a.K + kg * 16;
+  for (int i = 0; i < run; i += D)
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      acc = Traits<I8Pair>::mfma16(st[d], *(const i32x4*)(mine + (i + d < run ? s0 + i + d : 0) * 64), acc);
+      load(st[d], i + d + D);
+    }
+  part[threadIdx.x] = acc;
+  __syncthreads();
+  if (wave > 0) return;
+  // lane (r16, kg): choice r16, columns 4 kg .. + 3 (every column of a product is the same row)
+  const int n = tile * 16 + 4 * kg;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (r16 < top_k && n < a.N) {
+    const int e = a.solo.experts[r16];
+    if (e >= 0) {
+      i32x4 sum = {0, 0, 0, 0};
+      for (int w = 0; w < each; ++w) sum += part[(r16 * each + w) * 64 + lane];
+      const f32x4 sw = *(const f32x4*)(a.sw + (int64_t)e * a.N + n);
+      const float weight = a.solo.weights[r16], sx = RowScale<T>(most[r16]).scale;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v[q] = weight * ((float)sum[q] * (sx * sw[q]));
+    }
   }
-  if (token_tiles == 1) return run_q8_few<T, 1, 1, 1, 8, 4>(p, s);
-  if (token_tiles == 2) return run_q8_few<T, 1, 1, 2, 8, 4>(p, s);
-  return run_q8_few<T, 1, 1, 4, 8, 4>(p, s);
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] += __shfl_xor(v[q], d);
+  if (r16 == 0 && n < a.N) store_w<T, 4>((T*)a.y + n, v);
+}
+bool q8_solo(int64_t M, int64_t E, int64_t top_k, int64_t padded_k, int64_t padded_n) {
+  return M == 1 && E <= Q8_SOLO_MAX_E && padded_k <= 32768 && top_k * padded_n <= 40960;
+}
+template <typename T>
+hipError_t launch_q8_solo_down(const Q8Solo& solo, const T* h, const int8_t* w, const float* sw, T* y, int N, int cols, hipStream_t s) {
+  const int padded = (int)q8_padded(cols);
+  const Q8SoloDown a = {solo, h, w, sw, y, N, padded, cols};
+  const dim3 grid((unsigned)((N + 15) / 16));
+  const size_t lds = (size_t)solo.top_k * padded;
+  if (solo.top_k <= 8) hipLaunchKernelGGL((q8_solo_down_kernel<T, 8, 4>), grid, dim3(512), lds, s, a);
+  else hipLaunchKernelGGL((q8_solo_down_kernel<T, 16, 4>), grid, dim3(1024), lds, s, a);
+  return hipGetLastError();
 }
 
 // ------------------------------------------------------------------ routed choices
@@ -397,6 +619,8 @@ hipError_t launch_q8_combine(const float* parts, const float* weights, const int
 
 #define GMLP_INSTANTIATE(T)                                                                                                      \
   template hipError_t launch_q8_few<T>(const Q8Product&, int, int, hipStream_t);                                                 \
+  template hipError_t launch_q8_few_rows<T>(const Q8Product&, const T*, int, int, const Q8Solo*, hipStream_t);                   \
+  template hipError_t launch_q8_solo_down<T>(const Q8Solo&, const T*, const int8_t*, const float*, T*, int, int, hipStream_t);   \
   template hipError_t launch_q8_rows<T>(const T*, int8_t*, float*, int64_t, int64_t, int64_t, const int*, const int*, hipStream_t); \
   template hipError_t launch_q8_dequantize<T>(const int8_t*, const float*, T*, int64_t, int64_t, int64_t, hipStream_t);           \
   template hipError_t launch_q8_combine<T>(const float*, const float*, const int*, T*, int64_t, int64_t, int, hipStream_t);

@@ -12,7 +12,7 @@
 namespace gmlp {
 
 constexpr int Q8_MAX_COLS = 131072;   // 127 * 127 * 131072 < 2^31
-constexpr int Q8_FEW_ROWS = 64;       // token rows, of all or of an expert, that the weight-streaming kernels take
+constexpr int Q8_FEW_ROWS = 128;      // token rows, of all or of an expert, that the weight-streaming kernels take
 inline __host__ __device__ int64_t q8_padded(int64_t cols) { return (cols + 127) / 128 * 128; }
 inline __host__ __device__ int64_t q8_tiled_rows(int64_t rows) { return (rows + 15) / 16 * 16; }
 
@@ -55,9 +55,26 @@ struct Q8Product {
   float* partial;        // [splits][SETS][M][N] 32-bit sums, where splits > 1 (dense only)
 };
 
-// Weight streaming: the rows of a tile are at most 16 * token_tiles (1, 2 or 4).
+// Weight streaming: the rows of a tile are at most 16 * token_tiles (1, 2, 4 or 8).
 template <typename T>
 hipError_t launch_q8_few(const Q8Product& p, int sets, int token_tiles, hipStream_t s);
+// An expert layer's only token: its logits, and where its choices are left.
+constexpr int Q8_SOLO_MAX_E = 256;
+struct Q8Solo {
+  const void* logits;  // [E] of a GMLP_* type
+  int logits_dtype, E, top_k, normalize;
+  int* experts;        // [top_k], < 0: not run
+  float* weights;      // [top_k]
+};
+// The same of M rows [M][cols] as they are, where q8_own_rows allows it (p.x and p.sx are not used): dense, or (solo) the only token
+// through the matrices of each of its choices, out [top_k][N].
+bool q8_own_rows(int64_t M, int64_t padded);
+template <typename T>
+hipError_t launch_q8_few_rows(const Q8Product& p, const T* rows, int cols, int sets, const Q8Solo* solo, hipStream_t s);
+// y[N] = sum over the choices of weight * down(h), h [top_k][cols].  Where q8_solo says so.
+bool q8_solo(int64_t M, int64_t E, int64_t top_k, int64_t padded_k, int64_t padded_n);
+template <typename T>
+hipError_t launch_q8_solo_down(const Q8Solo& solo, const T* h, const int8_t* w, const float* sw, T* y, int N, int cols, hipStream_t s);
 // GEMM: tile_class LARGE (256 rows), WIDE or MEDIUM_FULL (128).
 template <typename T>
 hipError_t launch_q8_gemm(const Q8Product& p, int sets, hipStream_t s);

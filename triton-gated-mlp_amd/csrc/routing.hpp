@@ -39,6 +39,50 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __uint_as_float((uint32_t)__builtin_amdgcn_readlane((int)__float_as_uint(v), 63));
 }
 
+// One wavefront, one token: lane j < top_k gets the token's j-th choice and its weight.  The experts lie in lane order
+// (lane l: VPL l .. VPL l + VPL - 1), so among equal logits the lowest lane holds the lowest number.
+// (-inf: not available, weight 0 and expert -1 - number.)
+template <int VPL, typename F>
+__device__ __forceinline__ void choose(F&& logit, int E, int top_k, bool normalize, int lane, int& expert, float& weight) {
+  uint32_t key[VPL];
+  float value[VPL];
+#pragma unroll
+  for (int v = 0; v < VPL; ++v) {
+    const int e = lane * VPL + v;
+    value[v] = e < E ? logit(e) : -__builtin_inff();
+    key[v] = e < E ? logit_key(value[v]) : 0u;
+  }
+  uint32_t mine = 0, top = 0;
+  expert = 0;
+  for (int j = 0; j < top_k; ++j) {
+    uint32_t best = key[0];
+    int at = 0;
+#pragma unroll
+    for (int v = 1; v < VPL; ++v)
+      if (key[v] > best) best = key[v], at = v;
+    const uint32_t most = wave_max(best);
+    const int owner = __builtin_ctzll(__ballot(best == most));
+    const int e = __builtin_amdgcn_readlane(lane * VPL + at, owner);
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if (lane == owner && v == at) key[v] = 0u;
+    if (j == 0) top = most;
+    if (lane == j) mine = most, expert = e;
+  }
+  const float first = key_logit(top), own = key_logit(mine);
+  const bool none = first == -__builtin_inff();
+  const float e = lane < top_k && !none ? expf(own - first) : 0.f;
+  float all = e;
+  if (!normalize) {
+    all = 0.f;
+#pragma unroll
+    for (int v = 0; v < VPL; ++v)
+      if (lane * VPL + v < E && !none) all += expf(value[v] - first);
+  }
+  weight = none ? 0.f : e / wave_sum(all);
+  if (own == -__builtin_inff()) expert = -1 - expert;
+}
+
 // Four tokens to a wavefront, a row of 16 lanes each; lane l of a row has VPL experts from VPL l on.
 template <typename F>
 __device__ __forceinline__ uint32_t across_row(uint32_t v, F&& f) {
