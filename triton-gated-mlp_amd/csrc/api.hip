@@ -1704,7 +1704,7 @@ extern "C" {
 
 size_t gmlp_moe_balance_workspace_bytes(int64_t M, int64_t E) {
   if (M < 1 || M > kMaxDim || E < 1 || E > gmlp::EXPERTS_MAX_E) return 0;
-  return (size_t)gmlp::balance_workgroups(M) * gmlp::balance_partial((int)E) * sizeof(float);
+  return (size_t)gmlp::balance_workgroups(M, (int)E) * gmlp::balance_partial((int)E) * sizeof(float);
 }
 
 int gmlp_moe_balance_fwd(const void* logits, const uint8_t* mask, float* weights, int64_t* experts, int64_t* counts, float* loss,
@@ -1779,14 +1779,29 @@ struct Arena {
 int q8_token_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : rows <= 64 ? 4 : 8; }
 
 // How a dense product of more rows than the streaming kernels take runs.  A reduction tile of 128 integers costs what one of 64
-// 16-bit elements does (the same bytes and as many matrix instructions), so the estimates are theirs.
-GemmPlan plan_q8(int kind, int64_t M, int64_t N, int64_t padded) {
-  return cheapest(kind, tiles_of(kLarge, kind, M, N), tiles_of(kWide, kind, M, N), 0, tiles_of(kMedium, kind, M, N), padded / 128,
-                  (double)M * (double)N * (kind == GATEUP ? 2 : 1), kMaxSplits);
+// 16-bit elements does (the same bytes and as many matrix instructions), so the estimates are theirs.  `first`: output columns that
+// large tiles take in whole rounds, the others going to `rest` in a launch behind (0: one launch).
+struct Q8DensePlan {
+  GemmPlan all, rest;
+  int64_t first;
+};
+Q8DensePlan plan_q8(int kind, int64_t M, int64_t N, int64_t padded) {
+  auto pick = [&](int64_t cols, int64_t splits) {
+    return cheapest(kind, tiles_of(kLarge, kind, M, cols), tiles_of(kWide, kind, M, cols), 0, tiles_of(kMedium, kind, M, cols), padded / 128,
+                    (double)M * (double)cols * (kind == GATEUP ? 2 : 1), splits);
+  };
+  Q8DensePlan p = {pick(N, kMaxSplits), {}, 0};
+  const int64_t whole = whole_rounds(kind, M, N) * tile_cols(kind);
+  if (whole > 0) {
+    const GemmPlan rest = pick(N - whole, 1);
+    const double us = launch_us(kLarge, kind, tiles_of(kLarge, kind, M, whole), padded / 128, 1, 0) + rest.us;
+    if (us < p.all.us) p = {{gmlp::TILE_LARGE, 1, us}, rest, whole};
+  }
+  return p;
 }
 size_t q8_split_bytes(int kind, int64_t M, int64_t N, int64_t padded) {
   if (M <= gmlp::Q8_FEW_ROWS) return 0;
-  return split_workspace_bytes(plan_q8(kind, M, N, padded).splits, M, N, kind == GATEUP ? 2 : 1);
+  return split_workspace_bytes(plan_q8(kind, M, N, padded).all.splits, M, N, kind == GATEUP ? 2 : 1);
 }
 
 gmlp::Q8Product q8_product(const int8_t* x, const float* sx, int64_t M, int64_t N, int64_t cols) {
@@ -1800,13 +1815,20 @@ gmlp::Q8Product q8_product(const int8_t* x, const float* sx, int64_t M, int64_t 
 template <typename T>
 hipError_t run_q8_dense(gmlp::Q8Product& p, int sets, float* partial, hipStream_t s) {
   if (p.M <= gmlp::Q8_FEW_ROWS) return gmlp::launch_q8_few<T>(p, sets, q8_token_tiles(p.M), s);
-  const GemmPlan plan = plan_q8(sets == 2 ? GATEUP : LINEAR, p.M, p.N, p.K);
-  p.tile_class = plan.tile_class;
-  p.splits = plan.splits;
+  const Q8DensePlan plan = plan_q8(sets == 2 ? GATEUP : LINEAR, p.M, p.N, p.K);
+  p.splits = plan.all.splits;
   p.rotate = p.M <= 512;
-  p.group_m = pick_group(p.M, p.N, sets);
   p.partial = partial;
-  return gmlp::launch_q8_gemm<T>(p, sets, s);
+  auto columns = [&](int64_t from, int64_t to, int tile_class) {
+    p.tile_class = tile_class;
+    p.first_col = (int)from;
+    p.cols = (int)(to - from);
+    p.group_m = pick_group(p.M, to - from, sets);
+    return gmlp::launch_q8_gemm<T>(p, sets, s);
+  };
+  if (plan.first == 0) return columns(0, p.N, plan.all.tile_class);
+  if (hipError_t e = columns(0, plan.first, plan.all.tile_class)) return e;
+  return columns(plan.first, p.N, plan.rest.tile_class);
 }
 
 struct Q8LinearWorkspace {
@@ -2058,6 +2080,7 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
       p.tiles = routed.tiles; p.total = routed.total; p.most_tiles = (int)plan.tiles;
       if (!plan.gemm) return gmlp::launch_q8_few<T>(p, sets, plan.cap / 16, s);
       p.tile_class = plan.tile_class[sets == 2 ? 0 : 1];
+      p.cols = p.N;
       p.group_m = 8;
       return gmlp::launch_q8_gemm<T>(p, sets, s);
     };

@@ -15,62 +15,69 @@
 
 namespace gmlp {
 
-constexpr int BAL_THREADS = 256, BAL_ROWS = BAL_THREADS / 16;  // tokens of a workgroup at a time
+// Wavefronts of a workgroup in the first stage: sixteen, where their sums fit LDS.  (16384 tokens, 128 experts: one round of
+// 256 workgroups.  Four wavefronts and four rounds 15.5 us, a wavefront on a SIMD.)
+constexpr int bal_wavefronts(int vpl) { return vpl <= 16 ? 16 : 4; }
+constexpr int BAL_BWD_THREADS = 256;
+constexpr int64_t BAL_ALONE = 256;  // tokens that one workgroup takes, both stages in one launch
 
-// Sums of all workgroups' parts -> counts, loss, slope.  1024 threads.
+// Sums of all workgroups' parts -> counts, loss, slope.  1024 threads, and a chain of loads and barriers: eight loads of a thread are in
+// flight together, sums join in trees (64-bit atomics in LDS on one word, one after the other, took 4 us for 128 experts).
 __device__ __forceinline__ void balance_finish(const BalanceArgs& a, int parts) {
-  __shared__ double sum_p[1024];
-  __shared__ long long sum_c[1024];
-  __shared__ double in_loss[16];
-  __shared__ long long all_c, all_t;
-  const int tid = threadIdx.x, E = a.E, width = balance_partial(E);
+  __shared__ double sum_p[1024], sum_c[1024];  // (numbers of choices are exact up to 2^53)
+  __shared__ double in_wave[3][16];
+  const int tid = threadIdx.x, lane = tid & 63, E = a.E, width = balance_partial(E);
   // thread g * E + e adds up parts g, g + groups, ...
-  const int groups = 1024 / E, e = tid % E, g = tid / E;
-  double p = 0.0;
-  long long c = 0;
+  const int groups = parts < 1024 / E ? parts : 1024 / E, g = tid / E, e = tid - g * E;
+  double p = 0.0, c = 0.0, t = 0.0;
   if (g < groups)
+#pragma unroll 8
     for (int i = g; i < parts; i += groups) {
       p += (double)a.partial[(size_t)i * width + e];
-      c += __float_as_int(a.partial[(size_t)i * width + E + e]);
+      c += (double)__float_as_int(a.partial[(size_t)i * width + E + e]);
     }
-  sum_p[tid] = p;
-  sum_c[tid] = c;
-  if (tid == 0) all_c = 0, all_t = 0;
-  __syncthreads();
-  if (tid < E) {
-    for (int i = 1; i < groups; ++i) {
-      p += sum_p[i * E + tid];
-      c += sum_c[i * E + tid];
+  for (int i = tid; i < parts; i += 1024) t += (double)__float_as_int(a.partial[(size_t)i * width + 2 * E]);
+  int half = 1;
+  while (half < groups) half *= 2;
+  for (half /= 2; half > 0; half /= 2) {
+    sum_p[tid] = p;
+    sum_c[tid] = c;
+    __syncthreads();
+    if (g < half && g + half < groups) {
+      p += sum_p[tid + half * E];
+      c += sum_c[tid + half * E];
     }
-    a.counts[tid] = c;
-    if (c) atomicAdd((unsigned long long*)&all_c, (unsigned long long)c);
+    __syncthreads();
   }
-  long long t = 0;
-  for (int i = tid; i < parts; i += 1024) t += __float_as_int(a.partial[(size_t)i * width + 2 * E]);
-  if (t) atomicAdd((unsigned long long*)&all_t, (unsigned long long)t);
-  __syncthreads();
-  // (no tokens: a loss of 0, and no slope)
-  const double scale = all_c > 0 ? (double)E / ((double)all_c * (double)all_t) : 0.0;
-  double part = 0.0;
-  if (tid < E) {
-    const double slope = scale * (double)c;
-    a.slope[tid] = (float)slope;
-    part = slope * p;
-  }
+  if (tid >= E) p = c = 0.0;
+  double all[3] = {c, t, c * p};
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) part += __shfl_xor(part, d);
-  if ((tid & 63) == 0) in_loss[tid >> 6] = part;
+  for (int d = 32; d > 0; d >>= 1)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) all[k] += __shfl_xor(all[k], d);
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) in_wave[k][tid >> 6] = all[k];
   __syncthreads();
-  if (tid == 0) {
-    double loss = 0.0;
-    for (int i = 0; i < 16; ++i) loss += in_loss[i];
-    *a.loss = (float)loss;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) all[k] = in_wave[k][lane & 15];
+#pragma unroll
+  for (int d = 8; d > 0; d >>= 1)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) all[k] += __shfl_xor(all[k], d);
+  // (no tokens: a loss of 0, and no slope)
+  const double scale = all[0] > 0.0 ? (double)E / (all[0] * all[1]) : 0.0;
+  if (tid < E) {
+    a.counts[tid] = (int64_t)c;
+    a.slope[tid] = (float)(scale * c);
   }
+  if (tid == 0) *a.loss = (float)(scale * all[2]);
 }
 __global__ void __launch_bounds__(1024) balance_finish_kernel(BalanceArgs a, int parts) { balance_finish(a, parts); }
 
 template <int VPL, typename L>
-__global__ void __launch_bounds__(BAL_THREADS) balance_rows_kernel(BalanceArgs a) {
+__global__ void __launch_bounds__(bal_wavefronts(VPL) * 64) balance_rows_kernel(BalanceArgs a) {
+  constexpr int THREADS = bal_wavefronts(VPL) * 64, ROWS = THREADS / 16;
   extern __shared__ float wave_sums[];  // [wavefronts][balance_partial(E)]
   const int lane = threadIdx.x & 63, l = lane & 15, mine = threadIdx.x >> 4, E = a.E, top_k = a.top_k, width = balance_partial(E);
   const bool aligned = ((uintptr_t)a.logits & (sizeof(L) * VPL - 1)) == 0;
@@ -78,7 +85,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_kernel(BalanceArgs a
   int chosen[VPL], tokens = 0;
 #pragma unroll
   for (int v = 0; v < VPL; ++v) p[v] = 0.f, chosen[v] = 0;
-  for (int64_t base = (int64_t)blockIdx.x * BAL_ROWS; base < a.M; base += (int64_t)gridDim.x * BAL_ROWS) {
+  for (int64_t base = (int64_t)blockIdx.x * ROWS; base < a.M; base += (int64_t)gridDim.x * ROWS) {
     const int64_t token = base + mine, t = token < a.M ? token : a.M - 1;
     LogitRow<VPL, L> row;
     row.load((const L*)a.logits + t * E, aligned, E, l);
@@ -129,21 +136,27 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_rows_kernel(BalanceArgs a
     if (l == 0) own[2 * E] = __int_as_float(tokens);
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < width; i += BAL_THREADS) {
+  for (int i = threadIdx.x; i < width; i += THREADS) {
     float sum = 0.f;
     int n = 0;
 #pragma unroll
-    for (int w = 0; w < BAL_THREADS / 64; ++w) {
+    for (int w = 0; w < THREADS / 64; ++w) {
       const float x = wave_sums[w * width + i];
       if (i < E) sum += x;
       else n += __float_as_int(x);
     }
     a.partial[(size_t)blockIdx.x * width + i] = i < E ? sum : __int_as_float(n);
   }
+  if constexpr (THREADS == 1024)
+    if (gridDim.x == 1) {
+      __threadfence_block();
+      __syncthreads();
+      balance_finish(a, 1);
+    }
 }
 
 template <int VPL, typename L>
-__global__ void __launch_bounds__(BAL_THREADS) balance_bwd_kernel(BalanceArgs a) {
+__global__ void __launch_bounds__(BAL_BWD_THREADS) balance_bwd_kernel(BalanceArgs a) {
   const int lane = threadIdx.x & 63, l = lane & 15, mine = threadIdx.x >> 4, E = a.E, top_k = a.top_k;
   const bool aligned = ((uintptr_t)a.logits & (sizeof(L) * VPL - 1)) == 0;
   const bool aligned_out = ((uintptr_t)a.d_logits & (sizeof(L) * VPL - 1)) == 0;
@@ -151,7 +164,7 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_bwd_kernel(BalanceArgs a)
   float slope[VPL];
 #pragma unroll
   for (int v = 0; v < VPL; ++v) slope[v] = l * VPL + v < E && a.d_loss != nullptr ? a.slope[l * VPL + v] : 0.f;
-  for (int64_t base = (int64_t)blockIdx.x * BAL_ROWS; base < a.M; base += (int64_t)gridDim.x * BAL_ROWS) {
+  for (int64_t base = (int64_t)blockIdx.x * (BAL_BWD_THREADS / 16); base < a.M; base += (int64_t)gridDim.x * (BAL_BWD_THREADS / 16)) {
     const int64_t token = base + mine, t = token < a.M ? token : a.M - 1;
     LogitRow<VPL, L> row;
     row.load((const L*)a.logits + t * E, aligned, E, l);
@@ -220,9 +233,9 @@ __global__ void __launch_bounds__(BAL_THREADS) balance_bwd_kernel(BalanceArgs a)
   }
 }
 
-int balance_workgroups(int64_t M) {
-  const int64_t n = (M + BAL_ROWS - 1) / BAL_ROWS;
-  return (int)(n < 256 ? n : 256);
+int balance_workgroups(int64_t M, int E) {
+  const int64_t rows = E <= 256 ? 64 : 16, n = (M + rows - 1) / rows;
+  return E <= 256 && M <= BAL_ALONE ? 1 : (int)(n < 256 ? n : 256);
 }
 
 #define GMLP_BY_ROW(E, CALL)     \
@@ -234,20 +247,22 @@ int balance_workgroups(int64_t M) {
 
 template <typename L>
 hipError_t launch_balance_fwd(const BalanceArgs& a, hipStream_t s) {
-  const int wgs = balance_workgroups(a.M);
-  const size_t lds = (size_t)(BAL_THREADS / 64) * balance_partial(a.E) * sizeof(float);
-#define CALL(V) hipLaunchKernelGGL((balance_rows_kernel<V, L>), dim3(wgs), dim3(BAL_THREADS), lds, s, a)
+  const int wgs = balance_workgroups(a.M, a.E);
+#define CALL(V)                                                                                                  \
+  hipLaunchKernelGGL((balance_rows_kernel<V, L>), dim3(wgs), dim3(bal_wavefronts(V) * 64),                        \
+                     (size_t)bal_wavefronts(V) * balance_partial(a.E) * sizeof(float), s, a)
   GMLP_BY_ROW(a.E, CALL);
 #undef CALL
   if (hipError_t e = hipGetLastError()) return e;
+  if (wgs == 1 && a.E <= 256) return hipSuccess;
   hipLaunchKernelGGL(balance_finish_kernel, dim3(1), dim3(1024), 0, s, a, wgs);
   return hipGetLastError();
 }
 template <typename L>
 hipError_t launch_balance_bwd(const BalanceArgs& a, hipStream_t s) {
-  const int64_t n = (a.M + BAL_ROWS - 1) / BAL_ROWS;
+  const int64_t n = (a.M + BAL_BWD_THREADS / 16 - 1) / (BAL_BWD_THREADS / 16);
   const int wgs = (int)(n < 2048 ? n : 2048);
-#define CALL(V) hipLaunchKernelGGL((balance_bwd_kernel<V, L>), dim3(wgs), dim3(BAL_THREADS), 0, s, a)
+#define CALL(V) hipLaunchKernelGGL((balance_bwd_kernel<V, L>), dim3(wgs), dim3(BAL_BWD_THREADS), 0, s, a)
   GMLP_BY_ROW(a.E, CALL);
 #undef CALL
   return hipGetLastError();

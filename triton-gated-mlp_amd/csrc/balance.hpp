@@ -22,7 +22,7 @@ struct BalanceArgs {
 // What a workgroup of the first stage leaves: for each expert the sum of its probabilities and (as an int) its choices, and
 // the number of tokens.
 inline __host__ __device__ int balance_partial(int E) { return 2 * E + 1; }
-int balance_workgroups(int64_t M);
+int balance_workgroups(int64_t M, int E);
 
 template <typename L>
 hipError_t launch_balance_fwd(const BalanceArgs& a, hipStream_t s);

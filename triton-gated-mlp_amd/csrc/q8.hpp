@@ -52,6 +52,7 @@ struct Q8Product {
   int nxcd, cus;
   // GEMM only
   int tile_class, splits, rotate, group_m;
+  int first_col, cols;   // the output columns of this launch (all of them where splits > 1)
   float* partial;        // [splits][SETS][M][N] 32-bit sums, where splits > 1 (dense only)
 };
 

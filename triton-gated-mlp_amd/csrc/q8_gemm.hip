@@ -185,7 +185,7 @@ struct EpiQ8Partial : EpiPartial<I8Pair> {
 
 template <int BM, int BN, int WGN, int NB, typename Epi>
 __global__ void __launch_bounds__(2 * WGN * 64) gemm_q8_kernel_pipelined(Q8Product p, typename Epi::Args ea) {
-  const int tiles_n = (p.N + BN - 1) / BN;
+  const int tiles_n = (p.cols + BN - 1) / BN;
   const int tiles_m = p.tiles != nullptr ? p.total[0] : (p.M + BM - 1) / BM;
   const int each = tiles_m * tiles_n, all = each * (Epi::SPLIT ? p.splits : 1);
   if ((int)blockIdx.x >= all) return;
@@ -202,14 +202,14 @@ __global__ void __launch_bounds__(2 * WGN * 64) gemm_q8_kernel_pipelined(Q8Produ
     row = __builtin_amdgcn_readfirstlane(t.row);
     rows = __builtin_amdgcn_readfirstlane(t.rows);
   }
-  const int col = tn * BN;
+  const int col = p.first_col + tn * BN;
   const int64_t from = (expert * ((p.N + 15) / 16 * 16) + col) * p.K;
   GemmArgs ga = {};
   ga.A[0] = ga.A[1] = p.x + row * p.K;
   ga.B[0] = p.w[0] + from;
   ga.B[1] = NB == 2 ? p.w[1] + from : ga.B[0];
   ga.M = rows;
-  ga.N = min(BN, p.N - col);
+  ga.N = min(BN, p.first_col + p.cols - col);
   ga.K = ga.lda = ga.ldb = p.K / 2;
   ga.nseg = 1;
   ga.group_m = 1;
@@ -224,7 +224,7 @@ hipError_t launch_q8_class(const Q8Product& p, const typename Epi::Args& ea, hip
   typedef PipeConfig<I8Pair, BM, BN, 16, 2, WGN, false, false, NB, true> Cfg;
   constexpr auto kern = gemm_q8_kernel_pipelined<BM, BN, WGN, NB, Epi>;
   if (hipError_t e = allow_dynamic_lds(lds_kernel_of<kern, Cfg::LDS_BYTES>, s)) return e;
-  const int tiles_m = p.tiles != nullptr ? p.most_tiles : (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
+  const int tiles_m = p.tiles != nullptr ? p.most_tiles : (p.M + BM - 1) / BM, tiles_n = (p.cols + BN - 1) / BN;
   hipLaunchKernelGGL(kern, dim3((unsigned)(tiles_m * tiles_n * (Epi::SPLIT ? p.splits : 1))), dim3(Cfg::NW * 64), Cfg::LDS_BYTES, s, p, ea);
   return hipGetLastError();
 }
