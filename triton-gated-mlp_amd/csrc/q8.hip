@@ -407,32 +407,40 @@ hipError_t run_q8_few(const Q8Product& p, const void* rows, int cols, const Q8So
   hipLaunchKernelGGL(kern, grid, block, lds, s, a);
   return hipGetLastError();
 }
-// What the sizes choose.  Tiles of weight rows a workgroup: one, or two of a single matrix where they are two for every CU and more.
-// Wavefronts: eight for reductions from 8192 on, or from 2048 on where workgroups are few; otherwise four, with
-// stages two deep below 2048 and four deep beyond.  us, weights from memory, as (tiles, wavefronts, stages): 2048 x 2048, one row (1, 8, 4)
-// 3.2, (1, 4, 4) 3.6, (2, 8, 4) 4.3; 16384 x 1024 (2, 4, 2) 5.1, (1, 4, 4) 5.8, (1, 8, 4) 7.3; 131072 x 1024, 16 rows (2, 4, 2) 24.9, (1, 8, 4) 45;
-// 8192 x 28672, 16 rows (2, 8, 4) 37.2, (1, 8, 4) 41.1; gate and up of 14336 x 4096 (1, 4, 4) 20.3, (1, 8, 4) 21.2; of 28672 x 8192, 16 rows
-// (1, 8, 4) 72.0, (1, 4, 4) 74.5, (2, 4, 2) 90; of 65536 x 2048 (1, 4, 4) 43.6, (1, 8, 4) 47.3.  More token tiles: four wavefronts, and two
-// tiles of gate and up for 33 to 64 rows (11008 x 4096, 48 rows (2, 4, 4) 23.4, (1, 4, 4) 24.4, (1, 8, 4) 28.1).
+// What the sizes choose.  us, weights from memory, as (tiles of weight rows a workgroup, wavefronts, stages).
+// One token tile: two tiles of a single matrix where they are two for every CU and more, otherwise one.  Wavefronts: eight
+// for reductions from 8192 on, or from 2048 on where workgroups are few; otherwise four, with stages two deep below 2048 and four
+// deep beyond.  2048 x 2048, one row (1, 8, 4) 3.2, (1, 4, 4) 3.6, (2, 8, 4) 4.3; 16384 x 1024 (2, 4, 2) 5.1, (1, 4, 4) 5.8, (1, 8, 4) 7.3;
+// 131072 x 1024, 16 rows (2, 4, 2) 24.9, (1, 8, 4) 45; 8192 x 28672, 16 rows (2, 8, 4) 37.2, (1, 8, 4) 41.1; gate and up of 14336 x 4096
+// (1, 4, 4) 20.3, (1, 8, 4) 21.2; of 28672 x 8192, 16 rows (1, 8, 4) 72.0, (1, 4, 4) 74.5, (2, 4, 2) 90; of 65536 x 2048 (1, 4, 4) 43.6,
+// (1, 8, 4) 47.3.
+// More token tiles: every workgroup reads all of them from the caches, which is what bounds it unless it has several tiles of
+// weights for them: four of a single matrix (two for two token tiles) where there are three for every CU, two from two for every CU
+// on, two of gate and up.  128 rows, 14336 x 4096 (4, 4, 2) 21.5, (2, 4, 2) 25.0, (1, 4, 2) 40; gate and up of it (2, 4, 1) 34.7,
+// (2, 4, 2) 38.7, (1, 4, 2) 48.7; 5632 x 2048 (2, 4, 2) 13.0, (2, 4, 1) 14.0, (1, 4, 1) 14.7; 4096 x 14336 (1, 4, 2) 32.7, (2, 4, 2) 38.1.
+// 64 rows, 14336 x 4096 (4, 4, 2) 15.9, (1, 4, 1) 26.3; 4096 x 14336 (1, 4, 2) 21.9, (2, 8, 1) 25.9; 32 rows, 14336 x 4096 (2, 4, 2) 13.2,
+// (1, 8, 2) 18.0.
 template <typename T, int SETS, int R, int MT, bool F32, bool Q>
 hipError_t q8_few_depth(const Q8Product& p, const void* rows, int cols, const Q8Solo* solo, int entries, hipStream_t s) {
   const int steps = p.K / 64;
-  if constexpr (MT <= 2) {
-    const int64_t wgs = (int64_t)((p.N + 16 * R - 1) / (16 * R)) * entries;
+  const int64_t wgs = (int64_t)((p.N + 16 * R - 1) / (16 * R)) * entries;
+  if constexpr (MT == 1) {
     if (steps >= 128 || (steps >= 32 && wgs <= 2 * p.cus)) return run_q8_few<T, SETS, R, MT, 8, 4, F32, Q>(p, rows, cols, solo, s);
+    if (steps >= 32) return run_q8_few<T, SETS, R, MT, 4, 4, F32, Q>(p, rows, cols, solo, s);
+  } else if constexpr (MT == 8 && SETS == 2 && R == 2) {
+    if (wgs > p.cus) return run_q8_few<T, SETS, R, MT, 4, 1, F32, Q>(p, rows, cols, solo, s);
   }
-  if (steps >= 32) return run_q8_few<T, SETS, R, MT, 4, 4, F32, Q>(p, rows, cols, solo, s);
   return run_q8_few<T, SETS, R, MT, 4, 2, F32, Q>(p, rows, cols, solo, s);
 }
 template <typename T, int SETS, int MT, bool F32, bool Q>
 hipError_t q8_few_tiles(const Q8Product& p, const void* rows, int cols, const Q8Solo* solo, hipStream_t s) {
   const int entries = solo != nullptr ? solo->top_k : p.tiles != nullptr ? p.most_tiles : 1;
-  if constexpr (SETS == 1 && MT <= 4) {
-    if ((int64_t)((p.N + 15) / 16) * entries >= 2 * p.cus) return q8_few_depth<T, SETS, 2, MT, F32, Q>(p, rows, cols, solo, entries, s);
-    return q8_few_depth<T, SETS, 1, MT, F32, Q>(p, rows, cols, solo, entries, s);
-  } else {
-    return q8_few_depth<T, SETS, SETS == 2 && MT == 4 ? 2 : 1, MT, F32, Q>(p, rows, cols, solo, entries, s);
-  }
+  const int64_t tiles = (int64_t)((p.N + 15) / 16) * entries;
+  if constexpr (SETS == 1 && MT >= 4)
+    if (tiles >= 3 * p.cus) return q8_few_depth<T, SETS, 4, MT, F32, Q>(p, rows, cols, solo, entries, s);
+  if constexpr (SETS == 1 || MT > 1)
+    if (tiles >= (SETS == 2 ? 1 : 2) * p.cus) return q8_few_depth<T, SETS, 2, MT, F32, Q>(p, rows, cols, solo, entries, s);
+  return q8_few_depth<T, SETS, 1, MT, F32, Q>(p, rows, cols, solo, entries, s);
 }
 template <typename T>
 hipError_t launch_q8_few(const Q8Product& p, int sets, int token_tiles, hipStream_t s) {
@@ -590,29 +598,34 @@ hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8
   return hipGetLastError();
 }
 
+// Four columns a thread; four choices' parts are in flight together.
 template <typename T>
 __global__ void __launch_bounds__(256) q8_combine_kernel(const float* parts, const float* weights, const int* row_of, T* y, int64_t M,
                                                          int K, int top_k) {
-  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, t = unit / (K / 8);
+  const int64_t unit = (int64_t)blockIdx.x * 256 + threadIdx.x, t = unit / (K / 4);
   if (t >= M) return;
-  const int c = (int)(unit % (K / 8)) * 8;
-  float v[8] = {};
-  for (int j = 0; j < top_k; ++j) {
-    const int row = row_of[t * top_k + j];
-    if (row < 0) continue;
-    const float w = weights[t * top_k + j];
-    float part[8];
-    load_w<float, 4>(parts + (int64_t)row * K + c, part);
-    load_w<float, 4>(parts + (int64_t)row * K + c + 4, part + 4);
+  const int c = (int)(unit % (K / 4)) * 4;
+  float v[4] = {};
+  for (int first = 0; first < top_k; first += 4) {
+    f32x4 part[4];
+    float w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += w * part[i];
+    for (int j = 0; j < 4; ++j) {
+      const int row = first + j < top_k ? row_of[t * top_k + first + j] : -1;
+      w[j] = row >= 0 ? weights[t * top_k + first + j] : 0.f;
+      part[j] = row >= 0 ? __builtin_nontemporal_load((const f32x4*)(parts + (int64_t)row * K + c)) : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += w[j] * part[j][i];
   }
-  store_w<T, 8>(y + t * K + c, v);
+  store_w<T, 4>(y + t * K + c, v);
 }
 template <typename T>
 hipError_t launch_q8_combine(const float* parts, const float* weights, const int* row_of, T* y, int64_t M, int64_t K, int top_k,
                              hipStream_t s) {
-  hipLaunchKernelGGL(q8_combine_kernel<T>, dim3((unsigned)((M * (K / 8) + 255) / 256)), dim3(256), 0, s, parts, weights, row_of, y, M, (int)K,
+  hipLaunchKernelGGL(q8_combine_kernel<T>, dim3((unsigned)((M * (K / 4) + 255) / 256)), dim3(256), 0, s, parts, weights, row_of, y, M, (int)K,
                      top_k);
   return hipGetLastError();
 }
