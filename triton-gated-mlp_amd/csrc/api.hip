@@ -1857,39 +1857,46 @@ struct Q8MlpWorkspace {
   }
 };
 
-// An expert layer: rows of a tile (the GEMM's 128 or 256, the streaming kernels' 16 to 128).
+// An expert layer: rows of a tile (the GEMM's 128, or 256 in a list of its own, the streaming kernels' 16 to 128), and of the
+// GEMM the tile classes of gate/up and down, by their estimates for as many tiles as experts with half a tile left over each have.
 struct Q8MoePlan {
   int cap;
   bool gemm;
   int tile_class[2];
-  int64_t rows, tiles;
+  int64_t rows, tiles, large;
 };
 Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
   Q8MoePlan p = {};
   const int64_t each = cdiv(pairs, E);
-  if (each <= 12) p.cap = 16;
-  else if (each <= 24) p.cap = 32;
-  else if (each <= 48) p.cap = 64;
-  else if (each <= 96) p.cap = 128;
-  else {
-    p.gemm = true;
-    p.cap = each >= 512 ? 256 : 128;
-    p.tile_class[0] = p.tile_class[1] = each >= 512 ? gmlp::TILE_LARGE : gmlp::TILE_WIDE;
-  }
+  p.gemm = each > 96;
+  p.cap = each <= 12 ? 16 : each <= 24 ? 32 : each <= 48 ? 64 : 128;
   p.rows = gmlp::q8_plan_rows(pairs, E);
   p.tiles = gmlp::q8_plan_tiles(pairs, E, p.cap);
+  if (!p.gemm) return p;
+  p.large = gmlp::q8_plan_tiles(pairs, E, 256);
+  for (int i = 0; i < 2; ++i) {
+    const int kind = i == 0 ? GATEUP : LINEAR;
+    const int64_t cols = i == 0 ? N : K, kt = gmlp::q8_padded(i == 0 ? K : N) / 128;
+    double least = 1e30;
+    for (const TileCost* c : {&kLarge, &kWide, &kMedium}) {
+      const int64_t rows = pairs / c->rows + (E + 1) / 2;
+      const double us = launch_us(*c, kind, rows * cdiv(cols, tile_cols(kind) / c->col_div), kt, 1, 0);
+      if (us < least) least = us, p.tile_class[i] = c->tile_class;
+    }
+  }
   return p;
 }
 struct Q8MoeWorkspace {
-  size_t weights, experts, total, tiles, row_of, token_of, x, sx, h, q, sq, parts, bytes;
+  size_t weights, experts, total, tiles, large, row_of, token_of, x, sx, h, q, sq, parts, bytes;
   Q8MoeWorkspace(int64_t M, int64_t K, int64_t N, int64_t E, int64_t top_k) {
     Arena a;
     const int64_t pairs = M * top_k;
     const Q8MoePlan p = plan_q8_moe(pairs, K, N, E);
     weights = a.part(pairs * 4);
     experts = a.part(pairs * 8);
-    total = a.part(8);
+    total = a.part(3 * 4);
     tiles = a.part(p.tiles * (int64_t)sizeof(gmlp::Q8Tile));
+    large = a.part(p.large * (int64_t)sizeof(gmlp::Q8Tile));
     row_of = a.part(pairs * 4);
     token_of = a.part(p.rows * 4);
     x = a.part(p.rows * gmlp::q8_padded(K));
@@ -1968,6 +1975,7 @@ int gmlp_q8_linear_fwd(const void* x, const void* codes, const float* scales, co
     typedef decltype(tag) T;
     gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), M, C, R);
     p.w[0] = (const int8_t*)codes; p.sw[0] = scales; p.bias[0] = bias; p.out = y;
+    p.most_rows = (int)M;
     if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, (const T*)x, (int)R, 1, nullptr, s);
     if (hipError_t e = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, M, R, nullptr, nullptr, s))
       return e;
@@ -2007,6 +2015,7 @@ int gmlp_q8_mlp_fwd(const void* x, const void* codes_gate, const float* scales_g
     float* const partial = (float*)(base + ws.partial);
     // a product of rows [M][cols]; `at`, `scales`: where they become integers if that takes a launch of its own
     auto product = [&](gmlp::Q8Product& p, const T* rows, int64_t cols, size_t at, size_t scales, int sets) -> hipError_t {
+      p.most_rows = (int)M;
       if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
       if (hipError_t e = gmlp::launch_q8_rows<T>(rows, (int8_t*)(base + at), (float*)(base + scales), 1, M, cols, nullptr, nullptr, s)) return e;
       return run_q8_dense<T>(p, sets, partial, s);
@@ -2063,43 +2072,49 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
       gmlp::Q8Product p = q8_product(nullptr, nullptr, 1, N, K);
       p.w[0] = (const int8_t*)codes_gate; p.sw[0] = scales_gate;
       p.w[1] = (const int8_t*)codes_up; p.sw[1] = scales_up;
-      p.out = base + ws.h; p.act = act;
+      p.out = base + ws.h; p.act = act; p.most_rows = 1;
       if (hipError_t err = gmlp::launch_q8_few_rows<T>(p, (const T*)x, (int)K, 2, &solo, s)) return err;
       return gmlp::launch_q8_solo_down<T>(solo, (const T*)(base + ws.h), (const int8_t*)codes_down, scales_down, (T*)y, (int)K, (int)N, s);
     }));
-  const gmlp::Q8Plan routed = {(int*)(base + ws.total), (gmlp::Q8Tile*)(base + ws.tiles), (int*)(base + ws.row_of), (int*)(base + ws.token_of)};
-  hipError_t e = by_dtype(logits_dtype, [&](auto tag) {
+  const gmlp::Q8Plan routed = {(int*)(base + ws.total), (gmlp::Q8Tile*)(base + ws.tiles), plan.gemm ? (gmlp::Q8Tile*)(base + ws.large) : nullptr,
+                               (int*)(base + ws.row_of), (int*)(base + ws.token_of)};
+  const hipError_t e = by_dtype(logits_dtype, [&](auto tag) {
     typedef decltype(tag) L;
-    return gmlp::launch_route<L>((const L*)logits, weights, experts, M, (int)E, (int)top_k, normalize, s);
+    if (M <= gmlp::Q8_ROUTE_ROWS)
+      return gmlp::launch_q8_route_plan<L>((const L*)logits, weights, routed, (int)M, (int)E, (int)top_k, normalize, plan.cap, s);
+    if (hipError_t err = gmlp::launch_route<L>((const L*)logits, weights, experts, M, (int)E, (int)top_k, normalize, s)) return err;
+    return gmlp::launch_q8_plan(experts, weights, routed, (int)M, (int)E, (int)top_k, plan.cap, s);
   });
-  if (e == hipSuccess) e = gmlp::launch_q8_plan(experts, weights, routed, (int)M, (int)E, (int)top_k, plan.cap, s);
   if (e != hipSuccess) return hip_result(__func__, e);
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
-    auto product = [&](gmlp::Q8Product& p, int sets) {
+    // a product of the plan's rows, [..][cols] or (token_of) those tokens'; `at`, `scales`: where they become integers if that takes a
+    // launch of its own.  (An expert has no more rows than there are tokens.)
+    auto product = [&](gmlp::Q8Product& p, const T* rows, int64_t cols, const int* token_of, size_t at, size_t scales, int sets) -> hipError_t {
       p.tiles = routed.tiles; p.total = routed.total; p.most_tiles = (int)plan.tiles;
+      p.token_of = token_of;
+      p.most_rows = (int)M;
+      if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
+      if (hipError_t err = gmlp::launch_q8_rows<T>(rows, (int8_t*)(base + at), (float*)(base + scales), 1, plan.rows, cols, token_of,
+                                                   routed.total + 1, s))
+        return err;
       if (!plan.gemm) return gmlp::launch_q8_few<T>(p, sets, plan.cap / 16, s);
       p.tile_class = plan.tile_class[sets == 2 ? 0 : 1];
+      if (p.tile_class == gmlp::TILE_LARGE) p.tiles = routed.large, p.total = routed.total + 2, p.most_tiles = (int)plan.large;
       p.cols = p.N;
       p.group_m = 8;
       return gmlp::launch_q8_gemm<T>(p, sets, s);
     };
     T* const h = (T*)(base + ws.h);
     float* const parts = (float*)(base + ws.parts);
-    if (hipError_t err = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, plan.rows, K,
-                                                 routed.token_of, routed.total + 1, s))
-      return err;
     gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), plan.rows, N, K);
     p.w[0] = (const int8_t*)codes_gate; p.sw[0] = scales_gate;
     p.w[1] = (const int8_t*)codes_up; p.sw[1] = scales_up;
     p.out = h; p.act = act;
-    if (hipError_t err = product(p, 2)) return err;
-    if (hipError_t err = gmlp::launch_q8_rows<T>(h, (int8_t*)(base + ws.q), (float*)(base + ws.sq), 1, plan.rows, N, nullptr,
-                                                 routed.total + 1, s))
-      return err;
+    if (hipError_t err = product(p, (const T*)x, K, routed.token_of, ws.x, ws.sx, 2)) return err;
     p = q8_product((const int8_t*)(base + ws.q), (const float*)(base + ws.sq), plan.rows, K, N);
     p.w[0] = (const int8_t*)codes_down; p.sw[0] = scales_down; p.out = parts; p.out_f32 = 1;
-    if (hipError_t err = product(p, 1)) return err;
+    if (hipError_t err = product(p, h, N, nullptr, ws.q, ws.sq, 1)) return err;
     return gmlp::launch_q8_combine<T>(parts, weights, routed.row_of, (T*)y, M, K, (int)top_k, s);
   }));
 }

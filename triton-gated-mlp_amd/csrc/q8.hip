@@ -192,29 +192,31 @@ hipError_t launch_q8_dequantize(const int8_t* codes, const float* scales, T* w, 
 constexpr int Q8_OWN_ROWS = 4;
 struct Q8Few {
   Q8Product p;
-  const void* rows;  // Q: [M][cols]
+  const void* rows;  // Q: [rows][cols], those of a plan's tile in its order or (token_of) as tokens
+  const int* token_of;
   int cols;
   int strips;        // workgroups side by side, R tiles of weight rows each
   Q8Solo solo;       // Q and solo.logits: the only token of an expert layer
 };
 
 // `count` rows [cols] as integers in LDS, [count][padded], by NT threads, 16 numbers of a row at a time; a thread's first AHEAD
-// pieces are loaded by read_ahead, for the caller to have other loads behind them.
+// pieces are loaded by read_ahead, for the caller to have other loads behind them.  from (nullable): which of `rows` they are.
 template <typename T, int NT, int AHEAD>
 struct Q8RowsToLds {
   u32x4 ahead[AHEAD][2];
-  __device__ __forceinline__ void read(u32x4 (&v)[2], const T* rows, int cols, int padded, int count, int i) {
+  __device__ __forceinline__ void read(u32x4 (&v)[2], const T* rows, int cols, int padded, int count, int i, const int* from) {
     const int pieces = padded / 16, row = i / pieces, c = (i - row * pieces) * 16;
+    const int64_t at = from != nullptr && row < count ? from[row] : row;
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      v[h] = row < count && c + 8 * h < cols ? *(const u32x4*)(rows + (int64_t)row * cols + c + 8 * h) : u32x4{0, 0, 0, 0};
+      v[h] = row < count && c + 8 * h < cols ? *(const u32x4*)(rows + at * cols + c + 8 * h) : u32x4{0, 0, 0, 0};
   }
-  __device__ __forceinline__ void read_ahead(const T* rows, int cols, int padded, int count) {
+  __device__ __forceinline__ void read_ahead(const T* rows, int cols, int padded, int count, const int* from) {
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) read(ahead[i], rows, cols, padded, count, threadIdx.x + i * NT);
+    for (int i = 0; i < AHEAD; ++i) read(ahead[i], rows, cols, padded, count, threadIdx.x + i * NT, from);
   }
   // most[count], zeros on entry and behind a barrier: the rows' largest magnitudes (max_bits); `to` is there behind the next barrier
-  __device__ __forceinline__ void finish(const T* rows, int cols, int padded, int count, uint32_t* most, char* to) {
+  __device__ __forceinline__ void finish(const T* rows, int cols, int padded, int count, const int* from, uint32_t* most, char* to) {
     const int pieces = padded / 16, all = pieces * count;
     auto look = [&](const u32x4 (&v)[2], int i) __attribute__((always_inline)) {
       uint32_t m = 0;
@@ -237,7 +239,7 @@ struct Q8RowsToLds {
     for (int i = 0; i < AHEAD; ++i)
       if ((int)((threadIdx.x & ~63u) + i * NT) < all) look(ahead[i], threadIdx.x + i * NT);
     for (int i = threadIdx.x + AHEAD * NT; (int)((unsigned)i & ~63u) < all; i += NT) {
-      read(v, rows, cols, padded, count, i);
+      read(v, rows, cols, padded, count, i, from);
       look(v, i);
     }
     __syncthreads();
@@ -247,7 +249,7 @@ struct Q8RowsToLds {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) write(ahead[i], threadIdx.x + i * NT);
     for (int i = threadIdx.x + AHEAD * NT; i < all; i += NT) {
-      read(v, rows, cols, padded, count, i);
+      read(v, rows, cols, padded, count, i, from);
       write(v, i);
     }
   }
@@ -339,15 +341,17 @@ __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
         for (int m = 0; m < MT; ++m) acc[r * MT + m][b] = Traits<I8Pair>::mfma16(t.w[b][r], x[m], acc[r * MT + m][b]);
   };
   Q8RowsToLds<T, NW * 64, 2> rows;
+  const T* const own_from = (const T*)a.rows + (a.token_of == nullptr ? (int64_t)row * a.cols : 0);
+  const int* const own_tokens = a.token_of != nullptr ? a.token_of + row : nullptr;
   if constexpr (Q) {
-    rows.read_ahead((const T*)a.rows, a.cols, p.K, count);
+    rows.read_ahead(own_from, a.cols, p.K, count, own_tokens);
     if (threadIdx.x < Q8_OWN_ROWS) own_most[threadIdx.x] = 0;
   }
 #pragma unroll
   for (int d = 0; d < D; ++d) load(st[d], d);
   if constexpr (Q) {
     __syncthreads();
-    rows.finish((const T*)a.rows, a.cols, p.K, count, own_most, own_rows);
+    rows.finish(own_from, a.cols, p.K, count, own_tokens, own_most, own_rows);
     __syncthreads();
   }
   for (int i = 0; i < run; i += D)
@@ -400,10 +404,10 @@ __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
 
 template <typename T, int SETS, int R, int MT, int NW, int D, bool F32, bool Q>
 hipError_t run_q8_few(const Q8Product& p, const void* rows, int cols, const Q8Solo* solo, hipStream_t s) {
-  Q8Few a = {p, rows, cols, ((p.N + 15) / 16 + R - 1) / R, solo != nullptr ? *solo : Q8Solo{}};
+  Q8Few a = {p, rows, p.token_of, cols, ((p.N + 15) / 16 + R - 1) / R, solo != nullptr ? *solo : Q8Solo{}};
   const dim3 grid((unsigned)(a.strips * (solo != nullptr ? solo->top_k : p.tiles != nullptr ? p.most_tiles : 1))), block(NW * 64);
   constexpr auto kern = q8_few_kernel<T, SETS, R, MT, NW, D, F32, Q>;
-  const size_t lds = Q ? (size_t)p.M * p.K : 0;
+  const size_t lds = Q ? (size_t)p.most_rows * p.K : 0;
   hipLaunchKernelGGL(kern, grid, block, lds, s, a);
   return hipGetLastError();
 }
@@ -419,7 +423,7 @@ hipError_t run_q8_few(const Q8Product& p, const void* rows, int cols, const Q8So
 // on, two of gate and up.  128 rows, 14336 x 4096 (4, 4, 2) 21.5, (2, 4, 2) 25.0, (1, 4, 2) 40; gate and up of it (2, 4, 1) 34.7,
 // (2, 4, 2) 38.7, (1, 4, 2) 48.7; 5632 x 2048 (2, 4, 2) 13.0, (2, 4, 1) 14.0, (1, 4, 1) 14.7; 4096 x 14336 (1, 4, 2) 32.7, (2, 4, 2) 38.1.
 // 64 rows, 14336 x 4096 (4, 4, 2) 15.9, (1, 4, 1) 26.3; 4096 x 14336 (1, 4, 2) 21.9, (2, 8, 1) 25.9; 32 rows, 14336 x 4096 (2, 4, 2) 13.2,
-// (1, 8, 2) 18.0.
+// (1, 8, 2) 18.0; 4096 x 14336 (1, 8, 2) 15.3, (1, 4, 2) 18.7.
 template <typename T, int SETS, int R, int MT, bool F32, bool Q>
 hipError_t q8_few_depth(const Q8Product& p, const void* rows, int cols, const Q8Solo* solo, int entries, hipStream_t s) {
   const int steps = p.K / 64;
@@ -427,6 +431,8 @@ hipError_t q8_few_depth(const Q8Product& p, const void* rows, int cols, const Q8
   if constexpr (MT == 1) {
     if (steps >= 128 || (steps >= 32 && wgs <= 2 * p.cus)) return run_q8_few<T, SETS, R, MT, 8, 4, F32, Q>(p, rows, cols, solo, s);
     if (steps >= 32) return run_q8_few<T, SETS, R, MT, 4, 4, F32, Q>(p, rows, cols, solo, s);
+  } else if constexpr (MT == 2 && R == 1) {
+    if (steps >= 128) return run_q8_few<T, SETS, R, MT, 8, 2, F32, Q>(p, rows, cols, solo, s);
   } else if constexpr (MT == 8 && SETS == 2 && R == 2) {
     if (wgs > p.cus) return run_q8_few<T, SETS, R, MT, 4, 1, F32, Q>(p, rows, cols, solo, s);
   }
@@ -459,6 +465,7 @@ bool q8_own_rows(int64_t M, int64_t padded) { return M <= Q8_OWN_ROWS && M * pad
 template <typename T>
 hipError_t launch_q8_few_rows(const Q8Product& p, const T* rows, int cols, int sets, const Q8Solo* solo, hipStream_t s) {
   if (sets == 2) return q8_few_tiles<T, 2, 1, false, true>(p, rows, cols, solo, s);
+  if (p.out_f32) return q8_few_tiles<T, 1, 1, true, true>(p, rows, cols, solo, s);
   return q8_few_tiles<T, 1, 1, false, true>(p, rows, cols, solo, s);
 }
 
@@ -482,7 +489,7 @@ __global__ void __launch_bounds__(NW * 64) q8_solo_down_kernel(Q8SoloDown a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), top_k = a.solo.top_k;
   const int r16 = lane & 15, kg = lane >> 4, tile = (int)blockIdx.x;
   Q8RowsToLds<T, NW * 64, 4> rows;
-  rows.read_ahead((const T*)a.h, a.cols, a.K, top_k);  // (rows of choices that are not run are whatever memory holds)
+  rows.read_ahead((const T*)a.h, a.cols, a.K, top_k, nullptr);  // (rows of choices that are not run are whatever memory holds)
   if (threadIdx.x < 16) most[threadIdx.x] = 0;
   const int each = NW / top_k, choice = wave / each, me = wave - choice * each;  // NW >= top_k
   int expert = choice < top_k ? a.solo.experts[choice] : -1;
@@ -498,7 +505,7 @@ __global__ void __launch_bounds__(NW * 64) q8_solo_down_kernel(Q8SoloDown a) {
 #pragma unroll
   for (int d = 0; d < D; ++d) load(st[d], d);
   __syncthreads();
-  rows.finish((const T*)a.h, a.cols, a.K, top_k, most, integers);
+  rows.finish((const T*)a.h, a.cols, a.K, top_k, nullptr, most, integers);
   __syncthreads();
   i32x4 acc = {0, 0, 0, 0};
   const char* const mine = integers + (choice < top_k ? choice : 0) * a.K + kg * 16;
@@ -546,55 +553,141 @@ hipError_t launch_q8_solo_down(const Q8Solo& solo, const T* h, const int8_t* w, 
 }
 
 // ------------------------------------------------------------------ routed choices
-// One workgroup: choices of each expert are counted, experts laid out one behind the other from multiples of 16 rows on, and
-// every choice takes the next row of its expert.  (Which of an expert's rows it gets is up to the order of arrival; a row's
-// results do not depend on its place.)
-__global__ void __launch_bounds__(1024) q8_plan_kernel(const int64_t* experts, const float* weights, Q8Plan plan, int pairs, int E, int top_k,
-                                                       int cap, int most_rows) {
-  __shared__ int count[1024], next[1024], in_wave[2][16];
+// One workgroup: choices of each expert are counted, which gives each its place among its expert's, and experts laid out one behind
+// the other from multiples of 16 rows on.  (Which place is up to the order of arrival; a row's results do not depend on it.)  Bound
+// by the loads' latency, of which a thread has eight choices in flight, and by the additions in LDS: 16384 choices of 64 experts
+// 26 us with a choice at a time and a second addition for its place.
+struct Q8Choices {
+  int* count;  // [1024], zeros; then where an expert's rows begin
+  int (*in_wave)[16];
+};
+__device__ __forceinline__ void q8_lay_out(const Q8Choices& sh, const Q8Plan& plan, int E, int cap) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  count[tid] = 0;
-  for (int i = tid; i < most_rows; i += 1024) plan.token_of[i] = -1;
-  __syncthreads();
-  for (int i = tid; i < pairs; i += 1024)
-    if (weights[i] != 0.f) atomicAdd(&count[(int)experts[i]], 1);
-  __syncthreads();
-  // rows and tiles of the experts before this thread's
-  const int mine = tid < E ? count[tid] : 0;
-  const int rows = (mine + 15) / 16 * 16, tiles = (mine + cap - 1) / cap;
-  int upto[2] = {rows, tiles};
+  // rows and tiles (of each kind) of the experts before this thread's
+  const int mine = tid < E ? sh.count[tid] : 0;
+  const int per[3] = {(mine + 15) / 16 * 16, (mine + cap - 1) / cap, (mine + 255) / 256};
+  int upto[3] = {per[0], per[1], per[2]};
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1)
 #pragma unroll
-    for (int k = 0; k < 2; ++k) {
+    for (int k = 0; k < 3; ++k) {
       const int o = __shfl_up(upto[k], d);
       if (lane >= d) upto[k] += o;
     }
-  if (lane == 63) in_wave[0][wave] = upto[0], in_wave[1][wave] = upto[1];
+  if (lane == 63)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) sh.in_wave[k][wave] = upto[k];
   __syncthreads();
-  int before[2] = {upto[0] - rows, upto[1] - tiles}, total[2] = {0, 0};
+  int before[3], total[3] = {0, 0, 0};
+#pragma unroll
+  for (int k = 0; k < 3; ++k) before[k] = upto[k] - per[k];
   for (int w = 0; w < 16; ++w)
-    for (int k = 0; k < 2; ++k) {
-      if (w < wave) before[k] += in_wave[k][w];
-      total[k] += in_wave[k][w];
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (w < wave) before[k] += sh.in_wave[k][w];
+      total[k] += sh.in_wave[k][w];
     }
-  next[tid] = before[0];
-  for (int q = 0; q < tiles; ++q)
+  sh.count[tid] = before[0];
+  for (int q = 0; q < per[1]; ++q)
     plan.tiles[before[1] + q] = Q8Tile{tid, before[0] + q * cap, mine - q * cap < cap ? mine - q * cap : cap, 0};
-  if (tid == 0) plan.total[0] = total[1], plan.total[1] = total[0];
+  if (plan.large != nullptr)
+    for (int q = 0; q < per[2]; ++q)
+      plan.large[before[2] + q] = Q8Tile{tid, before[0] + q * 256, mine - q * 256 < 256 ? mine - q * 256 : 256, 0};
+  if (tid == 0) plan.total[0] = total[1], plan.total[1] = total[0], plan.total[2] = total[2];
   __syncthreads();
-  for (int i = tid; i < pairs; i += 1024) {
-    int row = -1;
-    if (weights[i] != 0.f) {
-      row = atomicAdd(&next[(int)experts[i]], 1);
-      plan.token_of[row] = i / top_k;
+}
+__global__ void __launch_bounds__(1024) q8_plan_kernel(const int64_t* experts, const float* weights, Q8Plan plan, int pairs, int E, int top_k,
+                                                       int cap, int most_rows) {
+  __shared__ int count[1024], in_wave[3][16];
+  constexpr int PER = 8;
+  const int tid = threadIdx.x;
+  const Q8Choices sh = {count, in_wave};
+  count[tid] = 0;
+  for (int i = tid; i < most_rows; i += 1024) plan.token_of[i] = -1;
+  __syncthreads();
+  int expert[PER], place[PER];
+  // (a second pass over more choices than a thread keeps finds their places in row_of)
+  auto pass = [&](int first, bool again) __attribute__((always_inline)) {
+    float w[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = first + k * 1024 + tid;
+      expert[k] = i < pairs ? (int)experts[i] : 0;
+      if (again) place[k] = i < pairs ? plan.row_of[i] : -1;
+      else w[k] = i < pairs ? weights[i] : 0.f;
     }
-    plan.row_of[i] = row;
+    if (!again)
+#pragma unroll
+      for (int k = 0; k < PER; ++k) place[k] = w[k] != 0.f ? atomicAdd(&count[expert[k]], 1) : -1;
+  };
+  for (int first = 0; first < pairs; first += PER * 1024) {
+    pass(first, false);
+    if (pairs > PER * 1024)
+#pragma unroll
+      for (int k = 0; k < PER; ++k)
+        if (first + k * 1024 + tid < pairs) plan.row_of[first + k * 1024 + tid] = place[k];
+  }
+  __syncthreads();
+  q8_lay_out(sh, plan, E, cap);
+  for (int first = 0; first < pairs; first += PER * 1024) {
+    if (pairs > PER * 1024) pass(first, true);
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int i = first + k * 1024 + tid;
+      if (i >= pairs) continue;
+      const int row = place[k] >= 0 ? count[expert[k]] + place[k] : -1;
+      plan.row_of[i] = row;
+      if (row >= 0) plan.token_of[row] = i / top_k;
+    }
   }
 }
 hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8Plan& plan, int M, int E, int top_k, int cap, hipStream_t s) {
   hipLaunchKernelGGL(q8_plan_kernel, dim3(1), dim3(1024), 0, s, experts, weights, plan, M * top_k, E, top_k, cap,
                      (int)q8_plan_rows((int64_t)M * top_k, E));
+  return hipGetLastError();
+}
+
+// Routing and plan of a few tokens in one launch: a wavefront chooses for one token after the other.
+template <int VPL, typename L>
+__global__ void __launch_bounds__(1024) q8_route_plan_kernel(const L* logits, float* weights, Q8Plan plan, int M, int E, int top_k, int normalize,
+                                                             int cap, int most_rows) {
+  __shared__ int count[1024], in_wave[3][16];
+  __shared__ short chosen[Q8_ROUTE_ROWS * 16];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const Q8Choices sh = {count, in_wave};
+  count[tid] = 0;
+  for (int i = tid; i < most_rows; i += 1024) plan.token_of[i] = -1;
+  __syncthreads();
+  for (int t = tid >> 6; t < M; t += 16) {
+    int e;
+    float w;
+    choose<VPL>([&](int i) { return (float)logits[(int64_t)t * E + i]; }, E, top_k, normalize != 0, lane, e, w);
+    if (lane < top_k) {
+      if (w == 0.f || e < 0) e = -1;
+      weights[t * top_k + lane] = w;
+      chosen[t * top_k + lane] = (short)e;
+      if (e >= 0) atomicAdd(&count[e], 1);
+    }
+  }
+  __syncthreads();
+  q8_lay_out(sh, plan, E, cap);
+  for (int i = tid; i < M * top_k; i += 1024) {
+    const int row = chosen[i] >= 0 ? atomicAdd(&count[chosen[i]], 1) : -1;
+    plan.row_of[i] = row;
+    if (row >= 0) plan.token_of[row] = i / top_k;
+  }
+}
+template <typename L>
+hipError_t launch_q8_route_plan(const L* logits, float* weights, const Q8Plan& plan, int M, int E, int top_k, int normalize, int cap,
+                                hipStream_t s) {
+#define CALL(V)                                                                                                          \
+  hipLaunchKernelGGL((q8_route_plan_kernel<V, L>), dim3(1), dim3(1024), 0, s, logits, weights, plan, M, E, top_k, normalize, cap, \
+                     (int)q8_plan_rows((int64_t)M * top_k, E))
+  if (E <= 64) CALL(1);
+  else if (E <= 128) CALL(2);
+  else if (E <= 256) CALL(4);
+  else CALL(8);
+#undef CALL
   return hipGetLastError();
 }
 
@@ -640,5 +733,8 @@ hipError_t launch_q8_combine(const float* parts, const float* weights, const int
 GMLP_INSTANTIATE(f16)
 GMLP_INSTANTIATE(bf16)
 #undef GMLP_INSTANTIATE
+template hipError_t launch_q8_route_plan<f16>(const f16*, float*, const Q8Plan&, int, int, int, int, int, hipStream_t);
+template hipError_t launch_q8_route_plan<bf16>(const bf16*, float*, const Q8Plan&, int, int, int, int, int, hipStream_t);
+template hipError_t launch_q8_route_plan<float>(const float*, float*, const Q8Plan&, int, int, int, int, int, hipStream_t);
 
 }  // namespace gmlp

@@ -23,8 +23,9 @@ struct Q8Tile {
 // The choices of a call in the order of their experts; device pointers into the caller's workspace.  An expert's rows begin at a
 // multiple of 16.
 struct Q8Plan {
-  int* total;        // [2] tiles in `tiles`, rows with those left empty between experts
+  int* total;        // [3] tiles in `tiles`, rows with those left empty between experts, tiles in `large`
   Q8Tile* tiles;     // in ascending order of expert and row
+  Q8Tile* large;     // the same rows in tiles of 256 (nullable)
   int* row_of;       // [M * top_k]: row of a choice, -1 where its expert is not run
   int* token_of;     // [rows]: -1 where a row is left empty
 };
@@ -49,6 +50,8 @@ struct Q8Product {
   const Q8Tile* tiles;
   const int* total;      // how many tiles there are
   int most_tiles;        // ... at most
+  const int* token_of;   // launch_q8_few_rows: the tiles' rows are those of these tokens (nullable: their own)
+  int most_rows;         // launch_q8_few_rows: rows of a tile, at most
   int nxcd, cus;
   // GEMM only
   int tile_class, splits, rotate, group_m;
@@ -67,9 +70,9 @@ struct Q8Solo {
   int* experts;        // [top_k], < 0: not run
   float* weights;      // [top_k]
 };
-// The same of M rows [M][cols] as they are, where q8_own_rows allows it (p.x and p.sx are not used): dense, or (solo) the only token
-// through the matrices of each of its choices, out [top_k][N].
-bool q8_own_rows(int64_t M, int64_t padded);
+// The same of rows [..][cols] as they are, p.most_rows in a tile, where q8_own_rows allows it (p.x and p.sx are not used): dense, of a
+// plan's tiles, or (solo) the only token through the matrices of each of its choices, out [top_k][N].
+bool q8_own_rows(int64_t most_rows, int64_t padded);
 template <typename T>
 hipError_t launch_q8_few_rows(const Q8Product& p, const T* rows, int cols, int sets, const Q8Solo* solo, hipStream_t s);
 // y[N] = sum over the choices of weight * down(h), h [top_k][cols].  Where q8_solo says so.
@@ -90,6 +93,12 @@ hipError_t launch_q8_dequantize(const int8_t* codes, const float* scales, T* w, 
 // The plan of routed choices; cap: rows of a tile.  A choice of weight 0 is not run.
 hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8Plan& plan, int M, int E, int top_k, int cap, hipStream_t s);
 // y[t] = sum over the choices of weight * parts[row]
+// Routing and plan of up to Q8_ROUTE_ROWS tokens from the logits on.  (2 of 64 experts for 64 tokens: 11.4 us, in two launches 4.7 and
+// 4.7; for 16 tokens 4.5.)
+constexpr int Q8_ROUTE_ROWS = 32;
+template <typename L>
+hipError_t launch_q8_route_plan(const L* logits, float* weights, const Q8Plan& plan, int M, int E, int top_k, int normalize, int cap,
+                                hipStream_t s);
 template <typename T>
 hipError_t launch_q8_combine(const float* parts, const float* weights, const int* row_of, T* y, int64_t M, int64_t K, int top_k,
                              hipStream_t s);
