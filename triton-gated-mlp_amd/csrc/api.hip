@@ -1976,7 +1976,7 @@ int gmlp_q8_linear_fwd(const void* x, const void* codes, const float* scales, co
     gmlp::Q8Product p = q8_product((const int8_t*)(base + ws.x), (const float*)(base + ws.sx), M, C, R);
     p.w[0] = (const int8_t*)codes; p.sw[0] = scales; p.bias[0] = bias; p.out = y;
     p.most_rows = (int)M;
-    if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, (const T*)x, (int)R, 1, nullptr, s);
+    if (gmlp::q8_own_rows(M, p.K, p.N, p.cus)) return gmlp::launch_q8_few_rows<T>(p, (const T*)x, (int)R, 1, nullptr, s);
     if (hipError_t e = gmlp::launch_q8_rows<T>((const T*)x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), 1, M, R, nullptr, nullptr, s))
       return e;
     return run_q8_dense<T>(p, 1, (float*)(base + ws.partial), s);
@@ -2016,7 +2016,7 @@ int gmlp_q8_mlp_fwd(const void* x, const void* codes_gate, const float* scales_g
     // a product of rows [M][cols]; `at`, `scales`: where they become integers if that takes a launch of its own
     auto product = [&](gmlp::Q8Product& p, const T* rows, int64_t cols, size_t at, size_t scales, int sets) -> hipError_t {
       p.most_rows = (int)M;
-      if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
+      if (gmlp::q8_own_rows(M, p.K, p.N, p.cus)) return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
       if (hipError_t e = gmlp::launch_q8_rows<T>(rows, (int8_t*)(base + at), (float*)(base + scales), 1, M, cols, nullptr, nullptr, s)) return e;
       return run_q8_dense<T>(p, sets, partial, s);
     };
@@ -2089,12 +2089,13 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
     // a product of the plan's rows, [..][cols] or (token_of) those tokens'; `at`, `scales`: where they become integers if that takes a
-    // launch of its own.  (An expert has no more rows than there are tokens.)
+    // launch of its own: from 4 rows an expert on.  (An expert has no more rows than there are tokens, and a tile no more than its own.)
     auto product = [&](gmlp::Q8Product& p, const T* rows, int64_t cols, const int* token_of, size_t at, size_t scales, int sets) -> hipError_t {
       p.tiles = routed.tiles; p.total = routed.total; p.most_tiles = (int)plan.tiles;
       p.token_of = token_of;
-      p.most_rows = (int)M;
-      if (gmlp::q8_own_rows(M, p.K)) return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
+      p.most_rows = (int)std::min<int64_t>(M, plan.cap);
+      if (M * top_k <= 4 * E && gmlp::q8_own_rows(p.most_rows, p.K, 0, p.cus))
+        return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
       if (hipError_t err = gmlp::launch_q8_rows<T>(rows, (int8_t*)(base + at), (float*)(base + scales), 1, plan.rows, cols, token_of,
                                                    routed.total + 1, s))
         return err;

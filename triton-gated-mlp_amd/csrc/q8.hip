@@ -186,10 +186,10 @@ hipError_t launch_q8_dequantize(const int8_t* codes, const float* scales, T* w, 
 // A workgroup: R tiles of 16 weight rows (of each matrix) and the token rows of a tile, up to 16 * MT.  Its wavefronts split the
 // reduction and add up through LDS (integers: in any order).  Bound by the weights' way from memory: a load is one KiB as it
 // lies, D of each kind in flight for a wavefront; tokens come from the caches, and past the end a load moves nothing.
-// Q: the token rows, 4 at most, come as they are and every workgroup makes integers of them for itself, in LDS, while its first
+// Q: the token rows, 16 at most, come as they are and every workgroup makes integers of them for itself, in LDS, while its first
 // weights are on their way: a launch less, and for one row no more time (one row of 4096 through two matrices of 14336 rows 20.3 us,
-// of integers 20.9; four rows of 2048 through 8192 7.9, 5.0 and 3 us of a launch).
-constexpr int Q8_OWN_ROWS = 4;
+// of integers 20.9).
+constexpr int Q8_OWN_ROWS = 16;
 struct Q8Few {
   Q8Product p;
   const void* rows;  // Q: [rows][cols], those of a plan's tile in its order or (token_of) as tokens
@@ -460,8 +460,14 @@ hipError_t launch_q8_few(const Q8Product& p, int sets, int token_tiles, hipStrea
   CALL(1, false);
 #undef CALL
 }
-// Rows of which every workgroup makes integers itself: 32 KiB of them at most.
-bool q8_own_rows(int64_t M, int64_t padded) { return M <= Q8_OWN_ROWS && M * padded <= 32768; }
+// Where every workgroup makes the integers itself.  A launch of their own takes 3 us; in every workgroup they take what it has rows
+// for: us, in the workgroups and in a launch, 4096 x 4096 of 4096, 6 rows 7.8, 8.5, 8 rows 8.7, 8.5; 14336 rows of 4096 columns 4 rows 12.6,
+// 15.0, 8 rows 15.4, 15.0; of 2048 columns 12 rows 11.6, 11.7, 16 rows 13.1, 11.8; 2048 of 2048, 16 rows 7.1, 8.6; an expert layer of 64
+// experts, 16 tokens, 8 of them each 72, 82.
+bool q8_own_rows(int64_t most_rows, int64_t padded, int64_t N, int cus) {
+  if (most_rows == 1) return padded <= 32768;
+  return most_rows <= Q8_OWN_ROWS && most_rows * padded <= (N <= 16 * cus ? 32768 : 24576);
+}
 template <typename T>
 hipError_t launch_q8_few_rows(const Q8Product& p, const T* rows, int cols, int sets, const Q8Solo* solo, hipStream_t s) {
   if (sets == 2) return q8_few_tiles<T, 2, 1, false, true>(p, rows, cols, solo, s);

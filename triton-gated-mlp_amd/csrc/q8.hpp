@@ -72,7 +72,7 @@ struct Q8Solo {
 };
 // The same of rows [..][cols] as they are, p.most_rows in a tile, where q8_own_rows allows it (p.x and p.sx are not used): dense, of a
 // plan's tiles, or (solo) the only token through the matrices of each of its choices, out [top_k][N].
-bool q8_own_rows(int64_t most_rows, int64_t padded);
+bool q8_own_rows(int64_t most_rows, int64_t padded, int64_t N, int cus);
 template <typename T>
 hipError_t launch_q8_few_rows(const Q8Product& p, const T* rows, int cols, int sets, const Q8Solo* solo, hipStream_t s);
 // y[N] = sum over the choices of weight * down(h), h [top_k][cols].  Where q8_solo says so.
