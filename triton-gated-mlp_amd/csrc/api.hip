@@ -1859,6 +1859,9 @@ struct Q8MlpWorkspace {
 
 // An expert layer: rows of a tile (the GEMM's 128, or 256 in a list of its own, the streaming kernels' 16 to 128), and of the
 // GEMM the tile classes of gate/up and down, by their estimates for as many tiles as experts with half a tile left over each have.
+// us by the rows of an expert on average, tiles of as many and of twice as many rows: 64 experts of 2048 x 1024, 10 rows (16, 32) 98, 105,
+// 21 rows (32, 64) 111, 122, 45 rows (64, 128) 133, 165, 56 rows 148, 169, 72 rows 185, 183; 8 of 4096 x 14336, 24 rows (32, 64) 254, 253, 42 rows
+// (64, 128) 277, 313, 52 rows 344, 316.  Beyond 96 rows the GEMM: 64 experts, 128 rows 190, 96 rows on the streaming kernels 196.
 struct Q8MoePlan {
   int cap;
   bool gemm;
@@ -1868,8 +1871,9 @@ struct Q8MoePlan {
 Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
   Q8MoePlan p = {};
   const int64_t each = cdiv(pairs, E);
+  // (an expert with more rows than a tile is read once for each of its tiles, small ones from the caches)
   p.gemm = each > 96;
-  p.cap = each <= 12 ? 16 : each <= 24 ? 32 : each <= 48 ? 64 : 128;
+  p.cap = each <= 12 ? 16 : each <= 24 ? 32 : each <= (K * N <= ((int64_t)1 << 23) ? 56 : 48) ? 64 : 128;
   p.rows = gmlp::q8_plan_rows(pairs, E);
   p.tiles = gmlp::q8_plan_tiles(pairs, E, p.cap);
   if (!p.gemm) return p;

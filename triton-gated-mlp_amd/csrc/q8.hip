@@ -653,26 +653,39 @@ hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8
   return hipGetLastError();
 }
 
-// Routing and plan of a few tokens in one launch: a wavefront chooses for one token after the other.
+// Routing and plan of a few tokens in one launch: 64 tokens at a time, four to a wavefront as in routing many.
 template <int VPL, typename L>
 __global__ void __launch_bounds__(1024) q8_route_plan_kernel(const L* logits, float* weights, Q8Plan plan, int M, int E, int top_k, int normalize,
                                                              int cap, int most_rows) {
   __shared__ int count[1024], in_wave[3][16];
   __shared__ short chosen[Q8_ROUTE_ROWS * 16];
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x, lane = tid & 63, l = tid & 15;
   const Q8Choices sh = {count, in_wave};
+  const bool aligned = ((uintptr_t)logits & (sizeof(L) * VPL - 1)) == 0;
   count[tid] = 0;
   for (int i = tid; i < most_rows; i += 1024) plan.token_of[i] = -1;
   __syncthreads();
-  for (int t = tid >> 6; t < M; t += 16) {
-    int e;
-    float w;
-    choose<VPL>([&](int i) { return (float)logits[(int64_t)t * E + i]; }, E, top_k, normalize != 0, lane, e, w);
-    if (lane < top_k) {
-      if (w == 0.f || e < 0) e = -1;
-      weights[t * top_k + lane] = w;
-      chosen[t * top_k + lane] = (short)e;
-      if (e >= 0) atomicAdd(&count[e], 1);
+  for (int base = 0; base < M; base += 64) {
+    const int token = base + (tid >> 4), t = token < M ? token : M - 1;
+    LogitRow<VPL, L> row;
+    row.load(logits + (int64_t)t * E, aligned, E, l);
+    row.choose(E, top_k, l);
+    const bool none = row.first == -__builtin_inff();
+    const float e = l < top_k && !none ? expf(row.own - row.first) : 0.f;
+    float all = e;
+    if (!normalize) {
+      all = 0.f;
+#pragma unroll
+      for (int v = 0; v < VPL; ++v)
+        if (l * VPL + v < E && !none) all += expf(row.value[v] - row.first);
+    }
+    all = row_sum(all, lane);
+    if (token < M && l < top_k) {
+      const float w = none ? 0.f : e / all;
+      const bool run = w != 0.f && row.own != -__builtin_inff();
+      weights[t * top_k + l] = w;
+      chosen[t * top_k + l] = (short)(run ? row.expert : -1);
+      if (run) atomicAdd(&count[row.expert], 1);
     }
   }
   __syncthreads();
@@ -689,10 +702,11 @@ hipError_t launch_q8_route_plan(const L* logits, float* weights, const Q8Plan& p
 #define CALL(V)                                                                                                          \
   hipLaunchKernelGGL((q8_route_plan_kernel<V, L>), dim3(1), dim3(1024), 0, s, logits, weights, plan, M, E, top_k, normalize, cap, \
                      (int)q8_plan_rows((int64_t)M * top_k, E))
-  if (E <= 64) CALL(1);
-  else if (E <= 128) CALL(2);
-  else if (E <= 256) CALL(4);
-  else CALL(8);
+  if (E <= 16) CALL(1);
+  else if (E <= 64) CALL(4);
+  else if (E <= 128) CALL(8);
+  else if (E <= 256) CALL(16);
+  else CALL(32);
 #undef CALL
   return hipGetLastError();
 }

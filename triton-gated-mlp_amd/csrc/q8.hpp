@@ -93,9 +93,9 @@ hipError_t launch_q8_dequantize(const int8_t* codes, const float* scales, T* w, 
 // The plan of routed choices; cap: rows of a tile.  A choice of weight 0 is not run.
 hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8Plan& plan, int M, int E, int top_k, int cap, hipStream_t s);
 // y[t] = sum over the choices of weight * parts[row]
-// Routing and plan of up to Q8_ROUTE_ROWS tokens from the logits on.  (2 of 64 experts for 64 tokens: 11.4 us, in two launches 4.7 and
-// 4.7; for 16 tokens 4.5.)
-constexpr int Q8_ROUTE_ROWS = 32;
+// Routing and plan of up to Q8_ROUTE_ROWS tokens from the logits on.  (8 of 64 experts, 64 tokens: 7.0 us, in two launches 4.7 and 4.7; for
+// 256 tokens 15.8, 5 and 6.)
+constexpr int Q8_ROUTE_ROWS = 128;
 template <typename L>
 hipError_t launch_q8_route_plan(const L* logits, float* weights, const Q8Plan& plan, int M, int E, int top_k, int normalize, int cap,
                                 hipStream_t s);
