@@ -150,7 +150,8 @@ def test_refusals_of_the_c_interface():
     assert linear(C=68) == -2 and linear(R=131080) == -2 and "32 bits" in err()
     assert linear(x=a + 8) == -3 and linear(bias=a + 2) == -3 and linear(scales=a + 4) == -3
     assert linear(n=need - 1) == -1 and "workspace" in err()
-    assert linear(M=1 << 28) == -2 and "too large" in err()
+    assert linear(M=1 << 24) == -2 and "2^24" in err()
+    assert linear(M=(1 << 24) - 1, C=1 << 20) == -2 and "too large" in err()
 
     need = lib.gmlp_q8_mlp_workspace_bytes(3, 64, 64, 1)
 
@@ -178,6 +179,7 @@ def test_refusals_of_the_c_interface():
         assert call(a, a, a, 0, 16, 128, 0, None) == -2 and call(a, a, a, 1, 12, 128, 0, None) == -2
         assert call(a, a, a, 1, 16, 128, 2, None) == -2 and call(a, a, a, 1, 16, 131080, 0, None) == -2
         assert call(a, a, a, 65536, 16, 128, 0, None) == -2 and call(a, a, a, 1 << 40, 16, 128, 0, None) == -2
+        assert call(a, a, a, 1, 1 << 24, 128, 0, None) == -2 and call(a, a, a, 1, 1 << 20, 1 << 17, 0, None) == -2
         assert call(a + 8, a, a, 1, 16, 128, 0, None) == -3
 
 
@@ -252,12 +254,12 @@ def test_rows_that_are_not_finite_are_nan_and_stand_alone():
         bad[[5, 9, 17]] = True
         assert torch.equal(q.scales.cpu().isnan(), bad) and (numbers_of(q)[bad] == 0).all()
         assert torch.equal(numbers_of(q)[~bad], integers64(w[~bad])[0])
-        for M in (24, 300):
+        for M in (8, 24, 300):
             x = normal((M, 264), 1.0, dtype, gen(4))
-            x[3, 100], x[M - 2, 1], x[M - 5] = math.nan, math.inf, 0
+            x[2, 100], x[M - 2, 1], x[M - 5] = math.nan, math.inf, 0
             y = quant.q8_linear_fwd(x.to(device()), q8((40, 264), dtype, gen(5))).cpu()
             rows = torch.zeros(M, dtype=torch.bool)
-            rows[[3, M - 2]] = True
+            rows[[2, M - 2]] = True
             assert torch.equal(y.isnan().any(1), rows) and torch.equal(y.isnan().all(1), rows) and (y[M - 5] == 0).all()
 
 
@@ -268,6 +270,7 @@ def test_rows_that_are_not_finite_are_nan_and_stand_alone():
     "M,R,C,bias",
     [
         (1, 8, 8, False), (1, 128, 16, True), (1, 2048, 2048, False), (2, 1160, 3096, True), (7, 264, 72, True), (1, 20000, 40, False),
+        (1, 40000, 24, True), (2, 40000, 72, False), (16, 2048, 264, True), (12, 136, 16400, False), (3, 1160, 8200, True),
         (16, 4096, 40, False), (17, 1000, 136, False), (32, 136, 1000, True), (33, 520, 264, True), (64, 1032, 520, False),
         (65, 264, 392, True), (77, 1160, 3096, True), (130, 4096, 264, False), (300, 1160, 264, False), (515, 8200, 520, True),
         (1024, 392, 2056, True), (2100, 264, 4104, False), (257, 136, 8200, False),
@@ -369,6 +372,9 @@ def test_q8_mlp(M, K, N, bias, act, dtype):
     [
         (1, 8, 8, 1, 1, "silu", True), (1, 1160, 520, 8, 2, "silu", True), (1, 264, 136, 64, 8, "gelu", False), (3, 136, 264, 60, 6, "relu", True),
         (16, 520, 392, 4, 2, "silu", False), (40, 264, 136, 5, 3, "silu", True), (96, 264, 136, 64, 8, "silu", True), (70, 136, 264, 3, 1, "tanh", True),
+        (1, 264, 136, 20, 16, "silu", True), (1, 520, 264, 200, 9, "relu", False), (1, 136, 264, 300, 3, "silu", True), (1, 40008, 16, 3, 2, "silu", True),
+        (2, 136, 264, 9, 9, "silu", True), (20, 264, 136, 100, 4, "silu", False), (10, 136, 264, 200, 3, "tanh", True), (7, 264, 136, 400, 5, "silu", True),
+        (128, 136, 264, 16, 2, "silu", True), (129, 136, 264, 16, 2, "silu", False), (260, 264, 136, 1, 1, "gelu", True), (700, 136, 264, 9, 1, "silu", True),
         (300, 264, 392, 8, 2, "silu", False), (600, 136, 520, 16, 4, "gelu", True), (1500, 136, 264, 4, 2, "silu", True), (130, 264, 136, 512, 16, "silu", True),
     ],
 )
@@ -399,6 +405,78 @@ def test_q8_moe_with_masked_experts_and_crowds(M, E, k):
     assert (y[M - 1] == 0).all()
     ref, bound = moe64(x, logits, k, True, "silu", dtype, lambda e: [weight_of(sliced(q, e)) for q in w])
     hold(y, ref, bound, dtype, M * N)
+
+
+@gpu
+@pytest.mark.parametrize("E", [4, 70, 300])
+def test_the_only_token_with_masked_experts(E):
+    dtype, K, N, k = torch.float16, 136, 264, 3
+    g = gen(E)
+    x, logits = normal((1, K), 1.0, dtype, g), normal((1, E), 1.0, torch.float32, g)
+    w = [q8((E, N, K), dtype, g), q8((E, N, K), dtype, g), q8((E, K, N), dtype, g)]
+    logits[0, 2:] = -math.inf  # two experts for three choices
+    y = moe.moe_mlp_fwd(on(x), on(logits), *w, k)
+    ref, bound = moe64(x, logits, k, True, "silu", dtype, lambda e: [weight_of(sliced(q, e)) for q in w])
+    hold(y, ref, bound, dtype, N)
+    logits[:] = -math.inf
+    assert (moe.moe_mlp_fwd(on(x), on(logits), *w, k) == 0).all()
+    logits[0, 1], logits[0, 3] = 0.0, -200.0  # a weight that is 0: its expert is not run
+    w[2].scales[3] = math.nan
+    assert moe.moe_mlp_fwd(on(x), on(logits), *w, 2).isfinite().all()
+
+
+# Shapes for every kernel that the rules choose: tiles of weight rows a workgroup, wavefronts and stages of the streaming kernels for
+# each number of token tiles, and the GEMM's classes with and without split reductions and a launch for the columns that whole rounds
+# leave.  References on the GPU, in float64, whose sums of integers are exact.
+@gpu
+@pytest.mark.parametrize(
+    "M,R,C",
+    [
+        (20, 264, 8200), (20, 8200, 520), (20, 2056, 520), (40, 264, 12360), (40, 264, 8200), (40, 2056, 520), (100, 264, 12360), (100, 264, 8200),
+        (100, 2056, 520), (129, 4096, 2056), (256, 14336, 1032), (512, 2048, 5640), (1000, 1160, 9000), (2048, 2048, 8200), (3000, 520, 16392), (4100, 264, 14344),
+    ],
+)
+def test_q8_linear_on_every_kernel(M, R, C):
+    dtype = torch.bfloat16 if M % 8 else torch.float16
+    g = gen(M + C)
+    x, q = on(normal((M, R), 1.0, dtype, g)), q8((C, R), dtype, g)
+    b = on(normal((C,), 0.5, dtype, g))
+    y = quant.q8_linear_fwd(x, q, b)
+    n, s = integers64(x)
+    ref = (n @ on(numbers_of(q)).T) * s * q.scales.double()
+    ref, bound = ref + b.double(), 8 * F * (ref.abs() + b.double().abs())
+    hold(y, ref.cpu(), bound.cpu(), dtype)
+
+
+@gpu
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize(
+    "M,K,N",
+    [
+        (5, 264, 4360), (5, 8200, 72), (20, 264, 4360), (20, 520, 264), (40, 264, 4360), (40, 520, 264), (100, 264, 8712), (100, 264, 4360), (100, 520, 264),
+        (160, 4096, 264), (300, 2048, 1032), (700, 1032, 2056), (2048, 520, 4104), (2300, 264, 6152),
+    ],
+)
+def test_q8_mlp_on_every_kernel(M, K, N, act):
+    """The hidden states, read through a down projection that picks one column for each output: 127·127/127 of its integer."""
+    dtype = torch.bfloat16
+    g = gen(M + N)
+    x = on(normal((M, K), 1.0, dtype, g))
+    w = [q8((N, K), dtype, g), q8((N, K), dtype, g)]
+    at = torch.arange(K, device="cuda") % N if K > N else torch.linspace(0, N - 1, K, device="cuda").long()
+    pick = torch.zeros(K, N, dtype=dtype, device="cuda")
+    pick[torch.arange(K, device="cuda"), at] = 1
+    y = quant.q8_mlp_fwd(x, w[0], None, w[1], None, quant.quantize_q8(pick), None, act_fn=act)
+    n, s = integers64(x)
+    gate, up = ((n @ on(numbers_of(q)).T) * s * q.scales.double() for q in w)
+    a = ACT[act](gate)
+    h = a * up
+    d = (1.13 * 8 * F * gate.abs() + 2e-6 * (1 + a.abs())) * (up.abs() + 8 * F * up.abs()) + 8 * F * a.abs() * up.abs() + 2 * F * h.abs()
+    lo, hi = (h - d).to(dtype), (h + d).to(dtype)
+    top = torch.maximum(lo.abs(), hi.abs()).double().amax(1, keepdim=True)
+    # a rounding to 16 bits, half a step of the row's integers and of y's own 16 bits
+    off = (y.double() - h[:, at]).abs()
+    assert (off <= (hi.double() - lo.double()).abs()[:, at] + 2 * U[dtype] * h[:, at].abs() + 0.51 * top / 127 + SUB[dtype]).all()
 
 
 @gpu
@@ -437,7 +515,7 @@ def test_logits_of_every_type_and_a_long_batch():
 
 
 @gpu
-@pytest.mark.parametrize("rows", [3, 100])
+@pytest.mark.parametrize("rows", [1, 3, 100, 500])
 def test_operators_on_another_stream_and_in_a_graph(rows):
     dtype, K, N, E = torch.bfloat16, 264, 392, 8
     g = gen(rows)

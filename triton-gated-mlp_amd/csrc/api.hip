@@ -1756,13 +1756,25 @@ int check_q8_cols(const char* fn, const char* name, int64_t cols) {
     return fail(GMLP_ESHAPE, "%s: %s = %lld exceeds the %d columns whose sums fit 32 bits", fn, name, (long long)cols, gmlp::Q8_MAX_COLS);
   return 0;
 }
-// Launches have fewer than 2^32 threads: a workgroup of 512 per tile of weight rows and 16 token rows at most, and of 256 per
-// 16 rows of integers.
+// Launches have fewer than 2^32 threads (of more the runtime starts a part only, without an error): 1024 threads for every 4 rows
+// of integers, a workgroup of 512 for every tile of weight rows and of token rows, a thread for 8 columns of a row.
+int check_q8_rows(const char* fn, int64_t rows) {
+  if (rows >= ((int64_t)1 << 24)) return fail(GMLP_ESHAPE, "%s: %lld rows: fewer than 2^24 are taken", fn, (long long)rows);
+  return 0;
+}
 int check_q8_sizes(const char* fn, int64_t rows, int64_t K, int64_t N, int64_t tiles) {
+  if (int rc = check_q8_rows(fn, rows)) return rc;
   const int64_t most = K > N ? K : N;
-  if (cdiv(rows, 16) >= ((int64_t)1 << 24) || tiles * cdiv(most, 16) >= ((int64_t)1 << 32) / 512 ||
-      rows * cdiv(most, 8) >= ((int64_t)1 << 40))
+  if (tiles * cdiv(most, 16) >= ((int64_t)1 << 32) / 512 || rows * cdiv(most, 8) >= ((int64_t)1 << 32))
     return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
+  return 0;
+}
+int check_q8_storage(const char* fn, int64_t count, int64_t rows, int64_t cols) {
+  if (int rc = check_storage(fn, count, rows, cols)) return rc;
+  if (int rc = check_q8_cols(fn, "cols", cols)) return rc;
+  if (int rc = check_q8_rows(fn, rows)) return rc;
+  if (count > 65535 || rows * cdiv(cols, 128) * 16 >= ((int64_t)1 << 32))
+    return fail(GMLP_ESHAPE, "%s: dimension too large (%lld matrices of %lld x %lld)", fn, (long long)count, (long long)rows, (long long)cols);
   return 0;
 }
 int64_t round256(int64_t n) { return (n + 255) / 256 * 256; }
@@ -1932,9 +1944,7 @@ extern "C" {
 int gmlp_q8_quantize(const void* w, void* codes, float* scales, int64_t count, int64_t rows, int64_t cols, int dtype, void* stream) {
   GMLP_REQUIRE_PTR(w); GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales);
   if (int rc = check_q8_type(__func__, dtype)) return rc;
-  if (int rc = check_storage(__func__, count, rows, cols)) return rc;
-  if (int rc = check_q8_cols(__func__, "cols", cols)) return rc;
-  if (count > 65535) return fail(GMLP_ESHAPE, "%s: count = %lld exceeds 65535", __func__, (long long)count);
+  if (int rc = check_q8_storage(__func__, count, rows, cols)) return rc;
   GMLP_REQUIRE_ALIGNED(w); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales);
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
@@ -1946,9 +1956,7 @@ int gmlp_q8_dequantize(const void* codes, const float* scales, void* w, int64_t 
                        void* stream) {
   GMLP_REQUIRE_PTR(codes); GMLP_REQUIRE_PTR(scales); GMLP_REQUIRE_PTR(w);
   if (int rc = check_q8_type(__func__, dtype)) return rc;
-  if (int rc = check_storage(__func__, count, rows, cols)) return rc;
-  if (int rc = check_q8_cols(__func__, "cols", cols)) return rc;
-  if (count > 65535) return fail(GMLP_ESHAPE, "%s: count = %lld exceeds 65535", __func__, (long long)count);
+  if (int rc = check_q8_storage(__func__, count, rows, cols)) return rc;
   GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(w);
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
