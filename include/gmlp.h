@@ -411,13 +411,13 @@ int gmlp_moe_balance_bwd(const void* logits, const uint8_t* mask, const float* w
  * columns: codes int8 [tiles][blocks][2 s][4 q][16 r][16]: columns 64 s + 16 q + 0..15 of the block, row r of the tile;
  * scales float [rows].  Several matrices of one size (experts) follow each other.
  *
- * gmlp_q8_quantize, gmlp_q8_dequantize (w = scale·n rounded to dtype): `count` matrices (at most 65535, of fewer than 2^24 rows).
+ * gmlp_q8_quantize, gmlp_q8_dequantize (w = scale·n rounded to dtype): `count` matrices (at most 65535, of at most 2^23 rows).
  * gmlp_q8_linear_fwd: y[M,C] = x[M,R]·Wᵀ + bias, W [C,R]; bias may be NULL.
  * gmlp_q8_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) rounded to dtype (in fp16 one past 65504 is infinite, and the
  *   token's outputs NaN), y = h·W_downᵀ + b_down, h in 8 bits again.
  * gmlp_q8_moe_fwd: y[m] = sum over m's experts e of weight·MLP_e(x[m]), routed as gmlp_moe_route does, the sum over experts in
  *   fp32; experts without tokens are not read, and a choice of weight 0 is not run.  M * top_k <= GMLP_Q8_MOE_MAX_PAIRS.
- * M < 2^24 in each.  workspace: as many bytes as the function beside each says.
+ * M is at most 2^23 in each.  workspace: as many bytes as the function beside each says.
  */
 #define GMLP_Q8_MOE_MAX_PAIRS 65536
 int gmlp_q8_quantize(const void* w, void* codes, float* scales, int64_t count, int64_t rows, int64_t cols, int dtype, void* stream);

@@ -38,10 +38,10 @@ def integers64(v):
     return n, (top.float() / 127.0).double()
 
 
-def numbers_of(q):
+def numbers_of(q, where="cpu"):
     """The integers of a single Q8Weight as float64 [rows, cols], looked up one place at a time."""
-    flat, blocks = q.codes.cpu().reshape(-1), q.codes.shape[-5]
-    r, c = torch.arange(q.rows).unsqueeze(1), torch.arange(q.cols).unsqueeze(0)
+    flat, blocks = q.codes.to(where).reshape(-1), q.codes.shape[-5]
+    r, c = torch.arange(q.rows, device=where).unsqueeze(1), torch.arange(q.cols, device=where).unsqueeze(0)
     at = ((r // 16) * blocks + c // 128) * 2048 + (c % 128 // 64) * 1024 + (c % 64 // 16) * 256 + (r % 16) * 16 + c % 16
     return flat[at].double()
 
@@ -150,8 +150,8 @@ def test_refusals_of_the_c_interface():
     assert linear(C=68) == -2 and linear(R=131080) == -2 and "32 bits" in err()
     assert linear(x=a + 8) == -3 and linear(bias=a + 2) == -3 and linear(scales=a + 4) == -3
     assert linear(n=need - 1) == -1 and "workspace" in err()
-    assert linear(M=1 << 24) == -2 and "2^24" in err()
-    assert linear(M=(1 << 24) - 1, C=1 << 20) == -2 and "too large" in err()
+    assert linear(M=(1 << 23) + 1) == -2 and "2^23" in err()
+    assert linear(M=1 << 23, C=1 << 20) == -2 and "too large" in err()
 
     need = lib.gmlp_q8_mlp_workspace_bytes(3, 64, 64, 1)
 
@@ -179,7 +179,7 @@ def test_refusals_of_the_c_interface():
         assert call(a, a, a, 0, 16, 128, 0, None) == -2 and call(a, a, a, 1, 12, 128, 0, None) == -2
         assert call(a, a, a, 1, 16, 128, 2, None) == -2 and call(a, a, a, 1, 16, 131080, 0, None) == -2
         assert call(a, a, a, 65536, 16, 128, 0, None) == -2 and call(a, a, a, 1 << 40, 16, 128, 0, None) == -2
-        assert call(a, a, a, 1, 1 << 24, 128, 0, None) == -2 and call(a, a, a, 1, 1 << 20, 1 << 17, 0, None) == -2
+        assert call(a, a, a, 1, (1 << 23) + 1, 128, 0, None) == -2 and call(a, a, a, 1, 1 << 20, 1 << 17, 0, None) == -2
         assert call(a + 8, a, a, 1, 16, 128, 0, None) == -3
 
 
@@ -426,40 +426,44 @@ def test_the_only_token_with_masked_experts(E):
 
 
 # Shapes for every kernel that the rules choose: tiles of weight rows a workgroup, wavefronts and stages of the streaming kernels for
-# each number of token tiles, and the GEMM's classes with and without split reductions and a launch for the columns that whole rounds
-# leave.  References on the GPU, in float64, whose sums of integers are exact.
+# each number of token tiles, rows made integers inside or before, and the GEMM's classes with and without split reductions and a launch
+# for the columns that whole rounds leave.  References on the GPU, in float64, whose sums of integers are exact.
 @gpu
+@pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize(
     "M,R,C",
     [
-        (20, 264, 8200), (20, 8200, 520), (20, 2056, 520), (40, 264, 12360), (40, 264, 8200), (40, 2056, 520), (100, 264, 12360), (100, 264, 8200),
-        (100, 2056, 520), (129, 4096, 2056), (256, 14336, 1032), (512, 2048, 5640), (1000, 1160, 9000), (2048, 2048, 8200), (3000, 520, 16392), (4100, 264, 14344),
+        (3, 264, 264), (3, 2056, 264), (3, 264, 8200), (3, 2056, 8200), (3, 2056, 16400), (16, 1600, 4104), (16, 1600, 8200), (16, 2056, 264),
+        (16, 2056, 8200), (16, 2056, 16400), (20, 264, 264), (20, 8200, 264), (20, 264, 8200), (40, 264, 264), (40, 264, 8200), (40, 264, 12296),
+        (100, 264, 264), (100, 264, 8200), (100, 264, 12296), (129, 264, 520), (129, 2056, 520), (129, 14344, 5640), (300, 4104, 20488),
+        (512, 2056, 20488), (1000, 2056, 16392), (2300, 4104, 10248),
     ],
 )
-def test_q8_linear_on_every_kernel(M, R, C):
-    dtype = torch.bfloat16 if M % 8 else torch.float16
+def test_q8_linear_on_every_kernel(M, R, C, dtype):
     g = gen(M + C)
     x, q = on(normal((M, R), 1.0, dtype, g)), q8((C, R), dtype, g)
     b = on(normal((C,), 0.5, dtype, g))
     y = quant.q8_linear_fwd(x, q, b)
     n, s = integers64(x)
-    ref = (n @ on(numbers_of(q)).T) * s * q.scales.double()
-    ref, bound = ref + b.double(), 8 * F * (ref.abs() + b.double().abs())
-    hold(y, ref.cpu(), bound.cpu(), dtype)
+    ref = (n @ numbers_of(q, x.device).T) * s * q.scales.double()
+    bound = 8 * F * (ref.abs() + b.double().abs())
+    hold(y, (ref + b.double()).cpu(), bound.cpu(), dtype)
 
 
 @gpu
-@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize(
-    "M,K,N",
+    "M,K,N,act",
     [
-        (5, 264, 4360), (5, 8200, 72), (20, 264, 4360), (20, 520, 264), (40, 264, 4360), (40, 520, 264), (100, 264, 8712), (100, 264, 4360), (100, 520, 264),
-        (160, 4096, 264), (300, 2048, 1032), (700, 1032, 2056), (2048, 520, 4104), (2300, 264, 6152),
+        (3, 264, 264, "silu"), (3, 2056, 8200, "silu"), (3, 8200, 264, "gelu"), (16, 1600, 4104, "silu"), (16, 2056, 8200, "silu"), (16, 8200, 264, "gelu"),
+        (20, 264, 264, "silu"), (20, 8200, 264, "silu"), (20, 264, 4104, "gelu"), (40, 264, 264, "silu"), (40, 264, 4104, "silu"), (100, 264, 264, "silu"),
+        (100, 264, 4104, "silu"), (100, 264, 8200, "gelu"), (129, 264, 520, "silu"), (129, 264, 520, "gelu"), (200, 2056, 520, "silu"),
+        (200, 2056, 520, "gelu"), (300, 14344, 2056, "silu"), (300, 14344, 2056, "tanh"), (129, 4104, 14344, "silu"), (129, 4104, 14344, "gelu"),
+        (129, 2056, 20488, "silu"), (129, 2056, 20488, "relu"), (512, 2056, 16392, "silu"), (512, 2056, 16392, "gelu"), (2048, 8200, 5640, "silu"),
     ],
 )
-def test_q8_mlp_on_every_kernel(M, K, N, act):
+def test_q8_mlp_on_every_kernel(M, K, N, act, dtype):
     """The hidden states, read through a down projection that picks one column for each output: 127·127/127 of its integer."""
-    dtype = torch.bfloat16
     g = gen(M + N)
     x = on(normal((M, K), 1.0, dtype, g))
     w = [q8((N, K), dtype, g), q8((N, K), dtype, g)]
@@ -468,7 +472,7 @@ def test_q8_mlp_on_every_kernel(M, K, N, act):
     pick[torch.arange(K, device="cuda"), at] = 1
     y = quant.q8_mlp_fwd(x, w[0], None, w[1], None, quant.quantize_q8(pick), None, act_fn=act)
     n, s = integers64(x)
-    gate, up = ((n @ on(numbers_of(q)).T) * s * q.scales.double() for q in w)
+    gate, up = ((n @ numbers_of(q, x.device).T) * s * q.scales.double() for q in w)
     a = ACT[act](gate)
     h = a * up
     d = (1.13 * 8 * F * gate.abs() + 2e-6 * (1 + a.abs())) * (up.abs() + 8 * F * up.abs()) + 8 * F * a.abs() * up.abs() + 2 * F * h.abs()
@@ -477,6 +481,52 @@ def test_q8_mlp_on_every_kernel(M, K, N, act):
     # a rounding to 16 bits, half a step of the row's integers and of y's own 16 bits
     off = (y.double() - h[:, at]).abs()
     assert (off <= (hi.double() - lo.double()).abs()[:, at] + 2 * U[dtype] * h[:, at].abs() + 0.51 * top / 127 + SUB[dtype]).all()
+
+
+# An expert's tokens through its layer alone: with one choice of weight 1 the same integers and sums.  An expert's sum is a float, rounded to
+# 16 bits when the choices are joined; a layer's alone may be rounded to 16 bits from the product itself, which for float16 an
+# instruction does.  A product v = n·(s_x·s_w) and its float rn32(v) lie between the same neighbouring 16-bit numbers a <= b (both
+# are floats, and rounding is monotonic), so that each result is a or b: one step apart at most.
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize(
+    "M,K,N,E",
+    [
+        (4, 264, 520, 1), (3, 264, 2056, 1), (2, 8200, 264, 1), (3, 8200, 2056, 1), (2, 16400, 2056, 1), (3, 2056, 8200, 1),
+        (10, 264, 520, 1), (10, 264, 2056, 1), (10, 8200, 264, 1), (10, 8200, 2056, 1), (10, 16400, 2056, 1), (10, 2056, 8200, 1),
+        (20, 264, 520, 1), (20, 264, 8200, 1), (20, 8200, 264, 1), (40, 264, 520, 1), (40, 8200, 4104, 1), (40, 12296, 264, 1),
+        (60, 264, 520, 1), (60, 8200, 4104, 1), (60, 12296, 8200, 1), (50, 264, 520, 6), (300, 264, 520, 9), (700, 520, 264, 9),
+        (300, 264, 264, 1), (900, 2056, 8200, 2), (1500, 4104, 2056, 5), (1500, 4104, 4104, 5), (4500, 2056, 4104, 2), (2300, 2056, 8200, 8),
+    ],
+)
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_q8_experts_on_every_kernel(M, K, N, E, act, dtype):
+    g = gen(M + K)
+    x, choice = on(normal((M, K), 1.0, dtype, g)), torch.arange(M) * 7 % E
+    if M // E > 128:
+        choice[torch.arange(M) % 10 == 9] = E - 1  # (one with more rows than the others; all of them by the GEMM)
+    logits = on(torch.nn.functional.one_hot(choice, E).float() * 5)
+    w = [q8((E, N, K), dtype, g), q8((E, N, K), dtype, g), q8((E, K, N), dtype, g)]
+    y = moe.moe_mlp_fwd(x, logits, *w, 1, act_fn=act)
+    for e in range(E):
+        rows = on((choice == e).nonzero()[:, 0])
+        gate, up, down = (sliced(q, e) for q in w)
+        alone = quant.q8_mlp_fwd(x[rows], gate, None, up, None, down, None, act_fn=act)
+        assert alone.isfinite().all() and ((alone == y[rows]) | ((alone.view(torch.int16).int() - y[rows].view(torch.int16).int()).abs() <= 1)).all()
+
+
+@gpu
+@pytest.mark.parametrize("M", [2, 128, 129])
+@pytest.mark.parametrize("logits_dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("E,k", [(3, 3), (16, 4), (60, 6), (100, 5), (250, 16), (500, 2)])
+def test_q8_experts_by_logits_of_each_type(M, logits_dtype, E, k):
+    dtype, K, N = torch.bfloat16, 72, 40
+    g = gen(E)
+    x, logits = normal((M, K), 1.0, dtype, g), normal((M, E), 2.0, logits_dtype, g)
+    w = [q8((E, N, K), dtype, g), q8((E, N, K), dtype, g), q8((E, K, N), dtype, g)]
+    y = moe.moe_mlp_fwd(on(x), on(logits), *w, k)
+    ref, bound = moe64(x, logits, k, True, "silu", dtype, lambda e: [weight_of(sliced(q, e)) for q in w])
+    hold(y, ref, bound, dtype, N)
 
 
 @gpu

@@ -1759,7 +1759,7 @@ int check_q8_cols(const char* fn, const char* name, int64_t cols) {
 // Launches have fewer than 2^32 threads (of more the runtime starts a part only, without an error): 1024 threads for every 4 rows
 // of integers, a workgroup of 512 for every tile of weight rows and of token rows, a thread for 8 columns of a row.
 int check_q8_rows(const char* fn, int64_t rows) {
-  if (rows >= ((int64_t)1 << 24)) return fail(GMLP_ESHAPE, "%s: %lld rows: fewer than 2^24 are taken", fn, (long long)rows);
+  if (rows > ((int64_t)1 << 23)) return fail(GMLP_ESHAPE, "%s: %lld rows: at most 2^23 are taken", fn, (long long)rows);
   return 0;
 }
 int check_q8_sizes(const char* fn, int64_t rows, int64_t K, int64_t N, int64_t tiles) {

@@ -430,7 +430,8 @@ hipError_t q8_few_depth(const Q8Product& p, const void* rows, int cols, const Q8
   const int64_t wgs = (int64_t)((p.N + 16 * R - 1) / (16 * R)) * entries;
   if constexpr (MT == 1) {
     if (steps >= 128 || (steps >= 32 && wgs <= 2 * p.cus)) return run_q8_few<T, SETS, R, MT, 8, 4, F32, Q>(p, rows, cols, solo, s);
-    if (steps >= 32) return run_q8_few<T, SETS, R, MT, 4, 4, F32, Q>(p, rows, cols, solo, s);
+    if constexpr (SETS == 2 || R == 2)  // (a single matrix has more workgroups than that of two tiles only)
+      if (steps >= 32) return run_q8_few<T, SETS, R, MT, 4, 4, F32, Q>(p, rows, cols, solo, s);
   } else if constexpr (MT == 2 && R == 1) {
     if (steps >= 128) return run_q8_few<T, SETS, R, MT, 8, 2, F32, Q>(p, rows, cols, solo, s);
   } else if constexpr (MT == 8 && SETS == 2 && R == 2) {
