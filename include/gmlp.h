@@ -416,7 +416,8 @@ int gmlp_moe_balance_bwd(const void* logits, const uint8_t* mask, const float* w
  * gmlp_q8_mlp_fwd: h = act(x·W_gateᵀ + b_gate) ⊙ (x·W_upᵀ + b_up) rounded to dtype (in fp16 one past 65504 is infinite, and the
  *   token's outputs NaN), y = h·W_downᵀ + b_down, h in 8 bits again.
  * gmlp_q8_moe_fwd: y[m] = sum over m's experts e of weight·MLP_e(x[m]), routed as gmlp_moe_route does, the sum over experts in
- *   fp32; experts without tokens are not read, and a choice of weight 0 is not run.  M * top_k <= GMLP_Q8_MOE_MAX_PAIRS.
+ *   fp32; experts without tokens are not read, and a choice of weight 0 is not run.  M * top_k <= GMLP_Q8_MOE_MAX_PAIRS,
+ *   and M * (K + 128) < 2^31 - 2^17.
  * M is at most 2^23 in each.  workspace: as many bytes as the function beside each says.
  */
 #define GMLP_Q8_MOE_MAX_PAIRS 65536

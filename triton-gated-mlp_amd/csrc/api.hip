@@ -1877,6 +1877,7 @@ struct Q8MlpWorkspace {
 struct Q8MoePlan {
   int cap;
   bool gemm;
+  bool by_token;  // token rows are found by their numbers
   int tile_class[2];
   int64_t rows, tiles, large;
 };
@@ -1886,6 +1887,10 @@ Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
   // (an expert with more rows than a tile is read once for each of its tiles, small ones from the caches)
   p.gemm = each > 96;
   p.cap = each <= 12 ? 16 : each <= 24 ? 32 : each <= (K * N <= ((int64_t)1 << 23) ? 56 : 48) ? 64 : 128;
+  // Small tiles find their token rows by their numbers: these become integers beside the routing, each once.  A load then touches 16 lines in
+  // the place of 8.  us, by number and laid out in the plan's order: 64 experts of 2048 x 1024, 24 rows (32) 107, 112; 16 of 2048 x 2816, 24
+  // rows 75, 79; 8 of 4096 x 14336, 24 rows 284, 254; in tiles of 128 rows, whose lanes need eight offsets, 64 experts, 96 rows 222, 196.
+  p.by_token = p.cap == 16 || (p.cap == 32 && K * N <= (int64_t)1 << 23);
   p.rows = gmlp::q8_plan_rows(pairs, E);
   p.tiles = gmlp::q8_plan_tiles(pairs, E, p.cap);
   if (!p.gemm) return p;
@@ -1915,8 +1920,8 @@ struct Q8MoeWorkspace {
     large = a.part(p.large * (int64_t)sizeof(gmlp::Q8Tile));
     row_of = a.part(pairs * 4);
     token_of = a.part(p.rows * 4);
-    x = a.part(p.rows * gmlp::q8_padded(K));
-    sx = a.part(p.rows * 4);
+    x = a.part((p.by_token ? M : p.rows) * gmlp::q8_padded(K));
+    sx = a.part((p.by_token ? M : p.rows) * 4);
     h = a.part(p.rows * N * 2);
     q = a.part(p.rows * gmlp::q8_padded(N));
     sq = a.part(p.rows * 4);
@@ -2068,6 +2073,8 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
     return fail(GMLP_ESHAPE, "%s: M * top_k = %lld exceeds the %d choices of a call", __func__, (long long)(M * top_k), GMLP_Q8_MOE_MAX_PAIRS);
   const Q8MoePlan plan = plan_q8_moe(M * top_k, K, N, E);
   if (int rc = check_q8_sizes(__func__, plan.rows, K, N, plan.tiles)) return rc;
+  if (M * gmlp::q8_padded(K) > gmlp::Q8_MAX_LINES)
+    return fail(GMLP_ESHAPE, "%s: M * K = %lld exceeds what a call takes", __func__, (long long)(M * K));
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(codes_up); GMLP_REQUIRE_ALIGNED(codes_down);
   GMLP_REQUIRE_ALIGNED(scales_gate); GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(scales_down);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
@@ -2090,27 +2097,39 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
     }));
   const gmlp::Q8Plan routed = {(int*)(base + ws.total), (gmlp::Q8Tile*)(base + ws.tiles), plan.gemm ? (gmlp::Q8Tile*)(base + ws.large) : nullptr,
                                (int*)(base + ws.row_of), (int*)(base + ws.token_of)};
+  // An expert has no more rows than there are tokens, and a tile no more than its own.
+  const int64_t most_rows = std::min<int64_t>(M, plan.cap);
+  // Made integers by the experts' workgroups: fewer than 2 rows an expert.  (us, so and before: 64 experts, 8 of them a token, 16 tokens 71.6,
+  // 73.5, 24 tokens 81.8, 79.6; 2 of 16, 16 tokens 56.7, 52.1, 8 tokens 39, 45; 4 of 128, 64 tokens 46.9, 47.6, 48 tokens 44.2, 44.7)
+  auto inside = [&](int64_t cols) {
+    return M * top_k < 2 * E && gmlp::q8_own_rows(most_rows, gmlp::q8_padded(cols), 0, num_cu());
+  };
+  const gmlp::Q8Lines tokens = {x, (int8_t*)(base + ws.x), (float*)(base + ws.sx), (int)M, (int)K, (int)gmlp::q8_padded(K), dtype};
+  const gmlp::Q8Lines* const lines = plan.by_token && !inside(K) ? &tokens : nullptr;
   const hipError_t e = by_dtype(logits_dtype, [&](auto tag) {
     typedef decltype(tag) L;
     if (M <= gmlp::Q8_ROUTE_ROWS)
-      return gmlp::launch_q8_route_plan<L>((const L*)logits, weights, routed, (int)M, (int)E, (int)top_k, normalize, plan.cap, s);
+      return gmlp::launch_q8_route_plan<L>((const L*)logits, weights, routed, (int)M, (int)E, (int)top_k, normalize, plan.cap, lines, s);
     if (hipError_t err = gmlp::launch_route<L>((const L*)logits, weights, experts, M, (int)E, (int)top_k, normalize, s)) return err;
-    return gmlp::launch_q8_plan(experts, weights, routed, (int)M, (int)E, (int)top_k, plan.cap, s);
+    return gmlp::launch_q8_plan(experts, weights, routed, (int)M, (int)E, (int)top_k, plan.cap, lines, s);
   });
   if (e != hipSuccess) return hip_result(__func__, e);
   return hip_result(__func__, by_half(dtype, [&](auto tag) {
     typedef decltype(tag) T;
     // a product of the plan's rows, [..][cols] or (token_of) those tokens'; `at`, `scales`: where they become integers if that takes a
-    // launch of its own: from 4 rows an expert on.  (An expert has no more rows than there are tokens, and a tile no more than its own.)
+    // launch of its own
     auto product = [&](gmlp::Q8Product& p, const T* rows, int64_t cols, const int* token_of, size_t at, size_t scales, int sets) -> hipError_t {
       p.tiles = routed.tiles; p.total = routed.total; p.most_tiles = (int)plan.tiles;
       p.token_of = token_of;
-      p.most_rows = (int)std::min<int64_t>(M, plan.cap);
-      if (M * top_k <= 4 * E && gmlp::q8_own_rows(p.most_rows, p.K, 0, p.cus))
-        return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
-      if (hipError_t err = gmlp::launch_q8_rows<T>(rows, (int8_t*)(base + at), (float*)(base + scales), 1, plan.rows, cols, token_of,
-                                                   routed.total + 1, s))
-        return err;
+      p.tokens = (int)M;
+      p.most_rows = (int)most_rows;
+      if (inside(cols)) return gmlp::launch_q8_few_rows<T>(p, rows, (int)cols, sets, nullptr, s);
+      if (token_of == nullptr || lines == nullptr) {
+        p.token_of = nullptr;
+        if (hipError_t err = gmlp::launch_q8_rows<T>(rows, (int8_t*)(base + at), (float*)(base + scales), 1, plan.rows, cols, token_of,
+                                                     routed.total + 1, s))
+          return err;
+      }
       if (!plan.gemm) return gmlp::launch_q8_few<T>(p, sets, plan.cap / 16, s);
       p.tile_class = plan.tile_class[sets == 2 ? 0 : 1];
       if (p.tile_class == gmlp::TILE_LARGE) p.tiles = routed.large, p.total = routed.total + 2, p.most_tiles = (int)plan.large;

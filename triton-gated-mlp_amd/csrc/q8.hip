@@ -71,27 +71,14 @@ __device__ __forceinline__ i32x4 q8_sixteen(const RowScale<T>& scale, const u32x
   return out;
 }
 
-// A workgroup of NT threads: ROWS rows of a tile.  A thread takes 16 numbers of a row at a time (32 bytes in, 16 out), PER times, and
-// keeps them while the row's largest is found; PER = 0: rows of any length, read twice.  Neighbouring threads take the ROWS
-// rows first, which lie together in the result.
-template <typename T, int NT, int ROWS, int PER>
-__global__ void __launch_bounds__(NT) q8_rows_kernel(const T* x, int8_t* codes, float* scales, int64_t rows, int cols, int padded,
-                                                     int tiles, const int* token_of, const int* rows_at) {
-  constexpr int LANES = NT / ROWS, NW = NT / 64, PARTS = 16 / ROWS;  // threads of a row
+// ROWS rows by NT threads.  A thread takes 16 numbers of a row at a time (32 bytes in, 16 out), PER times, and keeps them while the row's
+// largest is found; PER = 0: rows of any length, read twice.  Neighbouring threads take the ROWS rows first.  src: this thread's row, of
+// zeros if it is not `there`; put(c, integers of columns c..).  Returns the row's scale.
+template <typename T, int NT, int ROWS, int PER, typename Put>
+__device__ __forceinline__ float q8_some_rows(const T* src, bool there, int cols, int padded, Put&& put) {
+  constexpr int LANES = NT / ROWS, NW = NT / 64;  // threads of a row
   __shared__ uint32_t part[NW][ROWS];
   const int r = threadIdx.x % ROWS, l = threadIdx.x / ROWS;
-  // The workgroups of a tile are 8 apart: on the same die, whose cache joins what they write to a line.
-  const int64_t b = blockIdx.x, whole = (int64_t)tiles / 8 * 8 * PARTS;
-  const int64_t tile = b < whole ? b / (8 * PARTS) * 8 + b % 8 : b / PARTS, sub = b < whole ? b / 8 % PARTS : b % PARTS;
-  const int64_t at = tile * 16 + sub * ROWS + r, matrix = blockIdx.y;
-  int64_t from = at;
-  bool there = at < rows;
-  if (rows_at != nullptr && tile * 16 >= rows_at[0]) return;
-  if (token_of != nullptr) {
-    from = token_of[at];
-    there = from >= 0;
-  }
-  const T* const src = x + (matrix * rows + from) * cols;
   auto read = [&](u32x4 (&v)[2], int c) __attribute__((always_inline)) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) v[h] = there && c + 8 * h < cols ? *(const u32x4*)(src + c + 8 * h) : u32x4{0, 0, 0, 0};
@@ -122,21 +109,62 @@ __global__ void __launch_bounds__(NT) q8_rows_kernel(const T* x, int8_t* codes, 
 #pragma unroll
   for (int w = 0; w < NW; ++w) most = max(most, part[w][r]);
   const RowScale<T> scale(most);
-  if (l == 0 && at < rows) scales[matrix * rows + at] = there ? scale.scale : 0.f;
-  int8_t* const dst = codes + ((matrix * tiles + tile) * (int64_t)padded) * 16 + (at % 16) * 16;
-  auto write = [&](const u32x4 (&v)[2], int c) __attribute__((always_inline)) {
-    if (c < padded) *(i32x4*)(dst + (int64_t)(c / 16) * 256) = q8_sixteen<T>(scale, v);
-  };
   if constexpr (PER > 0) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) write(kept[i], (l + i * LANES) * 16);
+    for (int i = 0; i < PER; ++i)
+      if ((l + i * LANES) * 16 < padded) put((l + i * LANES) * 16, q8_sixteen<T>(scale, kept[i]));
   } else {
     for (int c = l * 16; c < padded; c += LANES * 16) {
       read(kept[0], c);
-      write(kept[0], c);
+      put(c, q8_sixteen<T>(scale, kept[0]));
     }
   }
+  return scale.scale;
 }
+
+// A workgroup: ROWS rows of a tile, which lie together in the result.
+template <typename T, int NT, int ROWS, int PER>
+__global__ void __launch_bounds__(NT) q8_rows_kernel(const T* x, int8_t* codes, float* scales, int64_t rows, int cols, int padded,
+                                                     int tiles, const int* token_of, const int* rows_at) {
+  constexpr int PARTS = 16 / ROWS;
+  const int r = threadIdx.x % ROWS;
+  // The workgroups of a tile are 8 apart: on the same die, whose cache joins what they write to a line.
+  const int64_t b = blockIdx.x, whole = (int64_t)tiles / 8 * 8 * PARTS;
+  const int64_t tile = b < whole ? b / (8 * PARTS) * 8 + b % 8 : b / PARTS, sub = b < whole ? b / 8 % PARTS : b % PARTS;
+  const int64_t at = tile * 16 + sub * ROWS + r, matrix = blockIdx.y;
+  int64_t from = at;
+  bool there = at < rows;
+  if (rows_at != nullptr && tile * 16 >= rows_at[0]) return;
+  if (token_of != nullptr) {
+    from = token_of[at];
+    there = from >= 0;
+  }
+  int8_t* const dst = codes + ((matrix * tiles + tile) * (int64_t)padded) * 16 + (at % 16) * 16;
+  const float scale = q8_some_rows<T, NT, ROWS, PER>(x + (matrix * rows + from) * cols, there, cols, padded,
+                                                     [&](int c, i32x4 n) { *(i32x4*)(dst + (int64_t)(c / 16) * 256) = n; });
+  if ((int)threadIdx.x < ROWS && at < rows) scales[matrix * rows + at] = there ? scale : 0.f;
+}
+
+// Four rows of `lines` by a workgroup of 1024, the `block`-th.
+template <typename T>
+__device__ __forceinline__ void q8_four_lines(const Q8Lines& a, int block) {
+  const int64_t at = (int64_t)block * 4 + threadIdx.x % 4;
+  const bool there = at < a.rows;
+  const T* const src = (const T*)a.x + at * a.cols;
+  int8_t* const dst = a.codes + at * a.padded;
+  auto put = [&](int c, i32x4 n) __attribute__((always_inline)) {
+    if (there) *(i32x4*)(dst + c) = n;
+  };
+  const float scale = a.padded <= 4096    ? q8_some_rows<T, 1024, 4, 1>(src, there, a.cols, a.padded, put)
+                      : a.padded <= 16384 ? q8_some_rows<T, 1024, 4, 4>(src, there, a.cols, a.padded, put)
+                                          : q8_some_rows<T, 1024, 4, 0>(src, there, a.cols, a.padded, put);
+  if (threadIdx.x < 4 && there) a.scales[at] = scale;
+}
+__device__ __forceinline__ void q8_lines_of(const Q8Lines& a, int block) {
+  if (a.dtype == 0) q8_four_lines<f16>(a, block);
+  else q8_four_lines<bf16>(a, block);
+}
+unsigned q8_lines_workgroups(const Q8Lines* lines) { return lines != nullptr ? (unsigned)((lines->rows + 3) / 4) : 0u; }
 
 template <typename T>
 hipError_t launch_q8_rows(const T* x, int8_t* codes, float* scales, int64_t count, int64_t rows, int64_t cols, const int* token_of,
@@ -308,13 +336,31 @@ __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
 #pragma unroll
   for (int b = 0; b < SETS; ++b)
     rw[b] = q8_make_rsrc(p.w[b] + ((int64_t)expert * all_tiles + first_tile) * pitch, (uint32_t)own * pitch);
-  const q8_rsrc rx = q8_make_rsrc(p.x + (int64_t)(row / 16) * pitch, (uint32_t)((count + 15) / 16) * pitch);
+  // GATHER: token rows that lie one behind the other are found by their numbers.  (Products of the columns beyond those that are there
+  // repeat the first one, and are not used.)
+  constexpr bool GATHER = SETS == 2 && !Q && MT <= 2;
+  const bool gathered = GATHER && a.token_of != nullptr;
+  const q8_rsrc rx = gathered ? q8_make_rsrc(p.x, (uint32_t)p.tokens * (uint32_t)p.K)
+                              : q8_make_rsrc(p.x + (int64_t)(row / 16) * pitch, (uint32_t)((count + 15) / 16) * pitch);
   const int s0 = steps * wave / NW, run = steps * (wave + 1) / NW - s0;
   const uint32_t lane_off = (uint32_t)lane * 16u;
+  uint32_t x_off[GATHER ? MT : 1];
+  const uint32_t x_step = gathered ? 64u : 1024u;
+  if constexpr (GATHER) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int j = 16 * m + (lane & 15);
+      x_off[m] = gathered ? (uint32_t)a.token_of[row + (j < count ? j : 0)] * (uint32_t)p.K + (uint32_t)(lane >> 4) * 16u
+                          : lane_off + (uint32_t)m * pitch;
+    }
+  }
   Q8Stage<SETS, R, MT, Q> st[D];
   auto load = [&](Q8Stage<SETS, R, MT, Q>& t, int i) __attribute__((always_inline)) {
     const uint32_t at = (uint32_t)(s0 + i) * 1024u;
-    if constexpr (!Q)
+    if constexpr (GATHER)
+#pragma unroll
+      for (int m = 0; m < MT; ++m) t.x[m] = q8_load16<0>(rx, x_off[m], i < run ? (uint32_t)(s0 + i) * x_step : Q8_PAST);
+    else if constexpr (!Q)
 #pragma unroll
       for (int m = 0; m < MT; ++m) t.x[m] = q8_load16<0>(rx, lane_off, i < run ? at + (uint32_t)m * pitch : Q8_PAST);
 #pragma unroll
@@ -378,7 +424,7 @@ __global__ void __launch_bounds__(NW * 64) q8_few_kernel(Q8Few a) {
       // lane: four output columns of one token row
       const int r = (first + i) / MT, j = 16 * ((first + i) % MT) + r16, n = (first_tile + r) * 16 + 4 * kg;
       if (j >= count || n >= p.N) continue;
-      const float sx = Q ? RowScale<T>(own_most[Q ? j : 0]).scale : p.sx[row + j];
+      const float sx = Q ? RowScale<T>(own_most[Q ? j : 0]).scale : p.sx[gathered ? a.token_of[row + j] : row + j];
       float v[SETS][4], o[4];
 #pragma unroll
       for (int b = 0; b < SETS; ++b) {
@@ -463,8 +509,7 @@ hipError_t launch_q8_few(const Q8Product& p, int sets, int token_tiles, hipStrea
 }
 // Where every workgroup makes the integers itself.  A launch of their own takes 3 us; in every workgroup they take what it has rows
 // for: us, in the workgroups and in a launch, 4096 x 4096 of 4096, 6 rows 7.8, 8.5, 8 rows 8.7, 8.5; 14336 rows of 4096 columns 4 rows 12.6,
-// 15.0, 8 rows 15.4, 15.0; of 2048 columns 12 rows 11.6, 11.7, 16 rows 13.1, 11.8; 2048 of 2048, 16 rows 7.1, 8.6; an expert layer of 64
-// experts, 16 tokens, 8 of them each 72, 82.
+// 15.0, 8 rows 15.4, 15.0; of 2048 columns 12 rows 11.6, 11.7, 16 rows 13.1, 11.8; 2048 of 2048, 16 rows 7.1, 8.6.
 bool q8_own_rows(int64_t most_rows, int64_t padded, int64_t N, int cus) {
   if (most_rows == 1) return padded <= 32768;
   return most_rows <= Q8_OWN_ROWS && most_rows * padded <= (N <= 16 * cus ? 32768 : 24576);
@@ -604,7 +649,8 @@ __device__ __forceinline__ void q8_lay_out(const Q8Choices& sh, const Q8Plan& pl
   __syncthreads();
 }
 __global__ void __launch_bounds__(1024) q8_plan_kernel(const int64_t* experts, const float* weights, Q8Plan plan, int pairs, int E, int top_k,
-                                                       int cap, int most_rows) {
+                                                       int cap, int most_rows, Q8Lines lines) {
+  if (blockIdx.x > 0) return q8_lines_of(lines, (int)blockIdx.x - 1);
   __shared__ int count[1024], in_wave[3][16];
   constexpr int PER = 8;
   const int tid = threadIdx.x;
@@ -648,16 +694,20 @@ __global__ void __launch_bounds__(1024) q8_plan_kernel(const int64_t* experts, c
     }
   }
 }
-hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8Plan& plan, int M, int E, int top_k, int cap, hipStream_t s) {
-  hipLaunchKernelGGL(q8_plan_kernel, dim3(1), dim3(1024), 0, s, experts, weights, plan, M * top_k, E, top_k, cap,
-                     (int)q8_plan_rows((int64_t)M * top_k, E));
+// (rows that no choice has are marked for launch_q8_rows only)
+static int q8_rows_to_mark(const Q8Lines* lines, int M, int E, int top_k) { return lines != nullptr ? 0 : (int)q8_plan_rows((int64_t)M * top_k, E); }
+hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8Plan& plan, int M, int E, int top_k, int cap,
+                          const Q8Lines* lines, hipStream_t s) {
+  hipLaunchKernelGGL(q8_plan_kernel, dim3(1 + q8_lines_workgroups(lines)), dim3(1024), 0, s, experts, weights, plan, M * top_k, E, top_k, cap,
+                     q8_rows_to_mark(lines, M, E, top_k), lines != nullptr ? *lines : Q8Lines{});
   return hipGetLastError();
 }
 
 // Routing and plan of a few tokens in one launch: 64 tokens at a time, four to a wavefront as in routing many.
 template <int VPL, typename L>
 __global__ void __launch_bounds__(1024) q8_route_plan_kernel(const L* logits, float* weights, Q8Plan plan, int M, int E, int top_k, int normalize,
-                                                             int cap, int most_rows) {
+                                                             int cap, int most_rows, Q8Lines lines) {
+  if (blockIdx.x > 0) return q8_lines_of(lines, (int)blockIdx.x - 1);
   __shared__ int count[1024], in_wave[3][16];
   __shared__ short chosen[Q8_ROUTE_ROWS * 16];
   const int tid = threadIdx.x, lane = tid & 63, l = tid & 15;
@@ -699,10 +749,10 @@ __global__ void __launch_bounds__(1024) q8_route_plan_kernel(const L* logits, fl
 }
 template <typename L>
 hipError_t launch_q8_route_plan(const L* logits, float* weights, const Q8Plan& plan, int M, int E, int top_k, int normalize, int cap,
-                                hipStream_t s) {
+                                const Q8Lines* lines, hipStream_t s) {
 #define CALL(V)                                                                                                          \
-  hipLaunchKernelGGL((q8_route_plan_kernel<V, L>), dim3(1), dim3(1024), 0, s, logits, weights, plan, M, E, top_k, normalize, cap, \
-                     (int)q8_plan_rows((int64_t)M * top_k, E))
+  hipLaunchKernelGGL((q8_route_plan_kernel<V, L>), dim3(1 + q8_lines_workgroups(lines)), dim3(1024), 0, s, logits, weights, plan, M, E, top_k, \
+                     normalize, cap, q8_rows_to_mark(lines, M, E, top_k), lines != nullptr ? *lines : Q8Lines{})
   if (E <= 16) CALL(1);
   else if (E <= 64) CALL(4);
   else if (E <= 128) CALL(8);
@@ -754,8 +804,8 @@ hipError_t launch_q8_combine(const float* parts, const float* weights, const int
 GMLP_INSTANTIATE(f16)
 GMLP_INSTANTIATE(bf16)
 #undef GMLP_INSTANTIATE
-template hipError_t launch_q8_route_plan<f16>(const f16*, float*, const Q8Plan&, int, int, int, int, int, hipStream_t);
-template hipError_t launch_q8_route_plan<bf16>(const bf16*, float*, const Q8Plan&, int, int, int, int, int, hipStream_t);
-template hipError_t launch_q8_route_plan<float>(const float*, float*, const Q8Plan&, int, int, int, int, int, hipStream_t);
+template hipError_t launch_q8_route_plan<f16>(const f16*, float*, const Q8Plan&, int, int, int, int, int, const Q8Lines*, hipStream_t);
+template hipError_t launch_q8_route_plan<bf16>(const bf16*, float*, const Q8Plan&, int, int, int, int, int, const Q8Lines*, hipStream_t);
+template hipError_t launch_q8_route_plan<float>(const float*, float*, const Q8Plan&, int, int, int, int, int, const Q8Lines*, hipStream_t);
 
 }  // namespace gmlp

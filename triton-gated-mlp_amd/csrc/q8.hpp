@@ -29,6 +29,15 @@ struct Q8Plan {
   int* row_of;       // [M * top_k]: row of a choice, -1 where its expert is not run
   int* token_of;     // [rows]: -1 where a row is left empty
 };
+// Token rows as integers one behind the other, [rows][padded], for the experts' workgroups to find by their numbers: each once, and
+// without the plan.
+struct Q8Lines {
+  const void* x;  // [rows][cols]
+  int8_t* codes;
+  float* scales;
+  int rows, cols, padded, dtype;
+};
+constexpr int64_t Q8_MAX_LINES = 0x7ffe0000;  // bytes: what offsets of 31 bits and a row reach
 inline int64_t q8_plan_rows(int64_t pairs, int64_t E) {  // at most
   const int64_t most = E + pairs / 16;
   return 16 * (pairs < most ? pairs : most);
@@ -50,7 +59,8 @@ struct Q8Product {
   const Q8Tile* tiles;
   const int* total;      // how many tiles there are
   int most_tiles;        // ... at most
-  const int* token_of;   // launch_q8_few_rows: the tiles' rows are those of these tokens (nullable: their own)
+  const int* token_of;   // streaming, SETS = 2 or launch_q8_few_rows: the tiles' rows are those of these tokens (nullable: their own);
+  int tokens;            // ... launch_q8_few: x and sx are Q8Lines of so many
   int most_rows;         // launch_q8_few_rows: rows of a tile, at most
   int nxcd, cus;
   // GEMM only
@@ -91,14 +101,16 @@ hipError_t launch_q8_rows(const T* x, int8_t* codes, float* scales, int64_t coun
 template <typename T>
 hipError_t launch_q8_dequantize(const int8_t* codes, const float* scales, T* w, int64_t count, int64_t rows, int64_t cols, hipStream_t s);
 // The plan of routed choices; cap: rows of a tile.  A choice of weight 0 is not run.
-hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8Plan& plan, int M, int E, int top_k, int cap, hipStream_t s);
-// y[t] = sum over the choices of weight * parts[row]
+// lines (nullable): what the launch's other workgroups do meanwhile; with it token_of is not -1 but left where no row is.
+hipError_t launch_q8_plan(const int64_t* experts, const float* weights, const Q8Plan& plan, int M, int E, int top_k, int cap,
+                          const Q8Lines* lines, hipStream_t s);
 // Routing and plan of up to Q8_ROUTE_ROWS tokens from the logits on.  (8 of 64 experts, 64 tokens: 7.0 us, in two launches 4.7 and 4.7; for
 // 256 tokens 15.8, 5 and 6.)
 constexpr int Q8_ROUTE_ROWS = 128;
 template <typename L>
 hipError_t launch_q8_route_plan(const L* logits, float* weights, const Q8Plan& plan, int M, int E, int top_k, int normalize, int cap,
-                                hipStream_t s);
+                                const Q8Lines* lines, hipStream_t s);
+// y[t] = sum over the choices of weight * parts[row]
 template <typename T>
 hipError_t launch_q8_combine(const float* parts, const float* weights, const int* row_of, T* y, int64_t M, int64_t K, int top_k,
                              hipStream_t s);

@@ -856,7 +856,7 @@ Tensor moe_mlp_q8(const Tensor& x_in, const Tensor& logits_in, const Q8& gate, c
   const Tensor x = Q8Matrix::aligned(x_in.contiguous()), logits = logits_in.contiguous();
   const Tensor y = at::empty(x.sizes(), x.options());
   if (M == 0) return y;
-  const int64_t piece = std::max<int64_t>(1, GMLP_Q8_MOE_MAX_PAIRS / top_k);
+  const int64_t piece = std::max<int64_t>(1, std::min<int64_t>(GMLP_Q8_MOE_MAX_PAIRS / top_k, ((int64_t)1 << 30) / (K + 128)));
   size_t bytes = lib.gmlp_q8_moe_workspace_bytes(std::min(M, piece), K, N, E, top_k, code);
   if (M > piece && M % piece) bytes = std::max(bytes, lib.gmlp_q8_moe_workspace_bytes(M % piece, K, N, E, top_k, code));
   const Tensor ws = scratch(bytes > 0 ? bytes : 16, x);  // (0: what the call below refuses)
