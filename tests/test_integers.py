@@ -492,7 +492,7 @@ def test_q8_mlp_on_every_kernel(M, K, N, act, dtype):
 @pytest.mark.parametrize(
     "M,K,N,E",
     [
-        (4, 264, 520, 1), (3, 264, 2056, 1), (2, 8200, 264, 1), (3, 8200, 2056, 1), (2, 16400, 2056, 1), (3, 2056, 8200, 1),
+        (3, 264, 2056, 2), (3, 4104, 2056, 2), (3, 8200, 2056, 2), (3, 2056, 8200, 2), (3, 8200, 264, 2), (4, 264, 520, 1), (3, 264, 2056, 1), (2, 8200, 264, 1), (3, 8200, 2056, 1), (2, 16400, 2056, 1), (3, 2056, 8200, 1),
         (10, 264, 520, 1), (10, 264, 2056, 1), (10, 8200, 264, 1), (10, 8200, 2056, 1), (10, 16400, 2056, 1), (10, 2056, 8200, 1),
         (20, 264, 520, 1), (20, 264, 8200, 1), (20, 8200, 264, 1), (40, 264, 520, 1), (40, 8200, 4104, 1), (40, 12296, 264, 1),
         (60, 264, 520, 1), (60, 8200, 4104, 1), (60, 12296, 8200, 1), (50, 264, 520, 6), (300, 264, 520, 9), (700, 520, 264, 9),

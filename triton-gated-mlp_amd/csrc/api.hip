@@ -1811,8 +1811,11 @@ Q8DensePlan plan_q8(int kind, int64_t M, int64_t N, int64_t padded) {
   }
   return p;
 }
+// Up to 64 rows weights are streamed, up to 128 but for a single matrix's long reductions.  us, streamed and by the GEMM, 100 rows: 4096 x 14336
+// 25, 33; 4096 x 4096 15, 17; 2048 x 2048 10.2, 13.9; 14336 x 4096 35, 28 (64 rows 27, 27); 2048 x 14336 16.7, 15.7.
+bool q8_streams(int kind, int64_t M, int64_t padded) { return M <= 64 || (M <= gmlp::Q8_FEW_ROWS && (kind == GATEUP || padded < 8192)); }
 size_t q8_split_bytes(int kind, int64_t M, int64_t N, int64_t padded) {
-  if (M <= gmlp::Q8_FEW_ROWS) return 0;
+  if (q8_streams(kind, M, padded)) return 0;
   return split_workspace_bytes(plan_q8(kind, M, N, padded).all.splits, M, N, kind == GATEUP ? 2 : 1);
 }
 
@@ -1826,8 +1829,9 @@ gmlp::Q8Product q8_product(const int8_t* x, const float* sx, int64_t M, int64_t 
 }
 template <typename T>
 hipError_t run_q8_dense(gmlp::Q8Product& p, int sets, float* partial, hipStream_t s) {
-  if (p.M <= gmlp::Q8_FEW_ROWS) return gmlp::launch_q8_few<T>(p, sets, q8_token_tiles(p.M), s);
-  const Q8DensePlan plan = plan_q8(sets == 2 ? GATEUP : LINEAR, p.M, p.N, p.K);
+  const int kind = sets == 2 ? GATEUP : LINEAR;
+  if (q8_streams(kind, p.M, p.K)) return gmlp::launch_q8_few<T>(p, sets, q8_token_tiles(p.M), s);
+  const Q8DensePlan plan = plan_q8(kind, p.M, p.N, p.K);
   p.splits = plan.all.splits;
   p.rotate = p.M <= 512;
   p.partial = partial;
@@ -1869,11 +1873,12 @@ struct Q8MlpWorkspace {
   }
 };
 
-// An expert layer: rows of a tile (the GEMM's 128, or 256 in a list of its own, the streaming kernels' 16 to 128), and of the
+// An expert layer: rows of a tile (the GEMM's 128, or 256 in a list of its own, the streaming kernels' 16 to 64), and of the
 // GEMM the tile classes of gate/up and down, by their estimates for as many tiles as experts with half a tile left over each have.
 // us by the rows of an expert on average, tiles of as many and of twice as many rows: 64 experts of 2048 x 1024, 10 rows (16, 32) 98, 105,
-// 21 rows (32, 64) 111, 122, 45 rows (64, 128) 133, 165, 56 rows 148, 169, 72 rows 185, 183; 8 of 4096 x 14336, 24 rows (32, 64) 254, 253, 42 rows
-// (64, 128) 277, 313, 52 rows 344, 316.  Beyond 96 rows the GEMM: 64 experts, 128 rows 190, 96 rows on the streaming kernels 196.
+// 21 rows (32, 64) 111, 122; 8 of 4096 x 14336, 24 rows 254, 253.  Streaming (64) and the GEMM: 64 experts, 40 rows 132, 126, 48 rows 134, 144,
+// 56 rows 146, 146, 64 rows (128) 174, 135; 8 of 4096 x 14336, 48 rows 289, 332, 64 rows (128) 330, 315; 16 of 2048 x 2816, 56 rows 92.6, 94.0, 64
+// rows (128) 103, 92; 128 of 1024 x 512, 48 rows 102, 89, 64 rows (128) 135, 89.
 struct Q8MoePlan {
   int cap;
   bool gemm;
@@ -1885,11 +1890,11 @@ Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
   Q8MoePlan p = {};
   const int64_t each = cdiv(pairs, E);
   // (an expert with more rows than a tile is read once for each of its tiles, small ones from the caches)
-  p.gemm = each > 96;
-  p.cap = each <= 12 ? 16 : each <= 24 ? 32 : each <= (K * N <= ((int64_t)1 << 23) ? 56 : 48) ? 64 : 128;
+  p.gemm = each > 48;
+  p.cap = each <= 12 ? 16 : each <= 24 ? 32 : p.gemm ? 128 : 64;
   // Small tiles find their token rows by their numbers: these become integers beside the routing, each once.  A load then touches 16 lines in
   // the place of 8.  us, by number and laid out in the plan's order: 64 experts of 2048 x 1024, 24 rows (32) 107, 112; 16 of 2048 x 2816, 24
-  // rows 75, 79; 8 of 4096 x 14336, 24 rows 284, 254; in tiles of 128 rows, whose lanes need eight offsets, 64 experts, 96 rows 222, 196.
+  // rows 75, 79; 8 of 4096 x 14336, 24 rows 284, 254.
   p.by_token = p.cap == 16 || (p.cap == 32 && K * N <= (int64_t)1 << 23);
   p.rows = gmlp::q8_plan_rows(pairs, E);
   p.tiles = gmlp::q8_plan_tiles(pairs, E, p.cap);

@@ -501,7 +501,8 @@ hipError_t launch_q8_few(const Q8Product& p, int sets, int token_tiles, hipStrea
   if (token_tiles == 1) return q8_few_tiles<T, SETS, 1, F32, false>(p, nullptr, 0, nullptr, s); \
   if (token_tiles == 2) return q8_few_tiles<T, SETS, 2, F32, false>(p, nullptr, 0, nullptr, s); \
   if (token_tiles == 4) return q8_few_tiles<T, SETS, 4, F32, false>(p, nullptr, 0, nullptr, s); \
-  return q8_few_tiles<T, SETS, 8, F32, false>(p, nullptr, 0, nullptr, s)
+  if constexpr (!F32) return q8_few_tiles<T, SETS, 8, F32, false>(p, nullptr, 0, nullptr, s); \
+  else return hipErrorInvalidValue  // (an expert's down projection: up to 64 rows)
   if (sets == 2) { CALL(2, false); }
   if (p.out_f32) { CALL(1, true); }
   CALL(1, false);
