@@ -131,6 +131,15 @@ def on(t):
 
 
 # ------------------------------------------------------------------ without a GPU
+def test_expert_layers_refuse_more_token_rows_than_offsets_reach():
+    lib = _cabi.lib()
+    raw = ctypes.create_string_buffer(4096 + 64)
+    a = (ctypes.addressof(raw) + 63) & ~63
+    moe_fwd = lambda M, K: lib.gmlp_q8_moe_fwd(a, a, a, a, a, a, a, a, a, M, K, 8, 512, 1, 1, 0, 0, 0, a, 0, None)
+    assert moe_fwd(16384, 131072) == -2 and "M * K" in lib.gmlp_last_error().decode()
+    assert moe_fwd(16383, 131072) == -1 and "workspace" in lib.gmlp_last_error().decode()
+
+
 def test_refusals_of_the_c_interface():
     lib = _cabi.lib()
     raw = ctypes.create_string_buffer(4096 + 64)

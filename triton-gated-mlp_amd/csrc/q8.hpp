@@ -12,7 +12,7 @@
 namespace gmlp {
 
 constexpr int Q8_MAX_COLS = 131072;   // 127 * 127 * 131072 < 2^31
-constexpr int Q8_FEW_ROWS = 128;      // token rows, of all or of an expert, that the weight-streaming kernels take
+constexpr int Q8_FEW_ROWS = 128;      // token rows that the weight-streaming kernels take at most
 inline __host__ __device__ int64_t q8_padded(int64_t cols) { return (cols + 127) / 128 * 128; }
 inline __host__ __device__ int64_t q8_tiled_rows(int64_t rows) { return (rows + 15) / 16 * 16; }
 
