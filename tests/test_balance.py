@@ -221,6 +221,24 @@ def test_what_is_not_finite():
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("E", [6, 40, 300])
+def test_what_is_not_finite_in_a_token_left_out_reaches_no_gradient_of_the_loss(E, normalize, dtype):
+    """A token that is in neither counts nor loss has a gradient of 0 for it, whatever its logits hold, and the others' are as without it."""
+    logits, _, _, dl = case(20, E, 2, dtype, E)
+    logits[3, 4], logits[9, 1], logits[12] = math.nan, math.inf, math.nan
+    rest = torch.ones(20, dtype=torch.bool, device=device())
+    rest[[3, 9, 12]] = False
+    x = logits.to(device()).requires_grad_()
+    (d,) = torch.autograd.grad(moe.moe_route_balanced(x, 2, normalize, token_mask=rest).loss, x, dl.to(device()))
+    good = logits.to(device())[rest].requires_grad_()
+    (g,) = torch.autograd.grad(moe.moe_route_balanced(good, 2, normalize).loss, good, dl.to(device()))
+    # (the same counts in both, and nothing else of the other tokens is in a token's gradient)
+    assert (d[~rest] == 0).all() and torch.equal(d[rest], g)
+
+
+@gpu
 def test_even_routing_has_loss_one():
     for M, E in ((64, 8), (4096, 128)):
         x = torch.full((M, E), -30.0)

@@ -203,7 +203,8 @@ __global__ void __launch_bounds__(BAL_BWD_THREADS) balance_bwd_kernel(BalanceArg
 #pragma unroll
     for (int v = 0; v < VPL; ++v) {
       d[v] = kept ? d_loss * (p[v] * (slope[v] - mean)) : 0.f;
-      if (!a.normalize) d[v] -= p[v] * mixed;
+      // (nothing is taken off without gradients of the weights: p of a token left out may be NaN)
+      if (!a.normalize && a.d_weights != nullptr) d[v] -= p[v] * mixed;
     }
     if (a.d_weights != nullptr) {
       const float own = a.normalize ? w * (dw - mixed) : w * dw;
