@@ -418,7 +418,8 @@ int gmlp_moe_balance_bwd(const void* logits, const uint8_t* mask, const float* w
  * gmlp_q8_moe_fwd: y[m] = sum over m's experts e of weight·MLP_e(x[m]), routed as gmlp_moe_route does, the sum over experts in
  *   fp32; experts without tokens are not read, and a choice of weight 0 is not run.  M * top_k <= GMLP_Q8_MOE_MAX_PAIRS,
  *   and M * (K + 128) < 2^31 - 2^17.
- * M is at most 2^23 in each.  workspace: as many bytes as the function beside each says.
+ * M is at most 2^23 in each.  A dense product has fewer than 2^27 output columns and ceil(M / 128) * ceil(columns / 64) < 2^24.
+ * workspace: as many bytes as the function beside each says.
  */
 #define GMLP_Q8_MOE_MAX_PAIRS 65536
 int gmlp_q8_quantize(const void* w, void* codes, float* scales, int64_t count, int64_t rows, int64_t cols, int dtype, void* stream);

@@ -140,6 +140,23 @@ def test_expert_layers_refuse_more_token_rows_than_offsets_reach():
     assert moe_fwd(16383, 131072) == -1 and "workspace" in lib.gmlp_last_error().decode()
 
 
+def test_what_a_launch_has_threads_for_is_taken_and_no_more():
+    lib = _cabi.lib()
+    raw = ctypes.create_string_buffer(4096 + 64)
+    a = (ctypes.addressof(raw) + 63) & ~63
+    err = lambda: lib.gmlp_last_error().decode()
+    linear = lambda M, C: lib.gmlp_q8_linear_fwd(a, a, a, None, a, M, 8, C, 0, a, 0, None)
+    for M, C in ((65536, 262144), (65536, (1 << 21) - 64), (1, (1 << 27) - 16), (1 << 20, (1 << 17) - 64)):
+        assert linear(M, C) == -1 and "workspace" in err()
+    for M, C in ((65536, 1 << 21), (1, 1 << 27), (1 << 21, 1 << 16), (1 << 21, 1 << 18)):
+        assert linear(M, C) == -2 and "too large" in err()
+    mlp = lambda M, K, N: lib.gmlp_q8_mlp_fwd(a, a, a, a, a, a, a, None, None, None, a, M, K, N, 0, 0, a, 0, None)
+    assert mlp(65536, 131072, 131072) == -1 and mlp(1 << 22, 131072, 64) == -2 and mlp(1 << 22, 64, 131072) == -2 and "too large" in err()
+    moe_fwd = lambda M, K, N, E, k: lib.gmlp_q8_moe_fwd(a, a, a, a, a, a, a, a, a, M, K, N, E, k, 1, 0, 0, 0, a, 0, None)
+    assert moe_fwd(65536, 8, 131072, 512, 1) == -1 and "workspace" in err()
+    assert moe_fwd(1, 131072, 131072, 512, 16) == -1 and moe_fwd(384, 131072, 131072, 512, 16) == -1 and moe_fwd(1536, 131072, 131072, 512, 16) == -1
+
+
 def test_refusals_of_the_c_interface():
     lib = _cabi.lib()
     raw = ctypes.create_string_buffer(4096 + 64)
@@ -347,6 +364,44 @@ def test_refusals_of_tensors():
         (lambda: quant.quantize_q8(x[0]), ValueError),
         (lambda: quant.quantize_q8(x[:, :260]), NotImplementedError),
         (lambda: quant.dequantize_q8(q, torch.float32), TypeError),
+# A long batch goes in pieces of 65536 rows, which its rows do not see.
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("more", [17, 300])
+def test_rows_around_the_cut_of_a_long_batch(more, dtype):
+    M, K, N = 65536 + more, 72, 40
+    g = gen(more)
+    x = on(normal((M, K), 1.0, dtype, g))
+    w = [q8((N, K), dtype, g), q8((N, K), dtype, g), q8((K, N), dtype, g)]
+    b = [normal((n,), 0.3, dtype, g) for n in (N, N, K)]
+    rows = torch.tensor([0, 1, 127, 40000, 65534, 65535, 65536, 65537, M - 2, M - 1])
+    y = quant.q8_linear_fwd(x, w[0], on(b[0]))
+    ref, bound = product64(x[on(rows)].cpu(), weight_of(w[0]), b[0])
+    hold(y[on(rows)], ref, bound, dtype)
+    assert torch.equal(y[:65536], quant.q8_linear_fwd(x[:65536], w[0], on(b[0])))
+    y = quant.q8_mlp_fwd(x, w[0], on(b[0]), w[1], on(b[1]), w[2], on(b[2]))
+    ref, bound = mlp64(x[on(rows)].cpu(), weight_of(w[0]), b[0], weight_of(w[1]), b[1], weight_of(w[2]), b[2], "silu", dtype)
+    hold(y[on(rows)], ref, bound, dtype, len(rows) * N)
+    assert torch.equal(y[:65536], quant.q8_mlp_fwd(x[:65536], w[0], on(b[0]), w[1], on(b[1]), w[2], on(b[2])))
+
+
+@gpu
+@pytest.mark.parametrize("M,C", [(65536 + 17, 262144), (3000, (1 << 23) - 8)])
+def test_a_long_batch_through_a_wide_weight(M, C):
+    """A vocabulary projection, and the widest weight that can be quantised.  (34 and 50 GB of outputs.)"""
+    dtype, K = torch.float16, 8
+    g = gen(C % 1000)
+    x, q = on(normal((M, K), 1.0, dtype, g)), quant.quantize_q8(torch.randn((C, K), device=device()).to(dtype))
+    y = quant.q8_linear_fwd(x, q)
+    rows = on(torch.tensor([0, 1, 127, 128, 2047, 2048, M - 1081, M - 18, M - 17, M - 1]))
+    cols = on(torch.cat([torch.arange(32), torch.randint(0, C, (200,), generator=g), torch.arange(C - 32, C)]))
+    n, s = integers64(x[rows])
+    ref = (n @ numbers_of(q, x.device)[cols].T) * s * q.scales.double()[cols]
+    hold(y[rows][:, cols], ref.cpu(), (8 * F * ref.abs()).cpu(), dtype)
+    del y
+    torch.cuda.empty_cache()
+
+
     ]:
         with pytest.raises(error):
             call()

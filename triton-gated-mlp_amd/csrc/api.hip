@@ -1756,18 +1756,23 @@ int check_q8_cols(const char* fn, const char* name, int64_t cols) {
     return fail(GMLP_ESHAPE, "%s: %s = %lld exceeds the %d columns whose sums fit 32 bits", fn, name, (long long)cols, gmlp::Q8_MAX_COLS);
   return 0;
 }
-// Launches have fewer than 2^32 threads (of more the runtime starts a part only, without an error): 1024 threads for every 4 rows
-// of integers, a workgroup of 512 for every tile of weight rows and of token rows, a thread for 8 columns of a row.
+// Launches have fewer than 2^32 threads (of more the runtime starts a part only, without an error): 1024 for every 4 rows of integers;
+// streaming at most 512 for a tile of 16 weight rows and one of token rows; the GEMM at most 256 for 64 output columns and 128 rows.
 int check_q8_rows(const char* fn, int64_t rows) {
   if (rows > ((int64_t)1 << 23)) return fail(GMLP_ESHAPE, "%s: %lld rows: at most 2^23 are taken", fn, (long long)rows);
   return 0;
 }
-int check_q8_sizes(const char* fn, int64_t rows, int64_t K, int64_t N, int64_t tiles) {
-  if (int rc = check_q8_rows(fn, rows)) return rc;
-  const int64_t most = K > N ? K : N;
-  if (tiles * cdiv(most, 16) >= ((int64_t)1 << 32) / 512 || rows * cdiv(most, 8) >= ((int64_t)1 << 32))
-    return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
+// tiles: of token rows, `streamed` or the GEMM's; cols: of the wider product's output
+int check_q8_threads(const char* fn, int64_t tiles, int64_t cols, bool streamed) {
+  const int64_t threads = streamed ? tiles * cdiv(cols, 16) * 512 : tiles * cdiv(cols, 64) * 256;
+  if (threads >= ((int64_t)1 << 32)) return fail(GMLP_ESHAPE, "%s: dimension too large", fn);
   return 0;
+}
+// A dense product of any number of rows.  (Its width is what a few rows can have, too.)
+int check_q8_dense(const char* fn, int64_t M, int64_t cols) {
+  if (int rc = check_q8_rows(fn, M)) return rc;
+  if (int rc = check_q8_threads(fn, 1, cols, true)) return rc;
+  return check_q8_threads(fn, cdiv(M, 128), cols, false);
 }
 int check_q8_storage(const char* fn, int64_t count, int64_t rows, int64_t cols) {
   if (int rc = check_storage(fn, count, rows, cols)) return rc;
@@ -1986,7 +1991,7 @@ int gmlp_q8_linear_fwd(const void* x, const void* codes, const float* scales, co
   if (int rc = check_dims(__func__, M, R, C)) return rc;
   if (int rc = check_q8_cols(__func__, "R", R)) return rc;
   if (int rc = check_mult8(__func__, "C", C)) return rc;
-  if (int rc = check_q8_sizes(__func__, M, R, C, cdiv(M, 128))) return rc;
+  if (int rc = check_q8_dense(__func__, M, C)) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes); GMLP_REQUIRE_ALIGNED(scales); GMLP_REQUIRE_ALIGNED(bias);
   GMLP_REQUIRE_ALIGNED(y); GMLP_REQUIRE_ALIGNED(workspace);
   const Q8LinearWorkspace ws(M, R, C);
@@ -2022,7 +2027,7 @@ int gmlp_q8_mlp_fwd(const void* x, const void* codes_gate, const float* scales_g
   if (int rc = check_dims(__func__, M, K, N)) return rc;
   if (int rc = check_q8_cols(__func__, "K", K)) return rc;
   if (int rc = check_q8_cols(__func__, "N", N)) return rc;
-  if (int rc = check_q8_sizes(__func__, M, K, N, cdiv(M, 128))) return rc;
+  if (int rc = check_q8_dense(__func__, M, std::max(K, N))) return rc;
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(scales_gate); GMLP_REQUIRE_ALIGNED(codes_up);
   GMLP_REQUIRE_ALIGNED(scales_up); GMLP_REQUIRE_ALIGNED(codes_down); GMLP_REQUIRE_ALIGNED(scales_down);
   GMLP_REQUIRE_ALIGNED(b_gate); GMLP_REQUIRE_ALIGNED(b_up); GMLP_REQUIRE_ALIGNED(b_down);
@@ -2077,7 +2082,7 @@ int gmlp_q8_moe_fwd(const void* x, const void* logits, const void* codes_gate, c
   if (M > GMLP_Q8_MOE_MAX_PAIRS / top_k)
     return fail(GMLP_ESHAPE, "%s: M * top_k = %lld exceeds the %d choices of a call", __func__, (long long)(M * top_k), GMLP_Q8_MOE_MAX_PAIRS);
   const Q8MoePlan plan = plan_q8_moe(M * top_k, K, N, E);
-  if (int rc = check_q8_sizes(__func__, plan.rows, K, N, plan.tiles)) return rc;
+  if (int rc = check_q8_threads(__func__, plan.tiles, std::max(K, N), !plan.gemm)) return rc;
   if (M * gmlp::q8_padded(K) > gmlp::Q8_MAX_LINES)
     return fail(GMLP_ESHAPE, "%s: M * K = %lld exceeds what a call takes", __func__, (long long)(M * K));
   GMLP_REQUIRE_ALIGNED(x); GMLP_REQUIRE_ALIGNED(codes_gate); GMLP_REQUIRE_ALIGNED(codes_up); GMLP_REQUIRE_ALIGNED(codes_down);
