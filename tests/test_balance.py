@@ -292,6 +292,21 @@ def test_shapes_strides_streams_and_repeats():
 
 
 @gpu
+@pytest.mark.parametrize("M,E,k", [(1, 3, 2), (64, 8, 2), (3000, 60, 4), (20000, 300, 3)])
+def test_what_a_step_keeps_for_its_gradient(M, E, k):
+    """Logits, mask, weights, experts and a slope for each expert, in tensors that hold nothing else."""
+    x = torch.randn((M, E), device=device()).requires_grad_()
+    mask = torch.ones(M, dtype=torch.bool, device=x.device)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+        got = moe.moe_route_balanced(x, k, token_mask=mask)
+    assert sorted(tuple(t.shape) for t in kept) == sorted([(M, E), (M,), (M, k), (M, k), (E,)])
+    assert all(t.untyped_storage().nbytes() == t.numel() * t.element_size() for t in kept)
+    del kept
+    torch.autograd.grad((got.weights.sum(), got.loss), x)
+
+
+@gpu
 def test_what_autograd_is_refused():
     x = torch.randn(6, 8, device=device()).requires_grad_()
     got = moe.moe_route_balanced(x, 2)

@@ -870,7 +870,7 @@ Tensor moe_mlp_q8(const Tensor& x_in, const Tensor& logits_in, const Q8& gate, c
 // ------------------------------------------------------------------ routing that is trained
 // d weights, d loss -> d logits
 struct RouteBackward : public ag::Node {
-  int64_t M = 0, E = 0, top_k = 0, slope_numel = 0;
+  int64_t M = 0, E = 0, top_k = 0;
   bool normalize = true;
   int code = 0;
   std::vector<int64_t> sizes, weights_sizes;
@@ -903,7 +903,7 @@ struct RouteBackward : public ag::Node {
       const Tensor logits = readable_as(logits_saved, M * E, options.dtype().toScalarType(), device);
       const Tensor weights = readable_as(weights_saved, M * top_k, at::kFloat, device);
       const Tensor experts = readable_as(experts_saved, M * top_k, at::kLong, device);
-      const Tensor slope = readable_as(slope_saved, slope_numel, at::kFloat, device);
+      const Tensor slope = readable_as(slope_saved, E, at::kFloat, device);
       const Tensor mask = mask_saved.defined() ? readable_as(mask_saved, M, at::kBool, device) : Tensor();
       const Tensor d_weights = grads[0].defined() ? readable_as(grads[0], M * top_k, at::kFloat, device) : Tensor();
       const Tensor d_loss = grads[1].defined() ? readable_as(grads[1], 1, at::kFloat, device) : Tensor();
@@ -952,14 +952,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_route_balanced(const Tensor& logi
     if (M > 0) {
       counts = at::empty({E}, i64);
       loss = at::empty({}, f32);
-      // the slopes, which the backward pass reads, and behind them the workspace in one allocation
-      const int64_t room = (E + 3) / 4 * 4;
+      slope = at::empty({E}, f32);  // (what the backward pass reads of the forward's sums)
       const size_t bytes = lib.gmlp_moe_balance_workspace_bytes(M, E);
-      slope = at::empty({room + (int64_t)(bytes / sizeof(float))}, f32);
-      float* const base = (float*)out_ptr(slope);
+      const Tensor ws = scratch(bytes > 0 ? bytes : 16, logits);  // (0: what the call refuses)
       check(lib.gmlp_moe_balance_fwd(ptr(logits), (const uint8_t*)ptr(mask), (float*)out_ptr(weights), (int64_t*)out_ptr(experts),
-                                     (int64_t*)out_ptr(counts), (float*)out_ptr(loss), base, M, E, top_k, normalize, code, base + room, bytes,
-                                     stream_of(logits)));
+                                     (int64_t*)out_ptr(counts), (float*)out_ptr(loss), (float*)out_ptr(slope), M, E, top_k, normalize, code,
+                                     out_ptr(ws), bytes, stream_of(logits)));
     } else {
       counts = at::zeros({E}, i64);
       loss = at::zeros({}, f32);
@@ -970,7 +968,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_route_balanced(const Tensor& logi
     auto node = std::shared_ptr<RouteBackward>(new RouteBackward(), ag::deleteNode);
     node->set_next_edges(ag::collect_next_edges(logits_in));
     node->M = M; node->E = E; node->top_k = top_k; node->normalize = normalize; node->code = code;
-    node->slope_numel = slope.numel();
     node->sizes = logits_in.sizes().vec();
     node->options = logits_in.options();
     node->logits_ = ag::SavedVariable(logits_in, false);
