@@ -271,6 +271,31 @@ def test_quantize_and_dequantize(shape, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,bits,unit", [(torch.float16, 11, 5), (torch.float16, 11, -15), (torch.bfloat16, 8, 113), (torch.bfloat16, 8, -7),
+                                             (torch.bfloat16, 8, -67), (torch.bfloat16, 8, -117)])
+def test_every_quotient_is_rounded_to_the_nearest(dtype, bits, unit):
+    """A row for every mantissa b of the largest, b 2^unit, and in it every mantissa a of numbers a 2^(unit - k) up to it, for each gap k
+    of exponents that leaves a quotient 127 a / (b 2^k) of a half or more; k = 9 leaves none.  In whole numbers."""
+    some = torch.arange(1 << (bits - 1), 1 << bits, device=device())
+    b = some[:, None]
+    numbers, expected = [b], [torch.full_like(b, 127)]
+    for k in range(10):
+        a = some[None, :] * (some[None, :] <= b if k == 0 else torch.ones_like(b))
+        sign = 1 - 2 * (some[None, :] + b + k & 1)
+        whole, rest = 127 * a // (b << k), 127 * a % (b << k)
+        up = (2 * rest > b << k) | ((2 * rest == b << k) & (whole % 2 == 1))
+        numbers.append((sign * a).double() * 2.0**-k)
+        expected.append(sign * (whole + up))
+    numbers, expected = torch.cat([n.double() for n in numbers], 1), torch.cat(expected, 1)
+    fill = -numbers.shape[1] % 8
+    w = (torch.nn.functional.pad(numbers, (0, fill)) * 2.0**unit).to(dtype)
+    assert torch.equal(w[:, : numbers.shape[1]].double(), numbers * 2.0**unit)
+    got = numbers_of(quant.quantize_q8(w), w.device)
+    assert torch.equal(got, torch.nn.functional.pad(expected, (0, fill)).double())
+    assert (expected[:, -len(some) :] == 0).all() and expected[:, -2 * len(some) :].any()
+
+
+@gpu
 def test_rows_that_are_not_finite_are_nan_and_stand_alone():
     for dtype in HALF:
         w = normal((24, 136), 1.0, dtype, gen(3))
@@ -309,6 +334,44 @@ def test_q8_linear(M, R, C, bias, dtype):
     y = quant.q8_linear_fwd(on(x), q, on(b))
     ref, bound = product64(x, weight_of(q), b)
     hold(y, ref, bound, dtype)
+
+
+# A long batch goes in pieces of 65536 rows, which its rows do not see.
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("more", [17, 300])
+def test_rows_around_the_cut_of_a_long_batch(more, dtype):
+    M, K, N = 65536 + more, 72, 40
+    g = gen(more)
+    x = on(normal((M, K), 1.0, dtype, g))
+    w = [q8((N, K), dtype, g), q8((N, K), dtype, g), q8((K, N), dtype, g)]
+    b = [normal((n,), 0.3, dtype, g) for n in (N, N, K)]
+    rows = torch.tensor([0, 1, 127, 40000, 65534, 65535, 65536, 65537, M - 2, M - 1])
+    y = quant.q8_linear_fwd(x, w[0], on(b[0]))
+    ref, bound = product64(x[on(rows)].cpu(), weight_of(w[0]), b[0])
+    hold(y[on(rows)], ref, bound, dtype)
+    assert torch.equal(y[:65536], quant.q8_linear_fwd(x[:65536], w[0], on(b[0])))
+    y = quant.q8_mlp_fwd(x, w[0], on(b[0]), w[1], on(b[1]), w[2], on(b[2]))
+    ref, bound = mlp64(x[on(rows)].cpu(), weight_of(w[0]), b[0], weight_of(w[1]), b[1], weight_of(w[2]), b[2], "silu", dtype)
+    hold(y[on(rows)], ref, bound, dtype, len(rows) * N)
+    assert torch.equal(y[:65536], quant.q8_mlp_fwd(x[:65536], w[0], on(b[0]), w[1], on(b[1]), w[2], on(b[2])))
+
+
+@gpu
+@pytest.mark.parametrize("M,C", [(65536 + 17, 262144), (3000, (1 << 23) - 8)])
+def test_a_long_batch_through_a_wide_weight(M, C):
+    """A vocabulary projection, and the widest weight that can be quantised.  (34 and 50 GB of outputs.)"""
+    dtype, K = torch.float16, 8
+    g = gen(C % 1000)
+    x, q = on(normal((M, K), 1.0, dtype, g)), quant.quantize_q8(torch.randn((C, K), device=device()).to(dtype))
+    y = quant.q8_linear_fwd(x, q)
+    rows = on(torch.tensor([0, 1, 127, 128, 2047, 2048, M - 1081, M - 18, M - 17, M - 1]))
+    cols = on(torch.cat([torch.arange(32), torch.randint(0, C, (200,), generator=g), torch.arange(C - 32, C)]))
+    n, s = integers64(x[rows])
+    ref = (n @ numbers_of(q, x.device)[cols].T) * s * q.scales.double()[cols]
+    hold(y[rows][:, cols], ref.cpu(), (8 * F * ref.abs()).cpu(), dtype)
+    del y
+    torch.cuda.empty_cache()
 
 
 @gpu
@@ -364,44 +427,6 @@ def test_refusals_of_tensors():
         (lambda: quant.quantize_q8(x[0]), ValueError),
         (lambda: quant.quantize_q8(x[:, :260]), NotImplementedError),
         (lambda: quant.dequantize_q8(q, torch.float32), TypeError),
-# A long batch goes in pieces of 65536 rows, which its rows do not see.
-@gpu
-@pytest.mark.parametrize("dtype", HALF)
-@pytest.mark.parametrize("more", [17, 300])
-def test_rows_around_the_cut_of_a_long_batch(more, dtype):
-    M, K, N = 65536 + more, 72, 40
-    g = gen(more)
-    x = on(normal((M, K), 1.0, dtype, g))
-    w = [q8((N, K), dtype, g), q8((N, K), dtype, g), q8((K, N), dtype, g)]
-    b = [normal((n,), 0.3, dtype, g) for n in (N, N, K)]
-    rows = torch.tensor([0, 1, 127, 40000, 65534, 65535, 65536, 65537, M - 2, M - 1])
-    y = quant.q8_linear_fwd(x, w[0], on(b[0]))
-    ref, bound = product64(x[on(rows)].cpu(), weight_of(w[0]), b[0])
-    hold(y[on(rows)], ref, bound, dtype)
-    assert torch.equal(y[:65536], quant.q8_linear_fwd(x[:65536], w[0], on(b[0])))
-    y = quant.q8_mlp_fwd(x, w[0], on(b[0]), w[1], on(b[1]), w[2], on(b[2]))
-    ref, bound = mlp64(x[on(rows)].cpu(), weight_of(w[0]), b[0], weight_of(w[1]), b[1], weight_of(w[2]), b[2], "silu", dtype)
-    hold(y[on(rows)], ref, bound, dtype, len(rows) * N)
-    assert torch.equal(y[:65536], quant.q8_mlp_fwd(x[:65536], w[0], on(b[0]), w[1], on(b[1]), w[2], on(b[2])))
-
-
-@gpu
-@pytest.mark.parametrize("M,C", [(65536 + 17, 262144), (3000, (1 << 23) - 8)])
-def test_a_long_batch_through_a_wide_weight(M, C):
-    """A vocabulary projection, and the widest weight that can be quantised.  (34 and 50 GB of outputs.)"""
-    dtype, K = torch.float16, 8
-    g = gen(C % 1000)
-    x, q = on(normal((M, K), 1.0, dtype, g)), quant.quantize_q8(torch.randn((C, K), device=device()).to(dtype))
-    y = quant.q8_linear_fwd(x, q)
-    rows = on(torch.tensor([0, 1, 127, 128, 2047, 2048, M - 1081, M - 18, M - 17, M - 1]))
-    cols = on(torch.cat([torch.arange(32), torch.randint(0, C, (200,), generator=g), torch.arange(C - 32, C)]))
-    n, s = integers64(x[rows])
-    ref = (n @ numbers_of(q, x.device)[cols].T) * s * q.scales.double()[cols]
-    hold(y[rows][:, cols], ref.cpu(), (8 * F * ref.abs()).cpu(), dtype)
-    del y
-    torch.cuda.empty_cache()
-
-
     ]:
         with pytest.raises(error):
             call()

@@ -26,10 +26,13 @@ __device__ __forceinline__ uint32_t max_bits(uint32_t most, uint32_t two) {
   const u16x2 a = __builtin_bit_cast(u16x2, most), b = __builtin_bit_cast(u16x2, two & 0x7fff7fffu);
   return __builtin_bit_cast(uint32_t, (u16x2)__builtin_elementwise_max(a, b));
 }
-// n = 127 v / top rounded half to even: a product of 127 v with fl(1 / top), one step of correction, and the addition of 1.5 2^23, whose
-// result has n in its low bits.  127 v and top have few bits: a quotient that is no half is 1 / (2 top) from one at least, 2^-12 in
-// units of n, far more than the two roundings; one that is a half is a number of fp32, and the corrected quotient is it (what
-// the first product is off by is exact in the fused multiply-add).  8 instructions a number in the place of the division's 15.
+// n = 127 v / top rounded half to even: a product u of 127 v with fl(1 / top), one step of correction, and the addition of 1.5 2^23, whose
+// result has n in its low bits.  With top = b and v = a 2^-k in units of top's last place, a and b of p bits (11 of fp16, 8 of bf16) and k
+// the gap of the exponents, the quotient q = 127 a / (b 2^k) is below 2^(8-k) and, if it is no half, at least 1 / (2 b 2^k) > 2^-(12+k)
+// from one: both shrink with the gap.  The first product is within 2^-23 q, so that its remainder, of 13 bits, is exact in the fused
+// multiply-add; the correction is within 2^-47 q of what is missing, and the result off by its own rounding, 2^-24 q < 2^-(16+k): on the side
+// of the half where q is.  A q that is a half is a number of fp32, which no rounding of what is within 2^-47 q of it misses.  From
+// k = 9 on n is 0.  8 instructions a number in the place of the division's 15.
 template <typename T>
 struct RowScale {
   float top, pre, by, scale;
