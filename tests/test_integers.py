@@ -295,6 +295,34 @@ def test_every_quotient_is_rounded_to_the_nearest(dtype, bits, unit):
     assert (expected[:, -len(some) :] == 0).all() and expected[:, -2 * len(some) :].any()
 
 
+# Every form in which rows become integers: by how many rows there are, and by their length (kept by the threads in 1, 2, 4 or 8 pieces, or read
+# twice).
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("cols", [264, 5000, 16392, 20488, 32768, 32776, 40008])
+@pytest.mark.parametrize("shape", [(24,), (1032,), (3, 360)])
+def test_dense_rows_of_every_length(shape, cols, dtype):
+    w = normal((*shape, cols), 1.0, dtype, gen(cols))
+    q = quant.quantize_q8(on(w))
+    # (divided on the CPU: on the GPU torch multiplies by fl(1/127))
+    assert torch.equal(q.scales.cpu(), w.abs().amax(-1).float() / 127.0)
+    for e in [None] if len(shape) == 1 else range(shape[0]):
+        n, _ = integers64(on(w if e is None else w[e]))
+        assert torch.equal(numbers_of(q if e is None else sliced(q, e), n.device), n)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("M,R,C", [(1032, 20488, 40), (1032, 32768, 24), (1040, 33000, 24), (1009, 16392, 136)])
+def test_q8_linear_of_many_long_rows(M, R, C, dtype):
+    g = gen(M + R)
+    x, q = normal((M, R), 1.0, dtype, g), q8((C, R), dtype, g)
+    y = quant.q8_linear_fwd(on(x), q)
+    n, s = integers64(on(x))
+    ref = (n @ numbers_of(q, n.device).T) * s * q.scales.double()
+    hold(y, ref.cpu(), 8 * F * ref.abs().cpu(), dtype)
+
+
 @gpu
 def test_rows_that_are_not_finite_are_nan_and_stand_alone():
     for dtype in HALF:
