@@ -873,7 +873,7 @@ struct RouteBackward : public ag::Node {
   int64_t M = 0, E = 0, top_k = 0;
   bool normalize = true;
   int code = 0;
-  std::vector<int64_t> sizes, weights_sizes;
+  std::vector<int64_t> sizes;
   at::TensorOptions options;  // of the logits
   ag::SavedVariable logits_, weights_, experts_, slope_, mask_;
 
@@ -952,12 +952,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_route_balanced(const Tensor& logi
     if (M > 0) {
       counts = at::empty({E}, i64);
       loss = at::empty({}, f32);
-      slope = at::empty({E}, f32);  // (what the backward pass reads of the forward's sums)
+      // The slopes lie ahead of the workspace, but for a step that is recorded: that keeps them and nothing else.
+      const int64_t room = (E + 3) / 4 * 4;
       const size_t bytes = lib.gmlp_moe_balance_workspace_bytes(M, E);
-      const Tensor ws = scratch(bytes > 0 ? bytes : 16, logits);  // (0: what the call refuses)
+      const Tensor ws = at::empty({room + (int64_t)(bytes / sizeof(float))}, f32);
+      float* const base = (float*)out_ptr(ws);
+      if (graph) slope = at::empty({E}, f32);
       check(lib.gmlp_moe_balance_fwd(ptr(logits), (const uint8_t*)ptr(mask), (float*)out_ptr(weights), (int64_t*)out_ptr(experts),
-                                     (int64_t*)out_ptr(counts), (float*)out_ptr(loss), (float*)out_ptr(slope), M, E, top_k, normalize, code,
-                                     out_ptr(ws), bytes, stream_of(logits)));
+                                     (int64_t*)out_ptr(counts), (float*)out_ptr(loss), graph ? (float*)out_ptr(slope) : base, M, E, top_k,
+                                     normalize, code, base + room, bytes, stream_of(logits)));
     } else {
       counts = at::zeros({E}, i64);
       loss = at::zeros({}, f32);
