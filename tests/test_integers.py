@@ -524,6 +524,29 @@ def test_q8_moe_with_masked_experts_and_crowds(M, E, k):
     hold(y, ref, bound, dtype, M * N)
 
 
+# The way an expert layer runs is chosen by the rows an expert has on average; routers have popular experts.  Up to 12, 24 and 48 rows an
+# expert and beyond, each with an expert that has many times as many and experts that have a few or none.
+@gpu
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize(
+    "M,K,N,E,k,act",
+    [
+        (40, 264, 520, 20, 2, "silu"), (100, 136, 264, 60, 6, "gelu"), (150, 264, 392, 16, 2, "silu"), (90, 4104, 2056, 8, 2, "relu"),
+        (200, 264, 136, 12, 2, "silu"), (320, 136, 520, 64, 8, "tanh"), (700, 264, 520, 10, 2, "silu"), (1200, 520, 264, 32, 4, "gelu"),
+    ],
+)
+def test_q8_moe_with_popular_experts(M, K, N, E, k, act, dtype):
+    g = gen(M + E)
+    x = normal((M, K), 1.0, dtype, g)
+    logits = normal((M, E), 1.5, torch.float32, g) - torch.linspace(0, 9, E)[torch.randperm(E, generator=g)]
+    rows = torch.bincount(route64(logits, k, True)[1].reshape(-1), minlength=E)
+    assert rows.max() > 3 * M * k / E and rows.min() < M * k / E / 3
+    w = [q8((E, N, K), dtype, g), q8((E, N, K), dtype, g), q8((E, K, N), dtype, g)]
+    y = moe.moe_mlp_fwd(on(x), on(logits), *w, k, act_fn=act)
+    ref, bound = moe64(x, logits, k, True, act, dtype, lambda e: [weight_of(sliced(q, e)) for q in w])
+    hold(y, ref, bound, dtype, M * N)
+
+
 @gpu
 @pytest.mark.parametrize("E", [4, 70, 300])
 def test_the_only_token_with_masked_experts(E):
