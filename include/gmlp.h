@@ -405,7 +405,8 @@ int gmlp_moe_balance_bwd(const void* logits, const uint8_t* mask, const float* w
  * 8-bit integer weights and activations, inference only, fp16 and bf16, any number of token rows.  A row of numbers v becomes
  * n = 127 v / max|v| rounded to nearest (even) and the scale max|v| / 127 (float): a row of a weight, once, or of token
  * rows, in each call.  A row with a number that is not finite has scale NaN and n = 0.  Products are sums of n, exact in
- * 32-bit integers, times both scales in fp32.
+ * 32-bit integers, times both scales in fp32.  (The two scales are multiplied first, in fp32: where their product overflows or is
+ * subnormal, which takes bf16 rows and weights far from 1, results are infinite, NaN or of few bits.)
  *
  * Storage of a matrix [rows, cols] (multiples of 8, cols at most 131072), padded with zeros to tiles of 16 rows and blocks of 128
  * columns: codes int8 [tiles][blocks][2 s][4 q][16 r][16]: columns 64 s + 16 q + 0..15 of the block, row r of the tile;

@@ -1817,7 +1817,9 @@ Q8DensePlan plan_q8(int kind, int64_t M, int64_t N, int64_t padded) {
   return p;
 }
 // Up to 64 rows weights are streamed, up to 128 but for a single matrix's long reductions.  us, streamed and by the GEMM, 100 rows: 4096 x 14336
-// 25, 33; 4096 x 4096 15, 17; 2048 x 2048 10.2, 13.9; 14336 x 4096 35, 28 (64 rows 27, 27); 2048 x 14336 16.7, 15.7.
+// 25, 33; 4096 x 4096 15, 17; 2048 x 2048 10.2, 13.9; 14336 x 4096 35, 28 (64 rows 27, 27); 2048 x 14336 16.7, 15.7.  Around the bound, columns x rows of
+// the weight: 6144 x 4096 19.8, 18.8; 6144 x 14336 30.9, 34.1; 7168 x 4096 21.9, 19.3; 8192 x 1024 23.9, 18.5; 8192 x 4096 25.5, 21.8; 8192 x 14336
+// 43, 33.
 bool q8_streams(int kind, int64_t M, int64_t padded) { return M <= 64 || (M <= gmlp::Q8_FEW_ROWS && (kind == GATEUP || padded < 8192)); }
 size_t q8_split_bytes(int kind, int64_t M, int64_t N, int64_t padded) {
   if (q8_streams(kind, M, padded)) return 0;
@@ -1898,8 +1900,9 @@ Q8MoePlan plan_q8_moe(int64_t pairs, int64_t K, int64_t N, int64_t E) {
   p.gemm = each > 48;
   p.cap = each <= 12 ? 16 : each <= 24 ? 32 : p.gemm ? 128 : 64;
   // Small tiles find their token rows by their numbers: these become integers beside the routing, each once.  A load then touches 16 lines in
-  // the place of 8.  us, by number and laid out in the plan's order: 64 experts of 2048 x 1024, 24 rows (32) 107, 112; 16 of 2048 x 2816, 24
-  // rows 75, 79; 8 of 4096 x 14336, 24 rows 284, 254.
+  // the place of 8.  us, by number and laid out in the plan's order, 24 rows an expert: 64 experts of 2048 x 1024 107, 112; 16 of 2048 x 2816
+  // 75, 79; 8 of 4096 x 14336 284, 254.  With 20 rows, of which fewer experts need two tiles: 16 of 2048 x 4096 96, 99; 8 of 4096 x 4096 85, 90; of
+  // 4096 x 8192 158, 161; of 4096 x 14336 258, 261: the bound leaves up to 5 % where the tiles are not full, for the 12 % where they are.
   p.by_token = p.cap == 16 || (p.cap == 32 && K * N <= (int64_t)1 << 23);
   p.rows = gmlp::q8_plan_rows(pairs, E);
   p.tiles = gmlp::q8_plan_tiles(pairs, E, p.cap);

@@ -42,9 +42,9 @@ class BalancedRouting(NamedTuple):
 
 
 def moe_route_balanced(logits: Tensor, top_k: int, normalize: bool = True, token_mask: Optional[Tensor] = None) -> BalancedRouting:
-    """moe_route for training: the same weights and experts, the number of choices that fell on each expert, and the balance loss
-    E · sum_e f_e·P_e, f_e being the expert's share of all choices and P_e the mean of its softmax probability over the tokens.  It is 1
-    where every expert gets as much.
+    """moe_route for training: the same experts and weights (bit for bit up to 256 experts; beyond, their sums have another order), the number
+    of choices that fell on each expert, and the balance loss E · sum_e f_e·P_e, f_e being the expert's share of all choices and P_e the
+    mean of its softmax probability over the tokens.  It is 1 where every expert gets as much.
 
     `weights` and `loss` have gradients for the logits (any of the two may be left unused); f counts as a constant.  `token_mask`
     (bool [...], the logits' leading dimensions) is False for tokens, padding for instance, that are in neither counts nor
